@@ -31,6 +31,7 @@ CODEC_ID = {"q4_k": 12, "q6_k": 14, "iq2_xxs": 16}
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 OP_DEQUANTIZE, OP_QUANTIZE, OP_MATMUL, OP_GATHER, OP_MOE_GLU, OP_SDPA = range(6)
 MAX_GROUP = 8
+PAGED_MAX_ROWS = 2048  # KQ_PAGED_MAX_ROWS
 SDPA_NOALLOC_SCRATCH_BYTES = 32 << 20  # KQ_SDPA_NOALLOC_SCRATCH_BYTES (include/kq_capi.h)
 # KQ_MATMUL_COUNTER_BYTES: arrival counters at the start of every matmul / gather
 # workspace (zero when allocated; the library leaves them zero)
@@ -48,6 +49,7 @@ EXPORTS = (
     "kq_sdpa_workspace_bytes", "kq_sdpa_decode_ragged", "kq_sdpa_decode_ragged_q8", "kq_sdpa_decode_gqa",
     "kq_sdpa_decode_gqa_q8", "kq_sdpa_decode_gqa_noalloc",
     "kq_sdpa_cascade_workspace_bytes", "kq_sdpa_decode_gqa_cascade", "kq_sdpa_decode_gqa_cascade_q8",
+    "kq_paged_plan", "kq_paged_write", "kq_paged_read", "kq_sdpa_paged_workspace_bytes", "kq_sdpa_paged",
     "kq_gguf_open", "kq_gguf_close", "kq_gguf_header", "kq_gguf_kv", "kq_gguf_tensor", "kq_gguf_type_size",
 )
 
@@ -108,6 +110,25 @@ class RouterOptions(ctypes.Structure):
     ]
 
 
+class PagedPool(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("k_biases", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("v_biases", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -157,6 +178,12 @@ _SIGS = {
                                        _i32, _i32, _i32, _i32, _f32, _int, _vp, _vp, _sz, _vp], _int),
     "kq_sdpa_decode_gqa_cascade": ([_vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64, _i32, _vp, _i32, _i32,
                                     _i32, _i32, _i32, _f32, _int, _vp, _vp, _sz, _vp], _int),
+    "kq_paged_plan": ([_vp, _vp, _vp, _i32, _vp, _i64, _i32, _vp, _i32, _vp, _i32, _i32] + [_vp] * 7, _int),
+    "kq_paged_write": ([ctypes.POINTER(PagedPool), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp], _int),
+    "kq_paged_read": ([ctypes.POINTER(PagedPool), _vp, _i32, _vp, _vp, _vp], _int),
+    "kq_sdpa_paged_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _int], _sz),
+    "kq_sdpa_paged": ([_vp, _i64, ctypes.POINTER(PagedPool), _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+                       _f32, _vp, _i64, _vp, _sz, _vp], _int),
     "kq_gguf_open": ([ctypes.c_char_p, ctypes.POINTER(_vp)], _int),
     "kq_gguf_close": ([_vp], None),
     "kq_gguf_header": ([_vp, ctypes.POINTER(ctypes.c_uint32)] + [ctypes.POINTER(_i64)] * 6, _int),

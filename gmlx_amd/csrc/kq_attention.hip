@@ -33,9 +33,7 @@
 #include <mutex>
 #include <type_traits>
 
-#include "kq_common.h"
-
-int device_cus();
+#include "kq_attn.h"
 
 namespace {
 
@@ -86,33 +84,6 @@ struct SdpaArgs {
     // wave finds its units without the scan over the rows' split counts
     int32_t direct;
 };
-
-template <bool BF>
-__device__ __forceinline__ floatx4 mfma(const half8_t &a, const half8_t &b, const floatx4 &c) {
-    if constexpr (!BF) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    } else {
-        typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-    }
-}
-
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (!BF) {
-        return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) |
-               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16);
-    } else {
-        return kq_f32x2_to_bf16_bits(a, b);
-    }
-}
-
-template <bool BF>
-__device__ __forceinline__ uint16_t from_f32(float f) {
-    if constexpr (!BF) return __builtin_bit_cast(uint16_t, (_Float16)f);
-    else return kq_f32_to_bf16_bits(f);
-}
 
 // Element index / D of (row, q head) in q and out, laid out [seq][Hq][qL][D]
 // (qL = 1: [row][Hq][D]).
@@ -201,18 +172,6 @@ __device__ __forceinline__ bool map_unit(const SdpaArgs &a, int u, int &b, int &
     return false;
 }
 
-// Largest of v over the four lane groups (lanes r, r + 16, r + 32, r + 48), in
-// every one of them: row swaps inside the VALU, where LDS shuffles put two
-// round trips into a tile's serial chain.
-__device__ __forceinline__ float max_over_groups(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t w = __builtin_bit_cast(
-        uint32_t, fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1])));
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
-}
-
 // Tokens per K/V tile: 32, or 16 at head dim 512, where a 32-token tile
 // alone would take 256 VGPRs.  A 16-token tile fills the first half of the
 // P.V MFMA's 32 k values; the other half gets zero P and zero V rows.
@@ -269,13 +228,6 @@ struct KVTile {
         for (int i = 0; i < 8; ++i) out[i] = i < VT ? v[dg][i] : u32x4{0u, 0u, 0u, 0u};
     }
 };
-
-// 16-bit float bits (fp16, or bf16 when BF) -> fp32
-template <bool BF>
-__device__ __forceinline__ float f16bits_to_f32(uint32_t h) {
-    if constexpr (BF) return __builtin_bit_cast(float, h << 16);
-    else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
-}
 
 // 8 unsigned bytes -> s * q + b with one rounding to the 16-bit type: the
 // affine dequantization of an 8-bit group-quantized KV cache, group of 64
@@ -542,12 +494,6 @@ struct KvSrc {
     const void *k, *v;
     const uint16_t *ks, *kb, *vs, *vb;
 };
-
-// A wave-uniform value the compiler cannot prove uniform, in scalar registers.
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
-}
 
 template <bool Q8>
 __device__ __forceinline__ KvSrc kv_src(const void *k, const void *v, const uint16_t *ks, const uint16_t *kb,
@@ -891,14 +837,6 @@ __global__ __launch_bounds__(256) void kq_sdpa_merge_kernel(SdpaArgs a) {
     w.x = (uint32_t)from_f32<BF>(acc.x * inv) | ((uint32_t)from_f32<BF>(acc.y * inv) << 16);
     w.y = (uint32_t)from_f32<BF>(acc.z * inv) | ((uint32_t)from_f32<BF>(acc.w * inv) << 16);
     *(uint2 *)(a.out + qo_index(a, b, hq) * D + 4 * q) = w;
-}
-
-int env_int(const char *name, int dflt) {
-    const char *s = getenv(name);
-    if (!s || !*s) return dflt;
-    char *end = nullptr;
-    const long v = strtol(s, &end, 10);
-    return (end && *end == 0 && v > 0 && v < (1 << 24)) ? (int)v : dflt;
 }
 
 // Tokens per split (multiples of the 32-token tile).  A split is one wave's

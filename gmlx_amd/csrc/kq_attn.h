@@ -1,0 +1,73 @@
+// Helpers that the decode and the paged attention kernels share: MFMA and
+// 16-bit conversions by element type, reductions over a wave's lane groups.
+#pragma once
+#include <stdlib.h>
+#include <type_traits>
+
+#include "kq_common.h"
+
+int device_cus();
+
+namespace {
+
+template <bool BF>
+__device__ __forceinline__ floatx4 mfma(const half8_t &a, const half8_t &b, const floatx4 &c) {
+    if constexpr (!BF) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    } else {
+        typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (!BF) {
+        return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) |
+               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16);
+    } else {
+        return kq_f32x2_to_bf16_bits(a, b);
+    }
+}
+
+template <bool BF>
+__device__ __forceinline__ uint16_t from_f32(float f) {
+    if constexpr (!BF) return __builtin_bit_cast(uint16_t, (_Float16)f);
+    else return kq_f32_to_bf16_bits(f);
+}
+
+// Largest of v over the four lane groups (lanes r, r + 16, r + 32, r + 48), in
+// every one of them: row swaps inside the VALU, where LDS shuffles put two
+// round trips into a tile's serial chain.
+__device__ __forceinline__ float max_over_groups(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t w = __builtin_bit_cast(
+        uint32_t, fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1])));
+    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+
+// 16-bit float bits (fp16, or bf16 when BF) -> fp32
+template <bool BF>
+__device__ __forceinline__ float f16bits_to_f32(uint32_t h) {
+    if constexpr (BF) return __builtin_bit_cast(float, h << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+
+// A wave-uniform value the compiler cannot prove uniform, in scalar registers.
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+int env_int(const char *name, int dflt) {
+    const char *s = getenv(name);
+    if (!s || !*s) return dflt;
+    char *end = nullptr;
+    const long v = strtol(s, &end, 10);
+    return (end && *end == 0 && v > 0 && v < (1 << 24)) ? (int)v : dflt;
+}
+
+}  // namespace

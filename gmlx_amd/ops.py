@@ -26,6 +26,7 @@ from __future__ import annotations
 import ctypes
 import os
 from collections import OrderedDict
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -40,7 +41,7 @@ __all__ = [
     "codecs", "codec_has_matmul", "codec_has_moe_glu", "dequantize", "quantize", "quantized_matmul",
     "quantized_matmul_grouped", "fused_mlp", "fused_mlp_status", "counts", "moe_route", "gather_qmm", "moe_glu_gather_kq", "gather_qmv_kq",
     "gather_qmv_mix_ns_kq", "moe_router_topk", "sdpa_decode_ragged", "sdpa_decode_gqa",
-    "ragged_decode_attention", "wire_k",
+    "ragged_decode_attention", "wire_k", "PagedPlan", "paged_plan", "paged_write", "paged_read", "sdpa_paged",
 ]
 
 
@@ -1187,4 +1188,230 @@ def sdpa_decode_gqa_cascade(queries, k_shared, v_shared, k_priv, v_priv, scale, 
     rc = L.kq_sdpa_decode_gqa_cascade(q.data_ptr(), kS.data_ptr(), vS.data_ptr(), shs, P, kP.data_ptr(),
                                       vP.data_ptr(), pbs, phs, S, stp, *common)
     check("kq_sdpa_decode_gqa_cascade", rc)
+    return out
+
+
+# ------------------------------------------------------------ paged KV cache
+
+class PagedPlan(NamedTuple):
+    """One step over a paged cache (paged_plan); int32 tensors on the device."""
+    cu_q: torch.Tensor        # [B + 1] running sum of the rows' new tokens
+    kv_lens: torch.Tensor     # [B] cached tokens once the new ones are written
+    slots: torch.Tensor       # [max_tokens] pool slot of each new token, -1: none
+    positions: torch.Tensor   # [max_tokens] its position in its row, -1: none
+    free_count: torch.Tensor  # [1] pages left on the free stack
+    refused: torch.Tensor     # [B] 1: no pages for this row, which stays as it was
+
+
+def _paged_call(fn, device, *args):
+    """One library call with `device` current (a launch goes to the current
+    device, whichever the stream's is)."""
+    f = getattr(lib(), fn)
+    if torch.cuda.current_device() == device.index:
+        rc = f(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = f(*args)
+    check(fn, rc)
+
+
+def _ints(t, name, shape, device):
+    """A contiguous int32 device tensor of `shape`."""
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or tuple(t.shape) != shape \
+            or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}")
+    return t.data_ptr()
+
+
+def _block_table(t, B, device):
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or t.dim() != 2 \
+            or t.shape[0] != B or t.shape[1] < 1 or t.stride(1) != 1 or (B > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"block_table must be int32 [{B}, pages] on {device}, its rows contiguous")
+    return t.data_ptr(), t.stride(0) if B > 1 else t.shape[1], t.shape[1]
+
+
+def paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens, keep_lens=None):
+    """Block tables and slot maps of one step over a paged cache, built on the
+    device from the requests' lengths, without a host synchronisation.
+
+    Row b has seq_lens[b] cached tokens, in the pages block_table[b, :]; it keeps
+    the first keep_lens[b] of them (default: all; fewer after rejected draft
+    tokens, 0 for a request that has ended) and gets room for new_lens[b] more.
+    Pages no longer needed go back on the free stack free_pages[:free_count],
+    then new ones come off its top, rows in order both times.  Returns a
+    PagedPlan; its slots are what paged_write takes, its cu_q and kv_lens what
+    sdpa_paged takes.  block_table and free_pages are updated in place;
+    seq_lens and free_count are not: the next step is given this one's kv_lens
+    and free_count (or copies them over, inside a HIP graph).  Called again on
+    the same inputs it gives the same.
+
+    The first row that the stack is too short for (or that would not fit the
+    table's width) and the later rows that need pages are refused: they stay as
+    they were, their tokens' slots are -1 and their attention is of no use.
+
+    seq_lens, new_lens, keep_lens int32 [B], B <= 2048; block_table int32
+    [B, pages]; free_pages int32 [n] with n the pool's pages; free_count int32
+    [1]; page_size a power of two from 16 to 1024; max_tokens >= the new tokens
+    of all rows (the length of slots and positions)."""
+    _fault("paged_plan")
+    _require_gpu(seq_lens, new_lens, block_table, free_pages, free_count)
+    dev, B, T = seq_lens.device, seq_lens.numel(), int(max_tokens)
+    if not 1 <= B <= _lib.PAGED_MAX_ROWS or T < 0:
+        raise ValueError(f"paged_plan: 1 to {_lib.PAGED_MAX_ROWS} rows and max_tokens >= 0, got {B} and {T}")
+    tab, tab_stride, width = _block_table(block_table, B, dev)
+    seq, new = _ints(seq_lens, "seq_lens", (B,), dev), _ints(new_lens, "new_lens", (B,), dev)
+    keep = None if keep_lens is None else _ints(keep_lens, "keep_lens", (B,), dev)
+    stack = _ints(free_pages, "free_pages", (free_pages.numel(),), dev)
+    count = _ints(free_count, "free_count", (1,), dev)
+    parts = torch.empty(3 * B + 2 + 2 * T, dtype=torch.int32, device=dev).split((B + 1, B, T, T, 1, B))
+    cu_q, kv, slots, pos, left, refused = (t.data_ptr() for t in parts)
+    _paged_call("kq_paged_plan", dev, seq, keep, new, B, tab, tab_stride, width, stack, free_pages.numel(), count,
+                int(page_size), T, cu_q, kv, slots or cu_q, pos or cu_q, left, refused, _stream(seq_lens))
+    return PagedPlan(*parts)
+
+
+def _paged_pool(k, v, scales, name):
+    """The C description of a pool [n_pages, Hkv, page_size, D], 16-bit or (with
+    the four scale / bias tensors [n_pages, Hkv, page_size, D / 64]) 8-bit."""
+    _require_gpu(k, v)
+    if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or v.device != k.device or v.dtype != k.dtype \
+            or k.stride(3) != 1:
+        raise ValueError(f"{name}: k_cache / v_cache must be [n_pages, Hkv, page_size, D] of one layout, D contiguous")
+    n, H, ps, D = k.shape
+    # (the stride of a dim of size 1 is never used)
+    strides = [s if size > 1 else 0 for s, size in zip(k.stride()[:2], (n, H))] + [k.stride(2)]
+    if all(t is None for t in scales):
+        if k.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"{name}: a 16-bit pool is float16 or bfloat16, got {k.dtype}")
+        return _lib.PagedPool(k.data_ptr(), v.data_ptr(), None, None, None, None, *strides, n, ps, H, D,
+                              _TORCH_DTYPE[k.dtype]), k.dtype
+    if any(t is None for t in scales):
+        raise ValueError(f"{name}: an 8-bit pool needs k_scales, k_biases, v_scales and v_biases")
+    if k.dtype != torch.uint8 or D % 64:
+        raise ValueError(f"{name}: an 8-bit pool holds uint8 values in groups of 64")
+    dt = scales[0].dtype
+    if dt not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{name}: scales and biases must be float16 or bfloat16, got {dt}")
+    for t in scales:
+        if not isinstance(t, torch.Tensor) or t.device != k.device or t.dtype != dt \
+                or tuple(t.shape) != (n, H, ps, D // 64) or (D > 64 and t.stride(3) != 1) \
+                or any(64 * t.stride(i) != k.stride(i) for i in range(3) if t.shape[i] > 1):
+            raise ValueError(f"{name}: scales and biases must be [n_pages, Hkv, page_size, D / 64] of one dtype, laid "
+                             "out as the values are (strides a 64th of theirs)")
+    return _lib.PagedPool(k.data_ptr(), v.data_ptr(), *(t.data_ptr() for t in scales), *strides, n, ps, H, D,
+                          _TORCH_DTYPE[dt]), dt
+
+
+def _token_rows(x, D, name):
+    """x [T, H, D] with D contiguous, the strides multiples of 8 and 16-byte
+    alignment (copied only where it has not): (x, token stride, head stride)."""
+    if x.dim() != 3 or x.shape[2] != D:
+        raise ValueError(f"{name} must be [tokens, heads, {D}]")
+    T, H, _ = x.shape
+    if (D > 1 and x.stride(2) != 1) or (T > 1 and x.stride(0) % 8) or (H > 1 and x.stride(1) % 8) or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x, x.stride(0) if T > 1 else H * D, x.stride(1) if H > 1 else D
+
+
+def paged_write(k, v, k_cache, v_cache, slots, k_scales=None, k_biases=None, v_scales=None, v_biases=None):
+    """Write new tokens' K / V rows [T, Hkv, D] to their slots of a paged cache,
+    in place.
+
+    k_cache / v_cache [n_pages, Hkv, page_size, D], any strides with D
+    contiguous (a [n_pages, page_size, Hkv, D] pool is passed permuted), of the
+    rows' dtype; or, with the four scale / bias tensors [n_pages, Hkv, page_size,
+    D / 64] in the rows' dtype, uint8: each 64 values are stored as
+    (x - bias) / scale rounded to 0..255, bias their smallest and scale a 255th
+    of their range (the 8-bit affine cache of sdpa_decode_gqa's quantized form).
+    slots int32 [T] (PagedPlan.slots): page * page_size + place; a slot outside
+    the pool (-1) writes nothing.  Slots are distinct: of two rows given the
+    same one, which values stay is not specified."""
+    _fault("paged_write")
+    pool, dt = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases), "paged_write")
+    _require_gpu(k, v)
+    if k.dtype != dt or v.dtype != dt or k.shape != v.shape or k.device != k_cache.device or v.device != k.device:
+        raise ValueError(f"paged_write: k and v must be [T, Hkv, D] of dtype {dt} on the cache's device")
+    if k.dim() != 3 or k.shape[1] != pool.Hkv:
+        raise ValueError(f"paged_write: k and v must be [T, {pool.Hkv}, {pool.D}]")
+    k, kt, kh = _token_rows(k, pool.D, "k")
+    v, vt, vh = _token_rows(v, pool.D, "v")
+    T = k.shape[0]
+    sl = _ints(slots, "slots", (T,), k.device)
+    if T:
+        _paged_call("kq_paged_write", k.device, ctypes.byref(pool), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, sl, T,
+                    _stream(k))
+
+
+def paged_read(k_cache, v_cache, slots, k_scales=None, k_biases=None, v_scales=None, v_biases=None):
+    """The K and V rows at `slots` of a paged cache, (k, v) each [T, Hkv, D]:
+    what paged_write stored there, an 8-bit cache's values as scale * q + bias
+    in the scales' dtype; zeros for a slot outside the pool."""
+    _fault("paged_read")
+    pool, dt = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases), "paged_read")
+    _require_gpu(slots)
+    T = slots.numel()
+    sl = _ints(slots, "slots", (T,), k_cache.device)
+    k, v = (torch.empty((T, pool.Hkv, pool.D), dtype=dt, device=k_cache.device) for _ in range(2))
+    if T:
+        _paged_call("kq_paged_read", k.device, ctypes.byref(pool), sl, T, k.data_ptr(), v.data_ptr(), _stream(k_cache))
+    return k, v
+
+
+def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=None, max_kv=None, k_scales=None,
+               k_biases=None, v_scales=None, v_biases=None, out=None):
+    """Attention of each row's new tokens over its pages of a paged cache: decode
+    rows, verify blocks and prompt chunks in one call, causal at the end.
+
+    q [T, Hq, D]: row b's tokens are q[cu_q[b]:cu_q[b + 1]], n of them, and the
+    last n of its kv_lens[b] cached tokens (written before the call); token i
+    attends keys 0 .. kv_lens[b] - n + i, query head hq with kv head
+    hq // (Hq / Hkv).  A token that sees no key gets zeros.  Returns [T, Hq, D]
+    in q's dtype; rows behind the last sequence (cu_q[B] ..) are left as they
+    are in `out` (unspecified where it is not given).
+
+    k_cache / v_cache and the scale / bias tensors as paged_write has them, in
+    q's dtype; block_table int32 [B, pages], kv_lens int32 [B], cu_q int32
+    [B + 1] on the device, read there only.  max_q (default T) and max_kv
+    (default pages * page_size): the most new and cached tokens of any row;
+    they size the launch, and of a row with more only the first max_q tokens
+    are computed and only the first max_kv keys attended.  Entries of the table
+    that are no page of the pool are not attended.  D in 64, 96, 128, 256, 512
+    (no 96 in 8 bits), Hq / Hkv up to 64.  A row's result is bitwise that of a
+    call on the row alone."""
+    _fault("sdpa_paged")
+    pool, dt = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases), "sdpa_paged")
+    _require_gpu(q, kv_lens)
+    dev, B = k_cache.device, kv_lens.numel()
+    if q.dim() != 3 or q.shape[2] != pool.D or q.dtype != dt or q.device != dev or q.shape[1] % pool.Hkv or \
+            not 1 <= q.shape[1] // pool.Hkv <= 64:
+        raise ValueError(f"sdpa_paged: q must be [T, Hq, {pool.D}] of dtype {dt} on the cache's device, Hq a multiple "
+                         f"of Hkv={pool.Hkv} up to 64 times it")
+    T, Hq, D = q.shape
+    tab, tab_stride, width = _block_table(block_table, B, dev)
+    lens, cu = _ints(kv_lens, "kv_lens", (B,), dev), _ints(cu_q, "cu_q", (B + 1,), dev)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=dt, device=dev)
+    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != dt or out.device != dev or \
+            out.stride(2) != 1 or out.stride(1) != D or (T > 1 and (out.stride(0) % 8 or out.stride(0) < Hq * D)) \
+            or out.data_ptr() % 16:
+        raise ValueError("sdpa_paged: out must be like q, its heads contiguous, 16-byte aligned")
+    if not T or not B:
+        return out
+    if q.stride(1) != D or (T > 1 and q.stride(0) < Hq * D):
+        q = q.contiguous()
+    q, qt, _ = _token_rows(q, D, "q")
+    mq = T if max_q is None else min(int(max_q), T)
+    mkv = min(width * pool.page_size, (1 << 31) - 1)
+    if max_kv is not None:
+        mkv = min(mkv, max(1, int(max_kv)) if max_kv >= 0 else -1)
+    if mq < 1 or mkv < 1:
+        raise ValueError("sdpa_paged: max_q must be positive and max_kv not negative")
+    need = lib().kq_sdpa_paged_workspace_bytes(T, B, Hq, pool.Hkv, D, mq, mkv, int(pool.k_scales is not None))
+    s = _stream(q)
+    ws = _WS.get("sdpa_paged", dev, s.value, need) if need else None
+    _paged_call("kq_sdpa_paged", dev, q.data_ptr(), qt, ctypes.byref(pool), tab, tab_stride, width, lens, cu, T, B, Hq,
+                mq, mkv, float(scale), out.data_ptr(), out.stride(0) if T > 1 else Hq * D,
+                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), s)
     return out

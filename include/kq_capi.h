@@ -457,6 +457,101 @@ int kq_sdpa_decode_gqa_cascade_q8(const void *q, const void *k_shared, const voi
                                   float scale, int dtype, void *out, void *workspace,
                                   size_t workspace_bytes, kq_stream_t stream);
 
+/* ---- paged KV cache --------------------------------------------------------- */
+/* A pool of pages that the rows of a batch share: k / v [n_pages][Hkv]
+ * [page_size][D] at any page, head and token strides, D contiguous values a
+ * token.  No counterpart in the reference's call sites: its engine keeps one
+ * left-padded cache per batch and gives prompt chunks to the stock attention.
+ *
+ * 16-bit pool (k_scales NULL): values of `dtype` (f16 or bf16), strides in
+ * elements and multiples of 8, k / v 16-byte aligned, D in {64, 96, 128, 256,
+ * 512}.
+ * 8-bit affine pool, group 64 (as kq_sdpa_decode_ragged_q8 has it): uint8
+ * values, value = scale * q + bias with one scale and one bias of `dtype` per
+ * 64 values at element index (byte offset) / 64 of the four arrays; strides in
+ * bytes and multiples of 64, token_stride == D (a head's tokens of a page lie
+ * one after the other), k / v 16-byte aligned, D in {64, 128, 256, 512}.
+ *
+ * Token t of a row lies in page block_table[row][t / page_size], place t %
+ * page_size; slot = page * page_size + place (n_pages * page_size < 2^31).
+ * page_size: a power of two from 16 to 1024. */
+typedef struct {
+    void *k, *v;
+    void *k_scales, *k_biases, *v_scales, *v_biases; /* all NULL: 16-bit pool */
+    int64_t page_stride, head_stride, token_stride;
+    int32_t n_pages, page_size, Hkv, D;
+    int32_t dtype;
+} kq_paged_pool;
+
+/* Block tables and slot maps of one step, from the rows' lengths, on the
+ * device: B rows (1..KQ_PAGED_MAX_ROWS) of seq_lens[b] cached tokens first keep
+ * keep_lens[b] of them (NULL: all; fewer where draft tokens were rejected or
+ * the request has ended), then get room for new_lens[b] more.  Pages that no
+ * kept or new token needs go on the free stack (free_pages[0 .. *free_count),
+ * of capacity n_stack) in row order; then new pages come off its top in row
+ * order.  The first row that the stack is too short for, or one whose pages
+ * would not fit table_width, is refused: it stays as it was, and so does every
+ * later row that needs a page.
+ *   cu_q [B + 1]      running sum of new_lens (refused rows' tokens included)
+ *   kv_lens [B]       kept + new (refused rows: seq_lens[b])
+ *   slots [max_tokens], positions [max_tokens]  of every new token, in cu_q's
+ *                     order; -1 for a refused row's tokens and past the last
+ *   free_count_out [1], refused [B] (0 or 1)
+ * block_table gets the new pages' ids and free_pages the released ones that
+ * stay; nothing else of them is written, and the inputs seq_lens and
+ * free_count are only read, so the same call made again gives the same.
+ * Outputs must not overlap inputs.  Negative lengths count as 0, seq_lens past
+ * table_width * page_size as that.  All int32 on the device. */
+#define KQ_PAGED_MAX_ROWS 2048
+int kq_paged_plan(const int32_t *seq_lens, const int32_t *keep_lens, const int32_t *new_lens, int32_t B,
+                  int32_t *block_table, int64_t table_stride, int32_t table_width, int32_t *free_pages,
+                  int32_t n_stack, const int32_t *free_count, int32_t page_size, int32_t max_tokens,
+                  int32_t *cu_q, int32_t *kv_lens, int32_t *slots, int32_t *positions, int32_t *free_count_out,
+                  int32_t *refused, kq_stream_t stream);
+
+/* Rows k / v [T][Hkv][D] of the pool's dtype (token and head strides in
+ * elements, multiples of 8, 16-byte aligned) into slots[t] of the pool; a slot
+ * outside the pool (negative, as the plan marks them) writes nothing.  An 8-bit
+ * pool quantises each 64 values: lo and hi their smallest and largest, scale =
+ * (hi - lo) / 255 and bias = lo, both rounded to dtype, q = (x - bias) / scale
+ * rounded to nearest even and clamped to 0..255 (0 where scale is 0).  Slots
+ * are distinct: of two rows given the same slot, which values stay there is
+ * not specified. */
+int kq_paged_write(const kq_paged_pool *pool, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                   const void *v, int64_t v_token_stride, int64_t v_head_stride, const int32_t *slots,
+                   int32_t T, kq_stream_t stream);
+
+/* The rows at slots[t] into k / v [T][Hkv][D] (contiguous, the pool's dtype, 8-bit
+ * values as scale * q + bias in fp32, rounded once); zeros for a slot outside
+ * the pool. */
+int kq_paged_read(const kq_paged_pool *pool, const int32_t *slots, int32_t T, void *k, void *v,
+                  kq_stream_t stream);
+
+/* Attention of each row's new tokens over its pages: row b's tokens are
+ * cu_q[b] .. cu_q[b + 1] of q [T][Hq][D] (token stride q_stride elements, a
+ * multiple of 8; heads contiguous), n of them, the last n of its kv_lens[b]
+ * cached ones.  Token i sees keys 0 .. kv_lens[b] - n + i (none where that is
+ * negative: zeros), and
+ *   out[t, hq] = softmax(scale * q[t, hq] . K_h^T) . V_h,  h = hq / (Hq / Hkv),
+ * with fp32 scores, statistics and sums.  out [T][Hq][D], token stride
+ * out_stride; rows of q behind the last sequence are not read and their output
+ * is left as it was.  Keys whose block table entry is no page of the pool are
+ * not seen.  A key that a token does not see cannot reach its output, whatever
+ * it holds (infinities and NaN included).
+ * max_q: the most new tokens of any row (of a longer row the first max_q are
+ * computed); max_kv: the most cached tokens (longer rows are cut to the first
+ * max_kv keys); both size the launch and the workspace only.  Hq % Hkv == 0, Hq / Hkv
+ * <= 64.
+ * Workspace: fp32 split partials, no zero-fill needed; 256-byte aligned; calls
+ * that share one are ordered.  A row's result is bitwise that of the call on
+ * the row alone. */
+size_t kq_sdpa_paged_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
+                                     int32_t max_kv, int q8);
+int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int32_t *block_table,
+                  int64_t table_stride, int32_t table_width, const int32_t *kv_lens, const int32_t *cu_q,
+                  int32_t T, int32_t B, int32_t Hq, int32_t max_q, int32_t max_kv, float scale, void *out,
+                  int64_t out_stride, void *workspace, size_t workspace_bytes, kq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

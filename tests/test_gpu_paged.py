@@ -1,0 +1,470 @@
+"""The paged KV cache's operators on the GPU: plans against plain Python, writes
+and reads against the definition, attention against fp64 numpy over each row's
+own keys."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as ref
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+# half a step of a rounding to the type, relative to the value
+HALF = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
+
+
+def _say(*a):
+    print(*a, flush=True)
+
+
+# ------------------------------------------------------------------- the plan
+
+def _device_plan(seq, new, table, stack, count, page, T, keep):
+    from gmlx_amd import ops
+    dev = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+    tab, st = dev(table), dev(stack)
+    args = (dev(seq), dev(new), tab, st, dev([count]), page, T)
+    p = ops.paged_plan(*args, keep_lens=None if keep is None else dev(keep))
+    got = [p.cu_q, p.kv_lens, p.slots, p.positions, p.free_count, p.refused, tab, st]
+    got = [x.cpu().numpy() for x in got]
+    again = ops.paged_plan(*args, keep_lens=None if keep is None else dev(keep))
+    for a, b in zip(got, [*again[:4], again.free_count, again.refused, tab, st]):
+        assert np.array_equal(a, b.cpu().numpy())  # the same call again gives the same
+    return got
+
+
+def _check_plan(seq, new, table, stack, count, page, T, keep=None):
+    got = _device_plan(seq, new, table, stack, count, page, T, keep)
+    want = ref.plan(seq, new, np.asarray(table), stack, count, page, T, keep)
+    names = ("cu_q", "kv_lens", "slots", "positions", "free_count", "refused", "table", "stack")
+    for name, a, b in zip(names, got, want):
+        assert np.array_equal(a.reshape(-1), np.asarray(b).reshape(-1)), name
+    return got
+
+
+def _rows(rng, B, page, width, used, spare):
+    """Rows of `used` tokens with their pages, and a free stack of the spare ones."""
+    have = [-(-u // page) for u in used]
+    n_pages = sum(have) + spare
+    order = rng.permutation(n_pages)
+    table, at = np.full((B, width), -7, np.int32), 0
+    for b, h in enumerate(have):
+        table[b, :h] = order[at:at + h]
+        at += h
+    stack = np.full(n_pages, -9, np.int32)
+    stack[:spare] = order[at:]
+    return table, stack, spare
+
+
+@pytest.mark.parametrize("B,page,hi,n", [(1, 16, 1, 1), (1, 16, 500, 4000), (3, 64, 300, 1), (8, 16, 4000, 5),
+                                         (65, 32, 900, 40), (300, 128, 9000, 3), (1025, 16, 200, 2),
+                                         (2048, 16, 100, 17)])
+def test_plan(B, page, hi, n):
+    rng = np.random.default_rng(B * page + n)
+    seq = rng.integers(0, hi + 1, B)
+    new = rng.integers(0, n + 1, B)
+    keep = np.where(rng.random(B) < 0.4, rng.integers(0, hi + 1, B), seq)  # (past seq: all of it)
+    keep[rng.random(B) < 0.1] = 0
+    width = (hi + n) // page + 2
+    table, stack, count = _rows(rng, B, page, width, seq, B * (n // page + 2))
+    T = int(new.sum()) + 5
+    _say("plan", B, page, hi, n, T)
+    _check_plan(seq, new, table, stack, count, page, T, keep)
+    _check_plan(seq, new, table, stack, count, page, T)
+    _check_plan(seq, new, table, stack, count, page, max(0, T - 9), keep)  # fewer slots than tokens
+    # a stack that runs out at some row, at once, and one that is just long enough
+    base = np.minimum(keep, seq)
+    need = np.maximum(-(-(base + new) // page) - -(-seq // page), 0).sum()
+    give = np.maximum(-(-seq // page) - -(-(base + new) // page), 0).sum()
+    for c in {0, max(0, int(need - give)), max(0, int(need - give) - 1), count // 7}:
+        _check_plan(seq, new, table, stack, c, page, T, keep)
+
+
+def test_plan_refuses_a_row_that_the_table_cannot_hold():
+    rng = np.random.default_rng(3)
+    table, stack, count = _rows(rng, 4, 16, 3, [40, 48, 0, 16], 9)
+    got = _check_plan([40, 48, 0, 16], [8, 1, 49, 20], table, stack, count, 16, 80)
+    assert got[5].tolist() == [0, 1, 1, 0]
+    # lengths that no state has: negative ones count as 0, past the table as its width
+    _check_plan([-5, 1000, 3, 7], [-1, 0, 2, 1], np.abs(table), stack, count, 16, 8, [0, 999, -4, 7])
+
+
+def test_plan_ends_requests_and_reuses_their_pages():
+    rng = np.random.default_rng(4)
+    seq = [100, 33, 17, 64]
+    table, stack, count = _rows(rng, 4, 16, 9, seq, 0)
+    # nothing free: row 1's and row 2's pages go back and rows 0 and 3 take them
+    got = _check_plan(seq, [16, 0, 0, 20], table, stack, count, 16, 36, [100, 0, 0, 64])
+    assert got[5].tolist() == [0, 0, 0, 0] and got[4].tolist() == [2]
+
+
+# -------------------------------------------------------------- write and read
+
+def _bits(t):
+    return t.contiguous().view(torch.uint8).cpu().numpy()
+
+
+def _pool(shape, dt, q8, layout, fill=None):
+    """k, v (and their scales and biases) [n_pages, Hkv, page, D] in a memory
+    layout: 'head' as shaped, 'token' [n_pages, page, Hkv, D] permuted, 'mixed'
+    K and V of a page side by side."""
+    n, H, P, D = shape
+
+    def make(D, dtype):
+        if layout == "token":
+            ts = [torch.zeros(n, P, H, D, dtype=dtype, device="cuda").permute(0, 2, 1, 3) for _ in range(2)]
+        elif layout == "mixed":
+            both = torch.zeros(n, 2, H, P, D, dtype=dtype, device="cuda")
+            ts = [both[:, 0], both[:, 1]]
+        else:
+            ts = [torch.zeros(n, H, P, D, dtype=dtype, device="cuda") for _ in range(2)]
+        if fill is not None:
+            for t in ts:
+                t.fill_(fill if dtype != torch.uint8 else 255)
+        return ts
+    if not q8:
+        return make(D, dt), {}
+    (ks, vs), (kb, vb) = make(D // 64, dt), make(D // 64, dt)
+    return make(D, torch.uint8), dict(k_scales=ks, k_biases=kb, v_scales=vs, v_biases=vb)
+
+
+def _quantised(x, dt):
+    """(q, scale, bias) of rows [..., D] by the definition, in fp64 but for the
+    16-bit rounding of the scale."""
+    g = x.double().cpu().unflatten(-1, (-1, 64))
+    lo, hi = g.amin(-1), g.amax(-1)
+    s = ((hi - lo) / 255).to(dt).double()
+    q = torch.where(s[..., None] == 0, 0.0, ((g - lo[..., None]) / s[..., None]).round().clamp(0, 255))
+    return q.flatten(-2).to(torch.uint8), s.to(dt), lo.to(dt)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D,H,P,T,layout", [(64, 1, 16, 1, "head"), (96, 3, 32, 37, "token"), (128, 8, 16, 33, "mixed"),
+                                            (256, 2, 64, 100, "head"), (512, 1, 128, 9, "token")])
+def test_write_and_read_16bit(dt, D, H, P, T, layout):
+    from gmlx_amd import ops
+    torch.manual_seed(D + T)
+    n = T // P + 3
+    (k, v), _ = _pool((n, H, P, D), dt, False, layout, fill=3.0)
+    # rows from a packed q|k|v block: strides of their own
+    rows = torch.randn(T, 3 * H, D, device="cuda").to(dt)
+    x, y = rows[:, H:2 * H], rows[:, 2 * H:]
+    slots = torch.randperm(n * P, device="cuda")[:T].int()
+    if T > 4:
+        slots[1], slots[3], slots[4] = -1, n * P, 2 ** 31 - 1  # no slots of the pool
+    _say("write16", dt, D, H, P, T, layout)
+    before = k.clone(), v.clone()
+    ops.paged_write(x, y, k, v, slots)
+    ok = (slots >= 0) & (slots < n * P)
+    s = slots[ok].long()
+    for pool, old, new in ((k, before[0], x), (v, before[1], y)):
+        old[s // P, :, s % P] = new[ok]
+        assert np.array_equal(_bits(pool), _bits(old))
+    got = ops.paged_read(k, v, slots)
+    for g, new in zip(got, (x, y)):
+        assert np.array_equal(_bits(g), _bits(torch.where(ok[:, None, None], new, 0)))
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D,H,P,T,layout", [(64, 1, 16, 1, "head"), (128, 8, 16, 33, "head"), (256, 2, 64, 100, "mixed"),
+                                            (512, 1, 128, 9, "head")])
+def test_write_and_read_8bit(dt, D, H, P, T, layout):
+    """Scales within one 16-bit step of the definition's (their fp32 quotient
+    rounds once before the 16-bit rounding), biases exact, values the nearest
+    of the stored scale, and read back as scale * q + bias rounded once."""
+    from gmlx_amd import ops
+    torch.manual_seed(D + T)
+    n = T // P + 2
+    (k, v), sc = _pool((n, H, P, D), dt, True, layout)
+    x, y = (torch.randn(T, H, D, device="cuda") * 3 + 1).to(dt), torch.randn(T, H, D, device="cuda").to(dt)
+    x[0, 0, :64] = 1.5  # a group of one value: scale 0
+    if T > 2:
+        y[1, 0, :64] *= 1e-6  # a tiny group
+        x[2, 0, 5] = 60000.0  # an outlier
+    slots = torch.randperm(n * P, device="cuda")[:T].int()
+    _say("write8", dt, D, H, P, T, layout)
+    ops.paged_write(x, y, k, v, slots, **sc)
+    got = ops.paged_read(k, v, slots, **sc)
+    s = slots.long()
+    for new, q, a, b, back in ((x, k, sc["k_scales"], sc["k_biases"], got[0]), (y, v, sc["v_scales"], sc["v_biases"], got[1])):
+        q, a, b = (t[s // P, :, s % P].cpu() for t in (q, a, b))
+        _, want_s, want_b = _quantised(new, dt)
+        assert torch.equal(b, want_b)
+        af, wf = a.double(), want_s.double()
+        tiny = torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+        assert ((af - wf).abs() <= wf * torch.finfo(dt).eps + tiny).all()
+        g, af, bf = new.double().cpu().unflatten(-1, (-1, 64)), af[..., None], b.double()[..., None]
+        ideal = torch.where(af == 0, 0.0, (g - bf) / af).clamp(0, 255)
+        # nearest: half a step, and the fp32 quotient's own rounding (2 roundings of values up to 255)
+        assert ((q.unflatten(-1, (-1, 64)).double() - ideal).abs() <= 0.5 + 255 * 2.0 ** -22).all()
+        val = (q.unflatten(-1, (-1, 64)).double() * af + bf).flatten(-2)
+        # one fp32 rounding, then the 16-bit one
+        room = val.abs() * (HALF[dt] + 2.0 ** -23) + tiny
+        assert ((back.cpu().double() - val).abs() <= room).all()
+
+
+# ------------------------------------------------------------------- attention
+
+class Batch:
+    """Rows of (new tokens, keys) over a pool whose other places hold NaN (8-bit:
+    NaN scales), with block tables that end in no pages."""
+
+    def __init__(self, rows, Hq, Hkv, D, P, dt, q8=False, layout="head", seed=0, spread=1.0, pad=0):
+        rng = np.random.default_rng(seed)
+        gen = torch.Generator().manual_seed(seed)
+        self.rows, self.dt, self.scale = rows, dt, D ** -0.5
+        have = [-(-kv // P) for _, kv in rows]
+        n_pages, width = sum(have) + 3, max(have + [1]) + 2
+        (k, v), sc = _pool((n_pages, Hkv, P, D), dt, q8, layout, fill=float("nan"))
+        order, at = rng.permutation(n_pages), 0
+        table = np.full((len(rows), width), -1, np.int32)
+        table[:, 1::2] = 2 ** 31 - 1
+        self.k, self.v, self.err = [], [], []
+        for b, (n, kv) in enumerate(rows):
+            table[b, :have[b]] = order[at:at + have[b]]
+            at += have[b]
+            t = torch.arange(kv)
+            page, off = torch.from_numpy(table[b].astype(np.int64))[t // P].cuda(), (t % P).cuda()
+            vals = []
+            for pool, which in ((k, "k"), (v, "v")):
+                x = (torch.randn(kv, Hkv, D, generator=gen) * spread).to(dt)
+                if q8:
+                    q, s, bi = _quantised(x, dt)
+                    pool[page, :, off] = q.cuda()
+                    sc[which + "_scales"][page, :, off] = s.cuda()
+                    sc[which + "_biases"][page, :, off] = bi.cuda()
+                    s, bi = (a.double()[..., None] for a in (s, bi))
+                    centred = (q.unflatten(-1, (-1, 64)).double() - 128) * s
+                    # 32-bit dequantisation by sums: s (q . k) + b (sum of q)
+                    vals += [(centred + 128 * s + bi).flatten(-2).transpose(0, 1).numpy(),
+                             centred.abs().flatten(-2).transpose(0, 1).numpy()]
+                else:
+                    pool[page, :, off] = x.cuda()
+                    vals += [x.double().transpose(0, 1).numpy(), x.double().abs().transpose(0, 1).numpy()]
+            self.k.append(vals[0])
+            self.v.append(vals[2])
+            self.err.append(vals[3])
+        T = sum(n for n, _ in rows)
+        self.q = torch.randn(T + pad, Hq, D, generator=gen).to(dt)
+        self.T = T
+        self.pool, self.scales = (k, v), sc
+        ints = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+        self.table, self.kv_lens = ints(table), ints([kv for _, kv in rows])
+        self.cu = np.concatenate([[0], np.cumsum([n for n, _ in rows])])
+        self.cu_q = ints(self.cu)
+
+    def run(self, **kw):
+        from gmlx_amd import ops
+        q = kw.pop("q", self.q.cuda())
+        return ops.sdpa_paged(q, *self.pool, self.table, self.kv_lens, self.cu_q, self.scale, **self.scales, **kw)
+
+    def check(self, out):
+        """Every element within: the output's rounding, the probabilities' (of
+        the values, or of the centred 8-bit ones that they multiply), and the
+        32-bit work of scores of up to 2^6 and sums over the keys."""
+        u = HALF[self.dt]
+        got = out.double().cpu().numpy()
+        for b, (n, kv) in enumerate(self.rows):
+            if not n:
+                continue
+            q = self.q[self.cu[b]:self.cu[b + 1]].double().numpy()
+            want, far = ref.attention(q, self.k[b], self.v[b], n, self.scale, self.err[b])
+            _, mean = ref.attention(q, self.k[b], self.v[b], n, self.scale)
+            smax = 1.5 * self.scale * np.abs(q).sum(-1).max() * max(1.0, np.abs(self.k[b]).max() if kv else 1.0)
+            # a score's products and sums (D + 4 roundings), the power's argument and value, the sums over kv keys
+            f32 = 2.0 ** -24 * (2 * (q.shape[-1] + 8) * smax + 2 * kv + 16)
+            room = u * np.abs(want) + u * (1 + u) * far + f32 * (mean + far) + 1e-7
+            d = np.abs(got[self.cu[b]:self.cu[b + 1]] - want)
+            assert np.isfinite(d).all() and (d <= room).all(), (b, n, kv, (d / room).max())
+
+
+SHAPES = [(128, 32, 8), (64, 8, 8), (96, 12, 3), (256, 16, 2), (128, 5, 1), (512, 8, 1), (64, 64, 2), (128, 48, 1)]
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D,Hq,Hkv", SHAPES)
+def test_attention_shapes(D, Hq, Hkv, dt):
+    rows = [(1, 1), (1, 15), (0, 40), (1, 16), (1, 33), (3, 3), (7, 7 + 64), (0, 0), (5, 2), (2, 0), (1, 700),
+            (40, 333), (1, 0)]
+    _say("attend", D, Hq, Hkv, dt)
+    b = Batch(rows, Hq, Hkv, D, 16, dt, seed=D + Hq)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D,Hq,Hkv", [s for s in SHAPES if s[0] != 96])
+def test_attention_8bit(D, Hq, Hkv, dt):
+    rows = [(1, 1), (1, 15), (0, 40), (1, 32), (3, 3), (7, 7 + 64), (5, 2), (2, 0), (1, 700), (40, 333)]
+    _say("attend8", D, Hq, Hkv, dt)
+    b = Batch(rows, Hq, Hkv, D, 32, dt, q8=True, seed=D + Hq)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("q8,layout", [(False, "token"), (False, "mixed"), (True, "mixed")])
+@pytest.mark.parametrize("P", [16, 64, 256, 1024])
+def test_attention_pages_and_layouts(P, q8, layout):
+    rows = [(1, P), (1, P + 1), (1, 2 * P - 1), (9, 2 * P + 5), (1, 1500), (70, 1200)]
+    _say("pages", P, q8, layout)
+    b = Batch(rows, 16, 2, 128, P, F16, q8=q8, layout=layout, seed=P)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("n,kv", [(1, 9000), (2, 5000), (16, 3100), (65, 2049), (129, 129), (300, 2500), (513, 1030)])
+@pytest.mark.parametrize("dt,q8", [(F16, False), (BF16, False), (BF16, True)])
+def test_attention_chunks(n, kv, dt, q8):
+    _say("chunk", n, kv, dt, q8)
+    b = Batch([(n, kv), (1, 77), (n // 2, kv // 3 + n)], 8, 2, 128, 64, dt, q8=q8, seed=n)
+    b.check(b.run())
+
+
+def test_attention_large_scores():
+    """Scores far apart: probabilities from 1 down to 2^-100 and below."""
+    for dt in (F16, BF16):
+        _say("large", dt)
+        b = Batch([(1, 600), (33, 400)], 8, 2, 64, 16, dt, seed=5, spread=5.0)
+        b.check(b.run())
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,q8", [(128, 32, 8, False), (128, 32, 8, True), (256, 16, 2, False), (64, 8, 8, False)])
+def test_row_equals_the_call_on_the_row_alone(D, Hq, Hkv, q8):
+    """Bit for bit, and the same at every call."""
+    from gmlx_amd import ops
+    rows = [(1, 5000), (1, 130), (200, 1700), (4, 2600), (1, 1), (37, 37)]
+    b = Batch(rows, Hq, Hkv, D, 16, BF16, q8=q8, seed=9)
+    full = b.run()
+    assert torch.equal(full, b.run())
+    for i, (n, kv) in enumerate(rows):
+        lo, hi = int(b.cu[i]), int(b.cu[i + 1])
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        _say("alone", D, q8, n, kv)
+        one = ops.sdpa_paged(b.q[lo:hi].cuda(), *b.pool, b.table[i:i + 1], b.kv_lens[i:i + 1], cu, b.scale, max_q=n,
+                             max_kv=kv, **b.scales)
+        assert torch.equal(one, full[lo:hi]), (n, kv)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("n,kv,Hq", [(5, 70, 8), (40, 90, 8), (150, 400, 8), (150, 400, 32)])
+def test_values_that_a_token_does_not_see(n, kv, Hq, dt):
+    """Infinities and NaN in the keys and values of later tokens leave earlier
+    ones as they are; the tokens that see them get what the sum gives."""
+    base = Batch([(n, kv), (1, 20)], Hq, 2, 128, 16, dt, seed=n)
+    clean = base.run()
+    k, v = base.pool
+    P = 16
+    hit = kv - n // 2 - 1          # a key in the middle of the chunk
+    page, off = int(base.table[0, hit // P]), hit % P
+    for bad, what in ((float("inf"), "v"), (float("-inf"), "v"), (float("nan"), "v"), (float("nan"), "k"),
+                      (float("inf"), "k")):
+        _say("hidden", bad, what, n, kv, dt)
+        pool = (v if what == "v" else k)
+        was = pool[page, :, off].clone()
+        pool[page, 1, off, 3] = bad
+        out = base.run()
+        pool[page, :, off] = was
+        first = hit - (kv - n)     # the first new token that sees it
+        half = Hq // 2
+        assert torch.equal(out[:first], clean[:first]) and torch.equal(out[n:], clean[n:])
+        assert torch.equal(out[:, :half], clean[:, :half])  # the other kv head
+        seen = out[first:n, half:]
+        if what == "v":
+            col = seen[:, :, 3].float()
+            # (a probability that rounds to 0 makes 0 * inf, so NaN is possible beside the infinity)
+            assert (torch.isnan(col).all() if bad != bad else (torch.isnan(col) | (col == bad)).all())
+            rest = [d for d in range(128) if d != 3]
+            assert torch.equal(seen[:, :, rest], clean[first:n, half:][:, :, rest])
+        elif bad != bad:
+            assert torch.isnan(seen).all()
+
+
+def test_hidden_scales_of_an_8bit_pool():
+    base = Batch([(40, 90), (1, 20)], 8, 2, 128, 16, F16, q8=True, seed=2)
+    clean = base.run()
+    hit, P = 70, 16
+    page, off, first = int(base.table[0, hit // P]), hit % P, 70 - 50
+    for name in ("v_scales", "v_biases", "k_scales"):
+        t = base.scales[name]
+        was = t[page, 1, off, 1].clone()
+        t[page, 1, off, 1] = float("nan")
+        out = base.run()
+        t[page, 1, off, 1] = was
+        _say("hidden scale", name)
+        assert torch.equal(out[:first], clean[:first]) and torch.equal(out[:, :4], clean[:, :4])
+        assert torch.isnan(out[first:40, 4:, 64:]).all()
+
+
+def test_pages_outside_the_pool_are_not_seen():
+    """Keys of a table entry that is no page of the pool are left out."""
+    from gmlx_amd import ops
+    for n, kv, bad in ((1, 200, -1), (1, 200, 10 ** 6), (30, 200, -1), (30, 200, 2 ** 31 - 1)):
+        b = Batch([(n, kv)], 8, 2, 128, 32, F16, seed=7)
+        tab = b.table.clone()
+        tab[0, 2] = bad
+        _say("bad page", n, kv, bad)
+        out = ops.sdpa_paged(b.q.cuda(), *b.pool, tab, b.kv_lens, b.cu_q, b.scale)
+        keep = [t for t in range(kv) if t // 32 != 2]
+        for i in range(n):
+            vis = [t for t in keep if t <= kv - n + i]
+            want, far = ref.attention(b.q[i:i + 1].double().numpy(), b.k[0][:, vis], b.v[0][:, vis], 1, b.scale)
+            d = np.abs(out[i:i + 1].double().cpu().numpy() - want)
+            assert (d <= HALF[F16] * (np.abs(want) + far) + 1e-4 * far).all()
+
+
+def test_rows_behind_the_last_sequence_and_strides():
+    """A padded batch into a given output; q a slice of a packed q|k|v block."""
+    for q8 in (False, True):
+        b = Batch([(1, 300), (20, 150), (0, 5)], 8, 2, 128, 16, BF16, q8=q8, seed=3, pad=11)
+        out = torch.full((32, 8, 128), 7.0, dtype=BF16, device="cuda")
+        packed = torch.full((32, 12 * 128), float("nan"), dtype=BF16, device="cuda")
+        packed[:21, :8 * 128] = b.q[:21].reshape(21, -1).cuda()
+        got = b.run(q=packed[:, :8 * 128].unflatten(1, (8, 128)), out=out)
+        assert got.data_ptr() == out.data_ptr() and (out[21:] == 7.0).all()
+        b.check(out[:21])
+        assert torch.equal(out[:21], b.run()[:21])
+        wide = torch.zeros(32, 16, 128, dtype=BF16, device="cuda")
+        b.run(out=wide[:, 3:11])
+        assert torch.equal(wide[:21, 3:11], out[:21]) and (wide[:, :3] == 0).all() and (wide[:, 11:] == 0).all()
+
+
+def test_bounds_cut_longer_rows():
+    """max_q and max_kv below the rows' lengths: the first max_q tokens are
+    computed, over the first max_kv keys."""
+    b = Batch([(6, 100), (2, 50)], 8, 2, 128, 16, F16, seed=3)
+    out = torch.full((8, 8, 128), 7.0, dtype=F16, device="cuda")
+    b.run(out=out, max_q=4)
+    full = b.run()
+    assert torch.equal(out[:4], full[:4]) and (out[4:6] == 7.0).all() and torch.equal(out[6:], full[6:])
+    b.run(out=out, max_kv=64)
+    assert torch.equal(out[6:], full[6:])
+    assert torch.isfinite(out).all()
+    # malformed tables: lengths past the table, a cu_q that runs backwards or past T
+    b.kv_lens = torch.tensor([10 ** 9, -3], dtype=torch.int32, device="cuda")
+    b.cu_q = torch.tensor([4, 2, 90], dtype=torch.int32, device="cuda")
+    b.run(out=out)
+    torch.cuda.synchronize()
+
+
+def test_large_pool_offsets():
+    """Pages that start past 2^31 and 2^32 bytes and elements of the pool."""
+    from gmlx_amd import ops
+    P, H, D = 64, 4, 128
+    n = (5 << 30) // (2 * P * H * D)  # 5 GiB of K, 2.7 G elements
+    dt = F16
+    k, v = (torch.zeros(n, H, P, D, dtype=dt, device="cuda") for _ in range(2))
+    pages = [n - 1, 1, n // 2 + 3, n - 2, (1 << 31) // (P * H * D) + 1]
+    kv = 5 * P - 7
+    x, y = (torch.randn(kv, H, D, device="cuda").to(dt) for _ in range(2))
+    slots = torch.tensor([pages[t // P] * P + t % P for t in range(kv)], dtype=torch.int32, device="cuda")
+    ops.paged_write(x, y, k, v, slots)
+    got = ops.paged_read(k, v, slots)
+    assert torch.equal(got[0], x) and torch.equal(got[1], y)
+    table = torch.tensor([pages], dtype=torch.int32, device="cuda")
+    for m in (1, 33):
+        q = torch.randn(m, 8, D, device="cuda").to(dt)
+        cu = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+        _say("large pool", m)
+        out = ops.sdpa_paged(q, k, v, table, torch.tensor([kv], dtype=torch.int32, device="cuda"), cu, D ** -0.5)
+        want, far = ref.attention(q.double().cpu().numpy(), x.double().cpu().numpy().transpose(1, 0, 2),
+                                  y.double().cpu().numpy().transpose(1, 0, 2), m, D ** -0.5)
+        d = np.abs(out.double().cpu().numpy() - want)
+        assert (d <= HALF[dt] * (np.abs(want) + far) + 1e-4 * far).all()

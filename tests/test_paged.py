@@ -1,0 +1,151 @@
+"""The paged cache's host side: refusals of the C ABI and of the ops, workspace
+sizes, and the plan reference's own invariants.  No GPU needed."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as ref
+
+
+def _lib():
+    from gmlx_amd import _lib as m
+    return m, m.lib()
+
+
+def _pool(**kw):
+    m, _ = _lib()
+    d = dict(k=1 << 20, v=1 << 21, k_scales=None, k_biases=None, v_scales=None, v_biases=None, page_stride=8 * 16 * 128,
+             head_stride=16 * 128, token_stride=128, n_pages=10, page_size=16, Hkv=8, D=128, dtype=m.DTYPE_F16)
+    d.update(kw)
+    return m.PagedPool(**d)
+
+
+Q8 = dict(k_scales=1 << 22, k_biases=1 << 23, v_scales=1 << 24, v_biases=1 << 25)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(k=None), "NULL_POINTER"), (dict(v=None), "NULL_POINTER"), (dict(dtype=0), "UNSUPPORTED_DTYPE"),
+    (dict(D=80), "BAD_SHAPE"), (dict(D=0), "BAD_SHAPE"), (dict(n_pages=0), "BAD_SHAPE"), (dict(Hkv=0), "BAD_SHAPE"),
+    (dict(page_size=8), "BAD_SHAPE"), (dict(page_size=48), "BAD_SHAPE"), (dict(page_size=2048), "BAD_SHAPE"),
+    (dict(n_pages=1 << 27), "BAD_SHAPE"), (dict(token_stride=64), "BAD_SHAPE"), (dict(token_stride=1 << 21), "BAD_SHAPE"),
+    (dict(page_stride=-8), "BAD_SHAPE"), (dict(k=(1 << 20) + 8), "BAD_ALIGN"), (dict(head_stride=2052), "BAD_ALIGN"),
+    (dict(**{**Q8, "v_biases": None}), "NULL_POINTER"), (dict(**Q8, D=96, token_stride=96), "BAD_ALIGN"),
+    (dict(**Q8, D=96, token_stride=128), "BAD_SHAPE"),
+    (dict(**Q8, token_stride=1024), "BAD_SHAPE"), (dict(**Q8, head_stride=2048 + 8), "BAD_ALIGN"),
+    (dict(**{**Q8, "k_scales": (1 << 22) + 1}), "BAD_ALIGN")])
+def test_pools_are_refused(change, code):
+    """By every entry point that takes a pool, before any launch."""
+    m, L = _lib()
+    want = getattr(m, "KQ_ERR_" + code)
+    p = ctypes.byref(_pool(**change))
+    x = 1 << 26
+    assert L.kq_paged_write(p, x, 1024, 128, x, 1024, 128, x, 4, None) == want
+    assert L.kq_paged_read(p, x, 4, x, x, None) == want
+    assert L.kq_sdpa_paged(p and x, 4096, p, x, 4, 4, x, x, 4, 2, 32, 4, 64, 0.1, x, 4096, None, 0, None) == want
+
+
+def test_calls_are_refused():
+    m, L = _lib()
+    ok, x = ctypes.byref(_pool()), 1 << 26
+    assert L.kq_paged_write(ok, None, 0, 0, None, 0, 0, None, 0, None) == m.KQ_OK  # nothing to write
+    assert L.kq_paged_write(ok, None, 1024, 128, x, 1024, 128, x, 4, None) == m.KQ_ERR_NULL_POINTER
+    assert L.kq_paged_write(ok, x, 1024, 128, x, 1024, 128, None, 4, None) == m.KQ_ERR_NULL_POINTER
+    assert L.kq_paged_write(ok, x + 2, 1024, 128, x, 1024, 128, x, 4, None) == m.KQ_ERR_BAD_ALIGN
+    assert L.kq_paged_write(ok, x, 1028, 128, x, 1024, 128, x, 4, None) == m.KQ_ERR_BAD_ALIGN
+    assert L.kq_paged_write(ok, x, 1024, 128, x, 1024, 128, x, -1, None) == m.KQ_ERR_BAD_SHAPE
+    assert L.kq_paged_write(ok, x, 1024, 128, x, 1024, 128, x, 1 << 25, None) == m.KQ_ERR_BAD_SHAPE
+    assert L.kq_paged_read(ok, x, 4, None, x, None) == m.KQ_ERR_NULL_POINTER
+    assert L.kq_paged_read(ok, x, 4, x + 8, x, None) == m.KQ_ERR_BAD_ALIGN
+
+    def sdpa(**kw):
+        d = dict(q=x, qs=4096, pool=ok, tab=x, ts=4, w=4, lens=x, cu=x, T=4, B=2, Hq=32, mq=4, mkv=64, out=x, os=4096,
+                 ws=None, n=0)
+        d.update(kw)
+        return L.kq_sdpa_paged(d["q"], d["qs"], d["pool"], d["tab"], d["ts"], d["w"], d["lens"], d["cu"], d["T"], d["B"],
+                               d["Hq"], d["mq"], d["mkv"], 0.1, d["out"], d["os"], d["ws"], d["n"], None)
+    assert sdpa(T=0) == m.KQ_OK and sdpa(B=0) == m.KQ_OK
+    for name in ("q", "tab", "lens", "cu", "out"):
+        assert sdpa(**{name: None}) == m.KQ_ERR_NULL_POINTER, name
+    for bad in (dict(T=-1), dict(B=-1), dict(Hq=12), dict(Hq=0), dict(Hq=8 * 65), dict(mq=0), dict(mkv=0), dict(w=0),
+                dict(ts=3), dict(qs=4088), dict(os=4088), dict(T=1 << 26)):
+        assert sdpa(**bad) == m.KQ_ERR_BAD_SHAPE, bad
+    for bad in (dict(q=x + 8), dict(out=x + 2), dict(qs=4100), dict(os=4100)):
+        assert sdpa(**bad) == m.KQ_ERR_BAD_ALIGN, bad
+    need = L.kq_sdpa_paged_workspace_bytes(4, 2, 32, 8, 128, 4, 1 << 16, 0)
+    assert need > 0
+    assert sdpa(mkv=1 << 16) == m.KQ_ERR_WORKSPACE_TOO_SMALL
+    assert sdpa(mkv=1 << 16, ws=x, n=need - 1) == m.KQ_ERR_WORKSPACE_TOO_SMALL
+    assert sdpa(mkv=1 << 16, ws=x + 16, n=need) == m.KQ_ERR_BAD_ALIGN
+
+    def plan(**kw):
+        d = dict(seq=x, keep=None, new=x, B=2, tab=x, ts=4, w=4, st=x, n=8, cnt=x, ps=16, T=4, cu=x, kv=x, sl=x, pos=x,
+                 left=x, ref=x)
+        d.update(kw)
+        return L.kq_paged_plan(d["seq"], d["keep"], d["new"], d["B"], d["tab"], d["ts"], d["w"], d["st"], d["n"], d["cnt"],
+                               d["ps"], d["T"], d["cu"], d["kv"], d["sl"], d["pos"], d["left"], d["ref"], None)
+    for name in ("seq", "new", "tab", "st", "cnt", "cu", "kv", "sl", "pos", "left", "ref"):
+        assert plan(**{name: None}) == m.KQ_ERR_NULL_POINTER, name
+    for bad in (dict(B=0), dict(B=2049), dict(w=0), dict(ts=3), dict(n=-1), dict(T=-1), dict(ps=8), dict(ps=24),
+                dict(ps=2048), dict(w=1 << 28, ts=1 << 28)):
+        assert plan(**bad) == m.KQ_ERR_BAD_SHAPE, bad
+
+
+def test_workspace_follows_the_longest_rows():
+    """One partial (D + 2 floats) a token, query head and split at most; none for
+    rows of one split; bounded for prompt chunks however long."""
+    _, L = _lib()
+
+    def f(T, B, kv, mq):
+        return L.kq_sdpa_paged_workspace_bytes(T, B, 32, 8, 128, mq, kv, 0)
+    assert f(8, 8, 64, 1) == 0 and f(0, 8, 4096, 1) == 0
+    assert 0 < f(8, 8, 4096, 1) <= f(8, 8, 131072, 1) <= 8 * 32 * 520 * 1024
+    assert f(65536, 1, 131072, 65536) <= 128 << 20
+
+
+def test_ops_refuse():
+    from gmlx_amd import KQError, ops
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+    sl = torch.zeros(3, dtype=torch.int32)
+    x = torch.zeros(3, 2, 64, dtype=torch.float16)
+    one = torch.zeros(1, dtype=torch.int32)
+    tab = torch.zeros(1, 4, dtype=torch.int32)
+    for call in (lambda: ops.paged_write(x, x, k, k, sl), lambda: ops.paged_read(k, k, sl),
+                 lambda: ops.sdpa_paged(x, k, k, tab, one, torch.zeros(2, dtype=torch.int32), 0.1),
+                 lambda: ops.paged_plan(one, one, tab, sl, one, 16, 4)):
+        with pytest.raises(ValueError, match="GPU only"):
+            call()
+
+
+@pytest.mark.parametrize("name", ["paged_plan", "paged_write", "paged_read", "sdpa_paged"])
+def test_faults_can_be_injected(name, monkeypatch):
+    from gmlx_amd import KQError, ops
+    monkeypatch.setenv("GMLX_HIP_FAULT", name)
+    t = torch.zeros(1)
+    args = {"paged_plan": (t, t, t, t, t, 16, 1), "paged_write": (t, t, t, t, t), "paged_read": (t, t, t),
+            "sdpa_paged": (t, t, t, t, t, t, 1.0)}[name]
+    with pytest.raises(KQError, match="fault injected"):
+        getattr(ops, name)(*args)
+
+
+def test_plan_reference_keeps_every_page_once():
+    """Over many steps every page is in one row's table or on the stack."""
+    rng = np.random.default_rng(0)
+    B, page, n_pages, width = 6, 16, 40, 30
+    seq, table = [0] * B, np.zeros((B, width), np.int32)
+    stack, count = list(range(n_pages)), n_pages
+    refusals = 0
+    for _ in range(300):
+        new = [int(x) for x in rng.integers(0, 60, B) * (rng.random(B) < 0.5)]
+        keep = [0 if rng.random() < 0.15 else int(s - rng.integers(0, 5) * (s > 5)) for s in seq]
+        cu, kv, slots, pos, count, refused, table, stack = ref.plan(seq, new, table, stack, count, page, sum(new), keep)
+        refusals += sum(refused)
+        seq = kv
+        held = [int(p) for b in range(B) for p in table[b, :-(-seq[b] // page)]]
+        assert sorted(held + list(stack[:count])) == list(range(n_pages))
+        for b in range(B):
+            if not refused[b]:
+                for s, p in zip(slots[cu[b]:cu[b + 1]], pos[cu[b]:cu[b + 1]]):
+                    assert s == table[b, p // page] * page + p % page
+    assert refusals > 20
