@@ -21,20 +21,34 @@ struct PagedArgs {
     int64_t q_stride, out_stride, page_stride, head_stride, table_stride;
     int32_t tok_stride, lps, n_pages, width;
     int32_t T, B, Hq, Hkv, G, max_q, max_kv;
+    int32_t group_cols;  // query columns of a chunk's workgroup
     float scale_log2;
     float *part, *ml;  // split partials: [slot][D] sums, [slot][2] (maximum, sum)
 };
 
+constexpr int kFewColumns = 16;     // rows of at most so many columns take the wave kernel
 constexpr int kSplitTokens = 512;   // least keys of a split
-constexpr int kSplitWaves = 2048;   // waves of a row that splitting aims at
+constexpr int kSplitWaves = 2048;   // waves that splitting a row of few columns aims at
+constexpr int kSplitGroups = 512;   // workgroups that splitting a chunk aims at
+
+__host__ __device__ __forceinline__ bool few_columns(int n, int G) { return (int64_t)n * G <= kFewColumns; }
+
+// Query columns of a chunk's workgroup: four waves of 32, or of 16 where 32
+// would take over 256 registers a lane for the sums and the queries.
+constexpr int group_columns(int D) { return D > 128 ? 64 : 128; }
+
+// Workgroups (waves, rows of few columns) of an unsplit row over one kv head.
+__host__ __device__ __forceinline__ int row_blocks(int n, int G, int group_cols) {
+    return few_columns(n, G) ? (n > 0) : (int)(((int64_t)n * G + group_cols - 1) / group_cols);
+}
 
 // Splits of a row of n tokens and kv keys: from the row and the head counts
 // alone, so that a row of a batch has the bits of the row alone.
-__host__ __device__ __forceinline__ int paged_splits(int n, int kv, int G, int Hkv) {
-    const int waves = (int)(((int64_t)n * G + 15) / 16) * Hkv;
-    if (waves == 0) return 1;
+__host__ __device__ __forceinline__ int paged_splits(int n, int kv, int G, int Hkv, int group_cols) {
+    const int units = row_blocks(n, G, group_cols) * Hkv;
+    if (units == 0) return 1;
     const int most = (kv + kSplitTokens - 1) / kSplitTokens;
-    const int want = (kSplitWaves + waves - 1) / waves;
+    const int want = ((few_columns(n, G) ? kSplitWaves : kSplitGroups) + units - 1) / units;
     return max(1, min(want, most));
 }
 
@@ -51,23 +65,26 @@ __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     r.full = min(max(a.cu_q[b + 1], r.q0), a.T) - r.q0;
     r.n = min(r.full, a.max_q);
     r.kv = (int)min((int64_t)max(min(a.kv_lens[b], a.max_kv), 0), (int64_t)a.width << a.lps);
-    r.blocks = (int)(((int64_t)r.n * a.G + 15) / 16);
-    r.splits = paged_splits(r.n, r.kv, a.G, a.Hkv);
+    r.blocks = row_blocks(r.n, a.G, a.group_cols);
+    r.splits = paged_splits(r.n, r.kv, a.G, a.Hkv, a.group_cols);
     return r;
 }
 
-__device__ __forceinline__ int64_t row_units(const PagedArgs &a, const Row &r) {
-    return (int64_t)r.blocks * r.splits * a.Hkv;
+// Units of the chunk kernel (CHUNK) or of the wave kernel.
+template <bool CHUNK>
+__device__ __forceinline__ int row_units(const PagedArgs &a, const Row &r) {
+    return few_columns(r.n, a.G) == CHUNK ? 0 : r.blocks * r.splits * a.Hkv;
 }
 
-__device__ __forceinline__ int64_t row_slots(const PagedArgs &a, const Row &r) {
-    return r.splits > 1 ? (int64_t)r.n * a.Hq * r.splits : 0;
+// (the host refuses calls whose unit or slot numbers pass 31 bits)
+__device__ __forceinline__ int row_slots(const PagedArgs &a, const Row &r) {
+    return r.splits > 1 ? r.n * a.Hq * r.splits : 0;
 }
 
-__device__ __forceinline__ int64_t wave_scan(int64_t v) {
+__device__ __forceinline__ int wave_scan(int v) {
     const int lane = kq_lane();
     for (int off = 1; off < 64; off <<= 1) {
-        const int64_t t = __shfl_up(v, off);
+        const int t = __shfl_up(v, off);
         if (lane >= off) v += t;
     }
     return v;
@@ -76,31 +93,69 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
 // The row that unit u belongs to, with u made its number within the row and
 // the row's first partial slot; false past the last unit.  The unit counts are
 // summed over the rows, 64 at a time, by every wave that asks.
-__device__ __forceinline__ bool find_unit(const PagedArgs &a, int64_t &u, int &b, Row &r, int64_t &slot0) {
+template <bool CHUNK>
+__device__ __forceinline__ bool find_unit(const PagedArgs &a, int &u, int &b, int &slot0) {
     const int lane = kq_lane();
-    int64_t slots = 0;
+    int slots = 0;
     for (int c0 = 0; c0 < a.B; c0 += 64) {
         const int row = c0 + lane;
-        int64_t mu = 0, ms = 0;
+        int mu = 0, ms = 0;
         if (row < a.B) {
             const Row x = row_at(a, row);
-            mu = row_units(a, x);
+            mu = row_units<CHUNK>(a, x);
             ms = row_slots(a, x);
         }
-        const int64_t iu = wave_scan(mu), is = wave_scan(ms);
-        const int64_t total = __shfl(iu, 63);
+        const int iu = wave_scan(mu), is = wave_scan(ms);
+        const int total = __builtin_amdgcn_readlane(iu, 63);
         if (u < total) {
             const int src = __builtin_ctzll(__ballot(u < iu));
-            b = __builtin_amdgcn_readfirstlane(c0 + src);
-            u -= __shfl(iu - mu, src);
-            slot0 = slots + __shfl(is - ms, src);
-            r = row_at(a, b);
+            b = c0 + src;
+            u -= __builtin_amdgcn_readlane(iu - mu, src);
+            slot0 = slots + __builtin_amdgcn_readlane(is - ms, src);
             return true;
         }
         u -= total;
-        slots += __shfl(is, 63);
+        slots += __builtin_amdgcn_readlane(is, 63);
     }
     return false;
+}
+
+// The row again for one wave, in scalar registers.
+__device__ __forceinline__ Row uniform_row(const PagedArgs &a, int b) {
+    Row r = row_at(a, b);
+    r.q0 = __builtin_amdgcn_readfirstlane(r.q0);
+    r.n = __builtin_amdgcn_readfirstlane(r.n);
+    r.full = __builtin_amdgcn_readfirstlane(r.full);
+    r.kv = __builtin_amdgcn_readfirstlane(r.kv);
+    r.blocks = __builtin_amdgcn_readfirstlane(r.blocks);
+    r.splits = __builtin_amdgcn_readfirstlane(r.splits);
+    return r;
+}
+
+// Whether a block table row's entries [p, last] all are pages of the pool.
+__device__ __forceinline__ bool pages_in_pool(const PagedArgs &a, const int32_t *tab, int p, int last) {
+    bool bad = false;
+    for (int i = p + kq_lane(); i <= last; i += 64) bad |= (uint32_t)tab[i] >= (uint32_t)a.n_pages;
+    return __builtin_amdgcn_ballot_w64(bad) == 0;
+}
+
+// 16-bit values whose exponent is all ones (infinities and NaN) as 0 in a
+// masked tile: there the product of a hidden key's value with its probability
+// 0 would be NaN.  `odd` collects whether there were any; the columns that see
+// one get it from add_odd.
+template <bool BF>
+__device__ __forceinline__ uint32_t finite2(uint32_t x, uint32_t &odd) {
+    constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kStep = BF ? 0x00800080u : 0x04000400u;
+    const uint32_t top = ((x & kExp) + kStep) & 0x80008000u;  // exponent + 1 carries into the sign's place
+    odd |= top;
+    return x & ~(top | (top - (top >> 15)));
+}
+
+// What an infinite or NaN value that a column sees does to its sum, else 0.
+template <bool BF>
+__device__ __forceinline__ float odd_part(uint32_t x) {
+    const float v = f16bits_to_f32<BF>(x);
+    return v - v == 0.f ? 0.f : v;
 }
 
 // Exponent shift of the probabilities: they and their sum are 2^kShift times
@@ -123,7 +178,7 @@ struct Geo {
 template <int D>
 struct TileAt {
     int64_t off[Geo<D>::CH];
-    bool ok[Geo<D>::CH];
+    uint32_t ok;  // bit ch
 };
 
 // One tile in registers, 16-bit pool.
@@ -253,7 +308,6 @@ struct State {
     floatx4 o[NO];
     float bias[SG];  // Q8: this lane's share of sum of p b
     float m_run, l_part;
-    int seen;  // keys that the column sees: 0 .. seen - 1
 
     // value 4 consecutive results start at: d of (o[j .. ], e)
     __device__ __forceinline__ void init() {
@@ -297,7 +351,7 @@ struct State {
     // MASK: some of the tile's keys are hidden from some column (vis: bit j for
     // this lane's j-th score).
     template <bool MASK, class Tile>
-    __device__ __forceinline__ void tile(const Tile &t, float scale_log2, uint32_t vis) {
+    __device__ __forceinline__ void tile(const Tile &t, float scale_log2, uint32_t vis, uint32_t &odd) {
         float s[8];
         scores(t, scale_log2, s);
         constexpr int N = 4 * CH;
@@ -328,7 +382,7 @@ struct State {
             for (int j = 0; j < SG; ++j) bias[j] *= alpha;
         }
         if constexpr (!Q8) {
-            pv16<MASK>(t, p, vis);
+            pv16<MASK>(t, p, odd);
         } else {
 #pragma unroll
             for (int grp = 0; grp < SG; ++grp) {
@@ -371,38 +425,20 @@ struct State {
     }
 
     template <bool MASK, class Tile>
-    __device__ __forceinline__ void pv16(const Tile &t, const float (&p)[8], uint32_t vis) {
+    __device__ __forceinline__ void pv16(const Tile &t, const float (&p)[8], uint32_t &odd) {
         const half8_t pf = __builtin_bit_cast(half8_t, u32x4{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3]),
                                                              pack2<BF>(p[4], p[5]), pack2<BF>(p[6], p[7])});
-        constexpr uint32_t kInf = BF ? 0x7F80u : 0x7C00u, kOne = BF ? 0x3F80u : 0x3C00u;
-        bool odd = false;
-        half8_t seen_f = pf;
-        if constexpr (MASK) {
-            // A hidden key's value times its probability 0 is NaN where the
-            // value is an infinity or NaN: look for those, and where there are
-            // any, take them out of the product and add them to the columns
-            // that see them (products of 0 / 1 matrices).
-#pragma unroll
-            for (int dg = 0; dg < Tile::NG; ++dg)
-#pragma unroll
-                for (int i = 0; i < Tile::VT; ++i)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t x = t.v[dg][i][w];
-                        odd |= (x & kInf) == kInf || (x & (kInf << 16)) == (kInf << 16);
-                    }
-            odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-            u32x4 f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                f[j] = ((vis >> (2 * j)) & 1 ? kOne : 0u) | ((vis >> (2 * j + 1)) & 1 ? kOne << 16 : 0u);
-            seen_f = __builtin_bit_cast(half8_t, f);
-        }
 #pragma unroll
         for (int dg = 0; dg < Tile::NG; ++dg) {
             u32x4 vr[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) vr[i] = i < Tile::VT ? t.v[dg][i] : u32x4{0u, 0u, 0u, 0u};
+            for (int i = 0; i < 8; ++i) {
+                vr[i] = i < Tile::VT ? t.v[dg][i] : u32x4{0u, 0u, 0u, 0u};
+                if constexpr (MASK) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) vr[i][w] = finite2<BF>(vr[i][w], odd);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
@@ -411,33 +447,23 @@ struct State {
                 f.y = __builtin_amdgcn_perm(vr[3][j >> 1], vr[2][j >> 1], sel);
                 f.z = __builtin_amdgcn_perm(vr[5][j >> 1], vr[4][j >> 1], sel);
                 f.w = __builtin_amdgcn_perm(vr[7][j >> 1], vr[6][j >> 1], sel);
-                if (MASK && odd) {
-                    u32x4 up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint32_t x = (f[w] >> (16 * half)) & 0xFFFFu;
-                            const bool bad = (x & kInf) == kInf, nan = (x & 0x7FFFu) > kInf;
-                            if (bad) {
-                                f[w] &= half ? 0x0000FFFFu : 0xFFFF0000u;
-                                if (nan || !(x & 0x8000u)) up[w] |= kOne << (16 * half);
-                                if (nan || (x & 0x8000u)) down[w] |= kOne << (16 * half);
-                            }
-                        }
-                    const floatx4 z = {0, 0, 0, 0};
-                    const floatx4 a = mfma<BF>(__builtin_bit_cast(half8_t, up), seen_f, z);
-                    const floatx4 b = mfma<BF>(__builtin_bit_cast(half8_t, down), seen_f, z);
-                    kq_mfma_drain();
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (a[e] > 0.f) o[dg * 8 + j][e] += INFINITY;
-                        if (b[e] > 0.f) o[dg * 8 + j][e] -= INFINITY;
-                    }
-                }
                 o[dg * 8 + j] = mfma<BF>(__builtin_bit_cast(half8_t, f), pf, o[dg * 8 + j]);
             }
         }
+    }
+
+    // Adds the infinite and NaN values of one key (its row of V) to the columns
+    // that see it.
+    __device__ __forceinline__ void add_odd(const uint16_t *v, bool sees) {
+        const int g = kq_lane() >> 4;
+#pragma unroll
+        for (int j = 0; j < NO; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 128 * (j >> 3) + 8 * (4 * g + e) + (j & 7);
+                const float x = d < D ? odd_part<BF>(v[d]) : 0.f;
+                if (sees) o[j][e] += x;
+            }
     }
 };
 
@@ -451,29 +477,21 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
     constexpr int TT = Geo<D>::TT, CH = Geo<D>::CH, NC = Geo<D>::NC;
     constexpr int NBUF = D >= 256 ? 1 : 2;
     const int lane = kq_lane(), r = lane & 15, g = lane >> 4;
-    for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
-        int64_t u = unit, slot0;
-        int b;
-        Row row;
-        if (!find_unit(a, u, b, row, slot0)) return;
-        const uint32_t nth = (uint32_t)u, rest = nth / (uint32_t)a.Hkv;
-        const int h = (int)(nth - rest * a.Hkv);
-        const int blk = (int)(rest / (uint32_t)row.splits), s = (int)(rest - (uint32_t)blk * row.splits);
+    for (int unit = blockIdx.x;; unit += gridDim.x) {
+        int u = unit, b, slot0;
+        if (!find_unit<false>(a, u, b, slot0)) return;
+        const Row row = uniform_row(a, b);
+        const int s = u / a.Hkv, h = u - s * a.Hkv;
 
         // this lane's column
-        const int64_t col = (int64_t)blk * 16 + r;
-        const bool live = col < (int64_t)row.n * a.G;
-        const int i = live ? (int)(col / a.G) : row.n - 1, head = live ? (int)(col - (int64_t)i * a.G) : 0;
-        const int hq = h * a.G + head;
+        const bool live = r < row.n * a.G;
+        const int i = live ? r / a.G : row.n - 1, hq = h * a.G + (live ? r - i * a.G : 0);
         State<D, BF, Q8> st;
         st.init();
-        const int first_i = (int)((int64_t)blk * 16 / a.G);
-        const int last_i = min((int)(((int64_t)blk * 16 + 15) / a.G), row.n - 1);
-        // keys seen: column i's, the block's least and most
-        const auto seen_by = [&](int tok) { return max(row.kv - row.full + tok + 1, 0); };
-        st.seen = live ? seen_by(i) : 0x7fffffff;
-        const int least = __builtin_amdgcn_readfirstlane(seen_by(first_i));
-        const int most = __builtin_amdgcn_readfirstlane(min(seen_by(last_i), row.kv));
+        // keys seen: the column's, the row's least and most
+        const int first = row.kv - row.full + 1;
+        const int seen = live ? max(first + i, 0) : 0x7fffffff;
+        const int least = max(first, 0), most = min(max(first + row.n - 1, 0), row.kv);
         // whole tiles, about the same for each split
         const int per = ((row.kv + row.splits - 1) / row.splits + TT - 1) / TT * TT;
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
@@ -510,50 +528,58 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
             const int64_t h_off = (int64_t)h * a.head_stride;
             auto at_tile = [&](int t0) {
                 TileAt<D> x;
+                x.ok = 0;
 #pragma unroll
                 for (int ch = 0; ch < CH; ++ch) {
                     // (chunks past the end repeat the last: their keys are hidden)
                     const int c = min((t0 >> 4) + ch, c_last), p = c >> sh;
-                    if (p - p0 >= 64) {
+                    if ((uint32_t)(p - p0) >= 64u) {
                         p0 = p;
                         ids = tab[min(p0 + lane, p_last)];
                     }
                     const int id = __builtin_amdgcn_readlane(ids, p - p0);
-                    x.ok[ch] = (uint32_t)id < (uint32_t)a.n_pages;
-                    x.off[ch] = uniform64((int64_t)(x.ok[ch] ? id : 0) * a.page_stride + h_off +
+                    const bool in = (uint32_t)id < (uint32_t)a.n_pages;
+                    x.ok |= in ? 1u << ch : 0u;
+                    x.off[ch] = uniform64((int64_t)(in ? id : 0) * a.page_stride + h_off +
                                           (int64_t)((c - (p << sh)) * 16) * a.tok_stride);
                 }
                 return x;
             };
+            // Tiles that every column sees whole run through the ring; the
+            // others (the last keys; all, where the table names no page) one
+            // by one before them, so that their code is there once.
+            int whole = min(least, t_end);
+            whole = whole <= t_begin || !pages_in_pool(a, tab, p0, p_last) ? t_begin : whole - (whole - t_begin) % TT;
             Tile ring[NBUF];
-            TileAt<D> at[NBUF];
+#pragma unroll 1
+            for (int t = whole; t < t_end; t += TT) {
+                const TileAt<D> at = at_tile(t);
+                ring[0].load(a, at);
+                const int lim = min(seen, t_end);
+                uint32_t vis = 0, odd = 0;
 #pragma unroll
-            for (int j = 0; j < NBUF - 1; ++j) {
-                at[j] = at_tile(t_begin + TT * j);
-                ring[j].load(a, at[j]);
+                for (int x = 0; x < 4 * CH; ++x)
+                    if (((at.ok >> (x >> 2)) & 1) && t + 16 * (x >> 2) + 4 * g + (x & 3) < lim) vis |= 1u << x;
+                st.template tile<true>(ring[0], a.scale_log2, vis, odd);
+                if constexpr (!Q8) {
+                    if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+#pragma unroll 1
+                        for (int k = 0; k < TT; ++k)
+                            st.add_odd((const uint16_t *)a.v + at.off[CH == 1 || k < 16 ? 0 : CH - 1] + (k & 15) * a.tok_stride,
+                                       ((at.ok >> (k >> 4)) & 1) && t + k < lim);
+                    }
+                }
             }
-            for (int t0 = t_begin; t0 < t_end; t0 += TT * NBUF) {
+            if (whole > t_begin) {
+                uint32_t odd;
 #pragma unroll
-                for (int j = 0; j < NBUF; ++j) {
-                    const int nx = (j + NBUF - 1) % NBUF;
-                    at[nx] = at_tile(t0 + TT * (j + NBUF - 1));
-                    ring[nx].load(a, at[nx]);
-                    __builtin_amdgcn_sched_barrier(0);
-                    const int t = t0 + TT * j;
-                    if (t < t_end) {
-                        bool whole = t + TT <= min(least, t_end);
+                for (int j = 0; j < NBUF - 1; ++j) ring[j].load(a, at_tile(t_begin + TT * j));
+                for (int t0 = t_begin; t0 < whole; t0 += TT * NBUF) {
 #pragma unroll
-                        for (int ch = 0; ch < CH; ++ch) whole &= at[j].ok[ch];
-                        if (whole) {
-                            st.template tile<false>(ring[j], a.scale_log2, 0);
-                        } else {
-                            const int lim = min(st.seen, t_end);
-                            uint32_t vis = 0;
-#pragma unroll
-                            for (int x = 0; x < 4 * CH; ++x)
-                                if (at[j].ok[x >> 2] && t + 16 * (x >> 2) + 4 * g + (x & 3) < lim) vis |= 1u << x;
-                            st.template tile<true>(ring[j], a.scale_log2, vis);
-                        }
+                    for (int j = 0; j < NBUF; ++j) {
+                        ring[(j + NBUF - 1) % NBUF].load(a, at_tile(t0 + TT * (j + NBUF - 1)));
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (t0 + TT * j < whole) st.template tile<false>(ring[j], a.scale_log2, 0, odd);
                     }
                 }
             }
@@ -574,7 +600,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
         const bool whole = row.splits == 1;
         const float mul = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
         uint16_t *op = a.out + (int64_t)(row.q0 + i) * a.out_stride + (int64_t)hq * D;
-        const int64_t slot = slot0 + ((int64_t)i * a.Hq + hq) * row.splits + s;
+        const int64_t slot = slot0 + (i * a.Hq + hq) * row.splits + s;
         float *pp = a.part + slot * D;
         // runs of W consecutive values: lane (column, g), o[j0 .. j0 + W)[e]
         constexpr int W = Q8 ? 4 : 8;
@@ -606,6 +632,540 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
     }
 }
 
+// ---- prompt chunks --------------------------------------------------------
+// Rows of more than 16 query columns: a workgroup of four waves takes 128
+// columns, 32 a wave (64 and 16 past head dim 128), and streams the keys in tiles of BN tokens through two
+// LDS stages, copied by direct-to-LDS loads one tile ahead; one barrier a tile.
+// v_mfma_f32_32x32x16: lane 32 h + c holds column c at tokens 8 (i / 4) + 4 h +
+// i % 4 (i < 16) of each 32, which are the P.V operand's eight tokens a lane of
+// two 16-token products; V's operand, eight tokens of one head dim a lane, is
+// read from the row-major tile by transposing LDS reads (ds_read_b64_tr_b16:
+// each group of 16 lanes reads 4 tokens x 16 values and gets a column a lane).
+//
+// An 8-bit pool's tile is written to LDS as 16-bit values by the waves that
+// would copy it: value = hi + lo, each in the queries' type, hi the value
+// s q + b rounded and lo the rest, both multiplied (twice the MFMAs), so that
+// no rounding of a dequantised value enters the result; dequantised to hi
+// alone, outputs were about twice as far from exact as the 16-bit pool's.
+template <int D, bool Q8>
+struct Chunk {
+    static constexpr int NP = Q8 ? 2 : 1;                              // planes: the values, or hi and lo
+    static constexpr int BN = D * NP <= 128 ? 64 : 32;                 // tokens a tile
+    static constexpr int NT = BN / 32;                                 // 32-token blocks
+    static constexpr int RC = D / 8;                                   // 16-byte pieces of a token's row
+    static constexpr int kRow = 2 * D;                                 // bytes
+    static constexpr int kPlane = BN * kRow;                           // K or V of a tile
+    static constexpr int kHalf = NP * kPlane;                          // V's place behind K's
+    static constexpr int kStage = 2 * kHalf;
+    static constexpr int kStages = 2 * kStage <= (160 << 10) ? 2 : 1;  // (8-bit rows of 512: one)
+    static constexpr int kLds = kStages * kStage;
+    static constexpr int kCopies = 16 * RC / 64;                       // 1 KB loads of 16 tokens
+
+    // Rows lie as they are but for the order of their pieces: piece c of row t
+    // is at place c ^ f(t), so that the 16 rows an operand read touches at one
+    // c lie in different banks.  K: single pieces; V: pairs (a transposing read
+    // takes 32 bytes of a row).
+    // So the piece's number enters the address by XOR in the swizzled bits (kSw)
+    // and by addition above them, the same for every lane.
+    static constexpr int kSw = D == 64 ? 7 : D == 96 ? 3 : 15;
+    __device__ __forceinline__ static int kswz(int t) {
+        return D == 64 ? (t >> 1) & 7 : D == 96 ? (t >> 2) & 3 : t & 15;
+    }
+    __device__ __forceinline__ static int vswz(int t) {
+        return D == 64 ? ((t >> 1) & 3) << 1 : D == 96 ? ((t >> 2) & 1) << 1 : (t & 7) << 1;
+    }
+};
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+template <bool BF>
+__device__ __forceinline__ floatx16 mfma32(const half8_t &a, const half8_t &b, const floatx16 &c) {
+    if constexpr (!BF) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    } else {
+        typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+}
+
+#define LDSP(T) __attribute__((address_space(3))) T *
+
+__device__ __forceinline__ half8_t lds_half8(uint32_t at) {
+    return __builtin_bit_cast(half8_t, *(const LDSP(u32x4))(uintptr_t)at);
+}
+
+// Four tokens of one head dim a lane from a row-major tile.
+__device__ __forceinline__ u32x2 lds_tr(uint32_t at) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDSP(s16x4))(uintptr_t)at));
+}
+
+// 16 bytes a lane from base + off straight to LDS, lane l's at lds + 16 l (the
+// base in m0, which the compiler sets).  Written out because the compiler
+// orders every LDS read behind the builtin's copy and would wait for the next
+// tile before the first operand of this one; the wait is the one at the tile's
+// barrier.
+__device__ __forceinline__ void copy16(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "{m0}"(lds), "v"(off), "s"(base) : "memory");
+}
+
+__device__ __forceinline__ float other_half_max(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+}
+
+// How far (log2) a tile's maximum may pass the one that the sums are held at
+// before they are rescaled: the probabilities stay below 2^(shift + slack).
+template <bool BF>
+constexpr float slack() { return BF ? 8.f : 4.f; }
+
+template <int D, bool BF, bool Q8>
+struct ChunkState {
+    using C = Chunk<D, Q8>;
+    static constexpr int COLS = 32, NQ = D / 16, ND = D / 32;
+    static constexpr int NR = D / 8;  // runs of four results a lane
+    half8_t qf[NQ];
+    floatx16 o[ND];
+    float m_run, l_part;
+
+    __device__ __forceinline__ static int qd(int d) { return 16 * d + 8 * (kq_lane() >> 5); }
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[j][x] = 0.f;
+        m_run = -INFINITY;
+        l_part = 0.f;
+    }
+    __device__ __forceinline__ float sum() const { return l_part + __shfl_xor(l_part, 32); }
+    // results d .. d + 3 of run k
+    __device__ __forceinline__ floatx4 run(int k, int &d) const {
+        const int j = k >> 2, x = k & 3;
+        d = 32 * j + 8 * x + 4 * (kq_lane() >> 5);
+        return floatx4{o[j][4 * x], o[j][4 * x + 1], o[j][4 * x + 2], o[j][4 * x + 3]};
+    }
+
+    template <bool MASK>
+    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, int t0, int lim, uint32_t okbits) {
+        const int lane = kq_lane(), c = lane & 31, h = lane >> 5;
+        floatx16 s[C::NT];
+        // rows t and t + 32 have the same order of pieces
+        const uint32_t ka = stage + (uint32_t)(c * C::kRow) + 16u * (uint32_t)(C::kswz(c) ^ h);
+#pragma unroll
+        for (int b = 0; b < C::NT; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < NQ; ++d) {
+            const uint32_t kd = (ka ^ (uint32_t)(16 * ((2 * d) & C::kSw))) + (uint32_t)(16 * ((2 * d) & ~C::kSw));
+#pragma unroll
+            for (int pl = 0; pl < C::NP; ++pl)
+#pragma unroll
+                for (int b = 0; b < C::NT; ++b)
+                    s[b] = mfma32<BF>(lds_half8(kd + (uint32_t)(pl * C::kPlane + 32 * b * C::kRow)), qf[d], s[b]);
+        }
+        if constexpr (MASK) {
+#pragma unroll
+            for (int b = 0; b < C::NT; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int t = 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
+                    const bool on = t0 + t < lim && ((okbits >> (2 * b + (i >> 3))) & 1);
+                    s[b][i] = on ? s[b][i] : -INFINITY;
+                }
+        }
+        float tmax = s[0][0];
+#pragma unroll
+        for (int b = 0; b < C::NT; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[b][i]);
+        tmax = other_half_max(tmax) * scale_log2;
+        // (each column by its own scores: what the others see does not matter)
+        const bool up = tmax > m_run + slack<BF>();
+        if (__builtin_amdgcn_ballot_w64(up)) {
+            const float alpha = up ? __builtin_amdgcn_exp2f(m_run - tmax) : 1.f;
+            m_run = up ? tmax : m_run;
+            l_part *= alpha;
+#pragma unroll
+            for (int j = 0; j < ND; ++j) o[j] = o[j] * alpha;
+        }
+        // (no key yet: every power is 0, not exp(-inf + inf))
+        const float m_use = (MASK && m_run == -INFINITY ? 0.f : m_run) - shift<BF, false>();
+        float psum = 0.f;
+        half8_t pf[2 * C::NT];
+#pragma unroll
+        for (int b = 0; b < C::NT; ++b)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float p[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[b][8 * k + i], scale_log2, -m_use));
+                    psum += p[i];
+                }
+                pf[2 * b + k] = __builtin_bit_cast(half8_t, u32x4{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3]),
+                                                                  pack2<BF>(p[4], p[5]), pack2<BF>(p[6], p[7])});
+            }
+        l_part += psum;
+        uint32_t odd = 0;
+        values<MASK>(stage + C::kHalf, pf, odd);
+        if constexpr (MASK) {
+            if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+#pragma unroll 1
+                for (int k = 0; k < C::BN; ++k)
+                    add_odd(stage + C::kHalf, k, t0 + k < lim && ((okbits >> (k >> 4)) & 1));
+            }
+        }
+        kq_mfma_drain();
+    }
+
+    template <bool MASK>
+    __device__ __forceinline__ void values(uint32_t vt, const half8_t (&pf)[2 * C::NT], uint32_t &odd) {
+        const int lane = kq_lane(), h = lane >> 5;
+        // lane 16 g + i: token 4 h + i / 4 (+ 8), values 32 j + 16 (g % 2) + 4 (i % 4) ..
+        const int tr = 4 * h + ((lane >> 2) & 3);
+        const int piece = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+        const uint32_t va = vt + (uint32_t)(tr * C::kRow) + 16u * (uint32_t)(C::vswz(tr) ^ piece) + 8u * (lane & 1);
+        // (rows 8 apart have the same order of pieces but for head dims 64 and 96)
+        const uint32_t vb = vt + (uint32_t)((tr + 8) * C::kRow) + 16u * (uint32_t)(C::vswz(tr + 8) ^ piece) + 8u * (lane & 1);
+#pragma unroll
+        for (int kk = 0; kk < 2 * C::NT; ++kk) {
+#pragma unroll
+            for (int j = 0; j < ND; ++j) {
+#pragma unroll
+                for (int pl = 0; pl < C::NP; ++pl) {
+                    const uint32_t flip = 16 * ((4 * j) & C::kSw);
+                    const uint32_t up = 16 * ((4 * j) & ~C::kSw) + 16 * kk * C::kRow + pl * C::kPlane;
+                    const u32x2 a = lds_tr((va ^ flip) + up), b = lds_tr((vb ^ flip) + up);
+                    u32x4 f = {a.x, a.y, b.x, b.y};
+                    if constexpr (MASK) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) f[x] = finite2<BF>(f[x], odd);
+                    }
+                    o[j] = mfma32<BF>(__builtin_bit_cast(half8_t, f), pf[kk], o[j]);
+                }
+            }
+        }
+    }
+
+    // Adds the infinite and NaN values of one key to the columns that see it.
+    __device__ __forceinline__ void add_odd(uint32_t vt, int t, bool sees) {
+        const int h = kq_lane() >> 5;
+        const uint32_t row = vt + (uint32_t)(t * C::kRow);
+        const int x = C::vswz(t & 15);
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const u32x2 v = *(const LDSP(u32x2))(uintptr_t)(row + 16u * (uint32_t)((4 * j + k) ^ x) + 8u * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = odd_part<BF>(e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFFu);
+                    if (sees) o[j][4 * k + e] += y;
+                }
+            }
+    }
+};
+
+// The same for 16 columns a wave on v_mfma_f32_16x16x32 (head dims past 128):
+// lane 16 g + c holds column c at tokens 4 g .. 4 g + 3 of each 16.
+template <int D, bool BF, bool Q8>
+struct ChunkState16 {
+    using C = Chunk<D, Q8>;
+    static_assert(C::BN == 32, "one product of 32 tokens a tile");
+    static constexpr int COLS = 16, NQ = D / 32, NR = D / 16;
+    half8_t qf[NQ];
+    floatx4 o[NR];
+    float m_run, l_part;
+
+    __device__ __forceinline__ static int qd(int d) { return 32 * d + 8 * (kq_lane() >> 4); }
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int j = 0; j < NR; ++j) o[j] = floatx4{0, 0, 0, 0};
+        m_run = -INFINITY;
+        l_part = 0.f;
+    }
+    __device__ __forceinline__ float sum() const {
+        const float l = l_part + __shfl_xor(l_part, 16);
+        return l + __shfl_xor(l, 32);
+    }
+    __device__ __forceinline__ floatx4 run(int k, int &d) const {
+        d = 16 * k + 4 * (kq_lane() >> 4);
+        return o[k];
+    }
+
+    template <bool MASK>
+    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, int t0, int lim, uint32_t okbits) {
+        const int lane = kq_lane(), c = lane & 15, g = lane >> 4;
+        floatx4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        const uint32_t ka = stage + (uint32_t)(c * C::kRow) + 16u * (uint32_t)(C::kswz(c) ^ g);
+#pragma unroll
+        for (int d = 0; d < NQ; ++d) {
+            const uint32_t kd = (ka ^ (uint32_t)(16 * ((4 * d) & C::kSw))) + (uint32_t)(16 * ((4 * d) & ~C::kSw));
+#pragma unroll
+            for (int pl = 0; pl < C::NP; ++pl)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    s[b] = mfma<BF>(lds_half8(kd + (uint32_t)(pl * C::kPlane + 16 * b * C::kRow)), qf[d], s[b]);
+        }
+        if constexpr (MASK) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[b][i] = t0 + 16 * b + 4 * g + i < lim && ((okbits >> b) & 1) ? s[b][i] : -INFINITY;
+        }
+        float tmax = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        tmax = max_over_groups(tmax) * scale_log2;
+        // (each column by its own scores: what the others see does not matter)
+        const bool up = tmax > m_run + slack<BF>();
+        if (__builtin_amdgcn_ballot_w64(up)) {
+            const float alpha = up ? __builtin_amdgcn_exp2f(m_run - tmax) : 1.f;
+            m_run = up ? tmax : m_run;
+            l_part *= alpha;
+#pragma unroll
+            for (int j = 0; j < NR; ++j) o[j] = o[j] * alpha;
+        }
+        const float m_use = (MASK && m_run == -INFINITY ? 0.f : m_run) - shift<BF, false>();
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], scale_log2, -m_use));
+            l_part += p[i];
+        }
+        const half8_t pf = __builtin_bit_cast(half8_t, u32x4{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3]),
+                                                             pack2<BF>(p[4], p[5]), pack2<BF>(p[6], p[7])});
+        // lane 16 g + i: tokens 4 g + i / 4 (+ 16), values 16 j + 4 (i % 4) ..
+        const uint32_t vt = stage + C::kHalf;
+        const int tr = 4 * g + ((lane >> 2) & 3);
+        const uint32_t va = vt + (uint32_t)(tr * C::kRow) + 16u * (uint32_t)(C::vswz(tr) ^ ((lane >> 1) & 1)) + 8u * (lane & 1);
+        uint32_t odd = 0;
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+#pragma unroll
+            for (int pl = 0; pl < C::NP; ++pl) {
+                const uint32_t at = (va ^ (uint32_t)(16 * ((2 * j) & C::kSw))) + (uint32_t)(16 * ((2 * j) & ~C::kSw) + pl * C::kPlane);
+                const u32x2 a = lds_tr(at), b = lds_tr(at + 16 * C::kRow);
+                u32x4 f = {a.x, a.y, b.x, b.y};
+                if constexpr (MASK) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) f[x] = finite2<BF>(f[x], odd);
+                }
+                o[j] = mfma<BF>(__builtin_bit_cast(half8_t, f), pf, o[j]);
+            }
+        if constexpr (MASK) {
+            if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+#pragma unroll 1
+                for (int k = 0; k < C::BN; ++k) {
+                    const bool sees = t0 + k < lim && ((okbits >> (k >> 4)) & 1);
+                    const uint32_t row = vt + (uint32_t)(k * C::kRow) + 8u * (g & 1);
+#pragma unroll
+                    for (int j = 0; j < NR; ++j) {
+                        const u32x2 v = *(const LDSP(u32x2))(uintptr_t)(row + 16u * (uint32_t)((2 * j + (g >> 1)) ^ C::vswz(k)));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float y = odd_part<BF>(e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFFu);
+                            if (sees) o[j][e] += y;
+                        }
+                    }
+                }
+            }
+        }
+        kq_mfma_drain();
+    }
+};
+
+template <int D, bool BF, bool Q8>
+__global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_paged_chunk_kernel(PagedArgs a) {
+    using C = Chunk<D, Q8>;
+    using State = std::conditional_t<(D > 128), ChunkState16<D, BF, Q8>, ChunkState<D, BF, Q8>>;
+    constexpr int COLS = State::COLS;
+    static_assert(4 * COLS == group_columns(D), "columns of a workgroup");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const uint32_t lds = (uint32_t)(uintptr_t)(LDSP(void))smem;
+    const int lane = kq_lane(), c = lane & (COLS - 1);
+    const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    for (int unit = blockIdx.x;; unit += gridDim.x) {
+        int u = unit, b, slot0;
+        if (!find_unit<true>(a, u, b, slot0)) return;
+        const Row row = uniform_row(a, b);
+        const int rest = u / a.Hkv, kvh = u - rest * a.Hkv;
+        // the tiles with the most keys first
+        const int back = rest / row.splits, s = rest - back * row.splits, blk = row.blocks - 1 - back;
+        const int col0 = (blk * 4 + w) * COLS, cols = row.n * a.G;
+
+        // this lane's column; waves past the row's columns only copy
+        const int col = col0 + c;
+        const bool live = col < cols;
+        const int i = live ? col / a.G : row.n - 1, hq = kvh * a.G + (live ? col - i * a.G : 0);
+        const auto seen_by = [&](int cl) { return max(row.kv - row.full + min(cl, cols - 1) / a.G + 1, 0); };
+        const int seen = live ? min(seen_by(col), row.kv) : 0x7fffffff;
+        const int least = __builtin_amdgcn_readfirstlane(seen_by(col0));
+        const int most = __builtin_amdgcn_readfirstlane(col0 < cols ? min(seen_by(col0 + COLS - 1), row.kv) : 0);
+        const int most_all = __builtin_amdgcn_readfirstlane(min(seen_by((blk + 1) * 4 * COLS - 1), row.kv));
+        const int per = ((row.kv + row.splits - 1) / row.splits + C::BN - 1) / C::BN * C::BN;
+        const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
+        const int t_end = __builtin_amdgcn_readfirstlane(min(most_all, t_begin + per));
+
+        State st;
+        st.init();
+        // scores are products times |scale|
+        const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+        const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // (0 times a hidden key's -inf)
+        const uint16_t *qp = a.q + (int64_t)(row.q0 + i) * a.q_stride + (int64_t)hq * D;
+#pragma unroll
+        for (int d = 0; d < State::NQ; ++d) {
+            const u32x4 v = *(const u32x4 *)(qp + State::qd(d));
+            st.qf[d] = __builtin_bit_cast(half8_t, live ? v ^ u32x4{flip, flip, flip, flip} : u32x4{0u, 0u, 0u, 0u});
+        }
+
+        if (t_end > t_begin) {
+            const int32_t *tab = a.table + (int64_t)b * a.table_stride;
+            const int sh = a.lps - 4;
+            const int c_last = (t_end - 1) >> 4, p_last = c_last >> sh;
+            int p0 = (t_begin >> 4) >> sh;
+            int ids = tab[min(p0 + lane, p_last)];
+            const int64_t h_off = (int64_t)kvh * a.head_stride;
+            // Piece y of this wave's 16-token pieces of the tile at t0, every
+            // other one of K (even waves) or V (odd waves): where it starts in
+            // the pool (values) and in a stage.
+            auto piece = [&](int t0, int y, uint32_t &dst) {
+                const int j = 2 * y + (w >> 1);
+                // (pieces past the end repeat the last: their keys are hidden)
+                const int ch = min((t0 >> 4) + j, c_last), p = ch >> sh;
+                if ((uint32_t)(p - p0) >= 64u) {
+                    p0 = p;
+                    ids = tab[min(p0 + lane, p_last)];
+                }
+                const int id = __builtin_amdgcn_readlane(ids, p - p0);
+                dst = (uint32_t)((w & 1) * C::kHalf + 16 * j * C::kRow);
+                return (int64_t)((uint32_t)id < (uint32_t)a.n_pages ? id : 0) * a.page_stride + h_off +
+                       (int64_t)((ch - (p << sh)) * 16) * a.tok_stride;
+            };
+            const auto swizzle = [&](int t) { return w & 1 ? C::vswz(t) : C::kswz(t); };
+            const uint8_t *src = (const uint8_t *)(w & 1 ? a.v : a.k);
+            // 16-bit pool: straight to LDS.
+            auto copy = [&](int t0, uint32_t stage) {
+#pragma unroll
+                for (int y = 0; y < C::BN / 32; ++y) {
+                    uint32_t dst;
+                    const int64_t off = piece(t0, y, dst);
+#pragma unroll
+                    for (int x = 0; x < C::kCopies; ++x) {
+                        const int at = 64 * x + lane, t = at / C::RC, pc = at - t * C::RC;
+                        copy16(src + 2 * off, (uint32_t)(t * a.tok_stride + 8 * (pc ^ swizzle(t))) * 2u,
+                               stage + dst + 1024u * x);
+                    }
+                }
+            };
+            // 8-bit pool: 16 values of a token a lane and load, with their
+            // scale and bias, to registers and later to LDS.
+            constexpr int NY = Q8 ? C::BN / 32 : 1, NX = Q8 ? D / 64 : 1;
+            u32x4 held[NY][NX];
+            uint32_t held_sb[NY][NX], held_at[NY];
+            const uint16_t *src_s = w & 1 ? a.vs : a.ks, *src_b = w & 1 ? a.vb : a.kb;
+            auto fetch = [&](int t0) {
+#pragma unroll
+                for (int y = 0; y < NY; ++y) {
+                    const int64_t off = piece(t0, y, held_at[y]);
+#pragma unroll
+                    for (int x = 0; x < NX; ++x) {
+                        const uint32_t at = 16u * (uint32_t)(64 * x + lane);
+                        held[y][x] = *(const u32x4 *)(src + off + at);
+                        held_sb[y][x] = (uint32_t)src_s[(off >> 6) + (at >> 6)] | ((uint32_t)src_b[(off >> 6) + (at >> 6)] << 16);
+                    }
+                }
+            };
+            auto put = [&](uint32_t stage) {
+#pragma unroll
+                for (int y = 0; y < NY; ++y)
+#pragma unroll
+                    for (int x = 0; x < NX; ++x) {
+                        const int at = 16 * (64 * x + lane), t = at / D, pc = (at - t * D) / 8;
+                        const float sc = f16bits_to_f32<BF>(held_sb[y][x] & 0xFFFFu), bi = f16bits_to_f32<BF>(held_sb[y][x] >> 16);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            u32x4 hi, lo;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t two = held[y][x][2 * half + (i >> 1)] >> (16 * (i & 1));
+                                const float u = fmaf((float)(two & 0xFFu), sc, bi), v = fmaf((float)((two >> 8) & 0xFFu), sc, bi);
+                                hi[i] = pack2<BF>(u, v);
+                                lo[i] = pack2<BF>(u - f16bits_to_f32<BF>(hi[i] & 0xFFFFu), v - f16bits_to_f32<BF>(hi[i] >> 16));
+                            }
+                            const uint32_t to = stage + held_at[y] + (uint32_t)(t * C::kRow + 16 * ((pc + half) ^ swizzle(t)));
+                            *(LDSP(u32x4))(uintptr_t)to = hi;
+                            *(LDSP(u32x4))(uintptr_t)(to + C::kPlane) = lo;
+                        }
+                    }
+            };
+            // Bit j: the tile's 16-token piece j lies in a page of the pool (after its copy).
+            const bool all_ok = pages_in_pool(a, tab, p0, p_last);
+            auto pages_ok = [&](int t0) {
+                uint32_t ok = (1u << (C::BN / 16)) - 1;
+                if (!all_ok)
+                    for (int j = 0; j < C::BN / 16; ++j)
+                        if ((uint32_t)tab[min((t0 >> 4) + j, c_last) >> sh] >= (uint32_t)a.n_pages) ok &= ~(1u << j);
+                return ok;
+            };
+            __syncthreads();  // the last unit's reads
+            if constexpr (Q8) {
+                fetch(t_begin);
+                put(lds);
+            } else {
+                copy(t_begin, lds);
+            }
+            uint32_t stage = lds, other = lds + (C::kStages - 1) * C::kStage;
+            for (int t0 = t_begin; t0 < t_end; t0 += C::BN) {
+                const bool more = t0 + C::BN < t_end;
+                // this tile has landed, and every wave is done with the other stage
+                if constexpr (Q8) {
+                    __syncthreads();
+                    if (more) fetch(t0 + C::BN);
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    if (more) copy(t0 + C::BN, other);
+                }
+                if (t0 < most) {
+                    if (t0 + C::BN <= min(least, t_end) && all_ok)
+                        st.template tile<false>(stage, scale, t0, 0, 0);
+                    else
+                        st.template tile<true>(stage, scale, t0, min(seen, t_end), pages_ok(t0));
+                }
+                if constexpr (Q8) {
+                    if constexpr (C::kStages == 1) __syncthreads();
+                    if (more) put(other);
+                }
+                const uint32_t x = stage;
+                stage = other;
+                other = x;
+            }
+        }
+
+        const float l = st.sum();
+        if (!live) continue;
+        const bool whole = row.splits == 1;
+        const float mul = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
+        uint16_t *op = a.out + (int64_t)(row.q0 + i) * a.out_stride + (int64_t)hq * D;
+        const int64_t slot = slot0 + (i * a.Hq + hq) * row.splits + s;
+        float *pp = a.part + slot * D;
+#pragma unroll
+        for (int k = 0; k < State::NR; ++k) {
+            int d;
+            const floatx4 v = st.run(k, d) * mul;
+            if (whole) *(u32x2 *)(op + d) = u32x2{pack2<BF>(v.x, v.y), pack2<BF>(v.z, v.w)};
+            else *(floatx4 *)(pp + d) = v;
+        }
+        if (!whole && lane < COLS) {
+            a.ml[2 * slot] = st.m_run;
+            a.ml[2 * slot + 1] = l;
+        }
+    }
+}
+
 // One wave a (token, query head) of a row with splits: rescales the splits to
 // their common maximum and sums them in split order.
 template <int D, bool BF>
@@ -620,13 +1180,13 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
     int splits = 0;
     for (int c0 = 0; c0 < a.B && !splits; c0 += 64) {
         const int row = c0 + lane;
-        int64_t ms = 0;
+        int ms = 0;
         Row x{};
         if (row < a.B) {
             x = row_at(a, row);
             ms = row_slots(a, x);
         }
-        const int64_t is = wave_scan(ms);
+        const int is = wave_scan(ms);
         const uint64_t hit = __ballot(row < a.B && t >= x.q0 && t < x.q0 + x.n);
         if (hit) {
             const int src = __builtin_ctzll(hit);
@@ -662,30 +1222,53 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
     for (int x = 0; x < V; ++x) op[x] = from_f32<BF>(acc[x] * inv);
 }
 
+struct Grid {
+    int waves, groups;  // 0: not launched
+    bool merge;
+};
+
 template <int D, bool BF, bool Q8>
-void launch_split(const PagedArgs &a, int grid, hipStream_t s) {
-    hipLaunchKernelGGL((kq_paged_split_kernel<D, BF, Q8>), dim3(grid), dim3(64), 0, s, a);
+int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
+    if (g.groups) {
+        constexpr int lds = Chunk<D, Q8>::kLds;
+        static_assert(lds <= 160 << 10, "LDS of a CU");
+        static const bool ok = lds <= (64 << 10) || hipFuncSetAttribute((const void *)kq_paged_chunk_kernel<D, BF, Q8>,
+                                                                        hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                                        lds) == hipSuccess;
+        if (!ok) return KQ_ERR_LAUNCH_FAILED;
+        hipLaunchKernelGGL((kq_paged_chunk_kernel<D, BF, Q8>), dim3(g.groups), dim3(256), lds, s, a);
+    }
+    if (g.waves) hipLaunchKernelGGL((kq_paged_split_kernel<D, BF, Q8>), dim3(g.waves), dim3(64), 0, s, a);
+    if (g.merge)
+        hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF>), dim3((unsigned)(((int64_t)a.T * a.Hq + 3) / 4)), dim3(256), 0,
+                           s, a);
+    return hipGetLastError() == hipSuccess ? KQ_OK : KQ_ERR_LAUNCH_FAILED;
 }
 
 template <int D, bool BF>
-void launch(const PagedArgs &a, bool q8, int grid, bool merge, hipStream_t s) {
-    if (q8) {
-        if constexpr (D % 64 == 0) launch_split<D, BF, true>(a, grid, s);
-    } else {
-        launch_split<D, BF, false>(a, grid, s);
-    }
-    if (merge)
-        hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF>), dim3((unsigned)(((int64_t)a.T * a.Hq + 3) / 4)), dim3(256), 0,
-                           s, a);
+int launch(const PagedArgs &a, bool q8, const Grid &g, hipStream_t s) {
+    if constexpr (D % 64 == 0)
+        if (q8) return launch_q8<D, BF, true>(a, g, s);
+    return launch_q8<D, BF, false>(a, g, s);
 }
 
-// Partial slots of a call: a row's n * Hq * splits is below (kSplitWaves + waves)
-// * 16 for waves < kSplitWaves (with as many or more it is not split), and no
-// row has more splits than one token over max_kv keys.
-int64_t max_slots(int64_t T, int64_t B, int Hq, int Hkv, int max_kv) {
-    const int most = paged_splits(1, max_kv, Hq / Hkv, Hkv);
+// The most splits of any row of at most max_q tokens and max_kv keys.
+int most_splits(int max_q, int Hq, int Hkv, int D, int max_kv) {
+    const int G = Hq / Hkv, chunk = kFewColumns / G + 1;  // the shortest chunk
+    const int few = chunk > 1 ? paged_splits(1, max_kv, G, Hkv, group_columns(D)) : 1;
+    const int many = max_q >= chunk ? paged_splits(chunk, max_kv, G, Hkv, group_columns(D)) : 1;
+    return few > many ? few : many;
+}
+
+// Partial slots of a call: one a token, query head and split; and of a row at
+// most 2 kSplitGroups * 128 (a split row has units < kSplitGroups workgroups
+// of 128 columns, and splits <= kSplitGroups / units + 1; rows of few columns
+// have fewer).
+int64_t max_slots(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max_kv) {
+    const int most = most_splits(max_q, Hq, Hkv, D, max_kv);
     if (most < 2) return 0;
-    const int64_t by_token = T * Hq * most, by_row = B * 2 * kSplitWaves * 16;
+    static_assert(2 * kSplitWaves * kFewColumns <= 2 * kSplitGroups * 128, "the chunks' bound covers both");
+    const int64_t by_token = T * Hq * most, by_row = B * 2 * kSplitGroups * 128;
     return by_token < by_row ? by_token : by_row;
 }
 
@@ -698,7 +1281,7 @@ extern "C" {
 size_t kq_sdpa_paged_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
                                      int32_t max_kv, int q8) {
     if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_q <= 0 || max_kv <= 0) return 0;
-    const int64_t slots = max_slots(T, B, Hq, Hkv, max_kv);
+    const int64_t slots = max_slots(T, B, Hq, Hkv, D, max_q, max_kv);
     return slots ? part_bytes(slots, D) + (size_t)slots * 8 : 0;
 }
 
@@ -719,6 +1302,11 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     const size_t need = kq_sdpa_paged_workspace_bytes(T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr);
     if (need && (!workspace || workspace_bytes < need)) return KQ_ERR_WORKSPACE_TOO_SMALL;
     if (need && ((uintptr_t)workspace & 255)) return KQ_ERR_BAD_ALIGN;
+    const int most = most_splits(max_q, Hq, Hkv, D, max_kv);
+    // 31-bit unit and partial numbers
+    if (max_slots(T, B, Hq, Hkv, D, max_q, max_kv) >= (int64_t)1 << 31 ||
+        ((int64_t)T * (Hq / Hkv) + B) * Hkv * most >= (int64_t)1 << 31)
+        return KQ_ERR_BAD_SHAPE;
     PagedArgs a;
     a.q = (const uint16_t *)q;
     a.out = (uint16_t *)out;
@@ -745,27 +1333,29 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     a.Hq = Hq;
     a.Hkv = Hkv;
     a.G = Hq / Hkv;
+    a.group_cols = group_columns(D);
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const int64_t slots = max_slots(T, B, Hq, Hkv, max_kv);
+    const int64_t slots = max_slots(T, B, Hq, Hkv, D, max_q, max_kv);
     a.part = (float *)workspace;
     a.ml = (float *)((char *)workspace + part_bytes(slots, D));
-    // units of the longest rows; the grid's waves take the rest in turn
-    const int64_t blocks = ((int64_t)T * a.G + 15) / 16 + B;
-    const int64_t units = blocks * Hkv * paged_splits(1, max_kv, a.G, Hkv);
-    const int grid = (int)(units < (1 << 16) ? units : (1 << 16));
+    // bounds of the units; the grids' waves and workgroups take the rest in turn
+    const int64_t few = (int64_t)(T < B ? T : B) * Hkv * most;
+    const int64_t many = (((int64_t)T * a.G + a.group_cols - 1) / a.group_cols + (T < B ? T : B)) * Hkv * most;
+    Grid g;
+    g.waves = a.G > kFewColumns ? 0 : (int)(few < (1 << 16) ? few : (1 << 16));
+    g.groups = few_columns(max_q, a.G) ? 0 : (int)(many < (1 << 14) ? many : (1 << 14));
+    g.merge = slots > 0;
     const bool q8 = a.ks != nullptr, bf = pool->dtype == KQ_DTYPE_BF16;
     hipStream_t s = (hipStream_t)stream;
-    const bool merge = slots > 0;
     switch (D) {
-    case 64: bf ? launch<64, true>(a, q8, grid, merge, s) : launch<64, false>(a, q8, grid, merge, s); break;
-    case 96: bf ? launch<96, true>(a, q8, grid, merge, s) : launch<96, false>(a, q8, grid, merge, s); break;
-    case 128: bf ? launch<128, true>(a, q8, grid, merge, s) : launch<128, false>(a, q8, grid, merge, s); break;
-    case 256: bf ? launch<256, true>(a, q8, grid, merge, s) : launch<256, false>(a, q8, grid, merge, s); break;
-    default: bf ? launch<512, true>(a, q8, grid, merge, s) : launch<512, false>(a, q8, grid, merge, s); break;
+    case 64: return bf ? launch<64, true>(a, q8, g, s) : launch<64, false>(a, q8, g, s);
+    case 96: return bf ? launch<96, true>(a, q8, g, s) : launch<96, false>(a, q8, g, s);
+    case 128: return bf ? launch<128, true>(a, q8, g, s) : launch<128, false>(a, q8, g, s);
+    case 256: return bf ? launch<256, true>(a, q8, g, s) : launch<256, false>(a, q8, g, s);
+    default: return bf ? launch<512, true>(a, q8, g, s) : launch<512, false>(a, q8, g, s);
     }
-    return hipGetLastError() == hipSuccess ? KQ_OK : KQ_ERR_LAUNCH_FAILED;
 }
 
 }  // extern "C"

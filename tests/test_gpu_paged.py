@@ -433,7 +433,11 @@ def test_bounds_cut_longer_rows():
     out = torch.full((8, 8, 128), 7.0, dtype=F16, device="cuda")
     b.run(out=out, max_q=4)
     full = b.run()
-    assert torch.equal(out[:4], full[:4]) and (out[4:6] == 7.0).all() and torch.equal(out[6:], full[6:])
+    assert (out[4:6] == 7.0).all() and torch.equal(out[6:], full[6:])
+    # (four tokens may take another kernel than six: the same sums in another order)
+    cut = full.clone()
+    cut[:4] = out[:4]
+    b.check(cut)
     b.run(out=out, max_kv=64)
     assert torch.equal(out[6:], full[6:])
     assert torch.isfinite(out).all()
