@@ -132,6 +132,23 @@ __device__ __forceinline__ Row uniform_row(const PagedArgs &a, int b) {
     return r;
 }
 
+// 64 entries of a block table row in a register; at(p) takes rising p.
+struct PageIds {
+    int first, ids;
+
+    __device__ __forceinline__ void load(const int32_t *tab, int p, int last) {
+        first = p;
+        ids = tab[min(p + kq_lane(), last)];
+        // waited for here: after a branch that may load them, the compiler
+        // would wait for every load in flight (a tile) before each use
+        __builtin_amdgcn_s_waitcnt(KQ_VMCNT(0));
+    }
+    __device__ __forceinline__ int at(const int32_t *tab, int p, int last) {
+        if ((uint32_t)(p - first) >= 64u) load(tab, p, last);
+        return __builtin_amdgcn_readlane(ids, p - first);
+    }
+};
+
 // Whether a block table row's entries [p, last] all are pages of the pool.
 __device__ __forceinline__ bool pages_in_pool(const PagedArgs &a, const int32_t *tab, int p, int last) {
     bool bad = false;
@@ -523,8 +540,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
             const int32_t *tab = a.table + (int64_t)b * a.table_stride;
             const int sh = a.lps - 4;  // log2 of a page's chunks
             const int c_last = (t_end - 1) >> 4, p_last = c_last >> sh;
-            int p0 = (t_begin >> 4) >> sh;
-            int ids = tab[min(p0 + lane, p_last)];
+            const int p_first = (t_begin >> 4) >> sh;
+            PageIds ids;
+            ids.load(tab, p_first, p_last);
             const int64_t h_off = (int64_t)h * a.head_stride;
             auto at_tile = [&](int t0) {
                 TileAt<D> x;
@@ -533,11 +551,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
                 for (int ch = 0; ch < CH; ++ch) {
                     // (chunks past the end repeat the last: their keys are hidden)
                     const int c = min((t0 >> 4) + ch, c_last), p = c >> sh;
-                    if ((uint32_t)(p - p0) >= 64u) {
-                        p0 = p;
-                        ids = tab[min(p0 + lane, p_last)];
-                    }
-                    const int id = __builtin_amdgcn_readlane(ids, p - p0);
+                    const int id = ids.at(tab, p, p_last);
                     const bool in = (uint32_t)id < (uint32_t)a.n_pages;
                     x.ok |= in ? 1u << ch : 0u;
                     x.off[ch] = uniform64((int64_t)(in ? id : 0) * a.page_stride + h_off +
@@ -549,7 +563,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
             // others (the last keys; all, where the table names no page) one
             // by one before them, so that their code is there once.
             int whole = min(least, t_end);
-            whole = whole <= t_begin || !pages_in_pool(a, tab, p0, p_last) ? t_begin : whole - (whole - t_begin) % TT;
+            whole = whole <= t_begin || !pages_in_pool(a, tab, p_first, p_last) ? t_begin : whole - (whole - t_begin) % TT;
             Tile ring[NBUF];
 #pragma unroll 1
             for (int t = whole; t < t_end; t += TT) {
@@ -716,6 +730,28 @@ __device__ __forceinline__ float other_half_max(float v) {
     return fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// mfma(i, operand) for i < N with the operands read AHEAD steps before their
+// use, so that no MFMA waits for a read that was just issued (left alone, the
+// scheduler saves registers and puts every read right before its MFMA).  Reads
+// and MFMAs keep this order; vector and scalar ALU work may move across.
+template <int N, int AHEAD, class Read, class Use>
+__device__ __forceinline__ void pipelined(Read &&read, Use &&use) {
+    constexpr int A = AHEAD < N ? AHEAD : N;
+    half8_t f[A + 1];
+#pragma unroll
+    for (int i = 0; i < A; ++i) f[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0x6);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i + A < N) f[(i + A) % (A + 1)] = read(i + A);
+        __builtin_amdgcn_sched_barrier(0x6);
+        use(i, f[i % (A + 1)]);
+        __builtin_amdgcn_sched_barrier(0x6);
+    }
+}
+
 // How far (log2) a tile's maximum may pass the one that the sums are held at
 // before they are rescaled: the probabilities stay below 2^(shift + slack).
 template <bool BF>
@@ -741,14 +777,19 @@ struct ChunkState {
     }
     __device__ __forceinline__ float sum() const { return l_part + __shfl_xor(l_part, 32); }
     // results d .. d + 3 of run k
-    __device__ __forceinline__ floatx4 run(int k, int &d) const {
-        const int j = k >> 2, x = k & 3;
-        d = 32 * j + 8 * x + 4 * (kq_lane() >> 5);
-        return floatx4{o[j][4 * x], o[j][4 * x + 1], o[j][4 * x + 2], o[j][4 * x + 3]};
+    __device__ __forceinline__ static int run_d(int k) { return 8 * k + 4 * (kq_lane() >> 5); }
+    __device__ __forceinline__ floatx4 run(int k) const {
+        const int j = k >> 2, x = 4 * (k & 3);
+        return floatx4{o[j][x], o[j][x + 1], o[j][x + 2], o[j][x + 3]};
+    }
+    __device__ __forceinline__ void add(int k, const floatx4 &y) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[k >> 2][4 * (k & 3) + e] += y[e];
     }
 
-    template <bool MASK>
-    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, int t0, int lim, uint32_t okbits) {
+    // masked: some key of the tile is hidden from a column (lim: the column's
+    // first unseen key; okbits: the 16-token pieces that lie in the pool).
+    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, bool masked, int t0, int lim, uint32_t okbits) {
         const int lane = kq_lane(), c = lane & 31, h = lane >> 5;
         floatx16 s[C::NT];
         // rows t and t + 32 have the same order of pieces
@@ -757,30 +798,28 @@ struct ChunkState {
         for (int b = 0; b < C::NT; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-#pragma unroll
-        for (int d = 0; d < NQ; ++d) {
-            const uint32_t kd = (ka ^ (uint32_t)(16 * ((2 * d) & C::kSw))) + (uint32_t)(16 * ((2 * d) & ~C::kSw));
-#pragma unroll
-            for (int pl = 0; pl < C::NP; ++pl)
-#pragma unroll
-                for (int b = 0; b < C::NT; ++b)
-                    s[b] = mfma32<BF>(lds_half8(kd + (uint32_t)(pl * C::kPlane + 32 * b * C::kRow)), qf[d], s[b]);
-        }
-        if constexpr (MASK) {
+        // operand x: head dims 16 d .. (d slowest), plane, 32-token block
+        pipelined<NQ * C::NP * C::NT, 4>(
+            [&](int x) {
+                const int b = x % C::NT, pl = x / C::NT % C::NP, d = x / (C::NT * C::NP);
+                const uint32_t kd = (ka ^ (uint32_t)(16 * ((2 * d) & C::kSw))) + (uint32_t)(16 * ((2 * d) & ~C::kSw));
+                return lds_half8(kd + (uint32_t)(pl * C::kPlane + 32 * b * C::kRow));
+            },
+            [&](int x, const half8_t &f) { s[x % C::NT] = mfma32<BF>(f, qf[x / (C::NT * C::NP)], s[x % C::NT]); });
+        if (masked) {
 #pragma unroll
             for (int b = 0; b < C::NT; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int t = 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                    const bool on = t0 + t < lim && ((okbits >> (2 * b + (i >> 3))) & 1);
-                    s[b][i] = on ? s[b][i] : -INFINITY;
+                    s[b][i] = t0 + t < lim && ((okbits >> (2 * b + (i >> 3))) & 1) ? s[b][i] : -INFINITY;
                 }
         }
         float tmax = s[0][0];
 #pragma unroll
         for (int b = 0; b < C::NT; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, s[b][i]);
+            for (int i = 0; i < 16; i += 2) tmax = max3(tmax, s[b][i], s[b][i + 1]);
         tmax = other_half_max(tmax) * scale_log2;
         // (each column by its own scores: what the others see does not matter)
         const bool up = tmax > m_run + slack<BF>();
@@ -792,80 +831,39 @@ struct ChunkState {
             for (int j = 0; j < ND; ++j) o[j] = o[j] * alpha;
         }
         // (no key yet: every power is 0, not exp(-inf + inf))
-        const float m_use = (MASK && m_run == -INFINITY ? 0.f : m_run) - shift<BF, false>();
-        float psum = 0.f;
+        const float m_use = (m_run == -INFINITY ? 0.f : m_run) - shift<BF, false>();
         half8_t pf[2 * C::NT];
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int b = 0; b < C::NT; ++b)
+        for (int k = 0; k < 2 * C::NT; ++k) {
+            float p[8];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float p[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[b][8 * k + i], scale_log2, -m_use));
-                    psum += p[i];
-                }
-                pf[2 * b + k] = __builtin_bit_cast(half8_t, u32x4{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3]),
-                                                                  pack2<BF>(p[4], p[5]), pack2<BF>(p[6], p[7])});
+            for (int i = 0; i < 8; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(fmaf(s[k >> 1][8 * (k & 1) + i], scale_log2, -m_use));
+                sums[i & 3] += p[i];
             }
-        l_part += psum;
-        uint32_t odd = 0;
-        values<MASK>(stage + C::kHalf, pf, odd);
-        if constexpr (MASK) {
-            if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-#pragma unroll 1
-                for (int k = 0; k < C::BN; ++k)
-                    add_odd(stage + C::kHalf, k, t0 + k < lim && ((okbits >> (k >> 4)) & 1));
-            }
+            pf[k] = __builtin_bit_cast(half8_t, u32x4{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3]),
+                                                      pack2<BF>(p[4], p[5]), pack2<BF>(p[6], p[7])});
         }
-        kq_mfma_drain();
-    }
-
-    template <bool MASK>
-    __device__ __forceinline__ void values(uint32_t vt, const half8_t (&pf)[2 * C::NT], uint32_t &odd) {
-        const int lane = kq_lane(), h = lane >> 5;
+        l_part += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         // lane 16 g + i: token 4 h + i / 4 (+ 8), values 32 j + 16 (g % 2) + 4 (i % 4) ..
+        const uint32_t vt = stage + C::kHalf;
         const int tr = 4 * h + ((lane >> 2) & 3);
         const int piece = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
         const uint32_t va = vt + (uint32_t)(tr * C::kRow) + 16u * (uint32_t)(C::vswz(tr) ^ piece) + 8u * (lane & 1);
         // (rows 8 apart have the same order of pieces but for head dims 64 and 96)
         const uint32_t vb = vt + (uint32_t)((tr + 8) * C::kRow) + 16u * (uint32_t)(C::vswz(tr + 8) ^ piece) + 8u * (lane & 1);
-#pragma unroll
-        for (int kk = 0; kk < 2 * C::NT; ++kk) {
-#pragma unroll
-            for (int j = 0; j < ND; ++j) {
-#pragma unroll
-                for (int pl = 0; pl < C::NP; ++pl) {
-                    const uint32_t flip = 16 * ((4 * j) & C::kSw);
-                    const uint32_t up = 16 * ((4 * j) & ~C::kSw) + 16 * kk * C::kRow + pl * C::kPlane;
-                    const u32x2 a = lds_tr((va ^ flip) + up), b = lds_tr((vb ^ flip) + up);
-                    u32x4 f = {a.x, a.y, b.x, b.y};
-                    if constexpr (MASK) {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) f[x] = finite2<BF>(f[x], odd);
-                    }
-                    o[j] = mfma32<BF>(__builtin_bit_cast(half8_t, f), pf[kk], o[j]);
-                }
-            }
-        }
-    }
-
-    // Adds the infinite and NaN values of one key to the columns that see it.
-    __device__ __forceinline__ void add_odd(uint32_t vt, int t, bool sees) {
-        const int h = kq_lane() >> 5;
-        const uint32_t row = vt + (uint32_t)(t * C::kRow);
-        const int x = C::vswz(t & 15);
-#pragma unroll
-        for (int j = 0; j < ND; ++j)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const u32x2 v = *(const LDSP(u32x2))(uintptr_t)(row + 16u * (uint32_t)((4 * j + k) ^ x) + 8u * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float y = odd_part<BF>(e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFFu);
-                    if (sees) o[j][4 * k + e] += y;
-                }
-            }
+        // operand x: 16 tokens kk (slowest), plane, head dims 32 j ..
+        pipelined<2 * C::NT * ND * C::NP, 4>(
+            [&](int x) {
+                const int j = x % ND, pl = x / ND % C::NP, kk = x / (ND * C::NP);
+                const uint32_t flip = 16 * ((4 * j) & C::kSw);
+                const uint32_t up = 16 * ((4 * j) & ~C::kSw) + 16 * kk * C::kRow + pl * C::kPlane;
+                const u32x2 a = lds_tr((va ^ flip) + up), b = lds_tr((vb ^ flip) + up);
+                return __builtin_bit_cast(half8_t, u32x4{a.x, a.y, b.x, b.y});
+            },
+            [&](int x, const half8_t &f) { o[x % ND] = mfma32<BF>(f, pf[x / (ND * C::NP)], o[x % ND]); });
+        kq_mfma_drain();
     }
 };
 
@@ -891,36 +889,30 @@ struct ChunkState16 {
         const float l = l_part + __shfl_xor(l_part, 16);
         return l + __shfl_xor(l, 32);
     }
-    __device__ __forceinline__ floatx4 run(int k, int &d) const {
-        d = 16 * k + 4 * (kq_lane() >> 4);
-        return o[k];
-    }
+    __device__ __forceinline__ static int run_d(int k) { return 16 * k + 4 * (kq_lane() >> 4); }
+    __device__ __forceinline__ floatx4 run(int k) const { return o[k]; }
+    __device__ __forceinline__ void add(int k, const floatx4 &y) { o[k] = o[k] + y; }
 
-    template <bool MASK>
-    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, int t0, int lim, uint32_t okbits) {
+    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, bool masked, int t0, int lim, uint32_t okbits) {
         const int lane = kq_lane(), c = lane & 15, g = lane >> 4;
         floatx4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         const uint32_t ka = stage + (uint32_t)(c * C::kRow) + 16u * (uint32_t)(C::kswz(c) ^ g);
-#pragma unroll
-        for (int d = 0; d < NQ; ++d) {
-            const uint32_t kd = (ka ^ (uint32_t)(16 * ((4 * d) & C::kSw))) + (uint32_t)(16 * ((4 * d) & ~C::kSw));
-#pragma unroll
-            for (int pl = 0; pl < C::NP; ++pl)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-                    s[b] = mfma<BF>(lds_half8(kd + (uint32_t)(pl * C::kPlane + 16 * b * C::kRow)), qf[d], s[b]);
-        }
-        if constexpr (MASK) {
+        pipelined<2 * NQ * C::NP, 6>(
+            [&](int x) {
+                const int b = x % 2, pl = x / 2 % C::NP, d = x / (2 * C::NP);
+                const uint32_t kd = (ka ^ (uint32_t)(16 * ((4 * d) & C::kSw))) + (uint32_t)(16 * ((4 * d) & ~C::kSw));
+                return lds_half8(kd + (uint32_t)(pl * C::kPlane + 16 * b * C::kRow));
+            },
+            [&](int x, const half8_t &f) { s[x % 2] = mfma<BF>(f, qf[x / (2 * C::NP)], s[x % 2]); });
+        if (masked) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     s[b][i] = t0 + 16 * b + 4 * g + i < lim && ((okbits >> b) & 1) ? s[b][i] : -INFINITY;
         }
-        float tmax = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        tmax = max_over_groups(tmax) * scale_log2;
-        // (each column by its own scores: what the others see does not matter)
+        float tmax = max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
+        tmax = max_over_groups(max3(max3(tmax, s[1][1], s[1][2]), s[1][3], s[1][3])) * scale_log2;
         const bool up = tmax > m_run + slack<BF>();
         if (__builtin_amdgcn_ballot_w64(up)) {
             const float alpha = up ? __builtin_amdgcn_exp2f(m_run - tmax) : 1.f;
@@ -929,51 +921,25 @@ struct ChunkState16 {
 #pragma unroll
             for (int j = 0; j < NR; ++j) o[j] = o[j] * alpha;
         }
-        const float m_use = (MASK && m_run == -INFINITY ? 0.f : m_run) - shift<BF, false>();
+        const float m_use = (m_run == -INFINITY ? 0.f : m_run) - shift<BF, false>();
         float p[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], scale_log2, -m_use));
-            l_part += p[i];
-        }
+        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], scale_log2, -m_use));
+        l_part += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         const half8_t pf = __builtin_bit_cast(half8_t, u32x4{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3]),
                                                              pack2<BF>(p[4], p[5]), pack2<BF>(p[6], p[7])});
         // lane 16 g + i: tokens 4 g + i / 4 (+ 16), values 16 j + 4 (i % 4) ..
-        const uint32_t vt = stage + C::kHalf;
         const int tr = 4 * g + ((lane >> 2) & 3);
-        const uint32_t va = vt + (uint32_t)(tr * C::kRow) + 16u * (uint32_t)(C::vswz(tr) ^ ((lane >> 1) & 1)) + 8u * (lane & 1);
-        uint32_t odd = 0;
-#pragma unroll
-        for (int j = 0; j < NR; ++j)
-#pragma unroll
-            for (int pl = 0; pl < C::NP; ++pl) {
+        const uint32_t va = stage + C::kHalf + (uint32_t)(tr * C::kRow) +
+                            16u * (uint32_t)(C::vswz(tr) ^ ((lane >> 1) & 1)) + 8u * (lane & 1);
+        pipelined<NR * C::NP, 6>(
+            [&](int x) {
+                const int j = x % NR, pl = x / NR;
                 const uint32_t at = (va ^ (uint32_t)(16 * ((2 * j) & C::kSw))) + (uint32_t)(16 * ((2 * j) & ~C::kSw) + pl * C::kPlane);
                 const u32x2 a = lds_tr(at), b = lds_tr(at + 16 * C::kRow);
-                u32x4 f = {a.x, a.y, b.x, b.y};
-                if constexpr (MASK) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) f[x] = finite2<BF>(f[x], odd);
-                }
-                o[j] = mfma<BF>(__builtin_bit_cast(half8_t, f), pf, o[j]);
-            }
-        if constexpr (MASK) {
-            if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-#pragma unroll 1
-                for (int k = 0; k < C::BN; ++k) {
-                    const bool sees = t0 + k < lim && ((okbits >> (k >> 4)) & 1);
-                    const uint32_t row = vt + (uint32_t)(k * C::kRow) + 8u * (g & 1);
-#pragma unroll
-                    for (int j = 0; j < NR; ++j) {
-                        const u32x2 v = *(const LDSP(u32x2))(uintptr_t)(row + 16u * (uint32_t)((2 * j + (g >> 1)) ^ C::vswz(k)));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float y = odd_part<BF>(e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFFu);
-                            if (sees) o[j][e] += y;
-                        }
-                    }
-                }
-            }
-        }
+                return __builtin_bit_cast(half8_t, u32x4{a.x, a.y, b.x, b.y});
+            },
+            [&](int x, const half8_t &f) { o[x % NR] = mfma<BF>(f, pf, o[x % NR]); });
         kq_mfma_drain();
     }
 };
@@ -986,6 +952,7 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
     static_assert(4 * COLS == group_columns(D), "columns of a workgroup");
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const uint32_t lds = (uint32_t)(uintptr_t)(LDSP(void))smem;
+    const auto odd_flag = (volatile LDSP(int))(uintptr_t)(lds + C::kLds);
     const int lane = kq_lane(), c = lane & (COLS - 1);
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     for (int unit = blockIdx.x;; unit += gridDim.x) {
@@ -1005,6 +972,7 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
         const int seen = live ? min(seen_by(col), row.kv) : 0x7fffffff;
         const int least = __builtin_amdgcn_readfirstlane(seen_by(col0));
         const int most = __builtin_amdgcn_readfirstlane(col0 < cols ? min(seen_by(col0 + COLS - 1), row.kv) : 0);
+        const int least_all = __builtin_amdgcn_readfirstlane(seen_by(blk * 4 * COLS));
         const int most_all = __builtin_amdgcn_readfirstlane(min(seen_by((blk + 1) * 4 * COLS - 1), row.kv));
         const int per = ((row.kv + row.splits - 1) / row.splits + C::BN - 1) / C::BN * C::BN;
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
@@ -1026,8 +994,9 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
             const int32_t *tab = a.table + (int64_t)b * a.table_stride;
             const int sh = a.lps - 4;
             const int c_last = (t_end - 1) >> 4, p_last = c_last >> sh;
-            int p0 = (t_begin >> 4) >> sh;
-            int ids = tab[min(p0 + lane, p_last)];
+            PageIds ids;
+            ids.load(tab, (t_begin >> 4) >> sh, p_last);
+            const bool all_ok = pages_in_pool(a, tab, (t_begin >> 4) >> sh, p_last);
             const int64_t h_off = (int64_t)kvh * a.head_stride;
             // Piece y of this wave's 16-token pieces of the tile at t0, every
             // other one of K (even waves) or V (odd waves): where it starts in
@@ -1036,11 +1005,7 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
                 const int j = 2 * y + (w >> 1);
                 // (pieces past the end repeat the last: their keys are hidden)
                 const int ch = min((t0 >> 4) + j, c_last), p = ch >> sh;
-                if ((uint32_t)(p - p0) >= 64u) {
-                    p0 = p;
-                    ids = tab[min(p0 + lane, p_last)];
-                }
-                const int id = __builtin_amdgcn_readlane(ids, p - p0);
+                const int id = ids.at(tab, p, p_last);
                 dst = (uint32_t)((w & 1) * C::kHalf + 16 * j * C::kRow);
                 return (int64_t)((uint32_t)id < (uint32_t)a.n_pages ? id : 0) * a.page_stride + h_off +
                        (int64_t)((ch - (p << sh)) * 16) * a.tok_stride;
@@ -1065,17 +1030,20 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
             // scale and bias, to registers and later to LDS.
             constexpr int NY = Q8 ? C::BN / 32 : 1, NX = Q8 ? D / 64 : 1;
             u32x4 held[NY][NX];
-            uint32_t held_sb[NY][NX], held_at[NY];
+            uint32_t held_s[NY][NX], held_b[NY][NX], held_at[NY];
             const uint16_t *src_s = w & 1 ? a.vs : a.ks, *src_b = w & 1 ? a.vb : a.kb;
             auto fetch = [&](int t0) {
 #pragma unroll
                 for (int y = 0; y < NY; ++y) {
                     const int64_t off = piece(t0, y, held_at[y]);
+                    const uint8_t *pv = src + off;
+                    const uint16_t *ps = src_s + (off >> 6), *pb = src_b + (off >> 6);
 #pragma unroll
                     for (int x = 0; x < NX; ++x) {
                         const uint32_t at = 16u * (uint32_t)(64 * x + lane);
-                        held[y][x] = *(const u32x4 *)(src + off + at);
-                        held_sb[y][x] = (uint32_t)src_s[(off >> 6) + (at >> 6)] | ((uint32_t)src_b[(off >> 6) + (at >> 6)] << 16);
+                        held[y][x] = *(const u32x4 *)(pv + at);
+                        held_s[y][x] = ps[at >> 6];
+                        held_b[y][x] = pb[at >> 6];
                     }
                 }
             };
@@ -1085,7 +1053,7 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
 #pragma unroll
                     for (int x = 0; x < NX; ++x) {
                         const int at = 16 * (64 * x + lane), t = at / D, pc = (at - t * D) / 8;
-                        const float sc = f16bits_to_f32<BF>(held_sb[y][x] & 0xFFFFu), bi = f16bits_to_f32<BF>(held_sb[y][x] >> 16);
+                        const float sc = f16bits_to_f32<BF>(held_s[y][x]), bi = f16bits_to_f32<BF>(held_b[y][x]);
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             u32x4 hi, lo;
@@ -1102,14 +1070,56 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
                         }
                     }
             };
-            // Bit j: the tile's 16-token piece j lies in a page of the pool (after its copy).
-            const bool all_ok = pages_in_pool(a, tab, p0, p_last);
+            // Bit j: the tile's 16-token piece j lies in a page of the pool.
             auto pages_ok = [&](int t0) {
                 uint32_t ok = (1u << (C::BN / 16)) - 1;
                 if (!all_ok)
                     for (int j = 0; j < C::BN / 16; ++j)
                         if ((uint32_t)tab[min((t0 >> 4) + j, c_last) >> sh] >= (uint32_t)a.n_pages) ok &= ~(1u << j);
                 return ok;
+            };
+            // In a tile with hidden keys, the product of a hidden key's value
+            // with its probability 0 would be NaN where the value is an
+            // infinity or NaN: such values are made 0 in LDS, and where there
+            // are any (tiles that say so in odd_flag), what they do to the
+            // columns that see them is added from the pool.
+            auto clean = [&](uint32_t stage, int t0) {
+                uint32_t odd = 0;
+                for (uint32_t at = stage + C::kHalf + 16u * threadIdx.x; at < stage + 2 * C::kHalf; at += 16u * 256u) {
+                    u32x4 v = *(const LDSP(u32x4))(uintptr_t)at;
+                    uint32_t here = 0;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] = finite2<BF>(v[x], here);
+                    if (here) *(LDSP(u32x4))(uintptr_t)at = v;
+                    odd |= here;
+                }
+                if (odd) *odd_flag = t0 + 1;
+                __syncthreads();
+            };
+            auto add_odd = [&](int t0, int lim) {
+#pragma unroll 1
+                for (int t = t0; t < min(t0 + C::BN, t_end); ++t) {
+                    const int id = __builtin_amdgcn_readfirstlane(tab[t >> a.lps]);
+                    if ((uint32_t)id >= (uint32_t)a.n_pages) continue;
+                    const int64_t off = (int64_t)id * a.page_stride + h_off + (int64_t)(t & ((1 << a.lps) - 1)) * a.tok_stride;
+#pragma unroll
+                    for (int k = 0; k < State::NR; ++k) {
+                        const int64_t at = off + State::run_d(k);
+                        floatx4 y;
+                        if constexpr (Q8) {
+                            const float sc = f16bits_to_f32<BF>(a.vs[at >> 6]), bi = f16bits_to_f32<BF>(a.vb[at >> 6]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float v = fmaf((float)((const uint8_t *)a.v)[at + e], sc, bi);
+                                y[e] = t < lim && v - v != 0.f ? v : 0.f;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) y[e] = t < lim ? odd_part<BF>(((const uint16_t *)a.v)[at + e]) : 0.f;
+                        }
+                        st.add(k, y);
+                    }
+                }
             };
             __syncthreads();  // the last unit's reads
             if constexpr (Q8) {
@@ -1118,6 +1128,7 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
             } else {
                 copy(t_begin, lds);
             }
+            if (threadIdx.x == 0) *odd_flag = 0;
             uint32_t stage = lds, other = lds + (C::kStages - 1) * C::kStage;
             for (int t0 = t_begin; t0 < t_end; t0 += C::BN) {
                 const bool more = t0 + C::BN < t_end;
@@ -1129,11 +1140,13 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
                     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                     if (more) copy(t0 + C::BN, other);
                 }
+                const bool hidden = !all_ok || t0 + C::BN > min(least_all, t_end);  // uniform over the workgroup
+                if (hidden) clean(stage, t0);
                 if (t0 < most) {
-                    if (t0 + C::BN <= min(least, t_end) && all_ok)
-                        st.template tile<false>(stage, scale, t0, 0, 0);
-                    else
-                        st.template tile<true>(stage, scale, t0, min(seen, t_end), pages_ok(t0));
+                    const int lim = min(seen, t_end);
+                    const bool masked = !all_ok || t0 + C::BN > min(least, t_end);
+                    st.tile(stage, scale, masked, t0, lim, masked ? pages_ok(t0) : 0u);
+                    if (hidden && *odd_flag == t0 + 1) add_odd(t0, lim);
                 }
                 if constexpr (Q8) {
                     if constexpr (C::kStages == 1) __syncthreads();
@@ -1154,8 +1167,8 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
         float *pp = a.part + slot * D;
 #pragma unroll
         for (int k = 0; k < State::NR; ++k) {
-            int d;
-            const floatx4 v = st.run(k, d) * mul;
+            const int d = State::run_d(k);
+            const floatx4 v = st.run(k) * mul;
             if (whole) *(u32x2 *)(op + d) = u32x2{pack2<BF>(v.x, v.y), pack2<BF>(v.z, v.w)};
             else *(floatx4 *)(pp + d) = v;
         }
@@ -1230,7 +1243,7 @@ struct Grid {
 template <int D, bool BF, bool Q8>
 int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
     if (g.groups) {
-        constexpr int lds = Chunk<D, Q8>::kLds;
+        constexpr int lds = Chunk<D, Q8>::kLds + 16;  // (and a flag)
         static_assert(lds <= 160 << 10, "LDS of a CU");
         static const bool ok = lds <= (64 << 10) || hipFuncSetAttribute((const void *)kq_paged_chunk_kernel<D, BF, Q8>,
                                                                         hipFuncAttributeMaxDynamicSharedMemorySize,
