@@ -37,15 +37,6 @@
 
 namespace {
 
-// Tokens per split of a ragged row, by the row's own length (split_rule).
-struct SplitRule {
-    int32_t one, to64, to128, to256, rest;
-
-    __host__ __device__ __forceinline__ int tokens(int len) const {
-        return len <= one ? one : len <= to64 ? 64 : len <= to128 ? 128 : len <= to256 ? 256 : rest;
-    }
-};
-
 struct SdpaArgs {
     const uint16_t *q, *k, *v;
     uint16_t *out;
@@ -109,11 +100,6 @@ __device__ __forceinline__ int64_t ragged_base(const SdpaArgs &a, int b, int h, 
     if (a.padded)
         return (int64_t)b * a.pad_batch_stride + (int64_t)h * a.pad_head_stride + (int64_t)padded_start(a, b) * D;
     return a.kv_off[b] + (int64_t)h * a.head_stride[b];
-}
-
-__host__ __device__ __forceinline__ int row_splits(const SplitRule &rule, int len) {
-    const int split = rule.tokens(len);
-    return len <= 0 ? 1 : (len + split - 1) / split;
 }
 
 __device__ __forceinline__ int cascade_start(const SdpaArgs &a, int sq) {
@@ -903,12 +889,7 @@ struct WsLayout {
 WsLayout ws_layout(int B, int Hq, int Hkv, int D, int max_len, bool q8, bool wide = false) {
     WsLayout w;
     w.rule = split_rule(B, Hq, Hkv, D, max_len, q8, wide);
-    // the most splits are those of max_len or of a row at a line below it
-    w.max_splits = row_splits(w.rule, max_len);
-    for (const int line : {w.rule.one, w.rule.to64, w.rule.to128, w.rule.to256}) {
-        const int n = line < max_len ? row_splits(w.rule, line) : 1;
-        if (n > w.max_splits) w.max_splits = n;
-    }
+    w.max_splits = most_row_splits(w.rule, max_len);
     const size_t slots = (size_t)B * Hkv * w.max_splits * (Hq / Hkv);
     w.part_bytes = (slots * D * 4 + 255) & ~(size_t)255;
     w.ml_bytes = slots * 2 * 4;

@@ -2,6 +2,8 @@
 // 16-bit conversions by element type, reductions over a wave's lane groups.
 #pragma once
 #include <stdlib.h>
+
+#include <initializer_list>
 #include <type_traits>
 
 #include "kq_common.h"
@@ -60,6 +62,31 @@ __device__ __forceinline__ float f16bits_to_f32(uint32_t h) {
 __device__ __forceinline__ int64_t uniform64(int64_t v) {
     return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
                      (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// Tokens per split of a row, by the row's own length.
+struct SplitRule {
+    int32_t one, to64, to128, to256, rest;
+
+    __host__ __device__ __forceinline__ int tokens(int len) const {
+        return len <= one ? one : len <= to64 ? 64 : len <= to128 ? 128 : len <= to256 ? 256 : rest;
+    }
+};
+
+__host__ __device__ __forceinline__ int row_splits(const SplitRule &rule, int len) {
+    const int split = rule.tokens(len);
+    return len <= 0 ? 1 : (len + split - 1) / split;
+}
+
+// The most splits of any row of at most max_len keys: those of max_len or of a
+// row at a line below it.
+int most_row_splits(const SplitRule &rule, int max_len) {
+    int most = row_splits(rule, max_len);
+    for (const int line : {rule.one, rule.to64, rule.to128, rule.to256}) {
+        const int n = line < max_len ? row_splits(rule, line) : 1;
+        if (n > most) most = n;
+    }
+    return most;
 }
 
 int env_int(const char *name, int dflt) {

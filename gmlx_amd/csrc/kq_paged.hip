@@ -24,12 +24,18 @@ struct PagedArgs {
     int32_t group_cols;  // query columns of a chunk's workgroup
     float scale_log2;
     float *part, *ml;  // split partials: [slot][D] sums, [slot][2] (maximum, sum)
+    SplitRule rule;    // rows of few columns
+    // slots a token and query head, or 0: a row's slots follow those of the rows
+    // before it (a chunk's tokens have fewer splits than a decode row's)
+    int32_t slot_stride;
+    int32_t direct;    // the wave kernel's grid is (split, kv head, row)
 };
 
 constexpr int kFewColumns = 16;     // rows of at most so many columns take the wave kernel
-constexpr int kSplitTokens = 512;   // least keys of a split
-constexpr int kSplitWaves = 2048;   // waves that splitting a row of few columns aims at
 constexpr int kSplitGroups = 512;   // workgroups that splitting a chunk aims at
+constexpr int kSplitTokens = 512;   // least keys of a chunk's split
+constexpr int kDirect = 1 << 15;    // waves, and merged tokens and heads, of a direct grid
+constexpr int kMergeGroups = 2048;  // workgroups of a merge that is not
 
 __host__ __device__ __forceinline__ bool few_columns(int n, int G) { return (int64_t)n * G <= kFewColumns; }
 
@@ -44,12 +50,10 @@ __host__ __device__ __forceinline__ int row_blocks(int n, int G, int group_cols)
 
 // Splits of a row of n tokens and kv keys: from the row and the head counts
 // alone, so that a row of a batch has the bits of the row alone.
-__host__ __device__ __forceinline__ int paged_splits(int n, int kv, int G, int Hkv, int group_cols) {
+__host__ __device__ __forceinline__ int paged_splits(const SplitRule &rule, int n, int kv, int G, int Hkv, int group_cols) {
+    if (few_columns(n, G)) return row_splits(rule, kv);
     const int units = row_blocks(n, G, group_cols) * Hkv;
-    if (units == 0) return 1;
-    const int most = (kv + kSplitTokens - 1) / kSplitTokens;
-    const int want = ((few_columns(n, G) ? kSplitWaves : kSplitGroups) + units - 1) / units;
-    return max(1, min(want, most));
+    return max(1, min(kSplitGroups / units, kv / kSplitTokens));
 }
 
 struct Row {
@@ -66,7 +70,7 @@ __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     r.n = min(r.full, a.max_q);
     r.kv = (int)min((int64_t)max(min(a.kv_lens[b], a.max_kv), 0), (int64_t)a.width << a.lps);
     r.blocks = row_blocks(r.n, a.G, a.group_cols);
-    r.splits = paged_splits(r.n, r.kv, a.G, a.Hkv, a.group_cols);
+    r.splits = paged_splits(a.rule, r.n, r.kv, a.G, a.Hkv, a.group_cols);
     return r;
 }
 
@@ -81,13 +85,21 @@ __device__ __forceinline__ int row_slots(const PagedArgs &a, const Row &r) {
     return r.splits > 1 ? r.n * a.Hq * r.splits : 0;
 }
 
+// Inclusive sum over the wave's lanes.
 __device__ __forceinline__ int wave_scan(int v) {
-    const int lane = kq_lane();
-    for (int off = 1; off < 64; off <<= 1) {
-        const int t = __shfl_up(v, off);
-        if (lane >= off) v += t;
-    }
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
     return v;
+}
+
+// Partial slot of split 0 of token i (of the row), query head hq.
+__device__ __forceinline__ int64_t slot_of(const PagedArgs &a, const Row &r, int slot0, int i, int hq) {
+    if (a.slot_stride) return ((int64_t)(r.q0 + i) * a.Hq + hq) * a.slot_stride;
+    return slot0 + (i * a.Hq + hq) * r.splits;
 }
 
 // The row that unit u belongs to, with u made its number within the row and
@@ -103,6 +115,34 @@ __device__ __forceinline__ bool find_unit(const PagedArgs &a, int &u, int &b, in
         if (row < a.B) {
             const Row x = row_at(a, row);
             mu = row_units<CHUNK>(a, x);
+            ms = row_slots(a, x);
+        }
+        const int iu = wave_scan(mu), is = wave_scan(ms);
+        const int total = __builtin_amdgcn_readlane(iu, 63);
+        if (u < total) {
+            const int src = __builtin_ctzll(__ballot(u < iu));
+            b = c0 + src;
+            u -= __builtin_amdgcn_readlane(iu - mu, src);
+            slot0 = slots + __builtin_amdgcn_readlane(is - ms, src);
+            return true;
+        }
+        u -= total;
+        slots += __builtin_amdgcn_readlane(is, 63);
+    }
+    return false;
+}
+
+// The same for the merge's units: four (token, query head) of a row that has
+// splits.
+__device__ __forceinline__ bool find_split_tokens(const PagedArgs &a, int &u, int &b, int &slot0) {
+    const int lane = kq_lane();
+    int slots = 0;
+    for (int c0 = 0; c0 < a.B; c0 += 64) {
+        const int row = c0 + lane;
+        int mu = 0, ms = 0;
+        if (row < a.B) {
+            const Row x = row_at(a, row);
+            mu = x.splits > 1 ? (x.n * a.Hq + 3) / 4 : 0;
             ms = row_slots(a, x);
         }
         const int iu = wave_scan(mu), is = wave_scan(ms);
@@ -495,10 +535,21 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
     constexpr int NBUF = D >= 256 ? 1 : 2;
     const int lane = kq_lane(), r = lane & 15, g = lane >> 4;
     for (int unit = blockIdx.x;; unit += gridDim.x) {
-        int u = unit, b, slot0;
-        if (!find_unit<false>(a, u, b, slot0)) return;
-        const Row row = uniform_row(a, b);
-        const int s = u / a.Hkv, h = u - s * a.Hkv;
+        int b, h, s, slot0 = 0;
+        Row row;
+        if (a.direct) {
+            s = unit;
+            h = blockIdx.y;
+            b = blockIdx.z;
+            row = uniform_row(a, b);
+            if (!few_columns(row.n, a.G) || row.n == 0 || s >= row.splits) return;
+        } else {
+            int u = unit;
+            if (!find_unit<false>(a, u, b, slot0)) return;
+            row = uniform_row(a, b);
+            s = u / a.Hkv;
+            h = u - s * a.Hkv;
+        }
 
         // this lane's column
         const bool live = r < row.n * a.G;
@@ -509,8 +560,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
         const int first = row.kv - row.full + 1;
         const int seen = live ? max(first + i, 0) : 0x7fffffff;
         const int least = max(first, 0), most = min(max(first + row.n - 1, 0), row.kv);
-        // whole tiles, about the same for each split
-        const int per = ((row.kv + row.splits - 1) / row.splits + TT - 1) / TT * TT;
+        const int per = a.rule.tokens(row.kv);
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
         const int t_end = __builtin_amdgcn_readfirstlane(min(most, t_begin + per));
         const uint16_t *qp = a.q + (int64_t)(row.q0 + i) * a.q_stride + (int64_t)hq * D;
@@ -614,7 +664,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
         const bool whole = row.splits == 1;
         const float mul = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
         uint16_t *op = a.out + (int64_t)(row.q0 + i) * a.out_stride + (int64_t)hq * D;
-        const int64_t slot = slot0 + (i * a.Hq + hq) * row.splits + s;
+        const int64_t slot = slot_of(a, row, slot0, i, hq) + s;
         float *pp = a.part + slot * D;
         // runs of W consecutive values: lane (column, g), o[j0 .. j0 + W)[e]
         constexpr int W = Q8 ? 4 : 8;
@@ -1163,7 +1213,7 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
         const bool whole = row.splits == 1;
         const float mul = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
         uint16_t *op = a.out + (int64_t)(row.q0 + i) * a.out_stride + (int64_t)hq * D;
-        const int64_t slot = slot0 + (i * a.Hq + hq) * row.splits + s;
+        const int64_t slot = slot_of(a, row, slot0, i, hq) + s;
         float *pp = a.part + slot * D;
 #pragma unroll
         for (int k = 0; k < State::NR; ++k) {
@@ -1179,65 +1229,168 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
     }
 }
 
-// One wave a (token, query head) of a row with splits: rescales the splits to
-// their common maximum and sums them in split order.
+// Scale of a split of maximum ms beside the common maximum m; a split without
+// keys holds zeros and counts nothing, one of NaN scores has a NaN sum l.
+__device__ __forceinline__ float split_scale(float ms, float m) {
+    return ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+}
+
+// (Token, query head) of n splits by one workgroup: thread t handles the float4
+// of outputs 4 q .. 4 q + 3 (q = t % (D / 4)) for the splits p, p + P, ... (p =
+// t / (D / 4) of P parts), rescaled to the common maximum; the P sums are added
+// in part order through LDS.
+template <int D, bool BF>
+__device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, int n, uint16_t *out) {
+    constexpr int Q = D / 4, P = 256 / Q;
+    __shared__ float red_m[4];
+    __shared__ float4 red_acc[P][Q];
+    __shared__ float red_l[P];
+    const int t = threadIdx.x, q = t % Q, part = t / Q;
+    const float *ml = a.ml + 2 * slot;
+    const float4 *po = (const float4 *)(a.part + slot * D) + q;
+    float m = -INFINITY;
+    for (int s = t; s < n; s += 256) m = fmaxf(m, ml[2 * s]);
+    // this thread's first splits, in flight beside the maximum's loads
+    constexpr int PRE = 4;
+    float4 o_pre[PRE];
+    float m_pre[PRE], l_pre[PRE];
+#pragma unroll
+    for (int k = 0; k < PRE; ++k) {
+        const int s = min(part + k * P, n - 1);
+        m_pre[k] = ml[2 * s];
+        l_pre[k] = ml[2 * s + 1];
+        o_pre[k] = po[(int64_t)s * Q];
+    }
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    __syncthreads();  // the last item's reads
+    if ((t & 63) == 0) red_m[t >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+    if (part < P) {  // (D = 96: threads 240 .. 255 hold no part)
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+        const auto add = [&](float ms, float ls, const float4 &o) {
+            const float f = split_scale(ms, m);
+            if (f == 0.f && ls == ls) return;
+            l += f * ls;
+            acc.x += f * o.x;
+            acc.y += f * o.y;
+            acc.z += f * o.z;
+            acc.w += f * o.w;
+        };
+#pragma unroll
+        for (int k = 0; k < PRE; ++k)
+            if (part + k * P < n) add(m_pre[k], l_pre[k], o_pre[k]);
+#pragma unroll 4
+        for (int s = part + PRE * P; s < n; s += P) add(ml[2 * s], ml[2 * s + 1], po[(int64_t)s * Q]);
+        red_acc[part][q] = acc;
+        if (q == 0) red_l[part] = l;
+    }
+    __syncthreads();
+    if (part == 0) {
+        float4 acc = red_acc[0][q];
+        float l = red_l[0];
+#pragma unroll
+        for (int k = 1; k < P; ++k) {
+            const float4 o = red_acc[k][q];
+            acc.x += o.x;
+            acc.y += o.y;
+            acc.z += o.z;
+            acc.w += o.w;
+            l += red_l[k];
+        }
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        *(u32x2 *)(out + 4 * q) = u32x2{pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv)};
+    }
+}
+
+// The same by one wave, for at most 64 splits (lane s holds split s's maximum and
+// sum), in the same order of sums.
+template <int D, bool BF>
+__device__ __forceinline__ void merge_wave(const PagedArgs &a, int64_t slot, int n, uint16_t *out) {
+    constexpr int P = 256 / (D / 4), V = D > 128 ? 4 : 2, R = D > 256 ? 2 : 1;  // R runs of V values a lane
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const int lane = kq_lane();
+    const float ms = lane < n ? a.ml[2 * (slot + lane)] : -INFINITY, ls = lane < n ? a.ml[2 * (slot + lane) + 1] : 0.f;
+    float m = ms;
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    const float f = split_scale(ms, m);
+    const auto lane_of = [](float v, int s) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), s));
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int d = (r * 64 + lane) * V;
+        const float *p = a.part + slot * D + min(d, D - V);
+        vec acc[P];
+        float l[P];
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            acc[k] = vec(0.f);
+            l[k] = 0.f;
+        }
+        for (int s0 = 0; s0 < n; s0 += P) {
+            vec o[P];
+#pragma unroll
+            for (int k = 0; k < P; ++k) o[k] = *(const vec *)(p + (int64_t)min(s0 + k, n - 1) * D);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                if (s0 + k >= n) break;
+                const float fs = lane_of(f, s0 + k), lk = lane_of(ls, s0 + k);
+                if (fs == 0.f && lk == lk) continue;
+                l[k] += fs * lk;
+#pragma unroll
+                for (int x = 0; x < V; ++x) acc[k][x] += fs * o[k][x];
+            }
+        }
+#pragma unroll
+        for (int k = 1; k < P; ++k) {
+            acc[0] = acc[0] + acc[k];
+            l[0] += l[k];
+        }
+        const float inv = l[0] > 0.f || l[0] != l[0] ? 1.f / l[0] : 0.f;
+        if (d < D) {
+#pragma unroll
+            for (int x = 0; x < V; x += 2) *(uint32_t *)(out + d + x) = pack2<BF>(acc[0][x] * inv, acc[0][x + 1] * inv);
+        }
+    }
+}
+
+// Workgroups take a token and query head each (direct), or four of a row's at a
+// time: a wave each where the row has at most 64 splits.
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
-    constexpr int V = D >= 256 ? D / 64 : 2;  // values a lane
-    const int lane = kq_lane();
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = (int)(item / a.Hq), hq = (int)(item - (int64_t)t * a.Hq);
-    if (t >= a.T) return;
-    // the token's row
-    int64_t slot = 0;
-    int splits = 0;
-    for (int c0 = 0; c0 < a.B && !splits; c0 += 64) {
-        const int row = c0 + lane;
-        int ms = 0;
-        Row x{};
-        if (row < a.B) {
-            x = row_at(a, row);
-            ms = row_slots(a, x);
-        }
-        const int is = wave_scan(ms);
-        const uint64_t hit = __ballot(row < a.B && t >= x.q0 && t < x.q0 + x.n);
-        if (hit) {
-            const int src = __builtin_ctzll(hit);
-            splits = __shfl(x.splits, src);
-            slot += __shfl(is - ms, src) + ((int64_t)(t - __shfl(x.q0, src)) * a.Hq + hq) * splits;
+    const auto out = [&](const Row &r, int x) {
+        const int i = x / a.Hq;
+        return a.out + (int64_t)(r.q0 + i) * a.out_stride + (int64_t)(x - i * a.Hq) * D;
+    };
+    const auto slot = [&](const Row &r, int slot0, int x) {
+        const int i = x / a.Hq;
+        return slot_of(a, r, slot0, i, x - i * a.Hq);
+    };
+    if (a.direct) {
+        const Row row = uniform_row(a, blockIdx.y);
+        const int x = blockIdx.x;
+        if (row.splits > 1 && x < row.n * a.Hq) merge_group<D, BF>(a, slot(row, 0, x), row.splits, out(row, x));
+        return;
+    }
+    const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    for (int item = blockIdx.x;; item += gridDim.x) {
+        int u = item, b, slot0;
+        if (!find_split_tokens(a, u, b, slot0)) return;
+        const Row row = uniform_row(a, b);
+        const int end = min(4 * u + 4, row.n * a.Hq);
+        if (row.splits <= 64) {
+            if (4 * u + w < end) merge_wave<D, BF>(a, slot(row, slot0, 4 * u + w), row.splits, out(row, 4 * u + w));
         } else {
-            slot += __shfl(is, 63);
+            for (int x = 4 * u; x < end; ++x) merge_group<D, BF>(a, slot(row, slot0, x), row.splits, out(row, x));
         }
     }
-    if (splits < 2) return;
-    const float *ml = a.ml + 2 * slot;
-    float m = -INFINITY;
-    for (int s = lane; s < splits; s += 64) m = fmaxf(m, ml[2 * s]);
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-    float acc[V], l = 0.f;
-#pragma unroll
-    for (int x = 0; x < V; ++x) acc[x] = 0.f;
-    const int d = lane * V;
-    if (d >= D) return;
-    for (int s = 0; s < splits; ++s) {
-        const float ms = ml[2 * s];
-        const float ls = ml[2 * s + 1];
-        const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-        if (f == 0.f && ls == ls) continue;  // (a split without keys holds zeros; one of NaN scores a NaN sum)
-        l += f * ls;
-        const float *p = a.part + (slot + s) * D + d;
-#pragma unroll
-        for (int x = 0; x < V; ++x) acc[x] += f * p[x];
-    }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    uint16_t *op = a.out + (int64_t)t * a.out_stride + (int64_t)hq * D + d;
-#pragma unroll
-    for (int x = 0; x < V; ++x) op[x] = from_f32<BF>(acc[x] * inv);
 }
 
 struct Grid {
-    int waves, groups;  // 0: not launched
-    bool merge;
+    dim3 waves, merge;
+    int groups;  // (x == 0, 0: not launched)
 };
 
 template <int D, bool BF, bool Q8>
@@ -1251,10 +1404,8 @@ int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
         if (!ok) return KQ_ERR_LAUNCH_FAILED;
         hipLaunchKernelGGL((kq_paged_chunk_kernel<D, BF, Q8>), dim3(g.groups), dim3(256), lds, s, a);
     }
-    if (g.waves) hipLaunchKernelGGL((kq_paged_split_kernel<D, BF, Q8>), dim3(g.waves), dim3(64), 0, s, a);
-    if (g.merge)
-        hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF>), dim3((unsigned)(((int64_t)a.T * a.Hq + 3) / 4)), dim3(256), 0,
-                           s, a);
+    if (g.waves.x) hipLaunchKernelGGL((kq_paged_split_kernel<D, BF, Q8>), g.waves, dim3(64), 0, s, a);
+    if (g.merge.x) hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF>), g.merge, dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? KQ_OK : KQ_ERR_LAUNCH_FAILED;
 }
 
@@ -1265,24 +1416,44 @@ int launch(const PagedArgs &a, bool q8, const Grid &g, hipStream_t s) {
     return launch_q8<D, BF, false>(a, g, s);
 }
 
-// The most splits of any row of at most max_q tokens and max_kv keys.
-int most_splits(int max_q, int Hq, int Hkv, int D, int max_kv) {
-    const int G = Hq / Hkv, chunk = kFewColumns / G + 1;  // the shortest chunk
-    const int few = chunk > 1 ? paged_splits(1, max_kv, G, Hkv, group_columns(D)) : 1;
-    const int many = max_q >= chunk ? paged_splits(chunk, max_kv, G, Hkv, group_columns(D)) : 1;
-    return few > many ? few : many;
+// Tokens per split of a row of few columns, by its own keys, as decode
+// attention over contiguous caches has them.
+SplitRule wave_rule(int Hq, int Hkv, int D, bool q8) {
+    if (D > 128) return SplitRule{q8 || D > 256 ? 0 : 128, 1024, 8192, 32768, 512};
+    if (q8) return SplitRule{Hq > 8 * Hkv ? 256 : 0, 1024, 2048, 32768, 512};
+    if (Hq > 8 * Hkv) return SplitRule{512, 0, 1024, 8192, 512};
+    return SplitRule{256, 512, Hq > 4 * Hkv ? 1024 : 4096, 8192, 512};
 }
 
-// Partial slots of a call: one a token, query head and split; and of a row at
-// most 2 kSplitGroups * 128 (a split row has units < kSplitGroups workgroups
-// of 128 columns, and splits <= kSplitGroups / units + 1; rows of few columns
-// have fewer).
-int64_t max_slots(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max_kv) {
-    const int most = most_splits(max_q, Hq, Hkv, D, max_kv);
-    if (most < 2) return 0;
-    static_assert(2 * kSplitWaves * kFewColumns <= 2 * kSplitGroups * 128, "the chunks' bound covers both");
-    const int64_t by_token = T * Hq * most, by_row = B * 2 * kSplitGroups * 128;
-    return by_token < by_row ? by_token : by_row;
+// What a call's splits can come to, from the bounds that the host knows.
+struct Plan {
+    SplitRule rule;
+    int few, many;    // the most splits of a row of few columns, of a chunk
+    int64_t slots;    // of the workspace
+    int slot_stride;  // (PagedArgs)
+};
+
+Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max_kv, bool q8) {
+    Plan p;
+    const int G = Hq / Hkv, chunk = kFewColumns / G + 1;  // tokens of the shortest chunk
+    p.rule = wave_rule(Hq, Hkv, D, q8);
+    p.few = chunk > 1 ? most_row_splits(p.rule, max_kv) : 1;
+    p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, group_columns(D)) : 1;
+    const int most = p.few > p.many ? p.few : p.many;
+    if (most < 2) {
+        p.slots = p.slot_stride = 0;
+        return p;
+    }
+    // one slot a token, query head and split; and of a row, of few columns at
+    // most kFewColumns of them a kv head, a chunk's at most kSplitGroups *
+    // 128 (one with splits has units < kSplitGroups workgroups of at most 128
+    // columns and splits <= kSplitGroups / units)
+    const int64_t by_token = T * Hq * most;
+    const int64_t few_row = (int64_t)kFewColumns * Hkv * p.few, many_row = p.many > 1 ? kSplitGroups * 128 : 0;
+    const int64_t by_row = B * (few_row > many_row ? few_row : many_row);
+    p.slots = by_token < by_row ? by_token : by_row;
+    p.slot_stride = by_token <= by_row ? most : 0;
+    return p;
 }
 
 size_t part_bytes(int64_t slots, int D) { return ((size_t)slots * D * 4 + 255) & ~(size_t)255; }
@@ -1294,7 +1465,7 @@ extern "C" {
 size_t kq_sdpa_paged_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
                                      int32_t max_kv, int q8) {
     if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_q <= 0 || max_kv <= 0) return 0;
-    const int64_t slots = max_slots(T, B, Hq, Hkv, D, max_q, max_kv);
+    const int64_t slots = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, q8 != 0).slots;
     return slots ? part_bytes(slots, D) + (size_t)slots * 8 : 0;
 }
 
@@ -1312,14 +1483,14 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     if ((int64_t)T * Hq > (1 << 30) || q_stride < (int64_t)Hq * D || out_stride < (int64_t)Hq * D)
         return KQ_ERR_BAD_SHAPE;
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_stride | out_stride) & 7)) return KQ_ERR_BAD_ALIGN;
-    const size_t need = kq_sdpa_paged_workspace_bytes(T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr);
+    const Plan plan = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr);
+    const int64_t most = plan.few > plan.many ? plan.few : plan.many;
+    // 31-bit unit and partial numbers
+    if (plan.slots >= (int64_t)1 << 31 || ((int64_t)T * (Hq / Hkv) + B) * Hkv * most >= (int64_t)1 << 31)
+        return KQ_ERR_BAD_SHAPE;
+    const size_t need = plan.slots ? part_bytes(plan.slots, D) + (size_t)plan.slots * 8 : 0;
     if (need && (!workspace || workspace_bytes < need)) return KQ_ERR_WORKSPACE_TOO_SMALL;
     if (need && ((uintptr_t)workspace & 255)) return KQ_ERR_BAD_ALIGN;
-    const int most = most_splits(max_q, Hq, Hkv, D, max_kv);
-    // 31-bit unit and partial numbers
-    if (max_slots(T, B, Hq, Hkv, D, max_q, max_kv) >= (int64_t)1 << 31 ||
-        ((int64_t)T * (Hq / Hkv) + B) * Hkv * most >= (int64_t)1 << 31)
-        return KQ_ERR_BAD_SHAPE;
     PagedArgs a;
     a.q = (const uint16_t *)q;
     a.out = (uint16_t *)out;
@@ -1350,16 +1521,30 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const int64_t slots = max_slots(T, B, Hq, Hkv, D, max_q, max_kv);
     a.part = (float *)workspace;
-    a.ml = (float *)((char *)workspace + part_bytes(slots, D));
-    // bounds of the units; the grids' waves and workgroups take the rest in turn
-    const int64_t few = (int64_t)(T < B ? T : B) * Hkv * most;
-    const int64_t many = (((int64_t)T * a.G + a.group_cols - 1) / a.group_cols + (T < B ? T : B)) * Hkv * most;
+    a.ml = (float *)((char *)workspace + part_bytes(plan.slots, D));
+    a.rule = plan.rule;
+    a.slot_stride = plan.slot_stride;
+    // Bounds of the units; past them the grids' waves and workgroups take the
+    // rest in turn.  Where a wave or workgroup for every unit that the longest
+    // rows would have is no large grid, each finds its own from its place there;
+    // else they sum over the rows' units.
     Grid g;
-    g.waves = a.G > kFewColumns ? 0 : (int)(few < (1 << 16) ? few : (1 << 16));
+    const int64_t rows = T < B ? T : B, waves = plan.few * (int64_t)Hkv * B;
+    const int64_t items = (int64_t)(max_q < T ? max_q : T) * Hq;
+    a.direct = (plan.slot_stride || !plan.slots) && B < (1 << 16) && Hkv < (1 << 16) && waves <= kDirect &&
+               items * B <= kDirect;
+    g.waves = g.merge = dim3(0);
+    if (a.G <= kFewColumns) {
+        const int64_t n = rows * Hkv * plan.few;
+        g.waves = a.direct ? dim3(plan.few, Hkv, B) : dim3((unsigned)(n < (1 << 16) ? n : (1 << 16)));
+    }
+    const int64_t many = (((int64_t)T * a.G + a.group_cols - 1) / a.group_cols + rows) * Hkv * plan.many;
     g.groups = few_columns(max_q, a.G) ? 0 : (int)(many < (1 << 14) ? many : (1 << 14));
-    g.merge = slots > 0;
+    if (plan.slots) {
+        const int64_t n = (int64_t)T * Hq / 4 + B;
+        g.merge = a.direct ? dim3((unsigned)items, B) : dim3((unsigned)(n < kMergeGroups ? n : kMergeGroups));
+    }
     const bool q8 = a.ks != nullptr, bf = pool->dtype == KQ_DTYPE_BF16;
     hipStream_t s = (hipStream_t)stream;
     switch (D) {
