@@ -179,10 +179,10 @@ _SIGS = {
     "kq_sdpa_decode_gqa_cascade": ([_vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64, _i32, _vp, _i32, _i32,
                                     _i32, _i32, _i32, _f32, _int, _vp, _vp, _sz, _vp], _int),
     "kq_paged_plan": ([_vp, _vp, _vp, _i32, _vp, _i64, _i32, _vp, _i32, _vp, _i32, _i32] + [_vp] * 7, _int),
-    "kq_paged_write": ([ctypes.POINTER(PagedPool), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp], _int),
-    "kq_paged_read": ([ctypes.POINTER(PagedPool), _vp, _i32, _vp, _vp, _vp], _int),
+    "kq_paged_write": ([_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp], _int),
+    "kq_paged_read": ([_vp, _vp, _i32, _vp, _vp, _vp], _int),
     "kq_sdpa_paged_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _int], _sz),
-    "kq_sdpa_paged": ([_vp, _i64, ctypes.POINTER(PagedPool), _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+    "kq_sdpa_paged": ([_vp, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
                        _f32, _vp, _i64, _vp, _sz, _vp], _int),
     "kq_gguf_open": ([ctypes.c_char_p, ctypes.POINTER(_vp)], _int),
     "kq_gguf_close": ([_vp], None),

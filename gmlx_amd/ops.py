@@ -25,8 +25,9 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from collections import OrderedDict
-from typing import NamedTuple, Optional
+from typing import NamedTuple
 
 import torch
 
@@ -1203,6 +1204,9 @@ class PagedPlan(NamedTuple):
     refused: torch.Tensor     # [B] 1: no pages for this row, which stays as it was
 
 
+_I32 = torch.int32
+
+
 def _paged_call(fn, device, *args):
     """One library call with `device` current (a launch goes to the current
     device, whichever the stream's is)."""
@@ -1212,22 +1216,99 @@ def _paged_call(fn, device, *args):
     else:
         with torch.cuda.device(device):
             rc = f(*args)
-    check(fn, rc)
+    if rc:
+        check(fn, rc)
 
 
-def _ints(t, name, shape, device):
-    """A contiguous int32 device tensor of `shape`."""
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or tuple(t.shape) != shape \
-            or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}")
+def _ints(t, name, n, device):
+    """The address of a contiguous int32 device tensor of n values."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _I32 or t.shape != (n,) or t.device != device or \
+            not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} values on {device}")
     return t.data_ptr()
 
 
 def _block_table(t, B, device):
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or t.dim() != 2 \
-            or t.shape[0] != B or t.shape[1] < 1 or t.stride(1) != 1 or (B > 1 and t.stride(0) < t.shape[1]):
+    if not isinstance(t, torch.Tensor) or t.dtype is not _I32 or t.dim() != 2 or t.device != device:
+        raise ValueError(f"block_table must be int32 [{B}, pages] on {device}")
+    (rows, width), (stride, one) = t.shape, t.stride()
+    if rows != B or width < 1 or (one != 1 and width > 1) or (B > 1 and stride < width):
         raise ValueError(f"block_table must be int32 [{B}, pages] on {device}, its rows contiguous")
-    return t.data_ptr(), t.stride(0) if B > 1 else t.shape[1], t.shape[1]
+    return t.data_ptr(), stride if B > 1 else width, width
+
+
+class _PoolLayout:
+    """A pool's shape, strides and types, checked: what kq_paged_pool holds
+    beside the addresses."""
+    PACK = struct.Struct("6P3q5i4x").pack  # kq_paged_pool
+
+    def __init__(self, k, v, scales):
+        if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or v.device != k.device or \
+                v.dtype != k.dtype or k.stride(3) != 1:
+            raise ValueError("k_cache / v_cache must be [n_pages, Hkv, page_size, D] of one layout, D contiguous")
+        n, H, ps, D = k.shape
+        if scales[0] is None:
+            dt = k.dtype
+            if dt not in (torch.float16, torch.bfloat16):
+                raise ValueError(f"a 16-bit pool is float16 or bfloat16, got {dt}")
+        else:
+            dt = scales[0].dtype
+            if k.dtype != torch.uint8 or D % 64:
+                raise ValueError("an 8-bit pool holds uint8 values in groups of 64")
+            if dt not in (torch.float16, torch.bfloat16):
+                raise ValueError(f"scales and biases must be float16 or bfloat16, got {dt}")
+            for t in scales:
+                if t.device != k.device or t.dtype != dt or t.shape != (n, H, ps, D // 64) or \
+                        (D > 64 and t.stride(3) != 1) or \
+                        any(64 * t.stride(i) != k.stride(i) for i in range(3) if t.shape[i] > 1):
+                    raise ValueError("scales and biases must be [n_pages, Hkv, page_size, D / 64] of one dtype, laid "
+                                     "out as the values are (strides a 64th of theirs)")
+        self.dtype, self.device, self.Hkv, self.D, self.page_size, self.q8 = dt, k.device, H, D, ps, int(scales[0] is not None)
+        # (the stride of a dim of size 1 is never used)
+        self.rest = (k.stride(0) if n > 1 else 0, k.stride(1) if H > 1 else 0, k.stride(2), n, ps, H, D, _TORCH_DTYPE[dt])
+
+
+_LAYOUTS = {}  # checked pool layouts by shapes, strides, types and devices
+
+
+def _paged_pool(k, v, scales):
+    """(layout, the bytes of its kq_paged_pool) of a pool [n_pages, Hkv,
+    page_size, D], 16-bit or (with the four scale / bias tensors [n_pages, Hkv,
+    page_size, D / 64]) 8-bit."""
+    a, b, c, d = scales
+    if a is None and b is None and c is None and d is None:
+        key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device)
+        lay = _LAYOUTS.get(key)
+        ptrs = (k.data_ptr(), v.data_ptr(), 0, 0, 0, 0)
+    else:
+        if a is None or b is None or c is None or d is None:
+            raise ValueError("an 8-bit pool needs k_scales, k_biases, v_scales and v_biases")
+        dev = k.device
+        if not (v.device == dev and a.device == dev and b.device == dev and c.device == dev and d.device == dev):
+            raise ValueError("a pool's tensors must be on one device")
+        key = (k.shape, k.stride(), k.dtype, dev, v.shape, v.stride(), v.dtype, a.shape, a.stride(), a.dtype, b.shape,
+               b.stride(), b.dtype, c.shape, c.stride(), c.dtype, d.shape, d.stride(), d.dtype)
+        lay = _LAYOUTS.get(key)
+        ptrs = (k.data_ptr(), v.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr())
+    if lay is None:
+        _require_gpu(k, v)
+        lay = _PoolLayout(k, v, scales)
+        if len(_LAYOUTS) >= 256:
+            _LAYOUTS.clear()
+        _LAYOUTS[key] = lay
+    return lay, _PoolLayout.PACK(*ptrs, *lay.rest)
+
+
+def _token_rows(x):
+    """x [T, H, D] with D contiguous, the strides multiples of 8 and 16-byte
+    alignment (copied only where it has not): (x, token stride, head stride)."""
+    (T, H, D), (t, h, one) = x.shape, x.stride()
+    if one != 1 or (t % 8 and T > 1) or (h % 8 and H > 1) or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+        return x, H * D, D
+    return x, t if T > 1 else H * D, h if H > 1 else D
 
 
 def paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens, keep_lens=None):
@@ -1254,65 +1335,23 @@ def paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_siz
     [1]; page_size a power of two from 16 to 1024; max_tokens >= the new tokens
     of all rows (the length of slots and positions)."""
     _fault("paged_plan")
-    _require_gpu(seq_lens, new_lens, block_table, free_pages, free_count)
+    _require_gpu(seq_lens)
     dev, B, T = seq_lens.device, seq_lens.numel(), int(max_tokens)
     if not 1 <= B <= _lib.PAGED_MAX_ROWS or T < 0:
         raise ValueError(f"paged_plan: 1 to {_lib.PAGED_MAX_ROWS} rows and max_tokens >= 0, got {B} and {T}")
     tab, tab_stride, width = _block_table(block_table, B, dev)
-    seq, new = _ints(seq_lens, "seq_lens", (B,), dev), _ints(new_lens, "new_lens", (B,), dev)
-    keep = None if keep_lens is None else _ints(keep_lens, "keep_lens", (B,), dev)
-    stack = _ints(free_pages, "free_pages", (free_pages.numel(),), dev)
-    count = _ints(free_count, "free_count", (1,), dev)
-    parts = torch.empty(3 * B + 2 + 2 * T, dtype=torch.int32, device=dev).split((B + 1, B, T, T, 1, B))
-    cu_q, kv, slots, pos, left, refused = (t.data_ptr() for t in parts)
-    _paged_call("kq_paged_plan", dev, seq, keep, new, B, tab, tab_stride, width, stack, free_pages.numel(), count,
-                int(page_size), T, cu_q, kv, slots or cu_q, pos or cu_q, left, refused, _stream(seq_lens))
-    return PagedPlan(*parts)
-
-
-def _paged_pool(k, v, scales, name):
-    """The C description of a pool [n_pages, Hkv, page_size, D], 16-bit or (with
-    the four scale / bias tensors [n_pages, Hkv, page_size, D / 64]) 8-bit."""
-    _require_gpu(k, v)
-    if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or v.device != k.device or v.dtype != k.dtype \
-            or k.stride(3) != 1:
-        raise ValueError(f"{name}: k_cache / v_cache must be [n_pages, Hkv, page_size, D] of one layout, D contiguous")
-    n, H, ps, D = k.shape
-    # (the stride of a dim of size 1 is never used)
-    strides = [s if size > 1 else 0 for s, size in zip(k.stride()[:2], (n, H))] + [k.stride(2)]
-    if all(t is None for t in scales):
-        if k.dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f"{name}: a 16-bit pool is float16 or bfloat16, got {k.dtype}")
-        return _lib.PagedPool(k.data_ptr(), v.data_ptr(), None, None, None, None, *strides, n, ps, H, D,
-                              _TORCH_DTYPE[k.dtype]), k.dtype
-    if any(t is None for t in scales):
-        raise ValueError(f"{name}: an 8-bit pool needs k_scales, k_biases, v_scales and v_biases")
-    if k.dtype != torch.uint8 or D % 64:
-        raise ValueError(f"{name}: an 8-bit pool holds uint8 values in groups of 64")
-    dt = scales[0].dtype
-    if dt not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{name}: scales and biases must be float16 or bfloat16, got {dt}")
-    for t in scales:
-        if not isinstance(t, torch.Tensor) or t.device != k.device or t.dtype != dt \
-                or tuple(t.shape) != (n, H, ps, D // 64) or (D > 64 and t.stride(3) != 1) \
-                or any(64 * t.stride(i) != k.stride(i) for i in range(3) if t.shape[i] > 1):
-            raise ValueError(f"{name}: scales and biases must be [n_pages, Hkv, page_size, D / 64] of one dtype, laid "
-                             "out as the values are (strides a 64th of theirs)")
-    return _lib.PagedPool(k.data_ptr(), v.data_ptr(), *(t.data_ptr() for t in scales), *strides, n, ps, H, D,
-                          _TORCH_DTYPE[dt]), dt
-
-
-def _token_rows(x, D, name):
-    """x [T, H, D] with D contiguous, the strides multiples of 8 and 16-byte
-    alignment (copied only where it has not): (x, token stride, head stride)."""
-    if x.dim() != 3 or x.shape[2] != D:
-        raise ValueError(f"{name} must be [tokens, heads, {D}]")
-    T, H, _ = x.shape
-    if (D > 1 and x.stride(2) != 1) or (T > 1 and x.stride(0) % 8) or (H > 1 and x.stride(1) % 8) or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-    return x, x.stride(0) if T > 1 else H * D, x.stride(1) if H > 1 else D
+    seq, new = _ints(seq_lens, "seq_lens", B, dev), _ints(new_lens, "new_lens", B, dev)
+    keep = None if keep_lens is None else _ints(keep_lens, "keep_lens", B, dev)
+    n_stack = free_pages.numel()
+    stack, count = _ints(free_pages, "free_pages", n_stack, dev), _ints(free_count, "free_count", 1, dev)
+    out = torch.empty(3 * B + 2 + 2 * T, dtype=_I32, device=dev)
+    cu = out.data_ptr()
+    kv = cu + 4 * (B + 1)
+    slots = kv + 4 * B
+    left = slots + 8 * T
+    _paged_call("kq_paged_plan", dev, seq, keep, new, B, tab, tab_stride, width, stack, n_stack, count, int(page_size),
+                T, cu, kv, slots, slots + 4 * T, left, left + 4, _stream(seq_lens))
+    return PagedPlan(*out.split_with_sizes((B + 1, B, T, T, 1, B)))
 
 
 def paged_write(k, v, k_cache, v_cache, slots, k_scales=None, k_biases=None, v_scales=None, v_biases=None):
@@ -1329,19 +1368,17 @@ def paged_write(k, v, k_cache, v_cache, slots, k_scales=None, k_biases=None, v_s
     the pool (-1) writes nothing.  Slots are distinct: of two rows given the
     same one, which values stay is not specified."""
     _fault("paged_write")
-    pool, dt = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases), "paged_write")
-    _require_gpu(k, v)
-    if k.dtype != dt or v.dtype != dt or k.shape != v.shape or k.device != k_cache.device or v.device != k.device:
-        raise ValueError(f"paged_write: k and v must be [T, Hkv, D] of dtype {dt} on the cache's device")
-    if k.dim() != 3 or k.shape[1] != pool.Hkv:
-        raise ValueError(f"paged_write: k and v must be [T, {pool.Hkv}, {pool.D}]")
-    k, kt, kh = _token_rows(k, pool.D, "k")
-    v, vt, vh = _token_rows(v, pool.D, "v")
-    T = k.shape[0]
-    sl = _ints(slots, "slots", (T,), k.device)
+    lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
+    dev, dt, shape = lay.device, lay.dtype, k.shape
+    if k.dtype is not dt or v.dtype is not dt or k.device != dev or v.device != dev or len(shape) != 3 or \
+            v.shape != shape or shape[1] != lay.Hkv or shape[2] != lay.D:
+        raise ValueError(f"paged_write: k and v must be [T, {lay.Hkv}, {lay.D}] of dtype {dt} on the cache's device")
+    k, kt, kh = _token_rows(k)
+    v, vt, vh = _token_rows(v)
+    T = shape[0]
+    sl = _ints(slots, "slots", T, dev)
     if T:
-        _paged_call("kq_paged_write", k.device, ctypes.byref(pool), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, sl, T,
-                    _stream(k))
+        _paged_call("kq_paged_write", dev, pool, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, sl, T, _stream(k))
 
 
 def paged_read(k_cache, v_cache, slots, k_scales=None, k_biases=None, v_scales=None, v_biases=None):
@@ -1349,13 +1386,13 @@ def paged_read(k_cache, v_cache, slots, k_scales=None, k_biases=None, v_scales=N
     what paged_write stored there, an 8-bit cache's values as scale * q + bias
     in the scales' dtype; zeros for a slot outside the pool."""
     _fault("paged_read")
-    pool, dt = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases), "paged_read")
-    _require_gpu(slots)
-    T = slots.numel()
-    sl = _ints(slots, "slots", (T,), k_cache.device)
-    k, v = (torch.empty((T, pool.Hkv, pool.D), dtype=dt, device=k_cache.device) for _ in range(2))
+    lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
+    dev, T = lay.device, slots.numel()
+    sl = _ints(slots, "slots", T, dev)
+    k = torch.empty((T, lay.Hkv, lay.D), dtype=lay.dtype, device=dev)
+    v = torch.empty_like(k)
     if T:
-        _paged_call("kq_paged_read", k.device, ctypes.byref(pool), sl, T, k.data_ptr(), v.data_ptr(), _stream(k_cache))
+        _paged_call("kq_paged_read", dev, pool, sl, T, k.data_ptr(), v.data_ptr(), _stream(k))
     return k, v
 
 
@@ -1381,37 +1418,47 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     (no 96 in 8 bits), Hq / Hkv up to 64.  A row's result is bitwise that of a
     call on the row alone."""
     _fault("sdpa_paged")
-    pool, dt = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases), "sdpa_paged")
-    _require_gpu(q, kv_lens)
-    dev, B = k_cache.device, kv_lens.numel()
-    if q.dim() != 3 or q.shape[2] != pool.D or q.dtype != dt or q.device != dev or q.shape[1] % pool.Hkv or \
-            not 1 <= q.shape[1] // pool.Hkv <= 64:
-        raise ValueError(f"sdpa_paged: q must be [T, Hq, {pool.D}] of dtype {dt} on the cache's device, Hq a multiple "
-                         f"of Hkv={pool.Hkv} up to 64 times it")
-    T, Hq, D = q.shape
+    lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
+    dev, dt, Hkv, D, B, shape = lay.device, lay.dtype, lay.Hkv, lay.D, kv_lens.numel(), q.shape
+    if q.dtype is not dt or q.device != dev or len(shape) != 3 or shape[2] != D or shape[1] % Hkv or \
+            not 1 <= shape[1] // Hkv <= 64:
+        raise ValueError(f"sdpa_paged: q must be [T, Hq, {D}] of dtype {dt} on the cache's device, Hq a multiple of "
+                         f"Hkv={Hkv} up to 64 times it")
+    T, Hq, _ = shape
     tab, tab_stride, width = _block_table(block_table, B, dev)
-    lens, cu = _ints(kv_lens, "kv_lens", (B,), dev), _ints(cu_q, "cu_q", (B + 1,), dev)
+    lens, cu = _ints(kv_lens, "kv_lens", B, dev), _ints(cu_q, "cu_q", B + 1, dev)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=dt, device=dev)
-    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != dt or out.device != dev or \
-            out.stride(2) != 1 or out.stride(1) != D or (T > 1 and (out.stride(0) % 8 or out.stride(0) < Hq * D)) \
-            or out.data_ptr() % 16:
-        raise ValueError("sdpa_paged: out must be like q, its heads contiguous, 16-byte aligned")
+        out, ot = torch.empty((T, Hq, D), dtype=dt, device=dev), Hq * D
+    else:
+        if not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != dt or out.device != dev:
+            raise ValueError("sdpa_paged: out must be like q")
+        ot, oh, one = out.stride()
+        ot = ot if T > 1 else Hq * D
+        if one != 1 or (oh != D and Hq > 1) or ot % 8 or ot < Hq * D or out.data_ptr() % 16:
+            raise ValueError("sdpa_paged: out must have contiguous heads, a token stride in multiples of 8, and be "
+                             "16-byte aligned")
     if not T or not B:
         return out
-    if q.stride(1) != D or (T > 1 and q.stride(0) < Hq * D):
+    qt, qh, one = q.stride()
+    if one != 1 or (qh != D and Hq > 1) or (T > 1 and (qt % 8 or qt < Hq * D)) or q.data_ptr() % 16:
         q = q.contiguous()
-    q, qt, _ = _token_rows(q, D, "q")
+        if q.data_ptr() % 16:
+            q = q.clone()
+        qt = Hq * D
+    elif T == 1:
+        qt = Hq * D
     mq = T if max_q is None else min(int(max_q), T)
-    mkv = min(width * pool.page_size, (1 << 31) - 1)
+    mkv = min(width * lay.page_size, (1 << 31) - 1)
     if max_kv is not None:
         mkv = min(mkv, max(1, int(max_kv)) if max_kv >= 0 else -1)
     if mq < 1 or mkv < 1:
         raise ValueError("sdpa_paged: max_q must be positive and max_kv not negative")
-    need = lib().kq_sdpa_paged_workspace_bytes(T, B, Hq, pool.Hkv, D, mq, mkv, int(pool.k_scales is not None))
+    need = lib().kq_sdpa_paged_workspace_bytes(T, B, Hq, Hkv, D, mq, mkv, lay.q8)
     s = _stream(q)
-    ws = _WS.get("sdpa_paged", dev, s.value, need) if need else None
-    _paged_call("kq_sdpa_paged", dev, q.data_ptr(), qt, ctypes.byref(pool), tab, tab_stride, width, lens, cu, T, B, Hq,
-                mq, mkv, float(scale), out.data_ptr(), out.stride(0) if T > 1 else Hq * D,
-                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), s)
+    ws_ptr, ws_len = None, 0
+    if need:
+        ws = _WS.get("sdpa_paged", dev, s.value, need)
+        ws_ptr, ws_len = ws.data_ptr(), ws.numel()
+    _paged_call("kq_sdpa_paged", dev, q.data_ptr(), qt, pool, tab, tab_stride, width, lens, cu, T, B, Hq, mq, mkv,
+                float(scale), out.data_ptr(), ot, ws_ptr, ws_len, s)
     return out
