@@ -28,16 +28,20 @@ struct PagedArgs {
     // slots a token and query head, or 0: a row's slots follow those of the rows
     // before it (a chunk's tokens have fewer splits than a decode row's)
     int32_t slot_stride;
-    int32_t direct;    // the wave kernel's grid is (split, kv head, row)
+    int32_t direct;    // the wave kernel's grid is (split, kv head, row), the merge's (token and head, row)
 };
 
-constexpr int kFewColumns = 16;     // rows of at most so many columns take the wave kernel
+constexpr int kFewColumns = 16;     // rows of at most so many columns split as decode rows do
 constexpr int kSplitGroups = 512;   // workgroups that splitting a chunk aims at
 constexpr int kSplitTokens = 512;   // least keys of a chunk's split
 constexpr int kDirect = 1 << 15;    // waves, and merged tokens and heads, of a direct grid
 constexpr int kMergeGroups = 2048;  // workgroups of a merge that is not
 
 __host__ __device__ __forceinline__ bool few_columns(int n, int G) { return (int64_t)n * G <= kFewColumns; }
+
+// Whether such rows run a wave each (at head dim 512 a wave's tile, sums and query
+// spill: the chunks' kernel takes all rows there).
+constexpr bool has_waves(int D) { return D <= 256; }
 
 // Query columns of a chunk's workgroup: four waves of 32, or of 16 where 32
 // would take over 256 registers a lane for the sums and the queries.
@@ -74,10 +78,17 @@ __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     return r;
 }
 
-// Units of the chunk kernel (CHUNK) or of the wave kernel.
-template <bool CHUNK>
-__device__ __forceinline__ int row_units(const PagedArgs &a, const Row &r) {
-    return few_columns(r.n, a.G) == CHUNK ? 0 : r.blocks * r.splits * a.Hkv;
+// Units of the wave kernel, of the chunk kernel, and of the merge (four tokens
+// and query heads of a row that has splits).
+__device__ __forceinline__ int wave_units(const PagedArgs &a, const Row &r) {
+    return few_columns(r.n, a.G) ? r.blocks * r.splits * a.Hkv : 0;
+}
+template <int D>
+__device__ __forceinline__ int chunk_units(const PagedArgs &a, const Row &r) {
+    return has_waves(D) && few_columns(r.n, a.G) ? 0 : r.blocks * r.splits * a.Hkv;
+}
+__device__ __forceinline__ int merge_units(const PagedArgs &a, const Row &r) {
+    return r.splits > 1 ? (r.n * a.Hq + 3) / 4 : 0;
 }
 
 // (the host refuses calls whose unit or slot numbers pass 31 bits)
@@ -102,79 +113,60 @@ __device__ __forceinline__ int64_t slot_of(const PagedArgs &a, const Row &r, int
     return slot0 + (i * a.Hq + hq) * r.splits;
 }
 
-// The row that unit u belongs to, with u made its number within the row and
-// the row's first partial slot; false past the last unit.  The unit counts are
-// summed over the rows, 64 at a time, by every wave that asks.
-template <bool CHUNK>
-__device__ __forceinline__ bool find_unit(const PagedArgs &a, int &u, int &b, int &slot0) {
-    const int lane = kq_lane();
-    int slots = 0;
-    for (int c0 = 0; c0 < a.B; c0 += 64) {
-        const int row = c0 + lane;
-        int mu = 0, ms = 0;
-        if (row < a.B) {
-            const Row x = row_at(a, row);
-            mu = row_units<CHUNK>(a, x);
-            ms = row_slots(a, x);
-        }
-        const int iu = wave_scan(mu), is = wave_scan(ms);
-        const int total = __builtin_amdgcn_readlane(iu, 63);
-        if (u < total) {
-            const int src = __builtin_ctzll(__ballot(u < iu));
-            b = c0 + src;
-            u -= __builtin_amdgcn_readlane(iu - mu, src);
-            slot0 = slots + __builtin_amdgcn_readlane(is - ms, src);
-            return true;
-        }
-        u -= total;
-        slots += __builtin_amdgcn_readlane(is, 63);
-    }
-    return false;
-}
-
-// The same for the merge's units: four (token, query head) of a row that has
-// splits.
-__device__ __forceinline__ bool find_split_tokens(const PagedArgs &a, int &u, int &b, int &slot0) {
-    const int lane = kq_lane();
-    int slots = 0;
-    for (int c0 = 0; c0 < a.B; c0 += 64) {
-        const int row = c0 + lane;
-        int mu = 0, ms = 0;
-        if (row < a.B) {
-            const Row x = row_at(a, row);
-            mu = x.splits > 1 ? (x.n * a.Hq + 3) / 4 : 0;
-            ms = row_slots(a, x);
-        }
-        const int iu = wave_scan(mu), is = wave_scan(ms);
-        const int total = __builtin_amdgcn_readlane(iu, 63);
-        if (u < total) {
-            const int src = __builtin_ctzll(__ballot(u < iu));
-            b = c0 + src;
-            u -= __builtin_amdgcn_readlane(iu - mu, src);
-            slot0 = slots + __builtin_amdgcn_readlane(is - ms, src);
-            return true;
-        }
-        u -= total;
-        slots += __builtin_amdgcn_readlane(is, 63);
-    }
-    return false;
-}
-
-// The row again for one wave, in scalar registers.
-__device__ __forceinline__ Row uniform_row(const PagedArgs &a, int b) {
-    Row r = row_at(a, b);
-    r.q0 = __builtin_amdgcn_readfirstlane(r.q0);
-    r.n = __builtin_amdgcn_readfirstlane(r.n);
-    r.full = __builtin_amdgcn_readfirstlane(r.full);
-    r.kv = __builtin_amdgcn_readfirstlane(r.kv);
-    r.blocks = __builtin_amdgcn_readfirstlane(r.blocks);
-    r.splits = __builtin_amdgcn_readfirstlane(r.splits);
+// Row x of lane src, in scalar registers.
+__device__ __forceinline__ Row lane_row(const Row &x, int src) {
+    Row r;
+    r.q0 = __builtin_amdgcn_readlane(x.q0, src);
+    r.n = __builtin_amdgcn_readlane(x.n, src);
+    r.full = __builtin_amdgcn_readlane(x.full, src);
+    r.kv = __builtin_amdgcn_readlane(x.kv, src);
+    r.blocks = __builtin_amdgcn_readlane(x.blocks, src);
+    r.splits = __builtin_amdgcn_readlane(x.splits, src);
     return r;
+}
+
+// The row b that unit u belongs to, with u made its number within the row, and
+// the row's first partial slot; false past the last unit.  units(row) is summed
+// over the rows, 64 at a time, by every wave that asks.
+template <class Units>
+__device__ __forceinline__ bool find_unit(const PagedArgs &a, Units &&units, int &u, int &b, Row &row, int &slot0) {
+    const int lane = kq_lane();
+    int slots = 0;
+    for (int c0 = 0; c0 < a.B; c0 += 64) {
+        int mu = 0, ms = 0;
+        Row x{};
+        if (c0 + lane < a.B) {
+            x = row_at(a, c0 + lane);
+            mu = units(x);
+            ms = row_slots(a, x);
+        }
+        const int iu = wave_scan(mu), is = wave_scan(ms);
+        const int total = __builtin_amdgcn_readlane(iu, 63);
+        if (u < total) {
+            const int src = __builtin_ctzll(__ballot(u < iu));
+            b = c0 + src;
+            u -= __builtin_amdgcn_readlane(iu - mu, src);
+            slot0 = slots + __builtin_amdgcn_readlane(is - ms, src);
+            row = lane_row(x, src);
+            return true;
+        }
+        u -= total;
+        slots += __builtin_amdgcn_readlane(is, 63);
+    }
+    return false;
 }
 
 // 64 entries of a block table row in a register; at(p) takes rising p.
 struct PageIds {
     int first, ids;
+
+    // Whether entries p .. last all are pages of the pool; loads the first 64.
+    __device__ __forceinline__ bool start(const PagedArgs &a, const int32_t *tab, int p, int last) {
+        load(tab, p, last);
+        bool bad = (uint32_t)ids >= (uint32_t)a.n_pages;
+        for (int i = p + 64 + kq_lane(); i <= last; i += 64) bad |= (uint32_t)tab[i] >= (uint32_t)a.n_pages;
+        return __builtin_amdgcn_ballot_w64(bad) == 0;
+    }
 
     __device__ __forceinline__ void load(const int32_t *tab, int p, int last) {
         first = p;
@@ -188,13 +180,6 @@ struct PageIds {
         return __builtin_amdgcn_readlane(ids, p - first);
     }
 };
-
-// Whether a block table row's entries [p, last] all are pages of the pool.
-__device__ __forceinline__ bool pages_in_pool(const PagedArgs &a, const int32_t *tab, int p, int last) {
-    bool bad = false;
-    for (int i = p + kq_lane(); i <= last; i += 64) bad |= (uint32_t)tab[i] >= (uint32_t)a.n_pages;
-    return __builtin_amdgcn_ballot_w64(bad) == 0;
-}
 
 // 16-bit values whose exponent is all ones (infinities and NaN) as 0 in a
 // masked tile: there the product of a hidden key's value with its probability
@@ -224,10 +209,10 @@ constexpr float shift() { return BF ? 0.f : Q8 ? 6.f : 10.f; }
 
 template <int D>
 struct Geo {
-    static constexpr int TT = D > 256 ? 16 : 32;  // tokens a tile
-    static constexpr int CH = TT / 16;            // 16-token chunks
-    static constexpr int VT = TT / 4;             // V rows a lane
-    static constexpr int NC = D / 32;             // 32-wide pieces of the head dim
+    static constexpr int TT = 32;       // tokens a tile
+    static constexpr int CH = TT / 16;  // 16-token chunks
+    static constexpr int VT = TT / 4;   // V rows a lane
+    static constexpr int NC = D / 32;   // 32-wide pieces of the head dim
 };
 
 // Where a tile's chunks start in the pool (elements or bytes; uniform), and
@@ -247,21 +232,20 @@ struct Tile16 {
 
     __device__ __forceinline__ void load(const PagedArgs &a, const TileAt<D> &at) {
         const int lane = kq_lane(), r = lane & 15, g = lane >> 4;
-        const uint32_t ko = (uint32_t)(r * a.tok_stride + 8 * g);
+        // uniform bases and 32-bit byte offsets of the lanes
+        const uint32_t ko = 2u * (uint32_t)(r * a.tok_stride + 8 * g), vo = 2u * (uint32_t)(4 * g * a.tok_stride);
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch) {
-            const uint16_t *kp = (const uint16_t *)a.k + at.off[ch];
+            const uint8_t *kp = (const uint8_t *)a.k + 2 * at.off[ch];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) k[ch][c] = *(const u32x4 *)(kp + (ko + 32 * c));
+            for (int c = 0; c < NC; ++c) k[ch][c] = *(const u32x4 *)(kp + 64 * c + ko);
         }
 #pragma unroll
-        for (int dg = 0; dg < NG; ++dg) {
-            const uint32_t d0 = min(128 * dg + 8 * r, D - 8);
+        for (int i = 0; i < VT; ++i) {
+            const uint8_t *vp = (const uint8_t *)a.v + 2 * (at.off[i >> 2] + (i & 3) * a.tok_stride);
 #pragma unroll
-            for (int i = 0; i < VT; ++i) {
-                const uint16_t *vp = (const uint16_t *)a.v + at.off[i >> 2];
-                v[dg][i] = *(const u32x4 *)(vp + ((uint32_t)((4 * g + (i & 3)) * a.tok_stride) + d0));
-            }
+            for (int dg = 0; dg < NG; ++dg)
+                v[dg][i] = *(const u32x4 *)(vp + 256 * dg + (vo + 2u * (uint32_t)min(8 * r, D - 8 - 128 * dg)));
         }
     }
 };
@@ -331,7 +315,7 @@ struct Tile8 {
             const uint8_t *kp = (const uint8_t *)a.k + at.off[ch];
 #pragma unroll
             for (int i = 0; i < NC / 2; ++i) {
-                const u32x4 w = *(const u32x4 *)(kp + (uint32_t)(r * D + 64 * i + 16 * g));
+                const u32x4 w = *(const u32x4 *)(kp + 64 * i + (uint32_t)(r * D + 16 * g));
                 k[ch][2 * i] = u32x2{w.x, w.y};
                 k[ch][2 * i + 1] = u32x2{w.z, w.w};
             }
@@ -349,8 +333,8 @@ struct Tile8 {
         for (int grp = 0; grp < SG; ++grp)
 #pragma unroll
             for (int i = 0; i < VT; ++i)
-                v[grp][i] = *(const uint32_t *)((const uint8_t *)a.v + at.off[i >> 2] +
-                                                (uint32_t)((4 * g + (i & 3)) * D + 64 * grp + 4 * r));
+                v[grp][i] = *(const uint32_t *)((const uint8_t *)a.v + at.off[i >> 2] + ((i & 3) * D + 64 * grp) +
+                                                (uint32_t)(4 * g * D + 4 * r));
     }
 };
 
@@ -411,7 +395,7 @@ struct State {
     __device__ __forceinline__ void tile(const Tile &t, float scale_log2, uint32_t vis, uint32_t &odd) {
         float s[8];
         scores(t, scale_log2, s);
-        constexpr int N = 4 * CH;
+        constexpr int N = 8;
         if constexpr (MASK) {
 #pragma unroll
             for (int j = 0; j < N; ++j) s[j] = (vis >> j) & 1 ? s[j] : -INFINITY;
@@ -427,7 +411,7 @@ struct State {
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
         float p[8], psum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = j < N ? __builtin_amdgcn_exp2f(s[j] - (m_use - shift<BF, Q8>())) : 0.f;
+        for (int j = 0; j < N; ++j) p[j] = __builtin_amdgcn_exp2f(s[j] - (m_use - shift<BF, Q8>()));
 #pragma unroll
         for (int j = 0; j < N; ++j) psum += p[j];
         l_part = l_part * alpha + psum;
@@ -446,10 +430,6 @@ struct State {
                 float ps[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (j >= N) {
-                        ps[j] = 0.f;
-                        continue;
-                    }
                     const float sc = t.of(t.vs[j >> 2][j & 3], grp), bi = t.of(t.vb[j >> 2][j & 3], grp);
                     // (a hidden key's scale and bias may be anything)
                     const bool on = !MASK || ((vis >> j) & 1);
@@ -461,7 +441,7 @@ struct State {
                 // byte j of tokens 0 .. 7 as one operand
                 uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = i < Tile::VT ? t.v[grp][i] : 0x80808080u;
+                for (int i = 0; i < 8; ++i) w[i] = t.v[grp][i];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     // (b0 b1 of two tokens) -> two words of one byte each of four tokens
@@ -490,7 +470,7 @@ struct State {
             u32x4 vr[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                vr[i] = i < Tile::VT ? t.v[dg][i] : u32x4{0u, 0u, 0u, 0u};
+                vr[i] = t.v[dg][i];
                 if constexpr (MASK) {
 #pragma unroll
                     for (int w = 0; w < 4; ++w) vr[i][w] = finite2<BF>(vr[i][w], odd);
@@ -514,39 +494,39 @@ struct State {
     __device__ __forceinline__ void add_odd(const uint16_t *v, bool sees) {
         const int g = kq_lane() >> 4;
 #pragma unroll
-        for (int j = 0; j < NO; ++j)
+        for (int j = 0; j < NO; ++j) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int d = 128 * (j >> 3) + 8 * (4 * g + e) + (j & 7);
-                const float x = d < D ? odd_part<BF>(v[d]) : 0.f;
-                if (sees) o[j][e] += x;
+                // (results past D are not stored)
+                const float x = odd_part<BF>(v[min(128 * (j >> 3) + 8 * (4 * g + e) + (j & 7), D - 1)]);
+                o[j][e] += sees ? x : 0.f;
             }
+            __builtin_amdgcn_sched_barrier(0);  // (few loads at a time: registers)
+        }
     }
 };
 
-// One wave a workgroup; unit = (row, 16-column block, split, kv head), the kv
-// heads fastest (with eight of them, one per XCD: the blocks of a head share
-// their keys in that XCD's L2).
-template <int D, bool BF, bool Q8>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void kq_paged_split_kernel(
-    PagedArgs a) {
+// Rows of few columns: one wave a unit = (row, split, kv head), the kv heads
+// fastest.  The wave takes the units `first`, `first` + `step`, ..., or with
+// DIRECT the one of its place in the grid.
+template <int D, bool BF, bool Q8, bool DIRECT>
+__device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int step) {
     using Tile = std::conditional_t<Q8, Tile8<D, BF>, Tile16<D, BF>>;
     constexpr int TT = Geo<D>::TT, CH = Geo<D>::CH, NC = Geo<D>::NC;
     constexpr int NBUF = D >= 256 ? 1 : 2;
     const int lane = kq_lane(), r = lane & 15, g = lane >> 4;
-    for (int unit = blockIdx.x;; unit += gridDim.x) {
+    for (int unit = first;; unit += step) {
         int b, h, s, slot0 = 0;
         Row row;
-        if (a.direct) {
+        if constexpr (DIRECT) {
             s = unit;
             h = blockIdx.y;
             b = blockIdx.z;
-            row = uniform_row(a, b);
+            row = lane_row(row_at(a, b), 0);
             if (!few_columns(row.n, a.G) || row.n == 0 || s >= row.splits) return;
         } else {
             int u = unit;
-            if (!find_unit<false>(a, u, b, slot0)) return;
-            row = uniform_row(a, b);
+            if (!find_unit(a, [&](const Row &x) { return wave_units(a, x); }, u, b, row, slot0)) return;
             s = u / a.Hkv;
             h = u - s * a.Hkv;
         }
@@ -590,9 +570,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
             const int32_t *tab = a.table + (int64_t)b * a.table_stride;
             const int sh = a.lps - 4;  // log2 of a page's chunks
             const int c_last = (t_end - 1) >> 4, p_last = c_last >> sh;
-            const int p_first = (t_begin >> 4) >> sh;
             PageIds ids;
-            ids.load(tab, p_first, p_last);
+            const bool all_ok = ids.start(a, tab, (t_begin >> 4) >> sh, p_last);
             const int64_t h_off = (int64_t)h * a.head_stride;
             auto at_tile = [&](int t0) {
                 TileAt<D> x;
@@ -613,7 +592,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
             // others (the last keys; all, where the table names no page) one
             // by one before them, so that their code is there once.
             int whole = min(least, t_end);
-            whole = whole <= t_begin || !pages_in_pool(a, tab, p_first, p_last) ? t_begin : whole - (whole - t_begin) % TT;
+            whole = whole <= t_begin || !all_ok ? t_begin : whole - (whole - t_begin) % TT;
             Tile ring[NBUF];
 #pragma unroll 1
             for (int t = whole; t < t_end; t += TT) {
@@ -629,7 +608,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
                     if (__builtin_amdgcn_ballot_w64(odd != 0)) {
 #pragma unroll 1
                         for (int k = 0; k < TT; ++k)
-                            st.add_odd((const uint16_t *)a.v + at.off[CH == 1 || k < 16 ? 0 : CH - 1] + (k & 15) * a.tok_stride,
+                            st.add_odd((const uint16_t *)a.v + (k < 16 ? at.off[0] : at.off[1]) + (k & 15) * a.tok_stride,
                                        ((at.ok >> (k >> 4)) & 1) && t + k < lim);
                     }
                 }
@@ -694,6 +673,12 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
             a.ml[2 * slot + 1] = l;
         }
     }
+}
+
+template <int D, bool BF, bool Q8, bool DIRECT>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void kq_paged_wave_kernel(
+    PagedArgs a) {
+    wave_work<D, BF, Q8, DIRECT>(a, blockIdx.x, gridDim.x);
 }
 
 // ---- prompt chunks --------------------------------------------------------
@@ -995,20 +980,19 @@ struct ChunkState16 {
 };
 
 template <int D, bool BF, bool Q8>
-__global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_paged_chunk_kernel(PagedArgs a) {
+__device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, int first, int step) {
     using C = Chunk<D, Q8>;
     using State = std::conditional_t<(D > 128), ChunkState16<D, BF, Q8>, ChunkState<D, BF, Q8>>;
     constexpr int COLS = State::COLS;
     static_assert(4 * COLS == group_columns(D), "columns of a workgroup");
-    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const uint32_t lds = (uint32_t)(uintptr_t)(LDSP(void))smem;
     const auto odd_flag = (volatile LDSP(int))(uintptr_t)(lds + C::kLds);
     const int lane = kq_lane(), c = lane & (COLS - 1);
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    for (int unit = blockIdx.x;; unit += gridDim.x) {
+    for (int unit = first;; unit += step) {
         int u = unit, b, slot0;
-        if (!find_unit<true>(a, u, b, slot0)) return;
-        const Row row = uniform_row(a, b);
+        Row row;
+        if (!find_unit(a, [&](const Row &x) { return chunk_units<D>(a, x); }, u, b, row, slot0)) return;
         const int rest = u / a.Hkv, kvh = u - rest * a.Hkv;
         // the tiles with the most keys first
         const int back = rest / row.splits, s = rest - back * row.splits, blk = row.blocks - 1 - back;
@@ -1024,7 +1008,8 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
         const int most = __builtin_amdgcn_readfirstlane(col0 < cols ? min(seen_by(col0 + COLS - 1), row.kv) : 0);
         const int least_all = __builtin_amdgcn_readfirstlane(seen_by(blk * 4 * COLS));
         const int most_all = __builtin_amdgcn_readfirstlane(min(seen_by((blk + 1) * 4 * COLS - 1), row.kv));
-        const int per = ((row.kv + row.splits - 1) / row.splits + C::BN - 1) / C::BN * C::BN;
+        const int per = few_columns(row.n, a.G) ? a.rule.tokens(row.kv)
+                                                : ((row.kv + row.splits - 1) / row.splits + C::BN - 1) / C::BN * C::BN;
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
         const int t_end = __builtin_amdgcn_readfirstlane(min(most_all, t_begin + per));
 
@@ -1045,8 +1030,7 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
             const int sh = a.lps - 4;
             const int c_last = (t_end - 1) >> 4, p_last = c_last >> sh;
             PageIds ids;
-            ids.load(tab, (t_begin >> 4) >> sh, p_last);
-            const bool all_ok = pages_in_pool(a, tab, (t_begin >> 4) >> sh, p_last);
+            const bool all_ok = ids.start(a, tab, (t_begin >> 4) >> sh, p_last);
             const int64_t h_off = (int64_t)kvh * a.head_stride;
             // Piece y of this wave's 16-token pieces of the tile at t0, every
             // other one of K (even waves) or V (odd waves): where it starts in
@@ -1168,6 +1152,7 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
                             for (int e = 0; e < 4; ++e) y[e] = t < lim ? odd_part<BF>(((const uint16_t *)a.v)[at + e]) : 0.f;
                         }
                         st.add(k, y);
+                        __builtin_amdgcn_sched_barrier(0);  // (few loads at a time: registers)
                     }
                 }
             };
@@ -1227,6 +1212,27 @@ __global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_p
             a.ml[2 * slot + 1] = l;
         }
     }
+}
+
+// Whether rows of few columns run beside chunks in one launch (past head dim 128
+// their tiles take more registers than two waves a SIMD can have).
+template <int D>
+constexpr bool kBeside = D <= 128;
+
+// The first `wave_groups` workgroups take rows of few columns, a wave a unit, the
+// others chunks: decode rows, which wait for memory, run beside a prompt
+// chunk's products.
+template <int D, bool BF, bool Q8>
+__global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_paged_kernel(PagedArgs a, int wave_groups) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    if constexpr (kBeside<D>) {
+        if ((int)blockIdx.x < wave_groups) {
+            const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+            wave_work<D, BF, Q8, false>(a, (int)(4 * blockIdx.x) + w, 4 * wave_groups);
+            return;
+        }
+    }
+    chunk_work<D, BF, Q8>(a, smem, (int)blockIdx.x - wave_groups, (int)gridDim.x - wave_groups);
 }
 
 // Scale of a split of maximum ms beside the common maximum m; a split without
@@ -1369,7 +1375,7 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
         return slot_of(a, r, slot0, i, x - i * a.Hq);
     };
     if (a.direct) {
-        const Row row = uniform_row(a, blockIdx.y);
+        const Row row = lane_row(row_at(a, blockIdx.y), 0);
         const int x = blockIdx.x;
         if (row.splits > 1 && x < row.n * a.Hq) merge_group<D, BF>(a, slot(row, 0, x), row.splits, out(row, x));
         return;
@@ -1377,8 +1383,8 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     for (int item = blockIdx.x;; item += gridDim.x) {
         int u = item, b, slot0;
-        if (!find_split_tokens(a, u, b, slot0)) return;
-        const Row row = uniform_row(a, b);
+        Row row;
+        if (!find_unit(a, [&](const Row &x) { return merge_units(a, x); }, u, b, row, slot0)) return;
         const int end = min(4 * u + 4, row.n * a.Hq);
         if (row.splits <= 64) {
             if (4 * u + w < end) merge_wave<D, BF>(a, slot(row, slot0, 4 * u + w), row.splits, out(row, 4 * u + w));
@@ -1389,8 +1395,9 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
 }
 
 struct Grid {
-    dim3 waves, merge;
-    int groups;  // (x == 0, 0: not launched)
+    dim3 waves, merge;   // x == 0: not launched
+    int groups;          // workgroups of chunks (0: none)
+    int wave_groups;     // and of rows of few columns beside them
 };
 
 template <int D, bool BF, bool Q8>
@@ -1398,13 +1405,18 @@ int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
     if (g.groups) {
         constexpr int lds = Chunk<D, Q8>::kLds + 16;  // (and a flag)
         static_assert(lds <= 160 << 10, "LDS of a CU");
-        static const bool ok = lds <= (64 << 10) || hipFuncSetAttribute((const void *)kq_paged_chunk_kernel<D, BF, Q8>,
-                                                                        hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                                        lds) == hipSuccess;
+        static const bool ok = hipFuncSetAttribute((const void *)kq_paged_kernel<D, BF, Q8>,
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
         if (!ok) return KQ_ERR_LAUNCH_FAILED;
-        hipLaunchKernelGGL((kq_paged_chunk_kernel<D, BF, Q8>), dim3(g.groups), dim3(256), lds, s, a);
+        const int beside = kBeside<D> ? g.wave_groups : 0;
+        hipLaunchKernelGGL((kq_paged_kernel<D, BF, Q8>), dim3(beside + g.groups), dim3(256), lds, s, a, beside);
     }
-    if (g.waves.x) hipLaunchKernelGGL((kq_paged_split_kernel<D, BF, Q8>), g.waves, dim3(64), 0, s, a);
+    if constexpr (has_waves(D)) {
+        if (g.waves.x && !(kBeside<D> && g.groups)) {
+            if (a.direct) hipLaunchKernelGGL((kq_paged_wave_kernel<D, BF, Q8, true>), g.waves, dim3(64), 0, s, a);
+            else hipLaunchKernelGGL((kq_paged_wave_kernel<D, BF, Q8, false>), g.waves, dim3(64), 0, s, a);
+        }
+    }
     if (g.merge.x) hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF>), g.merge, dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? KQ_OK : KQ_ERR_LAUNCH_FAILED;
 }
@@ -1535,12 +1547,17 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     a.direct = (plan.slot_stride || !plan.slots) && B < (1 << 16) && Hkv < (1 << 16) && waves <= kDirect &&
                items * B <= kDirect;
     g.waves = g.merge = dim3(0);
-    if (a.G <= kFewColumns) {
+    const int64_t many = (((int64_t)T * a.G + a.group_cols - 1) / a.group_cols + rows) * Hkv *
+                         (has_waves(D) ? plan.many : most);
+    g.groups = has_waves(D) && few_columns(max_q, a.G) ? 0 : (int)(many < (1 << 14) ? many : (1 << 14));
+    g.wave_groups = 0;
+    if (has_waves(D) && a.G <= kFewColumns) {
         const int64_t n = rows * Hkv * plan.few;
-        g.waves = a.direct ? dim3(plan.few, Hkv, B) : dim3((unsigned)(n < (1 << 16) ? n : (1 << 16)));
+        if (a.direct) g.waves = dim3(plan.few, Hkv, B);
+        else g.waves = dim3((unsigned)(n < (1 << 16) ? n : (1 << 16)));
+        // (a row that is a chunk leaves no more than the other tokens to these)
+        if (g.groups) g.wave_groups = (int)((n < (1 << 13) ? n : (1 << 13)) + 3) / 4;
     }
-    const int64_t many = (((int64_t)T * a.G + a.group_cols - 1) / a.group_cols + rows) * Hkv * plan.many;
-    g.groups = few_columns(max_q, a.G) ? 0 : (int)(many < (1 << 14) ? many : (1 << 14));
     if (plan.slots) {
         const int64_t n = (int64_t)T * Hq / 4 + B;
         g.merge = a.direct ? dim3((unsigned)items, B) : dim3((unsigned)(n < kMergeGroups ? n : kMergeGroups));
