@@ -35,7 +35,7 @@ constexpr int kFewColumns = 16;     // rows of at most so many columns split as 
 constexpr int kSplitGroups = 512;   // workgroups that splitting a chunk aims at
 constexpr int kSplitTokens = 512;   // least keys of a chunk's split
 constexpr int kDirect = 1 << 15;    // waves, and merged tokens and heads, of a direct grid
-constexpr int kMergeGroups = 2048;  // workgroups of a merge that is not
+constexpr int kMergeGroups = 1024;  // workgroups of a merge that is not
 
 __host__ __device__ __forceinline__ bool few_columns(int n, int G) { return (int64_t)n * G <= kFewColumns; }
 
@@ -78,8 +78,8 @@ __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     return r;
 }
 
-// Units of the wave kernel, of the chunk kernel, and of the merge (four tokens
-// and query heads of a row that has splits).
+// Units of the wave kernel, of the chunk kernel, and of the merge (merge_items
+// tokens and query heads of a row that has splits).
 __device__ __forceinline__ int wave_units(const PagedArgs &a, const Row &r) {
     return few_columns(r.n, a.G) ? r.blocks * r.splits * a.Hkv : 0;
 }
@@ -87,8 +87,13 @@ template <int D>
 __device__ __forceinline__ int chunk_units(const PagedArgs &a, const Row &r) {
     return has_waves(D) && few_columns(r.n, a.G) ? 0 : r.blocks * r.splits * a.Hkv;
 }
+// A workgroup's share of a merge: one item where all its threads add up the splits,
+// one a wave where a wave takes several rounds of loads for them, four a wave,
+// loaded ahead, where it takes one.
+__device__ __forceinline__ int merge_items(int splits) { return splits > 64 ? 1 : splits > 8 ? 4 : 16; }
 __device__ __forceinline__ int merge_units(const PagedArgs &a, const Row &r) {
-    return r.splits > 1 ? (r.n * a.Hq + 3) / 4 : 0;
+    const int items = merge_items(r.splits);
+    return r.splits > 1 ? (r.n * a.Hq + items - 1) / items : 0;
 }
 
 // (the host refuses calls whose unit or slot numbers pass 31 bits)
@@ -105,6 +110,22 @@ __device__ __forceinline__ int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
     return v;
+}
+
+// Largest over the wave's lanes, in scalar registers.
+__device__ __forceinline__ float wave_max(float v) {
+    const auto step = [&](auto ctrl, auto rows) {
+        const int low = __builtin_bit_cast(int, -INFINITY);
+        v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(low, __builtin_bit_cast(int, v), ctrl.value,
+                                                                          rows.value, 0xf, false)));
+    };
+    step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr:1, 2, 4, 8
+    step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15, 31
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // Partial slot of split 0 of token i (of the row), query head hq.
@@ -1267,7 +1288,7 @@ __device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, in
         l_pre[k] = ml[2 * s + 1];
         o_pre[k] = po[(int64_t)s * Q];
     }
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    m = wave_max(m);
     __syncthreads();  // the last item's reads
     if ((t & 63) == 0) red_m[t >> 6] = m;
     __syncthreads();
@@ -1287,7 +1308,7 @@ __device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, in
 #pragma unroll
         for (int k = 0; k < PRE; ++k)
             if (part + k * P < n) add(m_pre[k], l_pre[k], o_pre[k]);
-#pragma unroll 4
+#pragma unroll 8
         for (int s = part + PRE * P; s < n; s += P) add(ml[2 * s], ml[2 * s + 1], po[(int64_t)s * Q]);
         red_acc[part][q] = acc;
         if (q == 0) red_l[part] = l;
@@ -1310,61 +1331,74 @@ __device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, in
     }
 }
 
-// The same by one wave, for at most 64 splits (lane s holds split s's maximum and
-// sum), in the same order of sums.
+// The same by one wave, for at most 64 splits, in the same order of sums: lane s
+// holds split s's maximum and sum; the first P splits' sums are loaded beside
+// them, and before the item ahead of this one is finished.
 template <int D, bool BF>
-__device__ __forceinline__ void merge_wave(const PagedArgs &a, int64_t slot, int n, uint16_t *out) {
-    constexpr int P = 256 / (D / 4), V = D > 128 ? 4 : 2, R = D > 256 ? 2 : 1;  // R runs of V values a lane
+struct WaveMerge {
+    static constexpr int P = 256 / (D / 4), V = D > 128 ? 4 : 2, R = D > 256 ? 2 : 1;  // R runs of V values a lane
     typedef float vec __attribute__((ext_vector_type(V)));
-    const int lane = kq_lane();
-    const float ms = lane < n ? a.ml[2 * (slot + lane)] : -INFINITY, ls = lane < n ? a.ml[2 * (slot + lane) + 1] : 0.f;
-    float m = ms;
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-    const float f = split_scale(ms, m);
-    const auto lane_of = [](float v, int s) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), s));
-    };
+    float ms, ls;
+    vec o[R][P];
+
+    __device__ __forceinline__ void load(const PagedArgs &a, int64_t slot, int r, int s0, int n) {
+        const float *p = a.part + slot * D + min((r * 64 + kq_lane()) * V, D - V);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int d = (r * 64 + lane) * V;
-        const float *p = a.part + slot * D + min(d, D - V);
-        vec acc[P];
-        float l[P];
+        for (int k = 0; k < P; ++k)
+            if (s0 + k < n) o[r][k] = *(const vec *)(p + (int64_t)(s0 + k) * D);
+    }
+    __device__ __forceinline__ void start(const PagedArgs &a, int64_t slot, int n) {
+        const int lane = kq_lane();
+        ms = lane < n ? a.ml[2 * (slot + lane)] : -INFINITY;
+        ls = lane < n ? a.ml[2 * (slot + lane) + 1] : 0.f;
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
-            acc[k] = vec(0.f);
-            l[k] = 0.f;
-        }
-        for (int s0 = 0; s0 < n; s0 += P) {
-            vec o[P];
+        for (int r = 0; r < R; ++r) load(a, slot, r, 0, n);
+    }
+    __device__ __forceinline__ void finish(const PagedArgs &a, int64_t slot, int n, uint16_t *out) {
+        const float f = split_scale(ms, wave_max(ms));
+        const auto lane_of = [](float v, int s) {
+            return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), s));
+        };
 #pragma unroll
-            for (int k = 0; k < P; ++k) o[k] = *(const vec *)(p + (int64_t)min(s0 + k, n - 1) * D);
+        for (int r = 0; r < R; ++r) {
+            vec acc[P];
+            float l[P];
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                if (s0 + k >= n) break;
-                const float fs = lane_of(f, s0 + k), lk = lane_of(ls, s0 + k);
-                if (fs == 0.f && lk == lk) continue;
-                l[k] += fs * lk;
+                acc[k] = vec(0.f);
+                l[k] = 0.f;
+            }
+            for (int s0 = 0; s0 < n; s0 += P) {
+                if (s0 > 0) load(a, slot, r, s0, n);
 #pragma unroll
-                for (int x = 0; x < V; ++x) acc[k][x] += fs * o[k][x];
+                for (int k = 0; k < P; ++k) {
+                    if (s0 + k >= n) break;
+                    const float fs = lane_of(f, s0 + k), lk = lane_of(ls, s0 + k);
+                    if (fs == 0.f && lk == lk) continue;
+                    l[k] += fs * lk;
+#pragma unroll
+                    for (int x = 0; x < V; ++x) acc[k][x] += fs * o[r][k][x];
+                }
+            }
+#pragma unroll
+            for (int k = 1; k < P; ++k) {
+                acc[0] = acc[0] + acc[k];
+                l[0] += l[k];
+            }
+            const float inv = l[0] > 0.f || l[0] != l[0] ? 1.f / l[0] : 0.f;
+            const int d = (r * 64 + kq_lane()) * V;
+            if (d < D) {
+#pragma unroll
+                for (int x = 0; x < V; x += 2)
+                    *(uint32_t *)(out + d + x) = pack2<BF>(acc[0][x] * inv, acc[0][x + 1] * inv);
             }
         }
-#pragma unroll
-        for (int k = 1; k < P; ++k) {
-            acc[0] = acc[0] + acc[k];
-            l[0] += l[k];
-        }
-        const float inv = l[0] > 0.f || l[0] != l[0] ? 1.f / l[0] : 0.f;
-        if (d < D) {
-#pragma unroll
-            for (int x = 0; x < V; x += 2) *(uint32_t *)(out + d + x) = pack2<BF>(acc[0][x] * inv, acc[0][x + 1] * inv);
-        }
     }
-}
+};
 
-// Workgroups take a token and query head each (direct), or four of a row's at a
-// time: a wave each where the row has at most 64 splits.
-template <int D, bool BF>
+// Workgroups take a token and query head each (direct), or merge_items of a
+// row's at a time.
+template <int D, bool BF, bool DIRECT>
 __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
     const auto out = [&](const Row &r, int x) {
         const int i = x / a.Hq;
@@ -1374,7 +1408,7 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
         const int i = x / a.Hq;
         return slot_of(a, r, slot0, i, x - i * a.Hq);
     };
-    if (a.direct) {
+    if constexpr (DIRECT) {
         const Row row = lane_row(row_at(a, blockIdx.y), 0);
         const int x = blockIdx.x;
         if (row.splits > 1 && x < row.n * a.Hq) merge_group<D, BF>(a, slot(row, 0, x), row.splits, out(row, x));
@@ -1385,11 +1419,19 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
         int u = item, b, slot0;
         Row row;
         if (!find_unit(a, [&](const Row &x) { return merge_units(a, x); }, u, b, row, slot0)) return;
-        const int end = min(4 * u + 4, row.n * a.Hq);
-        if (row.splits <= 64) {
-            if (4 * u + w < end) merge_wave<D, BF>(a, slot(row, slot0, 4 * u + w), row.splits, out(row, 4 * u + w));
+        const int n = row.splits, items = merge_items(n), end = min((u + 1) * items, row.n * a.Hq);
+        if (n <= 64) {
+            int x = u * items + w;
+            if (x >= end) continue;
+            WaveMerge<D, BF> now, next;
+            now.start(a, slot(row, slot0, x), n);
+            for (; x < end; x += 4) {
+                if (x + 4 < end) next.start(a, slot(row, slot0, x + 4), n);
+                now.finish(a, slot(row, slot0, x), n, out(row, x));
+                now = next;
+            }
         } else {
-            for (int x = 4 * u; x < end; ++x) merge_group<D, BF>(a, slot(row, slot0, x), row.splits, out(row, x));
+            merge_group<D, BF>(a, slot(row, slot0, u), n, out(row, u));
         }
     }
 }
@@ -1417,7 +1459,10 @@ int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
             else hipLaunchKernelGGL((kq_paged_wave_kernel<D, BF, Q8, false>), g.waves, dim3(64), 0, s, a);
         }
     }
-    if (g.merge.x) hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF>), g.merge, dim3(256), 0, s, a);
+    if (g.merge.x) {
+        if (a.direct) hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF, true>), g.merge, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF, false>), g.merge, dim3(256), 0, s, a);
+    }
     return hipGetLastError() == hipSuccess ? KQ_OK : KQ_ERR_LAUNCH_FAILED;
 }
 
@@ -1559,7 +1604,7 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
         if (g.groups) g.wave_groups = (int)((n < (1 << 13) ? n : (1 << 13)) + 3) / 4;
     }
     if (plan.slots) {
-        const int64_t n = (int64_t)T * Hq / 4 + B;
+        const int64_t n = plan.few > 8 || plan.many > 8 ? items * B : (int64_t)T * Hq / 16 + B;
         g.merge = a.direct ? dim3((unsigned)items, B) : dim3((unsigned)(n < kMergeGroups ? n : kMergeGroups));
     }
     const bool q8 = a.ks != nullptr, bf = pool->dtype == KQ_DTYPE_BF16;
