@@ -21,7 +21,7 @@ struct PagedArgs {
     int64_t q_stride, out_stride, page_stride, head_stride, table_stride;
     int32_t tok_stride, lps, n_pages, width;
     int32_t T, B, Hq, Hkv, G, max_q, max_kv;
-    int32_t group_cols;  // query columns of a chunk's workgroup
+    int32_t group_cols, group_slots;
     float scale_log2;
     float *part, *ml;  // split partials: [slot][D] sums, [slot][2] (maximum, sum)
     SplitRule rule;    // rows of few columns
@@ -32,7 +32,6 @@ struct PagedArgs {
 };
 
 constexpr int kFewColumns = 16;     // rows of at most so many columns split as decode rows do
-constexpr int kSplitGroups = 512;   // workgroups that splitting a chunk aims at
 constexpr int kSplitTokens = 512;   // least keys of a chunk's split
 constexpr int kDirect = 1 << 15;    // waves, and merged tokens and heads, of a direct grid
 constexpr int kMergeGroups = 1024;  // workgroups of a merge that is not
@@ -43,9 +42,12 @@ __host__ __device__ __forceinline__ bool few_columns(int n, int G) { return (int
 // spill: the chunks' kernel takes all rows there).
 constexpr bool has_waves(int D) { return D <= 256; }
 
-// Query columns of a chunk's workgroup: four waves of 32, or of 16 where 32
-// would take over 256 registers a lane for the sums and the queries.
-constexpr int group_columns(int D) { return D > 128 ? 64 : 128; }
+// A chunk's workgroup: its waves, query columns (32 a wave, 16 where 32 would take
+// over 256 registers a lane for the sums and the queries), and how many such
+// workgroups the GPU holds at once, which splitting a chunk aims at.
+constexpr int chunk_waves(int D, bool q8) { return q8 && (D == 128 || D == 256) ? 8 : 4; }
+constexpr int group_columns(int D, bool q8) { return chunk_waves(D, q8) * (D > 128 ? 16 : 32); }
+constexpr int group_slots(int D, bool q8) { return D > 256 || chunk_waves(D, q8) > 4 ? 256 : 512; }
 
 // Workgroups (waves, rows of few columns) of an unsplit row over one kv head.
 __host__ __device__ __forceinline__ int row_blocks(int n, int G, int group_cols) {
@@ -54,10 +56,11 @@ __host__ __device__ __forceinline__ int row_blocks(int n, int G, int group_cols)
 
 // Splits of a row of n tokens and kv keys: from the row and the head counts
 // alone, so that a row of a batch has the bits of the row alone.
-__host__ __device__ __forceinline__ int paged_splits(const SplitRule &rule, int n, int kv, int G, int Hkv, int group_cols) {
+__host__ __device__ __forceinline__ int paged_splits(const SplitRule &rule, int n, int kv, int G, int Hkv, int group_cols,
+                                                            int group_slots) {
     if (few_columns(n, G)) return row_splits(rule, kv);
     const int units = row_blocks(n, G, group_cols) * Hkv;
-    return max(1, min(kSplitGroups / units, kv / kSplitTokens));
+    return max(1, min(group_slots / units, kv / kSplitTokens));
 }
 
 struct Row {
@@ -74,7 +77,7 @@ __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     r.n = min(r.full, a.max_q);
     r.kv = (int)min((int64_t)max(min(a.kv_lens[b], a.max_kv), 0), (int64_t)a.width << a.lps);
     r.blocks = row_blocks(r.n, a.G, a.group_cols);
-    r.splits = paged_splits(a.rule, r.n, r.kv, a.G, a.Hkv, a.group_cols);
+    r.splits = paged_splits(a.rule, r.n, r.kv, a.G, a.Hkv, a.group_cols, a.group_slots);
     return r;
 }
 
@@ -719,6 +722,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
 // alone, outputs were about twice as far from exact as the 16-bit pool's.
 template <int D, bool Q8>
 struct Chunk {
+    static constexpr int NW = chunk_waves(D, Q8);                      // waves
     static constexpr int NP = Q8 ? 2 : 1;                              // planes: the values, or hi and lo
     static constexpr int BN = D * NP <= 128 ? 64 : 32;                 // tokens a tile
     static constexpr int NT = BN / 32;                                 // 32-token blocks
@@ -1005,7 +1009,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
     using C = Chunk<D, Q8>;
     using State = std::conditional_t<(D > 128), ChunkState16<D, BF, Q8>, ChunkState<D, BF, Q8>>;
     constexpr int COLS = State::COLS;
-    static_assert(4 * COLS == group_columns(D), "columns of a workgroup");
+    static_assert(C::NW * COLS == group_columns(D, Q8), "columns of a workgroup");
     const uint32_t lds = (uint32_t)(uintptr_t)(LDSP(void))smem;
     const auto odd_flag = (volatile LDSP(int))(uintptr_t)(lds + C::kLds);
     const int lane = kq_lane(), c = lane & (COLS - 1);
@@ -1017,7 +1021,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
         const int rest = u / a.Hkv, kvh = u - rest * a.Hkv;
         // the tiles with the most keys first
         const int back = rest / row.splits, s = rest - back * row.splits, blk = row.blocks - 1 - back;
-        const int col0 = (blk * 4 + w) * COLS, cols = row.n * a.G;
+        const int col0 = (blk * C::NW + w) * COLS, cols = row.n * a.G;
 
         // this lane's column; waves past the row's columns only copy
         const int col = col0 + c;
@@ -1027,8 +1031,8 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
         const int seen = live ? min(seen_by(col), row.kv) : 0x7fffffff;
         const int least = __builtin_amdgcn_readfirstlane(seen_by(col0));
         const int most = __builtin_amdgcn_readfirstlane(col0 < cols ? min(seen_by(col0 + COLS - 1), row.kv) : 0);
-        const int least_all = __builtin_amdgcn_readfirstlane(seen_by(blk * 4 * COLS));
-        const int most_all = __builtin_amdgcn_readfirstlane(min(seen_by((blk + 1) * 4 * COLS - 1), row.kv));
+        const int least_all = __builtin_amdgcn_readfirstlane(seen_by(blk * C::NW * COLS));
+        const int most_all = __builtin_amdgcn_readfirstlane(min(seen_by((blk + 1) * C::NW * COLS - 1), row.kv));
         const int per = few_columns(row.n, a.G) ? a.rule.tokens(row.kv)
                                                 : ((row.kv + row.splits - 1) / row.splits + C::BN - 1) / C::BN * C::BN;
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
@@ -1053,24 +1057,26 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
             PageIds ids;
             const bool all_ok = ids.start(a, tab, (t_begin >> 4) >> sh, p_last);
             const int64_t h_off = (int64_t)kvh * a.head_stride;
-            // Piece y of this wave's 16-token pieces of the tile at t0, every
-            // other one of K (even waves) or V (odd waves): where it starts in
-            // the pool (values) and in a stage.
+            // Piece y of the RT tokens at a time of the tile at t0 that this
+            // wave copies, of K (even waves) or V (odd waves): where it starts
+            // in the pool (values) and in a stage.
+            constexpr int NY = C::NW == 4 ? C::BN / 32 : 1, RT = 2 * C::BN / (C::NW * NY);
+            static_assert(RT == 16 || RT == 8, "within 16 tokens");
             auto piece = [&](int t0, int y, uint32_t &dst) {
-                const int j = 2 * y + (w >> 1);
-                // (pieces past the end repeat the last: their keys are hidden)
-                const int ch = min((t0 >> 4) + j, c_last), p = ch >> sh;
+                const int t = RT * (C::NW / 2 * y + (w >> 1));
+                // (16 tokens past the end are the last ones again: their keys are hidden)
+                const int ch = min((t0 + t) >> 4, c_last), p = ch >> sh;
                 const int id = ids.at(tab, p, p_last);
-                dst = (uint32_t)((w & 1) * C::kHalf + 16 * j * C::kRow);
+                dst = (uint32_t)((w & 1) * C::kHalf + t * C::kRow);
                 return (int64_t)((uint32_t)id < (uint32_t)a.n_pages ? id : 0) * a.page_stride + h_off +
-                       (int64_t)((ch - (p << sh)) * 16) * a.tok_stride;
+                       (int64_t)((ch - (p << sh)) * 16 + (t & 15)) * a.tok_stride;
             };
             const auto swizzle = [&](int t) { return w & 1 ? C::vswz(t) : C::kswz(t); };
             const uint8_t *src = (const uint8_t *)(w & 1 ? a.v : a.k);
             // 16-bit pool: straight to LDS.
             auto copy = [&](int t0, uint32_t stage) {
 #pragma unroll
-                for (int y = 0; y < C::BN / 32; ++y) {
+                for (int y = 0; y < NY; ++y) {
                     uint32_t dst;
                     const int64_t off = piece(t0, y, dst);
 #pragma unroll
@@ -1083,7 +1089,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
             };
             // 8-bit pool: 16 values of a token a lane and load, with their
             // scale and bias, to registers and later to LDS.
-            constexpr int NY = Q8 ? C::BN / 32 : 1, NX = Q8 ? D / 64 : 1;
+            constexpr int NX = Q8 ? RT * D / 1024 : 1;
             u32x4 held[NY][NX];
             uint32_t held_s[NY][NX], held_b[NY][NX], held_at[NY];
             const uint16_t *src_s = w & 1 ? a.vs : a.ks, *src_b = w & 1 ? a.vb : a.kb;
@@ -1108,6 +1114,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
 #pragma unroll
                     for (int x = 0; x < NX; ++x) {
                         const int at = 16 * (64 * x + lane), t = at / D, pc = (at - t * D) / 8;
+                        const int turn = swizzle(t + (RT < 16 ? 8 * (w >> 1 & 1) : 0));
                         const float sc = f16bits_to_f32<BF>(held_s[y][x]), bi = f16bits_to_f32<BF>(held_b[y][x]);
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
@@ -1119,7 +1126,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
                                 hi[i] = pack2<BF>(u, v);
                                 lo[i] = pack2<BF>(u - f16bits_to_f32<BF>(hi[i] & 0xFFFFu), v - f16bits_to_f32<BF>(hi[i] >> 16));
                             }
-                            const uint32_t to = stage + held_at[y] + (uint32_t)(t * C::kRow + 16 * ((pc + half) ^ swizzle(t)));
+                            const uint32_t to = stage + held_at[y] + (uint32_t)(t * C::kRow + 16 * ((pc + half) ^ turn));
                             *(LDSP(u32x4))(uintptr_t)to = hi;
                             *(LDSP(u32x4))(uintptr_t)(to + C::kPlane) = lo;
                         }
@@ -1140,7 +1147,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
             // columns that see them is added from the pool.
             auto clean = [&](uint32_t stage, int t0) {
                 uint32_t odd = 0;
-                for (uint32_t at = stage + C::kHalf + 16u * threadIdx.x; at < stage + 2 * C::kHalf; at += 16u * 256u) {
+                for (uint32_t at = stage + C::kHalf + 16u * threadIdx.x; at < stage + 2 * C::kHalf; at += 16u * 64u * C::NW) {
                     u32x4 v = *(const LDSP(u32x4))(uintptr_t)at;
                     uint32_t here = 0;
 #pragma unroll
@@ -1244,12 +1251,13 @@ constexpr bool kBeside = D <= 128;
 // others chunks: decode rows, which wait for memory, run beside a prompt
 // chunk's products.
 template <int D, bool BF, bool Q8>
-__global__ __launch_bounds__(256, D > 256 || (D == 256 && Q8) ? 1 : 2) void kq_paged_kernel(PagedArgs a, int wave_groups) {
+__global__ __launch_bounds__(64 * chunk_waves(D, Q8), D > 256 ? 1 : 2) void kq_paged_kernel(PagedArgs a, int wave_groups) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     if constexpr (kBeside<D>) {
         if ((int)blockIdx.x < wave_groups) {
+            constexpr int NW = chunk_waves(D, Q8);
             const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-            wave_work<D, BF, Q8, false>(a, (int)(4 * blockIdx.x) + w, 4 * wave_groups);
+            wave_work<D, BF, Q8, false>(a, NW * (int)blockIdx.x + w, NW * wave_groups);
             return;
         }
     }
@@ -1439,7 +1447,7 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
 struct Grid {
     dim3 waves, merge;   // x == 0: not launched
     int groups;          // workgroups of chunks (0: none)
-    int wave_groups;     // and of rows of few columns beside them
+    int beside;          // waves of rows of few columns beside them
 };
 
 template <int D, bool BF, bool Q8>
@@ -1450,8 +1458,9 @@ int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
         static const bool ok = hipFuncSetAttribute((const void *)kq_paged_kernel<D, BF, Q8>,
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
         if (!ok) return KQ_ERR_LAUNCH_FAILED;
-        const int beside = kBeside<D> ? g.wave_groups : 0;
-        hipLaunchKernelGGL((kq_paged_kernel<D, BF, Q8>), dim3(beside + g.groups), dim3(256), lds, s, a, beside);
+        constexpr int NW = chunk_waves(D, Q8);
+        const int beside = kBeside<D> ? (g.beside + NW - 1) / NW : 0;
+        hipLaunchKernelGGL((kq_paged_kernel<D, BF, Q8>), dim3(beside + g.groups), dim3(64 * NW), lds, s, a, beside);
     }
     if constexpr (has_waves(D)) {
         if (g.waves.x && !(kBeside<D> && g.groups)) {
@@ -1495,18 +1504,17 @@ Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max
     const int G = Hq / Hkv, chunk = kFewColumns / G + 1;  // tokens of the shortest chunk
     p.rule = wave_rule(Hq, Hkv, D, q8);
     p.few = chunk > 1 ? most_row_splits(p.rule, max_kv) : 1;
-    p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, group_columns(D)) : 1;
+    p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, group_columns(D, q8), group_slots(D, q8)) : 1;
     const int most = p.few > p.many ? p.few : p.many;
     if (most < 2) {
         p.slots = p.slot_stride = 0;
         return p;
     }
     // one slot a token, query head and split; and of a row, of few columns at
-    // most kFewColumns of them a kv head, a chunk's at most kSplitGroups *
-    // 128 (one with splits has units < kSplitGroups workgroups of at most 128
-    // columns and splits <= kSplitGroups / units)
+    // most kFewColumns of them a kv head, a chunk's at most group_slots
+    // workgroups' columns (it has splits <= group_slots / workgroups)
     const int64_t by_token = T * Hq * most;
-    const int64_t few_row = (int64_t)kFewColumns * Hkv * p.few, many_row = p.many > 1 ? kSplitGroups * 128 : 0;
+    const int64_t few_row = (int64_t)kFewColumns * Hkv * p.few, many_row = p.many > 1 ? group_slots(D, q8) * group_columns(D, q8) : 0;
     const int64_t by_row = B * (few_row > many_row ? few_row : many_row);
     p.slots = by_token < by_row ? by_token : by_row;
     p.slot_stride = by_token <= by_row ? most : 0;
@@ -1574,7 +1582,8 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     a.Hq = Hq;
     a.Hkv = Hkv;
     a.G = Hq / Hkv;
-    a.group_cols = group_columns(D);
+    a.group_cols = group_columns(D, a.ks != nullptr);
+    a.group_slots = group_slots(D, a.ks != nullptr);
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.scale_log2 = scale * 1.4426950408889634f;
@@ -1595,13 +1604,12 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     const int64_t many = (((int64_t)T * a.G + a.group_cols - 1) / a.group_cols + rows) * Hkv *
                          (has_waves(D) ? plan.many : most);
     g.groups = has_waves(D) && few_columns(max_q, a.G) ? 0 : (int)(many < (1 << 14) ? many : (1 << 14));
-    g.wave_groups = 0;
+    g.beside = 0;
     if (has_waves(D) && a.G <= kFewColumns) {
         const int64_t n = rows * Hkv * plan.few;
         if (a.direct) g.waves = dim3(plan.few, Hkv, B);
         else g.waves = dim3((unsigned)(n < (1 << 16) ? n : (1 << 16)));
-        // (a row that is a chunk leaves no more than the other tokens to these)
-        if (g.groups) g.wave_groups = (int)((n < (1 << 13) ? n : (1 << 13)) + 3) / 4;
+        if (g.groups) g.beside = (int)(n < (1 << 13) ? n : (1 << 13));
     }
     if (plan.slots) {
         const int64_t n = plan.few > 8 || plan.many > 8 ? items * B : (int64_t)T * Hq / 16 + B;
