@@ -770,9 +770,9 @@ __device__ __forceinline__ half8_t lds_half8(uint32_t at) {
 }
 
 // Four tokens of one head dim a lane from a row-major tile.
-__device__ __forceinline__ u32x2 lds_tr(uint32_t at) {
+__device__ __forceinline__ u32x2 lds_tr(uint32_t at, uint32_t more) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDSP(s16x4))(uintptr_t)at));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDSP(s16x4))(uintptr_t)at + more / 8));
 }
 
 // 16 bytes a lane from base + off straight to LDS, lane l's at lds + 16 l (the
@@ -795,11 +795,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(
 // mfma(i, operand) for i < N with the operands read AHEAD steps before their
 // use, so that no MFMA waits for a read that was just issued (left alone, the
 // scheduler saves registers and puts every read right before its MFMA).  Reads
-// and MFMAs keep this order; vector and scalar ALU work may move across.
+// and MFMAs keep this order; vector and scalar ALU work may move across.  The
+// wave goes before the SIMD's other one meanwhile, whose softmax then fills the
+// gaps (a 2048-token chunk 257 -> 251 us).
 template <int N, int AHEAD, class Read, class Use>
 __device__ __forceinline__ void pipelined(Read &&read, Use &&use) {
     constexpr int A = AHEAD < N ? AHEAD : N;
     half8_t f[A + 1];
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < A; ++i) f[i] = read(i);
     __builtin_amdgcn_sched_barrier(0x6);
@@ -810,6 +813,7 @@ __device__ __forceinline__ void pipelined(Read &&read, Use &&use) {
         use(i, f[i % (A + 1)]);
         __builtin_amdgcn_sched_barrier(0x6);
     }
+    __builtin_amdgcn_s_setprio(0);
 }
 
 // How far (log2) a tile's maximum may pass the one that the sums are held at
@@ -919,7 +923,7 @@ struct ChunkState {
                 const int j = x % ND, pl = x / ND % C::NP, kk = x / (ND * C::NP);
                 const uint32_t flip = 16 * ((4 * j) & C::kSw);
                 const uint32_t up = 16 * ((4 * j) & ~C::kSw) + 16 * kk * C::kRow + pl * C::kPlane;
-                const u32x2 a = lds_tr((va ^ flip) + up), b = lds_tr((vb ^ flip) + up);
+                const u32x2 a = lds_tr(va ^ flip, up), b = lds_tr(vb ^ flip, up);
                 return __builtin_bit_cast(half8_t, u32x4{a.x, a.y, b.x, b.y});
             },
             [&](int x, const half8_t &f) { o[x % ND] = mfma32<BF>(f, pf[x / (ND * C::NP)], o[x % ND]); });
@@ -995,8 +999,9 @@ struct ChunkState16 {
         pipelined<NR * C::NP, 6>(
             [&](int x) {
                 const int j = x % NR, pl = x / NR;
-                const uint32_t at = (va ^ (uint32_t)(16 * ((2 * j) & C::kSw))) + (uint32_t)(16 * ((2 * j) & ~C::kSw) + pl * C::kPlane);
-                const u32x2 a = lds_tr(at), b = lds_tr(at + 16 * C::kRow);
+                const uint32_t at = va ^ (uint32_t)(16 * ((2 * j) & C::kSw));
+                const uint32_t up = (uint32_t)(16 * ((2 * j) & ~C::kSw) + pl * C::kPlane);
+                const u32x2 a = lds_tr(at, up), b = lds_tr(at, up + 16 * C::kRow);
                 return __builtin_bit_cast(half8_t, u32x4{a.x, a.y, b.x, b.y});
             },
             [&](int x, const half8_t &f) { o[x % NR] = mfma<BF>(f, pf, o[x % NR]); });
@@ -1485,6 +1490,7 @@ int launch(const PagedArgs &a, bool q8, const Grid &g, hipStream_t s) {
 // Tokens per split of a row of few columns, by its own keys, as decode
 // attention over contiguous caches has them.
 SplitRule wave_rule(int Hq, int Hkv, int D, bool q8) {
+    if (const int forced = env_int("GMLX_KQ_SDPA_SPLIT", 0)) return SplitRule{0, 0, 0, 0, (forced + 63) / 64 * 64};
     if (D > 128) return SplitRule{q8 || D > 256 ? 0 : 128, 1024, 8192, 32768, 512};
     if (q8) return SplitRule{Hq > 8 * Hkv ? 256 : 0, 1024, 2048, 32768, 512};
     if (Hq > 8 * Hkv) return SplitRule{512, 0, 1024, 8192, 512};
