@@ -22,21 +22,30 @@ struct PagedArgs {
     int32_t tok_stride, lps, n_pages, width;
     int32_t T, B, Hq, Hkv, G, max_q, max_kv;
     int32_t group_cols, group_slots;
+    int32_t few_limit;   // (few_columns)
+    int32_t few_cols;    // a wave's 16, or group_cols where the chunks' kernel takes all rows
     float scale_log2;
     float *part, *ml;  // split partials: [slot][D] sums, [slot][2] (maximum, sum)
     SplitRule rule;    // rows of few columns
     // slots a token and query head, or 0: a row's slots follow those of the rows
     // before it (a chunk's tokens have fewer splits than a decode row's)
     int32_t slot_stride;
+    int32_t few_blocks;  // the most 16-column blocks of a row of few columns
     int32_t direct;    // the wave kernel's grid is (split, kv head, row), the merge's (token and head, row)
 };
 
-constexpr int kFewColumns = 16;     // rows of at most so many columns split as decode rows do
 constexpr int kSplitTokens = 512;   // least keys of a chunk's split
 constexpr int kDirect = 1 << 15;    // waves, and merged tokens and heads, of a direct grid
 constexpr int kMergeGroups = 1024;  // workgroups of a merge that is not
 
-__host__ __device__ __forceinline__ bool few_columns(int n, int G) { return (int64_t)n * G <= kFewColumns; }
+// Rows of at most so many columns split as decode rows do and run in waves of 16
+// columns.  Two waves read a row's keys twice, and still beat a chunk's
+// workgroup with one of its waves at work where a tile costs conversions (8 bits:
+// blocks of 5 tokens in 8 rows 45 us against 72) or the GPU is idle anyway (16
+// bits: one row of 8 tokens and 4000 keys 14 against 24), but not where memory
+// bounds them (16 bits, 8 rows: 55 against 42).
+constexpr int few_limit(bool q8) { return q8 ? 32 : 16; }
+__host__ __device__ __forceinline__ bool few_columns(int n, int G, int limit) { return (int64_t)n * G <= limit; }
 
 // Whether such rows run a wave each (at head dim 512 a wave's tile, sums and query
 // spill: the chunks' kernel takes all rows there).
@@ -49,16 +58,16 @@ constexpr int chunk_waves(int D, bool q8) { return q8 && (D == 128 || D == 256) 
 constexpr int group_columns(int D, bool q8) { return chunk_waves(D, q8) * (D > 128 ? 16 : 32); }
 constexpr int group_slots(int D, bool q8) { return D > 256 || chunk_waves(D, q8) > 4 ? 256 : 512; }
 
-// Workgroups (waves, rows of few columns) of an unsplit row over one kv head.
-__host__ __device__ __forceinline__ int row_blocks(int n, int G, int group_cols) {
-    return few_columns(n, G) ? (n > 0) : (int)(((int64_t)n * G + group_cols - 1) / group_cols);
+// Blocks of `cols` query columns of a row.
+__host__ __device__ __forceinline__ int row_blocks(int n, int G, int cols) {
+    return (int)(((int64_t)n * G + cols - 1) / cols);
 }
 
 // Splits of a row of n tokens and kv keys: from the row and the head counts
 // alone, so that a row of a batch has the bits of the row alone.
-__host__ __device__ __forceinline__ int paged_splits(const SplitRule &rule, int n, int kv, int G, int Hkv, int group_cols,
-                                                            int group_slots) {
-    if (few_columns(n, G)) return row_splits(rule, kv);
+__host__ __device__ __forceinline__ int paged_splits(const SplitRule &rule, int n, int kv, int G, int Hkv, int few_limit,
+                                                            int group_cols, int group_slots) {
+    if (few_columns(n, G, few_limit)) return row_splits(rule, kv);
     const int units = row_blocks(n, G, group_cols) * Hkv;
     return max(1, min(group_slots / units, kv / kSplitTokens));
 }
@@ -76,19 +85,19 @@ __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     r.full = min(max(a.cu_q[b + 1], r.q0), a.T) - r.q0;
     r.n = min(r.full, a.max_q);
     r.kv = (int)min((int64_t)max(min(a.kv_lens[b], a.max_kv), 0), (int64_t)a.width << a.lps);
-    r.blocks = row_blocks(r.n, a.G, a.group_cols);
-    r.splits = paged_splits(a.rule, r.n, r.kv, a.G, a.Hkv, a.group_cols, a.group_slots);
+    r.blocks = row_blocks(r.n, a.G, few_columns(r.n, a.G, a.few_limit) ? a.few_cols : a.group_cols);
+    r.splits = paged_splits(a.rule, r.n, r.kv, a.G, a.Hkv, a.few_limit, a.group_cols, a.group_slots);
     return r;
 }
 
 // Units of the wave kernel, of the chunk kernel, and of the merge (merge_items
 // tokens and query heads of a row that has splits).
 __device__ __forceinline__ int wave_units(const PagedArgs &a, const Row &r) {
-    return few_columns(r.n, a.G) ? r.blocks * r.splits * a.Hkv : 0;
+    return few_columns(r.n, a.G, a.few_limit) ? r.blocks * r.splits * a.Hkv : 0;
 }
 template <int D>
 __device__ __forceinline__ int chunk_units(const PagedArgs &a, const Row &r) {
-    return has_waves(D) && few_columns(r.n, a.G) ? 0 : r.blocks * r.splits * a.Hkv;
+    return has_waves(D) && few_columns(r.n, a.G, a.few_limit) ? 0 : r.blocks * r.splits * a.Hkv;
 }
 // A workgroup's share of a merge: one item where all its threads add up the splits,
 // one a wave where a wave takes several rounds of loads for them, four a wave,
@@ -188,7 +197,10 @@ struct PageIds {
     __device__ __forceinline__ bool start(const PagedArgs &a, const int32_t *tab, int p, int last) {
         load(tab, p, last);
         bool bad = (uint32_t)ids >= (uint32_t)a.n_pages;
-        for (int i = p + 64 + kq_lane(); i <= last; i += 64) bad |= (uint32_t)tab[i] >= (uint32_t)a.n_pages;
+        // (every lane in every round: where lanes left such a loop one by one, the
+        // compiler has put register copies before the restore of EXEC behind it)
+        for (int i = p + 64; i <= last; i += 64)
+            bad |= (uint32_t)tab[min(i + kq_lane(), last)] >= (uint32_t)a.n_pages;
         return __builtin_amdgcn_ballot_w64(bad) == 0;
     }
 
@@ -540,30 +552,37 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
     constexpr int NBUF = D >= 256 ? 1 : 2;
     const int lane = kq_lane(), r = lane & 15, g = lane >> 4;
     for (int unit = first;; unit += step) {
-        int b, h, s, slot0 = 0;
+        // the 16-column blocks of a row (at most two) read the same keys: one after
+        // the other in the scan's order, eight apart, on one XCD, in the grid's
+        int b, h, s, blk, slot0 = 0;
         Row row;
         if constexpr (DIRECT) {
-            s = unit;
+            s = a.few_blocks > 1 ? unit / 16 * 8 + unit % 8 : unit;
+            blk = a.few_blocks > 1 ? unit / 8 % 2 : 0;
             h = blockIdx.y;
             b = blockIdx.z;
             row = lane_row(row_at(a, b), 0);
-            if (!few_columns(row.n, a.G) || row.n == 0 || s >= row.splits) return;
+            if (!few_columns(row.n, a.G, a.few_limit) || blk >= row.blocks || s >= row.splits) return;
         } else {
             int u = unit;
             if (!find_unit(a, [&](const Row &x) { return wave_units(a, x); }, u, b, row, slot0)) return;
-            s = u / a.Hkv;
-            h = u - s * a.Hkv;
+            const int head = u / row.blocks;
+            blk = u - head * row.blocks;
+            s = head / a.Hkv;
+            h = head - s * a.Hkv;
         }
 
         // this lane's column
-        const bool live = r < row.n * a.G;
-        const int i = live ? r / a.G : row.n - 1, hq = h * a.G + (live ? r - i * a.G : 0);
+        const int col = 16 * blk + r;
+        const bool live = col < row.n * a.G;
+        const int i = live ? col / a.G : row.n - 1, hq = h * a.G + (live ? col - i * a.G : 0);
         State<D, BF, Q8> st;
         st.init();
-        // keys seen: the column's, the row's least and most
+        // keys seen: the column's, the block's least and most
         const int first = row.kv - row.full + 1;
         const int seen = live ? max(first + i, 0) : 0x7fffffff;
-        const int least = max(first, 0), most = min(max(first + row.n - 1, 0), row.kv);
+        const int least = max(first + 16 * blk / a.G, 0);
+        const int most = min(max(first + min((16 * blk + 15) / a.G, row.n - 1), 0), row.kv);
         const int per = a.rule.tokens(row.kv);
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
         const int t_end = __builtin_amdgcn_readfirstlane(min(most, t_begin + per));
@@ -1038,7 +1057,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
         const int most = __builtin_amdgcn_readfirstlane(col0 < cols ? min(seen_by(col0 + COLS - 1), row.kv) : 0);
         const int least_all = __builtin_amdgcn_readfirstlane(seen_by(blk * C::NW * COLS));
         const int most_all = __builtin_amdgcn_readfirstlane(min(seen_by((blk + 1) * C::NW * COLS - 1), row.kv));
-        const int per = few_columns(row.n, a.G) ? a.rule.tokens(row.kv)
+        const int per = few_columns(row.n, a.G, a.few_limit) ? a.rule.tokens(row.kv)
                                                 : ((row.kv + row.splits - 1) / row.splits + C::BN - 1) / C::BN * C::BN;
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
         const int t_end = __builtin_amdgcn_readfirstlane(min(most_all, t_begin + per));
@@ -1507,20 +1526,20 @@ struct Plan {
 
 Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max_kv, bool q8) {
     Plan p;
-    const int G = Hq / Hkv, chunk = kFewColumns / G + 1;  // tokens of the shortest chunk
+    const int G = Hq / Hkv, limit = few_limit(q8), chunk = limit / G + 1;  // tokens of the shortest chunk
     p.rule = wave_rule(Hq, Hkv, D, q8);
     p.few = chunk > 1 ? most_row_splits(p.rule, max_kv) : 1;
-    p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, group_columns(D, q8), group_slots(D, q8)) : 1;
+    p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, limit, group_columns(D, q8), group_slots(D, q8)) : 1;
     const int most = p.few > p.many ? p.few : p.many;
     if (most < 2) {
         p.slots = p.slot_stride = 0;
         return p;
     }
     // one slot a token, query head and split; and of a row, of few columns at
-    // most kFewColumns of them a kv head, a chunk's at most group_slots
+    // most few_limit of them a kv head, a chunk's at most group_slots
     // workgroups' columns (it has splits <= group_slots / workgroups)
     const int64_t by_token = T * Hq * most;
-    const int64_t few_row = (int64_t)kFewColumns * Hkv * p.few, many_row = p.many > 1 ? group_slots(D, q8) * group_columns(D, q8) : 0;
+    const int64_t few_row = (int64_t)limit * Hkv * p.few, many_row = p.many > 1 ? group_slots(D, q8) * group_columns(D, q8) : 0;
     const int64_t by_row = B * (few_row > many_row ? few_row : many_row);
     p.slots = by_token < by_row ? by_token : by_row;
     p.slot_stride = by_token <= by_row ? most : 0;
@@ -1590,6 +1609,8 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     a.G = Hq / Hkv;
     a.group_cols = group_columns(D, a.ks != nullptr);
     a.group_slots = group_slots(D, a.ks != nullptr);
+    a.few_limit = few_limit(a.ks != nullptr);
+    a.few_cols = has_waves(D) ? 16 : a.group_cols;
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.scale_log2 = scale * 1.4426950408889634f;
@@ -1602,18 +1623,19 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     // rows would have is no large grid, each finds its own from its place there;
     // else they sum over the rows' units.
     Grid g;
-    const int64_t rows = T < B ? T : B, waves = plan.few * (int64_t)Hkv * B;
+    a.few_blocks = (int)(((int64_t)max_q * a.G < a.few_limit ? (int64_t)max_q * a.G : a.few_limit) + 15) / 16;
+    const int64_t rows = T < B ? T : B, waves = (int64_t)plan.few * a.few_blocks * Hkv * B;
     const int64_t items = (int64_t)(max_q < T ? max_q : T) * Hq;
     a.direct = (plan.slot_stride || !plan.slots) && B < (1 << 16) && Hkv < (1 << 16) && waves <= kDirect &&
                items * B <= kDirect;
     g.waves = g.merge = dim3(0);
     const int64_t many = (((int64_t)T * a.G + a.group_cols - 1) / a.group_cols + rows) * Hkv *
                          (has_waves(D) ? plan.many : most);
-    g.groups = has_waves(D) && few_columns(max_q, a.G) ? 0 : (int)(many < (1 << 14) ? many : (1 << 14));
+    g.groups = has_waves(D) && few_columns(max_q, a.G, a.few_limit) ? 0 : (int)(many < (1 << 14) ? many : (1 << 14));
     g.beside = 0;
-    if (has_waves(D) && a.G <= kFewColumns) {
-        const int64_t n = rows * Hkv * plan.few;
-        if (a.direct) g.waves = dim3(plan.few, Hkv, B);
+    if (has_waves(D) && a.G <= a.few_limit) {
+        const int64_t n = rows * Hkv * plan.few * a.few_blocks;
+        if (a.direct) g.waves = dim3(a.few_blocks > 1 ? (plan.few + 7) / 8 * 16 : plan.few, Hkv, B);
         else g.waves = dim3((unsigned)(n < (1 << 16) ? n : (1 << 16)));
         if (g.groups) g.beside = (int)(n < (1 << 13) ? n : (1 << 13));
     }

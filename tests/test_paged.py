@@ -1,6 +1,9 @@
 """The paged cache's host side: refusals of the C ABI and of the ops, workspace
 sizes, and the plan reference's own invariants.  No GPU needed."""
 import ctypes
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -149,3 +152,51 @@ def test_plan_reference_keeps_every_page_once():
                 for s, p in zip(slots[cu[b]:cu[b + 1]], pos[cu[b]:cu[b + 1]]):
                     assert s == table[b, p // page] * page + p % page
     assert refusals > 20
+
+
+def _before_exec(text):
+    """(kernel, label, instruction) of vector instructions between the start of a
+    block that lanes join again and its restore of EXEC: those lanes would skip
+    them.  Such blocks are where a `s_cbranch_execz` goes, and behind loops that
+    lanes leave one by one."""
+    joins = set(re.findall(r"s_cbranch_execz\s+(\.LBB\w+)", text))
+    kernel = block = last = None
+    found, seen = [], []
+    for line in text.splitlines():
+        name = re.match(r"([A-Za-z_]\w*):", line)
+        label = re.match(r"(\.LBB\w+):|; (%bb\.\w+):", line)
+        code = line.split(";")[0].strip()
+        if name:
+            kernel, block = name.group(1), None
+        elif label:
+            joined = label.group(1) in joins or (label.group(2) and last == "s_cbranch_execnz")
+            block, seen = (label.group(0) if joined else None), []
+        elif code and not code.startswith("."):
+            last = code.split()[0]
+            if block is None:
+                continue
+            if re.match(r"s_(or|andn2)_b64 exec, exec|s_mov_b64 exec|s_(or|andn2)_saveexec", code):
+                found += [(kernel, block, x) for x in seen]
+                block = None
+            elif re.match(r"s_c?branch|s_and_saveexec|s_endpgm|s_barrier", code):
+                block = None
+            elif re.match(r"(v|ds|global|flat|buffer|scratch)_", code) and not re.match(r"v_(readlane|writelane|readfirstlane)", code):
+                seen.append(code)
+    return found
+
+
+def test_register_copies_stand_behind_the_restore_of_exec(tmp_path):
+    """Of the attention kernels as compiled: where the compiler splits a live
+    range at a block that lanes join again, it can put the copy before the
+    restore of EXEC, which lost addresses where no lane had been in the branch."""
+    bad = "k:\n\ts_cbranch_execz .LBB0_2\n; %bb.1:\n\tv_mov_b32 v0, v1\n.LBB0_2:\n\tv_accvgpr_write_b32 a0, v2\n" \
+          "\ts_or_b64 exec, exec, s[0:1]\n"
+    assert _before_exec(bad) == [("k", ".LBB0_2:", "v_accvgpr_write_b32 a0, v2")]
+    assert not _before_exec(bad.replace("\tv_accvgpr_write_b32 a0, v2\n", ""))
+    from gmlx_amd import build
+    out = tmp_path / "kq_paged.s"
+    subprocess.run([build.HIPCC, *build.FLAGS, "-S", os.path.join(build.CSRC, "kq_paged.hip"), "-o", str(out),
+                    "--offload-device-only"], check=True, capture_output=True)
+    text = out.read_text()
+    assert "kq_paged_wave_kernel" in text
+    assert not _before_exec(text)
