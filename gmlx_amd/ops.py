@@ -1457,7 +1457,10 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     s = _stream(q)
     ws_ptr, ws_len = None, 0
     if need:
-        ws = _WS.get("sdpa_paged", dev, s.value, need)
+        # (a captured call's own, from its graph's pool: graphs captured on one
+        # stream may be replayed on two at once)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if torch.cuda.is_current_stream_capturing() else \
+            _WS.get("sdpa_paged", dev, s.value, need)
         ws_ptr, ws_len = ws.data_ptr(), ws.numel()
     _paged_call("kq_sdpa_paged", dev, q.data_ptr(), qt, pool, tab, tab_stride, width, lens, cu, T, B, Hq, mq, mkv,
                 float(scale), out.data_ptr(), ot, ws_ptr, ws_len, s)

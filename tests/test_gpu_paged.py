@@ -472,3 +472,236 @@ def test_large_pool_offsets():
                                   y.double().cpu().numpy().transpose(1, 0, 2), m, D ** -0.5)
         d = np.abs(out.double().cpu().numpy() - want)
         assert (d <= HALF[dt] * (np.abs(want) + far) + 1e-4 * far).all()
+
+
+# --------------------------------------------------------- the operators together
+
+class Serving:
+    """A pool, its tables and a step over them: plan, write, attend."""
+
+    def __init__(self, B, Hq, Hkv, D, P, n_pages, width, dt, q8):
+        from gmlx_amd import ops
+        self.ops, self.dt, self.P, self.Hq, self.Hkv, self.D = ops, dt, P, Hq, Hkv, D
+        self.scale = D ** -0.5
+        (self.k, self.v), self.sc = _pool((n_pages, Hkv, P, D), dt, q8, "mixed", fill=float("nan"))
+        i32 = dict(dtype=torch.int32, device="cuda")
+        self.table = torch.full((B, width), -1, **i32)
+        self.free = torch.randperm(n_pages, generator=torch.Generator().manual_seed(B)).to(**i32)
+        self.count = torch.tensor([n_pages], **i32)
+        self.seq = torch.zeros(B, **i32)
+
+    def step(self, new, keep, q, k, v, max_q, out=None):
+        """In place of the state, as a captured graph has it."""
+        ops = self.ops
+        p = ops.paged_plan(self.seq, new, self.table, self.free, self.count, self.P, q.shape[0], keep_lens=keep)
+        self.seq.copy_(p.kv_lens)
+        self.count.copy_(p.free_count)
+        ops.paged_write(k, v, self.k, self.v, p.slots, **self.sc)
+        out = ops.sdpa_paged(q, self.k, self.v, self.table, p.kv_lens, p.cu_q, self.scale, max_q=max_q, out=out, **self.sc)
+        return p, out
+
+    def state(self):
+        return [self.table, self.free, self.count, self.seq, self.k, self.v, *self.sc.values()]
+
+    def row(self, b):
+        """The row's cached K and V in fp64 (Hkv, kv, D), and what a probability's
+        rounding multiplies: |V|, of an 8-bit pool the centred values'."""
+        kv = int(self.seq[b])
+        t = torch.arange(kv, device="cuda")
+        page, off = self.table[b].long()[t // self.P], t % self.P
+        vals = []
+        for pool, x in ((self.k, "k"), (self.v, "v")):
+            z = pool[page, :, off].double()
+            far = z.abs()
+            if self.sc:
+                s, bi = (self.sc[x + name][page, :, off].double().repeat_interleave(64, -1) for name in ("_scales", "_biases"))
+                z, far = z * s + bi, ((z - 128) * s).abs()
+            vals += [z, far]
+        return [x.transpose(0, 1).cpu().numpy() for x in (vals[0], vals[2], vals[3])]
+
+    def check(self, q, out, b, lo, n):
+        k, v, err = self.row(b)
+        kv = k.shape[1]
+        x = q[lo:lo + n].double().cpu().numpy()
+        want, far = ref.attention(x, k, v, n, self.scale, err)
+        _, mean = ref.attention(x, k, v, n, self.scale)
+        u = HALF[self.dt]
+        smax = 1.5 * self.scale * np.abs(x).sum(-1).max() * max(1.0, np.abs(k).max())
+        f32 = 2.0 ** -24 * (2 * (x.shape[-1] + 8) * smax + 2 * kv + 16)  # (as Batch.check counts)
+        room = u * np.abs(want) + u * (1 + u) * far + f32 * (mean + far) + 1e-7
+        d = np.abs(out[lo:lo + n].double().cpu().numpy() - want)
+        assert np.isfinite(d).all() and (d <= room).all(), (b, n, kv, (d / room).max())
+
+
+# (new tokens, tokens kept) of four rows a step: prompts, decoding, drafts of
+# which some are rejected, an ended request whose row and pages go to the next
+# one, a row that the pool has no pages for
+STEPS = [([70, 0, 5, 33], None), ([1, 40, 1, 1], None), ([1, 1, 1, 1], None), ([5, 5, 5, 5], None),
+         ([5, 1, 5, 2], [74, 46, 10, 37]), ([130, 1, 0, 1], [0, 47, 14, 39]), ([1, 1, 1, 1000], None),
+         ([1, 1, 1, 1], [130, 47, 14, 0]), ([0, 0, 0, 17], None)]
+
+
+def _inputs(s, T, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    new = lambda h: torch.randn(T, h, s.D, device="cuda", generator=gen).to(s.dt)  # noqa: E731
+    return new(s.Hq), new(s.Hkv), new(s.Hkv)
+
+
+@pytest.mark.parametrize("dt,q8,Hq,Hkv,D", [(BF16, False, 8, 2, 128), (F16, True, 8, 2, 128), (F16, False, 4, 4, 64),
+                                           (BF16, True, 16, 2, 256)])
+def test_steps_of_a_serving_loop(dt, q8, Hq, Hkv, D):
+    s = Serving(4, Hq, Hkv, D, 16, 40, 70, dt, q8)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    model = [torch.zeros(0, Hkv, D, dtype=dt, device="cuda") for _ in range(4)]  # keys in order
+    for i, (new, keep) in enumerate(STEPS):
+        T = sum(new) + 3  # (padded)
+        q, k, v = _inputs(s, T, i)
+        _say("step", i, dt, q8, D, new, keep)
+        p, out = s.step(torch.tensor(new, **i32), None if keep is None else torch.tensor(keep, **i32), q, k, v, max(new))
+        refused, lo = p.refused.tolist(), 0
+        assert refused == [0, 0, 0, int(new[3] == 1000)]
+        for b, n in enumerate(new):
+            if not refused[b]:
+                kept = model[b] if keep is None else model[b][:keep[b]]
+                model[b] = torch.cat([kept, k[lo:lo + n]])
+                if not q8:
+                    assert np.array_equal(s.row(b)[0], model[b].double().transpose(0, 1).cpu().numpy())
+                if n:
+                    s.check(q, out, b, lo, n)
+            assert int(s.seq[b]) == len(model[b])
+            lo += n
+        pages = [int(x) for b in range(4) for x in s.table[b, :-(-len(model[b]) // 16)]]
+        pages += s.free[:int(s.count)].tolist()
+        assert sorted(pages) == list(range(40))  # every page once
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_step_captured_and_replayed(q8):
+    """A step of two new tokens a row, of which the next keeps one or both, in a
+    graph that updates the state in place; eager work between the replays; every
+    replay bit for bit as the eager step."""
+    B, i32 = 6, dict(dtype=torch.int32, device="cuda")
+
+    def fresh():
+        s = Serving(B, 8, 2, 128, 16, 200, 40, BF16, q8)
+        q, k, v = _inputs(s, 6 * 90, 99)
+        s.step(torch.tensor([90, 1, 33, 500 - 300, 16, 2], **i32), None, q, k, v, 200)
+        return s
+    eager, live = fresh(), fresh()
+    T = 2 * B
+    new = torch.full((B,), 2, **i32)
+    hold = [*_inputs(live, T, 0), torch.zeros(B, **i32)]
+    hold[3].copy_(live.seq)
+    outs = torch.zeros(T, 8, 128, dtype=BF16, device="cuda")
+    saved = [x.clone() for x in live.state()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # (builds what the first call builds, on another stream than the tensors')
+        live.step(new, hold[3], *hold[:3], 2, out=outs)
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip(live.state(), saved):
+        x.copy_(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        live.step(new, hold[3], *hold[:3], 2, out=outs)
+    for x, y in zip(live.state(), saved):
+        x.copy_(y)
+    for i in range(7):
+        q, k, v = _inputs(live, T, 100 + i)
+        keep = eager.seq - torch.tensor([(i + b) % 2 if i else 0 for b in range(B)], **i32)
+        for x, y in zip(hold, (q, k, v, keep)):
+            x.copy_(y)
+        _say("replay", i, q8)
+        graph.replay()
+        _, want = eager.step(new, keep, q, k, v, 2)
+        torch.cuda.synchronize()
+        assert torch.equal(outs, want)
+        for x, y in zip(live.state(), eager.state()):
+            assert np.array_equal(_bits(x), _bits(y))
+
+
+def test_two_graphs_replayed_at_once():
+    """Each call of a graph has a workspace of its own: two graphs captured one
+    after the other, replayed on two streams, beside eager calls on a third."""
+    from gmlx_amd import ops
+    batches = [Batch([(1, 6000), (1, 3000), (1, 9000)], 8, 2, 128, 16, F16, seed=1),
+               Batch([(1, 8000), (1, 7000)], 8, 2, 128, 16, F16, seed=2)]
+    want = [b.run() for b in batches]
+    qs = [b.q.cuda() for b in batches]
+    graphs, outs = [], []
+    for b, q in zip(batches, qs):
+        g, out = torch.cuda.CUDAGraph(), torch.zeros_like(q)
+        with torch.cuda.graph(g):
+            for _ in range(20):
+                ops.sdpa_paged(q, *b.pool, b.table, b.kv_lens, b.cu_q, b.scale, out=out)
+        graphs.append(g)
+        outs.append(out)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for i in range(4):
+        for out in outs:
+            out.zero_()
+        _say("two graphs", i)
+        for st, g in zip(streams, graphs):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                g.replay()
+        more = [b.run() for b in batches for _ in range(5)]
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+        for out, w in zip(outs, want):
+            assert torch.equal(out, w)
+        for j, m in enumerate(more):
+            assert torch.equal(m, want[j // 5])
+
+
+def test_ops_refuse_what_they_cannot_take():
+    """By an error, before any launch."""
+    from gmlx_amd import ops
+    b = Batch([(1, 40), (2, 20)], 8, 2, 128, 16, F16, seed=1)
+    e = Batch([(1, 40), (2, 20)], 8, 2, 128, 16, F16, q8=True, seed=1)
+    (k, v), q = b.pool, b.q.cuda()
+    x = torch.zeros(3, 2, 128, dtype=F16, device="cuda")
+    slots = torch.zeros(3, dtype=torch.int32, device="cuda")
+
+    def attend(**kw):
+        a = dict(q=q, k_cache=k, v_cache=v, block_table=b.table, kv_lens=b.kv_lens, cu_q=b.cu_q, scale=1.0)
+        ops.sdpa_paged(**{**a, **kw})
+    with_scales = dict(k_cache=e.pool[0], v_cache=e.pool[1], **e.scales)
+    for bad in (dict(q=q.bfloat16()), dict(q=q[:, :3]), dict(q=q[0]), dict(q=q[..., :64]), dict(q=q.cpu()),
+                dict(k_cache=k[:, :, :, :64]), dict(v_cache=v[:2]), dict(k_cache=k.bfloat16()),
+                dict(k_cache=k.float(), v_cache=v.float()), dict(k_cache=k.transpose(2, 3), v_cache=v.transpose(2, 3)),
+                dict(block_table=b.table.long()), dict(block_table=b.table[:1]), dict(block_table=b.table.cpu()),
+                dict(kv_lens=b.kv_lens.long()), dict(cu_q=b.cu_q[:2]), dict(max_q=0), dict(max_kv=-1),
+                dict(out=torch.empty(3, 8, 128, device="cuda")), dict(out=torch.empty(4, 8, 128, dtype=F16, device="cuda")),
+                dict(out=torch.empty(3, 128, 8, dtype=F16, device="cuda").transpose(1, 2)),
+                dict(k_cache=e.pool[0], v_cache=e.pool[1]), {**with_scales, "v_biases": None},
+                {**with_scales, "k_scales": e.scales["k_scales"].bfloat16()},
+                {**with_scales, "k_scales": e.scales["k_scales"][:2]}, {**with_scales, "k_cache": k, "v_cache": v}):
+        with pytest.raises((ValueError, RuntimeError)):
+            attend(**bad)
+    for bad in (dict(k=x.float()), dict(k=x[:2]), dict(v=x[:, :1]), dict(slots=slots.long()), dict(slots=slots[:2]),
+                dict(v_cache=v.bfloat16())):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.paged_write(**{**dict(k=x, v=x, k_cache=k, v_cache=v, slots=slots), **bad})
+    one = torch.ones(2, dtype=torch.int32, device="cuda")
+    plan = dict(seq_lens=one, new_lens=one, block_table=b.table, free_pages=slots, free_count=one[:1], page_size=16,
+                max_tokens=2)
+    for bad in (dict(new_lens=one[:1]), dict(page_size=24), dict(page_size=8), dict(max_tokens=-1),
+                dict(free_count=one), dict(keep_lens=one.long()), dict(block_table=b.table[:1]),
+                dict(seq_lens=torch.ones(3000, dtype=torch.int32, device="cuda"))):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.paged_plan(**{**plan, **bad})
+    attend()
+
+
+def test_calls_without_tokens_or_keys():
+    from gmlx_amd import ops
+    b = Batch([(0, 40), (0, 0)], 8, 2, 128, 16, F16, seed=1)
+    assert b.run().shape == (0, 8, 128)
+    x = torch.zeros(0, 2, 128, dtype=F16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    ops.paged_write(x, x, *b.pool, none)
+    assert ops.paged_read(*b.pool, none)[0].shape == (0, 2, 128)
+    out = torch.full((3, 8, 128), 7.0, dtype=F16, device="cuda")  # all rows padding
+    b.run(q=torch.ones_like(out), out=out)
+    assert (out == 7.0).all()
