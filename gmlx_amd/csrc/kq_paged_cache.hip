@@ -172,10 +172,12 @@ __global__ __launch_bounds__(kPlanThreads) void kq_paged_plan_kernel(PlanArgs a)
         if (i < n_add) {
             const int b = row_of(r.cu, a.B, i);
             if (r.base[b] >= 0) {
-                p = r.base[b] + i - r.cu[b];
-                const int nth = p >> a.lps, fresh = nth - r.pages[b];
-                // (a row that gives pages has want in r.pages, past its last token)
-                const int page = fresh < 0 ? a.table[b * a.table_stride + nth] : stack(total - 1 - (r.take[b] + fresh));
+                p = (int)((uint32_t)r.base[b] + (uint32_t)i - (uint32_t)r.cu[b]);
+                const int nth = p >> a.lps, fresh = nth - r.pages[b], from = total - 1 - (r.take[b] + fresh);
+                // (a row that gives pages has want in r.pages, past its last token;
+                // p and from are only negative where new_lens add up past 31 bits)
+                const int page = p < 0 || (fresh >= 0 && from < 0) ? -1
+                                 : fresh < 0 ? a.table[b * a.table_stride + nth] : stack(from);
                 slot = page < 0 || page >= (0x7fffffff >> a.lps) ? -1 : (page << a.lps) + (p & (P - 1));
             }
         }
@@ -209,12 +211,13 @@ __device__ __forceinline__ int64_t slot_offset(const CopyArgs &a, int slot, int 
     return page * a.p.page_stride + h * a.p.head_stride + (slot & ((1 << a.lps) - 1)) * a.p.token_stride;
 }
 
-// Smallest and largest of v over a group's 8 threads.
-__device__ __forceinline__ void group_range(float &lo, float &hi) {
+// Smallest, largest and sum of what a group's 8 threads hold.
+__device__ __forceinline__ void group_range(float &lo, float &hi, float &odd) {
 #pragma unroll
     for (int off = 1; off < 8; off <<= 1) {
         lo = fminf(lo, __shfl_xor(lo, off));
         hi = fmaxf(hi, __shfl_xor(hi, off));
+        odd += __shfl_xor(odd, off);
     }
 }
 
@@ -237,16 +240,17 @@ __global__ __launch_bounds__(256) void kq_paged_write_kernel(CopyArgs a) {
             x[2 * i] = f16bits_to_f32<BF>(w[i] & 0xFFFFu);
             x[2 * i + 1] = f16bits_to_f32<BF>(w[i] >> 16);
         }
-        float lo = x[0], hi = x[0];
+        float lo = x[0], hi = x[0], odd = x[0] - x[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) {
             lo = fminf(lo, x[i]);
             hi = fmaxf(hi, x[i]);
+            odd += x[i] - x[i];  // NaN from an infinity or NaN (which fminf drops), else 0
         }
-        group_range(lo, hi);
+        group_range(lo, hi, odd);
         // the scale as it is stored: the values are rounded against what is
         // read back; a bias of 16 bits holds lo exactly
-        const uint16_t s16 = from_f32<BF>((hi - lo) / 255.f);
+        const uint16_t s16 = from_f32<BF>((hi - lo) / 255.f + odd);
         const float s = f16bits_to_f32<BF>(s16);
         uint32_t q[2] = {0, 0};
 #pragma unroll
@@ -339,6 +343,8 @@ int kq_paged_plan(const int32_t *seq_lens, const int32_t *keep_lens, const int32
         return KQ_ERR_BAD_SHAPE;
     if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return KQ_ERR_BAD_SHAPE;
     if ((int64_t)table_width * page_size >= (int64_t)1 << 31) return KQ_ERR_BAD_SHAPE;
+    // 31-bit sums of pages
+    if ((int64_t)B * table_width >= 1 << 30 || n_stack >= 1 << 30) return KQ_ERR_BAD_SHAPE;
     const PlanArgs a{seq_lens,       keep_lens, new_lens,     free_count,  block_table, free_pages,
                      cu_q,           kv_lens,   slots,        positions,   free_count_out, refused,
                      table_stride,   B,         table_width,  n_stack,     __builtin_ctz(page_size), max_tokens};

@@ -1363,7 +1363,8 @@ def paged_write(k, v, k_cache, v_cache, slots, k_scales=None, k_biases=None, v_s
     rows' dtype; or, with the four scale / bias tensors [n_pages, Hkv, page_size,
     D / 64] in the rows' dtype, uint8: each 64 values are stored as
     (x - bias) / scale rounded to 0..255, bias their smallest and scale a 255th
-    of their range (the 8-bit affine cache of sdpa_decode_gqa's quantized form).
+    of their range (the 8-bit affine cache of sdpa_decode_gqa's quantized form);
+    64 values with an infinity or NaN among them read back as NaN.
     slots int32 [T] (PagedPlan.slots): page * page_size + place; a slot outside
     the pool (-1) writes nothing.  Slots are distinct: of two rows given the
     same one, which values stay is not specified."""
@@ -1450,9 +1451,9 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     mq = T if max_q is None else min(int(max_q), T)
     mkv = min(width * lay.page_size, (1 << 31) - 1)
     if max_kv is not None:
-        mkv = min(mkv, max(1, int(max_kv)) if max_kv >= 0 else -1)
+        mkv = min(mkv, int(max_kv))
     if mq < 1 or mkv < 1:
-        raise ValueError("sdpa_paged: max_q must be positive and max_kv not negative")
+        raise ValueError("sdpa_paged: max_q and max_kv must be positive")
     need = lib().kq_sdpa_paged_workspace_bytes(T, B, Hq, Hkv, D, mq, mkv, lay.q8)
     s = _stream(q)
     ws_ptr, ws_len = None, 0

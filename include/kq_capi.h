@@ -501,7 +501,9 @@ typedef struct {
  * stay; nothing else of them is written, and the inputs seq_lens and
  * free_count are only read, so the same call made again gives the same.
  * Outputs must not overlap inputs.  Negative lengths count as 0, seq_lens past
- * table_width * page_size as that.  All int32 on the device. */
+ * table_width * page_size as that; the new tokens of all rows are fewer than
+ * 2^31 (of more, cu_q, slots and positions are of no use).  All int32 on the
+ * device.  B * table_width and n_stack below 2^30. */
 #define KQ_PAGED_MAX_ROWS 2048
 int kq_paged_plan(const int32_t *seq_lens, const int32_t *keep_lens, const int32_t *new_lens, int32_t B,
                   int32_t *block_table, int64_t table_stride, int32_t table_width, int32_t *free_pages,
@@ -514,7 +516,8 @@ int kq_paged_plan(const int32_t *seq_lens, const int32_t *keep_lens, const int32
  * outside the pool (negative, as the plan marks them) writes nothing.  An 8-bit
  * pool quantises each 64 values: lo and hi their smallest and largest, scale =
  * (hi - lo) / 255 and bias = lo, both rounded to dtype, q = (x - bias) / scale
- * rounded to nearest even and clamped to 0..255 (0 where scale is 0).  Slots
+ * rounded to nearest even and clamped to 0..255 (0 where scale is 0); a group
+ * that holds an infinity or NaN gets a NaN scale: all of it reads as NaN.  Slots
  * are distinct: of two rows given the same slot, which values stay there is
  * not specified. */
 int kq_paged_write(const kq_paged_pool *pool, const void *k, int64_t k_token_stride, int64_t k_head_stride,
@@ -540,8 +543,8 @@ int kq_paged_read(const kq_paged_pool *pool, const int32_t *slots, int32_t T, vo
  * it holds (infinities and NaN included).
  * max_q: the most new tokens of any row (of a longer row the first max_q are
  * computed); max_kv: the most cached tokens (longer rows are cut to the first
- * max_kv keys); both size the launch and the workspace only.  Hq % Hkv == 0, Hq / Hkv
- * <= 64.
+ * max_kv keys), up to 2^30; both size the launch and the workspace only.  Hq %
+ * Hkv == 0, Hq / Hkv <= 64.
  * Workspace: fp32 split partials, no zero-fill needed; 256-byte aligned; calls
  * that share one are ordered.  A row's result is bitwise that of the call on
  * the row alone. */

@@ -90,6 +90,19 @@ def test_plan_refuses_a_row_that_the_table_cannot_hold():
     _check_plan([-5, 1000, 3, 7], [-1, 0, 2, 1], np.abs(table), stack, count, 16, 8, [0, 999, -4, 7])
 
 
+def test_plan_of_lengths_that_pass_31_bits_together():
+    """Rows too long for the table are refused, the free pages stay, and nothing
+    outside the tables is read or written."""
+    rng = np.random.default_rng(5)
+    table, stack, count = _rows(rng, 4, 16, 3, [16, 20, 0, 5], 6)
+    big = 2 ** 31 - 1
+    got = _device_plan([16, 20, 0, 5], [big, big, big, big], table, stack, count, 16, 3000, None)
+    assert got[5].tolist() == [1, 1, 1, 1] and got[4].tolist() == [6] and (got[2] == -1).all()
+    assert np.array_equal(got[6], table) and np.array_equal(got[7], stack)
+    got = _device_plan([16, 20, 0, 5], [big, big, 3, 3], table, stack, count, 16, 3000, None)
+    assert got[5].tolist() == [1, 1, 0, 0] and ((got[2] >= -1) & (got[2] < 16 * len(stack))).all()
+
+
 def test_plan_ends_requests_and_reuses_their_pages():
     rng = np.random.default_rng(4)
     seq = [100, 33, 17, 64]
@@ -202,6 +215,27 @@ def test_write_and_read_8bit(dt, D, H, P, T, layout):
         # one fp32 rounding, then the 16-bit one
         room = val.abs() * (HALF[dt] + 2.0 ** -23) + tiny
         assert ((back.cpu().double() - val).abs() <= room).all()
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_write_8bit_groups_that_are_not_finite(dt):
+    """The group reads as NaN, the others as before; none hides one as a number."""
+    from gmlx_amd import ops
+    (k, v), sc = _pool((2, 2, 16, 128), dt, True, "head")
+    x = torch.randn(5, 2, 128, device="cuda").to(dt)
+    slots = torch.arange(5, dtype=torch.int32, device="cuda") + 7
+    ops.paged_write(x, x, k, v, slots, **sc)
+    clean = ops.paged_read(k, v, slots, **sc)[0]
+    y = x.clone()
+    y[0, 0, 3], y[1, 1, 64], y[2, 0, 127], y[3, 0, 0] = float("nan"), float("inf"), float("-inf"), float("nan")
+    y[3, 0, 1:64] = 1.0
+    ops.paged_write(y, x, k, v, slots, **sc)
+    got = ops.paged_read(k, v, slots, **sc)
+    bad = torch.zeros(5, 2, 2, dtype=torch.bool, device="cuda")
+    bad[0, 0, 0] = bad[1, 1, 1] = bad[2, 0, 1] = bad[3, 0, 0] = True
+    bad = bad.repeat_interleave(64, -1)
+    assert torch.isnan(got[0][bad]).all() and torch.equal(got[0][~bad], clean[~bad])
+    assert torch.equal(got[1], clean)
 
 
 # ------------------------------------------------------------------- attention
@@ -671,7 +705,7 @@ def test_ops_refuse_what_they_cannot_take():
                 dict(k_cache=k[:, :, :, :64]), dict(v_cache=v[:2]), dict(k_cache=k.bfloat16()),
                 dict(k_cache=k.float(), v_cache=v.float()), dict(k_cache=k.transpose(2, 3), v_cache=v.transpose(2, 3)),
                 dict(block_table=b.table.long()), dict(block_table=b.table[:1]), dict(block_table=b.table.cpu()),
-                dict(kv_lens=b.kv_lens.long()), dict(cu_q=b.cu_q[:2]), dict(max_q=0), dict(max_kv=-1),
+                dict(kv_lens=b.kv_lens.long()), dict(cu_q=b.cu_q[:2]), dict(max_q=0), dict(max_kv=-1), dict(max_kv=0),
                 dict(out=torch.empty(3, 8, 128, device="cuda")), dict(out=torch.empty(4, 8, 128, dtype=F16, device="cuda")),
                 dict(out=torch.empty(3, 128, 8, dtype=F16, device="cuda").transpose(1, 2)),
                 dict(k_cache=e.pool[0], v_cache=e.pool[1]), {**with_scales, "v_biases": None},

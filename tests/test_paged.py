@@ -72,7 +72,7 @@ def test_calls_are_refused():
     for name in ("q", "tab", "lens", "cu", "out"):
         assert sdpa(**{name: None}) == m.KQ_ERR_NULL_POINTER, name
     for bad in (dict(T=-1), dict(B=-1), dict(Hq=12), dict(Hq=0), dict(Hq=8 * 65), dict(mq=0), dict(mkv=0), dict(w=0),
-                dict(ts=3), dict(qs=4088), dict(os=4088), dict(T=1 << 26)):
+                dict(ts=3), dict(qs=4088), dict(os=4088), dict(T=1 << 26), dict(mkv=(1 << 30) + 1)):
         assert sdpa(**bad) == m.KQ_ERR_BAD_SHAPE, bad
     for bad in (dict(q=x + 8), dict(out=x + 2), dict(qs=4100), dict(os=4100)):
         assert sdpa(**bad) == m.KQ_ERR_BAD_ALIGN, bad
@@ -91,7 +91,7 @@ def test_calls_are_refused():
     for name in ("seq", "new", "tab", "st", "cnt", "cu", "kv", "sl", "pos", "left", "ref"):
         assert plan(**{name: None}) == m.KQ_ERR_NULL_POINTER, name
     for bad in (dict(B=0), dict(B=2049), dict(w=0), dict(ts=3), dict(n=-1), dict(T=-1), dict(ps=8), dict(ps=24),
-                dict(ps=2048), dict(w=1 << 28, ts=1 << 28)):
+                dict(ps=2048), dict(w=1 << 28, ts=1 << 28), dict(B=2048, w=1 << 19, ts=1 << 19), dict(n=1 << 30)):
         assert plan(**bad) == m.KQ_ERR_BAD_SHAPE, bad
 
 
