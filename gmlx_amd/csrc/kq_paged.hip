@@ -7,7 +7,23 @@
 //   S^T[tok, col] = K[tok, d] . q^T[d, col],  O^T[d, col] += V^T[d, tok] . P^T[tok, col]
 // so that a lane's scores are the P.V operand it needs (lane 16 g + r holds
 // column r at tokens 4g .. 4g+3 of each 16), and the softmax statistics of a
-// column live in the four lanes that hold it.
+// column live in the four lanes that hold it.  One pass over the keys: a
+// column's running maximum m, sum l of 2^(s - m) and sums O of 2^(s - m) v, all
+// fp32; where a row is split, a merge adds the splits' (m, l, O) in split order.
+//
+// Rounded to 16 bits are the probabilities (an MFMA operand: half a step each,
+// relative, averaged over the keys) and the output, nothing else; 8-bit pools
+// multiply integers or hi + lo planes, exact to fp32.  Probabilities in hi + lo
+// too would double P.V's products and take the error (2-norm, bf16) from 0.0023 to
+// the 0.0017 of the output's own rounding.
+//
+// Few query columns (decode, verify): bound by HBM, one wave a unit streams its
+// keys through registers; 16 rows of 1 k to 131 k keys, head dim 128, 2.01 GB
+// in 371 us, 5.4 TB/s.  Chunks: bound by the MFMA, exp and LDS pipes together,
+// tiles in LDS shared by the workgroup's columns; 2048 tokens behind 6000, head
+// dim 128, 236 GFLOP in 248 us, 950 TFLOP/s (1.19 PFLOP/s for a plain 8192^3
+// product on the same card): MFMA pipes busy 45 % of the cycles, LDS 35 %, a
+// third of that in bank conflicts.
 #include "kq_paged.h"
 
 namespace {
@@ -34,9 +50,18 @@ struct PagedArgs {
     int32_t direct;    // the wave kernel's grid is (split, kv head, row), the merge's (token and head, row)
 };
 
-constexpr int kSplitTokens = 512;   // least keys of a chunk's split
-constexpr int kDirect = 1 << 15;    // waves, and merged tokens and heads, of a direct grid
-constexpr int kMergeGroups = 1024;  // workgroups of a merge that is not
+// Least keys of a chunk's split, where the GPU has room for more workgroups: 512
+// against 256 / 1024 (us): one chunk of 333 tokens over 4200 keys 50 / 50 / 54, 16
+// over 4000 24 / 19 / 40, four of 100 over 1000 34 / 43 / 34, 8 rows of 8 over 2 k
+// to 6 k 43 / 51 / 49, two chunks beside 14 decode rows 147 / 170 / 145.
+constexpr int kSplitTokens = 512;
+// Most waves, and merged tokens and heads, of grids in which each finds its place
+// without a sum over the rows: three rows of 400 to 1700 keys 10.8 us (16.5 with
+// the sum), 8 rows of 4 tokens 43.9 (45), four of 4000 at head dim 512 30 (38);
+// beyond, waves without work cost more than the sums (16 rows of up to 131 k keys
+// 398 against 395, 8-bit 241 against 237.5, at the limit).
+constexpr int kDirect = 1 << 15;
+constexpr int kMergeGroups = 1024;  // workgroups of a merge that is no such grid
 
 // Rows of at most so many columns split as decode rows do and run in waves of 16
 // columns.  Two waves read a row's keys twice, and still beat a chunk's
@@ -51,9 +76,12 @@ __host__ __device__ __forceinline__ bool few_columns(int n, int G, int limit) { 
 // spill: the chunks' kernel takes all rows there).
 constexpr bool has_waves(int D) { return D <= 256; }
 
-// A chunk's workgroup: its waves, query columns (32 a wave, 16 where 32 would take
-// over 256 registers a lane for the sums and the queries), and how many such
-// workgroups the GPU holds at once, which splitting a chunk aims at.
+// A chunk's workgroup: its waves (eight share an 8-bit tile's conversion: 333
+// tokens over 4200 keys at head dim 256 142 us on four, 82 on eight; at 128 85 and
+// 73), query columns (32 a wave, 16 where 32 would take over 256 registers a lane
+// for the sums and the queries: at head dim 256 2048 tokens over 8048 keys 278 us,
+// with 32 400), and how many such workgroups the GPU holds at once, which
+// splitting a chunk aims at (512; half of it: 333 over 4200 50 -> 65).
 constexpr int chunk_waves(int D, bool q8) { return q8 && (D == 128 || D == 256) ? 8 : 4; }
 constexpr int group_columns(int D, bool q8) { return chunk_waves(D, q8) * (D > 128 ? 16 : 32); }
 constexpr int group_slots(int D, bool q8) { return D > 256 || chunk_waves(D, q8) > 4 ? 256 : 512; }
@@ -101,7 +129,8 @@ __device__ __forceinline__ int chunk_units(const PagedArgs &a, const Row &r) {
 }
 // A workgroup's share of a merge: one item where all its threads add up the splits,
 // one a wave where a wave takes several rounds of loads for them, four a wave,
-// loaded ahead, where it takes one.
+// each loaded ahead of the one before, where it takes one (500 tokens in 4 splits
+// beside decode rows 68 us; with one a wave there too 73).
 __device__ __forceinline__ int merge_items(int splits) { return splits > 64 ? 1 : splits > 8 ? 4 : 16; }
 __device__ __forceinline__ int merge_units(const PagedArgs &a, const Row &r) {
     const int items = merge_items(r.splits);
@@ -725,9 +754,10 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
 }
 
 // ---- prompt chunks --------------------------------------------------------
-// Rows of more than 16 query columns: a workgroup of four waves takes 128
-// columns, 32 a wave (64 and 16 past head dim 128), and streams the keys in tiles of BN tokens through two
-// LDS stages, copied by direct-to-LDS loads one tile ahead; one barrier a tile.
+// Rows of more query columns: a workgroup takes 128 (64 for 16-bit pools past
+// head dim 128, 256 for 8-bit ones at 128), 32 or 16 a wave, and streams the keys
+// in tiles of BN tokens through two LDS stages, copied by direct-to-LDS loads one
+// tile ahead; one barrier a tile.
 // v_mfma_f32_32x32x16: lane 32 h + c holds column c at tokens 8 (i / 4) + 4 h +
 // i % 4 (i < 16) of each 32, which are the P.V operand's eight tokens a lane of
 // two 16-token products; V's operand, eight tokens of one head dim a lane, is
@@ -1266,14 +1296,15 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
     }
 }
 
-// Whether rows of few columns run beside chunks in one launch (past head dim 128
-// their tiles take more registers than two waves a SIMD can have).
+// Whether rows of few columns run beside chunks in one launch: a chunk of 500
+// tokens and seven decode rows 68 us, in two launches 75 (past head dim 128 their
+// tiles take more registers than two waves a SIMD can have).
 template <int D>
 constexpr bool kBeside = D <= 128;
 
 // The first `wave_groups` workgroups take rows of few columns, a wave a unit, the
 // others chunks: decode rows, which wait for memory, run beside a prompt
-// chunk's products.
+// chunk's products.  (Eight of each kind in turn instead: 68 -> 81 us.)
 template <int D, bool BF, bool Q8>
 __global__ __launch_bounds__(64 * chunk_waves(D, Q8), D > 256 ? 1 : 2) void kq_paged_kernel(PagedArgs a, int wave_groups) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];

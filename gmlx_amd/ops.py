@@ -20,6 +20,16 @@ Op names and argument orders follow the reference's calls:
                                                  gmlx/deepseek_v4_model.py:1179-1187
   sdpa_decode_gqa(q, k, v, scale, starts=)       gmlx/gemma4_batched_sdpa.py:221-222
   ragged_decode_attention(q, k, v, pads, scale)  gmlx/qwen35_attn.py:395-493
+
+A paged KV cache, which the reference has no counterpart of (its engine keeps one
+left-padded cache a batch): paged_plan (block tables and slots of a step),
+paged_write, paged_read, and sdpa_paged, the attention of decode rows, verify
+blocks and prompt chunks over it.  A step, eager or captured (the state is then
+copied over in place, as here):
+  p = paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_size, T, keep_lens=kept)
+  seq_lens.copy_(p.kv_lens); free_count.copy_(p.free_count)
+  for each layer: paged_write(k, v, k_cache, v_cache, p.slots)
+                  o = sdpa_paged(q, k_cache, v_cache, block_table, p.kv_lens, p.cu_q, scale, max_q=, max_kv=)
 """
 from __future__ import annotations
 

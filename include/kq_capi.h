@@ -1,11 +1,12 @@
 /*
  * kq_capi.h -- C ABI of libgmlx_amd.so, the MI355X (gfx950) K-quant
  * batched-decode hot path: GGUF Q4_K / Q6_K / IQ2_XXS dequant-fused matmuls
- * (dense, grouped, MoE expert gather) and ragged GQA decode attention.
+ * (dense, grouped, MoE expert gather), ragged GQA decode attention, and a paged
+ * KV cache with the attention over it.
  *
- * Every entry point replaces one op of the un-vendored mlx-kquant package that
- * gmlx binds (pyproject.toml:26-34); the reference call site each replaces is
- * cited beside it.  Conventions:
+ * Every entry point but the paged cache's replaces one op of the un-vendored
+ * mlx-kquant package that gmlx binds (pyproject.toml:26-34); the reference call
+ * site each replaces is cited beside it.  Conventions:
  *   - all pointers are device pointers unless stated; the caller owns every
  *     buffer (outputs and workspace included); the library never allocates,
  *     frees or synchronizes;
