@@ -1417,7 +1417,7 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     attends keys 0 .. kv_lens[b] - n + i, query head hq with kv head
     hq // (Hq / Hkv).  A token that sees no key gets zeros.  Returns [T, Hq, D]
     in q's dtype; rows behind the last sequence (cu_q[B] ..) are left as they
-    are in `out` (unspecified where it is not given).
+    are in `out` (unspecified where it is not given; `out` may be q).
 
     k_cache / v_cache and the scale / bias tensors as paged_write has them, in
     q's dtype; block_table int32 [B, pages], kv_lens int32 [B], cu_q int32

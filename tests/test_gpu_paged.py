@@ -739,3 +739,69 @@ def test_calls_without_tokens_or_keys():
     out = torch.full((3, 8, 128), 7.0, dtype=F16, device="cuda")  # all rows padding
     b.run(q=torch.ones_like(out), out=out)
     assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_many_rows(q8):
+    """More rows than a wave scans at once, chunks among them, in a workspace
+    whose slots follow one another."""
+    rng = np.random.default_rng(8)
+    rows = [(1, int(kv)) for kv in rng.integers(1, 900, 140)]
+    for i in range(10):
+        rows.insert(int(rng.integers(0, len(rows))), (int(rng.integers(2, 120)), int(rng.integers(400, 900))))
+    rows[70:70] = [(0, 30), (0, 0), (3, 1)]
+    _say("many rows", len(rows), q8)
+    b = Batch(rows, 8, 2, 64, 32, F16, q8=q8, seed=4)
+    out = b.run()
+    b.check(out)
+    # the longest chunk and a decode row behind it, alone
+    longest = max(range(len(rows)), key=lambda r: rows[r][0])
+    for r in (longest, len(rows) - 1):
+        lo, hi = int(b.cu[r]), int(b.cu[r + 1])
+        from gmlx_amd import ops
+        one = ops.sdpa_paged(b.q[lo:hi].cuda(), *b.pool, b.table[r:r + 1], b.kv_lens[r:r + 1],
+                             torch.tensor([0, hi - lo], dtype=torch.int32, device="cuda"), b.scale, **b.scales)
+        assert torch.equal(one, out[lo:hi])
+
+
+@pytest.mark.parametrize("D,Hq,q8", [(64, 2, False), (128, 4, True), (256, 1, False)])
+def test_long_prompt(D, Hq, q8):
+    """A prompt of 4100 tokens and one of 3000 behind 2000: sampled tokens."""
+    rows = [(4100, 4100), (3000, 5000)]
+    b = Batch(rows, Hq, 1, D, 64, BF16, q8=q8, seed=D)
+    _say("long prompt", D, Hq, q8)
+    out = b.run().double().cpu().numpy()
+    u, rng = HALF[BF16], np.random.default_rng(D)
+    for r, (n, kv) in enumerate(rows):
+        for i in [0, 1, n - 1, *rng.integers(0, n, 12)]:
+            t, see = int(b.cu[r]) + int(i), kv - n + int(i) + 1
+            q, k, v = b.q[t:t + 1].double().numpy(), b.k[r][:, :see], b.v[r][:, :see]
+            want, far = ref.attention(q, k, v, 1, b.scale, b.err[r][:, :see])
+            _, mean = ref.attention(q, k, v, 1, b.scale)
+            smax = 1.5 * b.scale * np.abs(q).sum(-1).max() * max(1.0, np.abs(k).max())
+            f32 = 2.0 ** -24 * (2 * (D + 8) * smax + 2 * see + 16)  # (as Batch.check counts)
+            room = u * np.abs(want) + u * (1 + u) * far + f32 * (mean + far) + 1e-7
+            assert (np.abs(out[t:t + 1] - want) <= room).all(), (r, i)
+
+
+def test_rows_that_share_pages():
+    """A common prefix in the same pages: every row as with pages of its own."""
+    from gmlx_amd import ops
+    P, H, D, n = 16, 2, 128, 12
+    k, v = (torch.randn(n, H, P, D, device="cuda").to(BF16) for _ in range(2))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    shared = torch.tensor([[0, 1, 2, 3, 4], [0, 1, 2, 5, 6], [0, 1, 2, 3, 4]], **i32)
+    lens, cu = torch.tensor([75, 66, 50], **i32), torch.tensor([0, 1, 21, 22], **i32)
+    q = torch.randn(22, 8, D, device="cuda").to(BF16)
+    out = ops.sdpa_paged(q, k, v, shared, lens, cu, 0.1)
+    own = torch.randperm(15, device="cuda").int().view(3, 5)
+    k2, v2 = (torch.zeros(15, H, P, D, dtype=BF16, device="cuda") for _ in range(2))
+    k2[own.long()], v2[own.long()] = k[shared.long()], v[shared.long()]
+    assert torch.equal(out, ops.sdpa_paged(q, k2, v2, own, lens, cu, 0.1))
+
+
+def test_output_in_place_of_the_queries():
+    b = Batch([(1, 3000), (60, 700), (3, 40)], 8, 2, 128, 16, BF16, seed=6)
+    want, q = b.run(), b.q.cuda()
+    b.run(q=q, out=q)
+    assert torch.equal(q, want)
