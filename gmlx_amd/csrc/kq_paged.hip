@@ -127,12 +127,15 @@ template <int D>
 __device__ __forceinline__ int chunk_units(const PagedArgs &a, const Row &r) {
     return has_waves(D) && few_columns(r.n, a.G, a.few_limit) ? 0 : r.blocks * r.splits * a.Hkv;
 }
-// A workgroup's share of a merge: one item where all its threads add up the splits,
+// A workgroup's share of a merge: a quarter of one item where all its threads add up
+// its splits (one row of 131072 keys 105 us, a whole item a workgroup 113),
 // one a wave where a wave takes several rounds of loads for them, four a wave,
 // each loaded ahead of the one before, where it takes one (500 tokens in 4 splits
 // beside decode rows 68 us; with one a wave there too 73).
-__device__ __forceinline__ int merge_items(int splits) { return splits > 64 ? 1 : splits > 8 ? 4 : 16; }
+constexpr int kSlices = 4;
+__device__ __forceinline__ int merge_items(int splits) { return splits > 8 ? 4 : 16; }
 __device__ __forceinline__ int merge_units(const PagedArgs &a, const Row &r) {
+    if (r.splits > 64) return r.n * a.Hq * kSlices;
     const int items = merge_items(r.splits);
     return r.splits > 1 ? (r.n * a.Hq + items - 1) / items : 0;
 }
@@ -1325,19 +1328,19 @@ __device__ __forceinline__ float split_scale(float ms, float m) {
     return ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
 }
 
-// (Token, query head) of n splits by one workgroup: thread t handles the float4
-// of outputs 4 q .. 4 q + 3 (q = t % (D / 4)) for the splits p, p + P, ... (p =
-// t / (D / 4) of P parts), rescaled to the common maximum; the P sums are added
-// in part order through LDS.
-template <int D, bool BF>
-__device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, int n, uint16_t *out) {
-    constexpr int Q = D / 4, P = 256 / Q;
+// (Token, query head) of n splits by one workgroup, or of many splits a quarter
+// of its outputs by each of four (SL): thread t handles the float4 of outputs 4 q
+// .. 4 q + 3 (q = t % Q) for the splits p, p + P, ... (p = t / Q of P parts),
+// rescaled to the common maximum; the P sums are added in part order through LDS.
+template <int D, bool BF, int SL>
+__device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, int n, int slice, uint16_t *out) {
+    constexpr int Q = D / 4 / SL, P = 256 / Q;
     __shared__ float red_m[4];
     __shared__ float4 red_acc[P][Q];
     __shared__ float red_l[P];
     const int t = threadIdx.x, q = t % Q, part = t / Q;
     const float *ml = a.ml + 2 * slot;
-    const float4 *po = (const float4 *)(a.part + slot * D) + q;
+    const float4 *po = (const float4 *)(a.part + slot * D) + slice * Q + q;
     float m = -INFINITY;
     for (int s = t; s < n; s += 256) m = fmaxf(m, ml[2 * s]);
     // this thread's first splits, in flight beside the maximum's loads
@@ -1349,14 +1352,14 @@ __device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, in
         const int s = min(part + k * P, n - 1);
         m_pre[k] = ml[2 * s];
         l_pre[k] = ml[2 * s + 1];
-        o_pre[k] = po[(int64_t)s * Q];
+        o_pre[k] = po[(int64_t)s * (D / 4)];
     }
     m = wave_max(m);
     __syncthreads();  // the last item's reads
     if ((t & 63) == 0) red_m[t >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
-    if (part < P) {  // (D = 96: threads 240 .. 255 hold no part)
+    if (part < P) {  // (D = 96: the last threads hold no part)
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float l = 0.f;
         const auto add = [&](float ms, float ls, const float4 &o) {
@@ -1372,7 +1375,7 @@ __device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, in
         for (int k = 0; k < PRE; ++k)
             if (part + k * P < n) add(m_pre[k], l_pre[k], o_pre[k]);
 #pragma unroll 8
-        for (int s = part + PRE * P; s < n; s += P) add(ml[2 * s], ml[2 * s + 1], po[(int64_t)s * Q]);
+        for (int s = part + PRE * P; s < n; s += P) add(ml[2 * s], ml[2 * s + 1], po[(int64_t)s * (D / 4)]);
         red_acc[part][q] = acc;
         if (q == 0) red_l[part] = l;
     }
@@ -1390,7 +1393,7 @@ __device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, in
             l += red_l[k];
         }
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-        *(u32x2 *)(out + 4 * q) = u32x2{pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv)};
+        *(u32x2 *)(out + 4 * (slice * Q + q)) = u32x2{pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv)};
     }
 }
 
@@ -1474,7 +1477,9 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
     if constexpr (DIRECT) {
         const Row row = lane_row(row_at(a, blockIdx.y), 0);
         const int x = blockIdx.x;
-        if (row.splits > 1 && x < row.n * a.Hq) merge_group<D, BF>(a, slot(row, 0, x), row.splits, out(row, x));
+        if (row.splits <= 1 || x >= row.n * a.Hq) return;
+        if (row.splits > 64) merge_group<D, BF, kSlices>(a, slot(row, 0, x), row.splits, blockIdx.z, out(row, x));
+        else if (blockIdx.z == 0) merge_group<D, BF, 1>(a, slot(row, 0, x), row.splits, 0, out(row, x));
         return;
     }
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -1494,7 +1499,8 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
                 now = next;
             }
         } else {
-            merge_group<D, BF>(a, slot(row, slot0, u), n, out(row, u));
+            const int x = u / kSlices;
+            merge_group<D, BF, kSlices>(a, slot(row, slot0, x), n, u - x * kSlices, out(row, x));
         }
     }
 }
@@ -1672,8 +1678,8 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
         if (g.groups) g.beside = (int)(n < (1 << 13) ? n : (1 << 13));
     }
     if (plan.slots) {
-        const int64_t n = plan.few > 8 || plan.many > 8 ? items * B : (int64_t)T * Hq / 16 + B;
-        g.merge = a.direct ? dim3((unsigned)items, B) : dim3((unsigned)(n < kMergeGroups ? n : kMergeGroups));
+        const int64_t n = most > 64 ? kSlices * items * B : most > 8 ? items * B : (int64_t)T * Hq / 16 + B;
+        g.merge = a.direct ? dim3((unsigned)items, B, most > 64 ? kSlices : 1) : dim3((unsigned)(n < kMergeGroups ? n : kMergeGroups));
     }
     const bool q8 = a.ks != nullptr, bf = pool->dtype == KQ_DTYPE_BF16;
     hipStream_t s = (hipStream_t)stream;

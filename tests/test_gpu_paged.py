@@ -805,3 +805,22 @@ def test_output_in_place_of_the_queries():
     want, q = b.run(), b.q.cuda()
     b.run(q=q, out=q)
     assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,q8", [(64, 8, 2, False), (96, 6, 3, False), (128, 8, 2, True), (256, 4, 2, False),
+                                         (512, 2, 1, False)])
+def test_rows_of_many_splits(D, Hq, Hkv, q8, monkeypatch):
+    """More splits than a wave's lanes, with direct grids and with a chunk beside
+    them, whose grids are not; the bits of the long row are the same."""
+    monkeypatch.setenv("GMLX_KQ_SDPA_SPLIT", "64")
+    rows = [(1, 9000), (2, 4500), (1, 300), (0, 7)]
+    _say("many splits", D, q8)
+    a = Batch(rows, Hq, Hkv, D, 32, BF16, q8=q8, seed=D)
+    b = Batch(rows + [(60, 900)], Hq, Hkv, D, 32, BF16, q8=q8, seed=D)
+    out, more = a.run(), b.run()
+    a.check(out)
+    b.check(more)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    from gmlx_amd import ops
+    one = ops.sdpa_paged(b.q[:1].cuda(), *b.pool, b.table[:1], b.kv_lens[:1], cu, b.scale, **b.scales)
+    assert torch.equal(one, more[:1])
