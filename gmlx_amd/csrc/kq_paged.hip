@@ -321,6 +321,7 @@ struct Tile16 {
 // 8 bytes as 16-bit floats of their integer values less Z (0 or 128), exactly.
 template <bool BF, int Z>
 __device__ __forceinline__ u32x4 bytes8(u32x2 q) {
+    static_assert(Z == 0 || Z == 128, "as they are, or signed");
     if constexpr (!BF) {
         const half2_t z = {(_Float16)(1024.f + Z), (_Float16)(1024.f + Z)};
         auto pair = [&](uint32_t w, uint32_t sel) {
@@ -331,9 +332,17 @@ __device__ __forceinline__ u32x4 bytes8(u32x2 q) {
         // fp32 values of at most 8 significant bits: their upper halves are
         // the bf16 values
         auto pair = [&](uint32_t w, int j) {
-            const float x = (float)((w >> (8 * j)) & 0xFFu) - (float)Z, y = (float)((w >> (8 * j + 8)) & 0xFFu) - (float)Z;
+            float x, y;
+            if constexpr (Z == 0) {
+                x = (float)((w >> (8 * j)) & 0xFFu);
+                y = (float)((w >> (8 * j + 8)) & 0xFFu);
+            } else {  // (signed bytes convert in one step)
+                x = (float)(int8_t)(w >> (8 * j));
+                y = (float)(int8_t)(w >> (8 * j + 8));
+            }
             return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
         };
+        if constexpr (Z != 0) q = u32x2{q.x ^ 0x80808080u, q.y ^ 0x80808080u};
         return u32x4{pair(q.x, 0), pair(q.x, 2), pair(q.y, 0), pair(q.y, 2)};
     }
 }
