@@ -824,3 +824,19 @@ def test_rows_of_many_splits(D, Hq, Hkv, q8, monkeypatch):
     from gmlx_amd import ops
     one = ops.sdpa_paged(b.q[:1].cuda(), *b.pool, b.table[:1], b.kv_lens[:1], cu, b.scale, **b.scales)
     assert torch.equal(one, more[:1])
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("D", [64, 256])
+def test_scales_of_zero_and_below(D, q8):
+    """A negative scale is the positive one of -q (whose products the matrix cores
+    need not round to the opposite of q's: each against fp64); 0 weighs all alike."""
+    b = Batch([(1, 700), (3, 90), (70, 500)], 8, 2, D, 32, F16, q8=q8, seed=D)
+    q = b.q.cuda()
+    b.scale = -b.scale
+    out = b.run()
+    b.scale, b.q = -b.scale, -b.q
+    b.check(out)
+    zero = b.run(q=torch.zeros_like(q))
+    b.scale = 0.0
+    assert torch.equal(b.run(), zero) and torch.isfinite(zero).all()
