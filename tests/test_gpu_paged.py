@@ -840,3 +840,20 @@ def test_scales_of_zero_and_below(D, q8):
     zero = b.run(q=torch.zeros_like(q))
     b.scale = 0.0
     assert torch.equal(b.run(), zero) and torch.isfinite(zero).all()
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,q8", [(64, 4, 1, False), (128, 4, 2, True), (256, 2, 1, False)])
+def test_long_contexts(D, Hq, Hkv, q8):
+    """Rows of 40 k to 70 k keys; each row's bits alone with its own bound, too."""
+    from gmlx_amd import ops
+    rows = [(1, 65535), (1, 65536), (2, 70001), (1, 40000)]
+    _say("long contexts", D, q8)
+    b = Batch(rows, Hq, Hkv, D, 256, F16, q8=q8, seed=D)
+    out = b.run()
+    b.check(out)
+    for r, (n, kv) in enumerate(rows):
+        lo = int(b.cu[r])
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        one = ops.sdpa_paged(b.q[lo:lo + n].cuda(), *b.pool, b.table[r:r + 1], b.kv_lens[r:r + 1], cu, b.scale, max_q=n,
+                             max_kv=kv, **b.scales)
+        assert torch.equal(one, out[lo:lo + n]), (n, kv)
