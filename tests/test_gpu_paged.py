@@ -857,3 +857,40 @@ def test_long_contexts(D, Hq, Hkv, q8):
         one = ops.sdpa_paged(b.q[lo:lo + n].cuda(), *b.pool, b.table[r:r + 1], b.kv_lens[r:r + 1], cu, b.scale, max_q=n,
                              max_kv=kv, **b.scales)
         assert torch.equal(one, out[lo:lo + n]), (n, kv)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 8, 2), (128, 8, 2), (256, 8, 2), (512, 4, 1)])
+def test_8bit_values_past_the_largest_fp16(D, Hq, Hkv):
+    """A group from 0 to 65504 has the scale 257, and its largest value is 65535:
+    in K and in V, for a decode row and a chunk over the same pages."""
+    from gmlx_amd import ops
+    gen, kv, P = torch.Generator(device="cuda").manual_seed(D), 333, 32
+    n = -(-kv // P)
+    (k, v), sc = _pool((n, Hkv, P, D), F16, True, "head")
+    x, y = (torch.rand(kv, Hkv, D, device="cuda", generator=gen) * 60000 for _ in range(2))
+    x[:, :, 5::64] = y[::2, :, 5::64] = 65504.0
+    x[:, :, 6::64] = y[:, :, 6::64] = 0.0
+    ops.paged_write(x.half(), y.half(), k, v, torch.arange(kv, dtype=torch.int32, device="cuda"), **sc)
+    vals = []
+    for pool, name in ((k, "k"), (v, "v")):
+        q, s, bi = (t.transpose(1, 2).reshape(n * P, Hkv, -1)[:kv].double()
+                    for t in (pool, sc[name + "_scales"], sc[name + "_biases"]))
+        s, bi = s.repeat_interleave(64, -1), bi.repeat_interleave(64, -1)
+        # (rounded probabilities multiply the values, or the centred integers times the scale)
+        vals += [(s * q + bi).transpose(0, 1).cpu().numpy(),
+                 torch.maximum((s * q + bi).abs(), (s * (q - 128)).abs()).transpose(0, 1).cpu().numpy()]
+    assert vals[0].max() == vals[2].max() == 65535.0
+    for m in (1, 40):
+        q = (torch.randn(m, Hq, D, device="cuda", generator=gen) * 1e-4).half()
+        i32 = dict(dtype=torch.int32, device="cuda")
+        _say("past fp16", D, m)
+        out = ops.sdpa_paged(q, k, v, torch.arange(n, **i32)[None], torch.tensor([kv], **i32),
+                             torch.tensor([0, m], **i32), D ** -0.5, **sc)
+        qd = q.double().cpu().numpy()
+        want, far = ref.attention(qd, vals[0], vals[2], m, D ** -0.5, vals[3])
+        smax = 1.5 * D ** -0.5 * np.abs(qd).sum(-1).max() * np.abs(vals[0]).max()
+        # (as Batch.check counts, and the rounding of a value's second half: 2^-22)
+        f32 = 2.0 ** -24 * (2 * (D + 8) * smax + 2 * kv + 16) + 2.0 ** -22
+        room = HALF[F16] * np.abs(want) + HALF[F16] * (1 + HALF[F16]) * far + f32 * 2 * far + 1e-7
+        d = np.abs(out.double().cpu().numpy() - want)
+        assert np.isfinite(d).all() and (d <= room).all(), (m, (d / room).max())
