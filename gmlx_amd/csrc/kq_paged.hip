@@ -102,18 +102,21 @@ __host__ __device__ __forceinline__ int paged_splits(const SplitRule &rule, int 
 }
 
 struct Row {
-    int q0;       // first query row
-    int n, full;  // tokens computed, tokens of the row
-    int kv;       // keys
+    int q0;      // first query row
+    int n;       // tokens computed
+    int kv;      // keys attended: the row's, cut by max_kv and the table's width
+    int before;  // cached tokens before the new ones, uncut (below 0: more new ones than cached)
     int blocks, splits;
 };
 
 __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     Row r;
     r.q0 = min(max(a.cu_q[b], 0), a.T);
-    r.full = min(max(a.cu_q[b + 1], r.q0), a.T) - r.q0;
-    r.n = min(r.full, a.max_q);
-    r.kv = (int)min((int64_t)max(min(a.kv_lens[b], a.max_kv), 0), (int64_t)a.width << a.lps);
+    const int n = min(max(a.cu_q[b + 1], r.q0), a.T) - r.q0, kv = max(a.kv_lens[b], 0);
+    r.n = min(n, a.max_q);
+    r.kv = (int)min((int64_t)min(kv, a.max_kv), (int64_t)a.width << a.lps);
+    // what a token sees goes by the row as it is, of which a cut leaves keys out
+    r.before = kv - n;
     r.blocks = row_blocks(r.n, a.G, few_columns(r.n, a.G, a.few_limit) ? a.few_cols : a.group_cols);
     r.splits = paged_splits(a.rule, r.n, r.kv, a.G, a.Hkv, a.few_limit, a.group_cols, a.group_slots);
     return r;
@@ -184,8 +187,8 @@ __device__ __forceinline__ Row lane_row(const Row &x, int src) {
     Row r;
     r.q0 = __builtin_amdgcn_readlane(x.q0, src);
     r.n = __builtin_amdgcn_readlane(x.n, src);
-    r.full = __builtin_amdgcn_readlane(x.full, src);
     r.kv = __builtin_amdgcn_readlane(x.kv, src);
+    r.before = __builtin_amdgcn_readlane(x.before, src);
     r.blocks = __builtin_amdgcn_readlane(x.blocks, src);
     r.splits = __builtin_amdgcn_readlane(x.splits, src);
     return r;
@@ -621,7 +624,7 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
         State<D, BF, Q8> st;
         st.init();
         // keys seen: the column's, the block's least and most
-        const int first = row.kv - row.full + 1;
+        const int first = row.before + 1;
         const int seen = live ? max(first + i, 0) : 0x7fffffff;
         const int least = max(first + 16 * blk / a.G, 0);
         const int most = min(max(first + min((16 * blk + 15) / a.G, row.n - 1), 0), row.kv);
@@ -1103,7 +1106,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
         const int col = col0 + c;
         const bool live = col < cols;
         const int i = live ? col / a.G : row.n - 1, hq = kvh * a.G + (live ? col - i * a.G : 0);
-        const auto seen_by = [&](int cl) { return max(row.kv - row.full + min(cl, cols - 1) / a.G + 1, 0); };
+        const auto seen_by = [&](int cl) { return max(row.before + 1 + min(cl, cols - 1) / a.G, 0); };
         const int seen = live ? min(seen_by(col), row.kv) : 0x7fffffff;
         const int least = __builtin_amdgcn_readfirstlane(seen_by(col0));
         const int most = __builtin_amdgcn_readfirstlane(col0 < cols ? min(seen_by(col0 + COLS - 1), row.kv) : 0);

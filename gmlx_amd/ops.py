@@ -1424,7 +1424,8 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     [B + 1] on the device, read there only.  max_q (default T) and max_kv
     (default pages * page_size): the most new and cached tokens of any row;
     they size the launch, and of a row with more only the first max_q tokens
-    are computed and only the first max_kv keys attended.  Entries of the table
+    are computed and only the first max_kv keys attended (token i sees those of
+    them up to kv_lens[b] - n + i).  Entries of the table
     that are no page of the pool are not attended.  D in 64, 96, 128, 256, 512
     (no 96 in 8 bits), Hq / Hkv up to 64.  A row's result is bitwise that of a
     call on the row alone."""

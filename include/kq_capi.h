@@ -545,9 +545,10 @@ int kq_paged_read(const kq_paged_pool *pool, const int32_t *slots, int32_t T, vo
  * not seen.  A key that a token does not see cannot reach its output, whatever
  * it holds (infinities and NaN included).
  * max_q: the most new tokens of any row (of a longer row the first max_q are
- * computed); max_kv: the most cached tokens (longer rows are cut to the first
- * max_kv keys), up to 2^30; both size the launch and the workspace only.  Hq %
- * Hkv == 0, Hq / Hkv <= 64.
+ * computed); max_kv: the most cached tokens, up to 2^30.  Of a row with more, or
+ * with more than table_width pages hold, only the first of its keys are attended:
+ * token i sees keys up to kv_lens[b] - n + i as ever, of those.  Both size the
+ * launch and the workspace only.  Hq % Hkv == 0, Hq / Hkv <= 64.
  * Workspace: fp32 split partials, no zero-fill needed; 256-byte aligned; calls
  * that share one are ordered.  A row's result is bitwise that of the call on
  * the row alone. */

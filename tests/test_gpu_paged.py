@@ -894,3 +894,39 @@ def test_8bit_values_past_the_largest_fp16(D, Hq, Hkv):
         room = HALF[F16] * np.abs(want) + HALF[F16] * (1 + HALF[F16]) * far + f32 * 2 * far + 1e-7
         d = np.abs(out.double().cpu().numpy() - want)
         assert np.isfinite(d).all() and (d <= room).all(), (m, (d / room).max())
+
+
+def _check_tokens(b, out, cut, take=None):
+    """As Batch.check, token by token, of rows cut to their first `cut` keys (and
+    `take` tokens): token i sees keys up to kv - n + i, of those."""
+    u, got = HALF[b.dt], out.double().cpu().numpy()
+    for r, (n, kv) in enumerate(b.rows):
+        for i in range(n if take is None else min(n, take)):
+            t, see = int(b.cu[r]) + i, max(0, min(kv - n + i + 1, cut))
+            q, k, v = b.q[t:t + 1].double().numpy(), b.k[r][:, :see], b.v[r][:, :see]
+            want, far = ref.attention(q, k, v, 1, b.scale, b.err[r][:, :see])
+            _, mean = ref.attention(q, k, v, 1, b.scale)
+            smax = 1.5 * b.scale * np.abs(q).sum(-1).max() * max(1.0, np.abs(k).max() if see else 1.0)
+            f32 = 2.0 ** -24 * (2 * (q.shape[-1] + 8) * smax + 2 * see + 16)
+            room = u * np.abs(want) + u * (1 + u) * far + f32 * (mean + far) + 1e-7
+            d = np.abs(got[t:t + 1] - want)
+            assert np.isfinite(d).all() and (d <= room).all(), (r, n, kv, i, cut, (d / room).max())
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,q8,dt", [(128, 8, 2, False, F16), (128, 8, 2, True, BF16), (256, 4, 2, False, BF16),
+                                            (256, 4, 2, True, F16), (64, 4, 4, True, F16), (96, 6, 2, False, F16),
+                                            (512, 2, 1, False, F16)])
+def test_cut_rows_keep_their_causal_line(D, Hq, Hkv, q8, dt):
+    """max_kv, or a table narrower than a row, leaves keys out and moves nothing:
+    fewer keys than new tokens among them."""
+    from gmlx_amd import ops
+    rows = [(6, 100), (2, 50), (1, 700), (90, 90), (40, 333), (1, 64), (3, 5), (40, 1300)]
+    b = Batch(rows, Hq, Hkv, D, 16, dt, q8=q8, seed=D)
+    for cut in (1, 17, 64, 200, 1290):
+        _say("cut", D, q8, cut)
+        _check_tokens(b, b.run(max_kv=cut), cut)
+    full = torch.full((b.T, Hq, D), 7.0, dtype=dt, device="cuda")
+    b.run(max_kv=48, max_q=5, out=full)
+    _check_tokens(b, full, 48, take=5)
+    narrow = ops.sdpa_paged(b.q.cuda(), *b.pool, b.table[:, :4].contiguous(), b.kv_lens, b.cu_q, b.scale, **b.scales)
+    _check_tokens(b, narrow, 64)
