@@ -1608,15 +1608,32 @@ Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max
 
 size_t part_bytes(int64_t slots, int D) { return ((size_t)slots * D * 4 + 255) & ~(size_t)255; }
 
+// Whether 32-bit numbers count a call's tokens and heads, partials and units (a
+// grid's step past the last of them too).  Units of the two kernels apart, since
+// a chunk of many columns has few splits however many keys it has: blocks and
+// splits of a row come to group_slots / Hkv, or to its blocks alone.
+bool numbers_fit(const Plan &p, int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max_kv, bool q8) {
+    constexpr int64_t kMost = ((int64_t)1 << 31) - (1 << 17);
+    if (T * Hq > (1 << 30) || B > (1 << 20) || max_kv > (1 << 30) || p.slots >= (int64_t)1 << 31) return false;
+    const int G = Hq / Hkv, limit = few_limit(q8), cols = group_columns(D, q8);
+    const int64_t rows = T < B ? T : B;
+    const int few_blocks = has_waves(D) ? (limit + 15) / 16 : 1;
+    const int64_t few = G <= limit ? rows * few_blocks * Hkv * p.few : 0;
+    const int64_t many = rows * group_slots(D, q8) + (T * G / cols + rows) * Hkv;
+    return has_waves(D) ? few < kMost && many < kMost : few + many < kMost;
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t kq_sdpa_paged_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
                                      int32_t max_kv, int q8) {
-    if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_q <= 0 || max_kv <= 0) return 0;
-    const int64_t slots = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, q8 != 0).slots;
-    return slots ? part_bytes(slots, D) + (size_t)slots * 8 : 0;
+    if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_q <= 0 || max_kv <= 0 || max_kv > (1 << 30) ||
+        (int64_t)T * Hq > (1 << 30))
+        return 0;
+    const Plan p = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, q8 != 0);
+    return p.slots && numbers_fit(p, T, B, Hq, Hkv, D, max_q, max_kv, q8 != 0) ? part_bytes(p.slots, D) + (size_t)p.slots * 8 : 0;
 }
 
 int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int32_t *block_table,
@@ -1627,18 +1644,16 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     if (T == 0 || B == 0) return KQ_OK;
     if (!q || !block_table || !kv_lens || !cu_q || !out) return KQ_ERR_NULL_POINTER;
     const int Hkv = pool->Hkv, D = pool->D;
-    if (T < 0 || B < 0 || B > (1 << 20) || Hq <= 0 || Hq % Hkv || Hq / Hkv > 64 || max_q < 1 || max_kv < 1 ||
+    if (T < 0 || B < 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 64 || max_q < 1 || max_kv < 1 ||
         table_width < 1 || table_stride < table_width)
         return KQ_ERR_BAD_SHAPE;
-    // (31-bit token numbers, a split past the last key among them)
+    // (31-bit key numbers, a split past the last key among them)
     if ((int64_t)T * Hq > (1 << 30) || max_kv > (1 << 30) || q_stride < (int64_t)Hq * D || out_stride < (int64_t)Hq * D)
         return KQ_ERR_BAD_SHAPE;
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_stride | out_stride) & 7)) return KQ_ERR_BAD_ALIGN;
     const Plan plan = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr);
     const int64_t most = plan.few > plan.many ? plan.few : plan.many;
-    // 31-bit unit and partial numbers
-    if (plan.slots >= (int64_t)1 << 31 || ((int64_t)T * (Hq / Hkv) + B) * Hkv * most >= (int64_t)1 << 31)
-        return KQ_ERR_BAD_SHAPE;
+    if (!numbers_fit(plan, T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr)) return KQ_ERR_BAD_SHAPE;
     const size_t need = plan.slots ? part_bytes(plan.slots, D) + (size_t)plan.slots * 8 : 0;
     if (need && (!workspace || workspace_bytes < need)) return KQ_ERR_WORKSPACE_TOO_SMALL;
     if (need && ((uintptr_t)workspace & 255)) return KQ_ERR_BAD_ALIGN;

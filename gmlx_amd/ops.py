@@ -1422,13 +1422,13 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     k_cache / v_cache and the scale / bias tensors as paged_write has them, in
     q's dtype; block_table int32 [B, pages], kv_lens int32 [B], cu_q int32
     [B + 1] on the device, read there only.  max_q (default T) and max_kv
-    (default pages * page_size): the most new and cached tokens of any row;
-    they size the launch, and of a row with more only the first max_q tokens
-    are computed and only the first max_kv keys attended (token i sees those of
-    them up to kv_lens[b] - n + i).  Entries of the table
-    that are no page of the pool are not attended.  D in 64, 96, 128, 256, 512
-    (no 96 in 8 bits), Hq / Hkv up to 64.  A row's result is bitwise that of a
-    call on the row alone."""
+    (default pages * page_size, at most 2^30): the most new and cached tokens of
+    any row; they size the launch, and of a row with more only the first max_q
+    tokens are computed and only the first max_kv keys attended (token i sees
+    those of them up to kv_lens[b] - n + i).  Entries of the table that are no
+    page of the pool are not attended.  D in 64, 96, 128, 256, 512 (no 96 in 8
+    bits), Hq / Hkv up to 64.  A row's result is bitwise that of a call on the
+    row alone."""
     _fault("sdpa_paged")
     lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
     dev, dt, Hkv, D, B, shape = lay.device, lay.dtype, lay.Hkv, lay.D, kv_lens.numel(), q.shape
@@ -1460,7 +1460,7 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     elif T == 1:
         qt = Hq * D
     mq = T if max_q is None else min(int(max_q), T)
-    mkv = min(width * lay.page_size, (1 << 31) - 1)
+    mkv = min(width * lay.page_size, 1 << 30)
     if max_kv is not None:
         mkv = min(mkv, int(max_kv))
     if mq < 1 or mkv < 1:

@@ -549,6 +549,10 @@ int kq_paged_read(const kq_paged_pool *pool, const int32_t *slots, int32_t T, vo
  * with more than table_width pages hold, only the first of its keys are attended:
  * token i sees keys up to kv_lens[b] - n + i as ever, of those.  Both size the
  * launch and the workspace only.  Hq % Hkv == 0, Hq / Hkv <= 64.
+ * Limits (KQ_ERR_BAD_SHAPE; the workspace's size is then 0): T * Hq <= 2^30, B <=
+ * 2^20, fewer than 2^31 partials (a workspace of 8 + 4 D bytes each), and, rows of
+ * few columns having at most max_kv / 512 splits past 32768 keys, min(T, B) * Hkv
+ * splits below 2^30.
  * Workspace: fp32 split partials, no zero-fill needed; 256-byte aligned; calls
  * that share one are ordered.  A row's result is bitwise that of the call on
  * the row alone. */

@@ -930,3 +930,17 @@ def test_cut_rows_keep_their_causal_line(D, Hq, Hkv, q8, dt):
     _check_tokens(b, full, 48, take=5)
     narrow = ops.sdpa_paged(b.q.cuda(), *b.pool, b.table[:, :4].contiguous(), b.kv_lens, b.cu_q, b.scale, **b.scales)
     _check_tokens(b, narrow, 64)
+
+
+def test_tables_of_more_keys_than_a_row_can_have():
+    """The default bound of a table of 2^31 places is the most keys of a row."""
+    from gmlx_amd import ops
+    i32 = dict(dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(3, 1, 1024, 64, device="cuda").half() for _ in range(2))
+    table = torch.full((1, 1 << 21), -1, **i32)
+    table[0, :3] = torch.tensor([2, 0, 1], **i32)
+    q = torch.randn(1, 2, 64, device="cuda").half()
+    lens, cu = torch.tensor([2500], **i32), torch.tensor([0, 1], **i32)
+    want = ops.sdpa_paged(q, k, v, table[:, :3].contiguous(), lens, cu, 0.125)
+    _say("wide table")
+    assert torch.equal(ops.sdpa_paged(q, k, v, table, lens, cu, 0.125), want)

@@ -200,3 +200,35 @@ def test_register_copies_stand_behind_the_restore_of_exec(tmp_path):
     text = out.read_text()
     assert "kq_paged_wave_kernel" in text
     assert not _before_exec(text)
+
+
+def _sdpa(T, B, Hq, mkv, mq=None, ws=None, n=0, scale=0.1, **pool):
+    """kq_sdpa_paged of a pool of pages, on addresses that no launch would get to."""
+    m, L = _lib()
+    x = 1 << 26
+    return L.kq_sdpa_paged(x, Hq * 128, ctypes.byref(_pool(**pool)), x, 1 << 17, 1 << 17, x, x, T, B, Hq, mq or T, mkv, scale,
+                           x, Hq * 128, ws, n, None)
+
+
+@pytest.mark.parametrize("T,B,Hq", [(16384, 1, 64), (16384, 64, 64), (32768, 1, 32), (8192, 2048, 128), (1 << 20, 16, 8),
+                                    (2048, 2048, 32)])
+def test_long_prompts_over_long_tables_are_taken(T, B, Hq):
+    """A chunk has few splits however many keys there may be: not refused, and
+    its partials bounded (a million keys; asked without the workspace)."""
+    m, L = _lib()
+    need = L.kq_sdpa_paged_workspace_bytes(T, B, Hq, 8, 128, T, 1 << 20, 0)
+    few = min(T, B * (16 // (Hq // 8)))  # tokens of rows of up to 16 columns, in splits of 512 keys
+    assert 0 < need <= (few * Hq * 2048 + B * 512 * 128) * (128 * 4 + 8) + 256
+    assert _sdpa(T, B, Hq, 1 << 20) == m.KQ_ERR_WORKSPACE_TOO_SMALL
+    assert _sdpa(T, B, Hq, 1 << 20, ws=1 << 30, n=need - 1) == m.KQ_ERR_WORKSPACE_TOO_SMALL
+
+
+def test_calls_past_31_bit_numbers_are_refused():
+    """Partials, or waves, that 32-bit numbers cannot count."""
+    m, L = _lib()
+    for T, B, Hq, mq, kv in ((1 << 20, 1 << 20, 8, 1, 1 << 30), (1 << 19, 1 << 19, 8, 1, 1 << 27)):
+        assert _sdpa(T, B, Hq, kv, mq=mq) == m.KQ_ERR_BAD_SHAPE
+        assert L.kq_sdpa_paged_workspace_bytes(T, B, Hq, 8, 128, mq, kv, 0) == 0
+    # arguments that the call refuses by themselves need no workspace either
+    assert L.kq_sdpa_paged_workspace_bytes(2 ** 31 - 1, 4, 2 ** 31 - 1, 1, 128, 4, 2 ** 31 - 1, 0) == 0
+    assert L.kq_sdpa_paged_workspace_bytes(4, 4, 8, 8, 128, 4, (1 << 30) + 1, 0) == 0
