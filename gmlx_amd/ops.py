@@ -1469,11 +1469,12 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     s = _stream(q)
     ws_ptr, ws_len = None, 0
     if need:
-        # (a captured call's own, from its graph's pool: graphs captured on one
-        # stream may be replayed on two at once)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if torch.cuda.is_current_stream_capturing() else \
-            _WS.get("sdpa_paged", dev, s.value, need)
-        ws_ptr, ws_len = ws.data_ptr(), ws.numel()
+        # the call's own, given back in stream order: partials are written before
+        # they are read, and a long step's are too many to keep for later ones (a
+        # captured call's are its graph's: graphs captured on one stream may be
+        # replayed on two at once)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws_ptr, ws_len = ws.data_ptr(), need
     _paged_call("kq_sdpa_paged", dev, q.data_ptr(), qt, pool, tab, tab_stride, width, lens, cu, T, B, Hq, mq, mkv,
                 float(scale), out.data_ptr(), ot, ws_ptr, ws_len, s)
     return out

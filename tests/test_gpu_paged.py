@@ -944,3 +944,23 @@ def test_tables_of_more_keys_than_a_row_can_have():
     want = ops.sdpa_paged(q, k, v, table[:, :3].contiguous(), lens, cu, 0.125)
     _say("wide table")
     assert torch.equal(ops.sdpa_paged(q, k, v, table, lens, cu, 0.125), want)
+
+
+def test_calls_keep_no_memory():
+    """An eager call's partials go back to torch's allocator with the call: as
+    large as asked for, none kept for later calls or other streams."""
+    b = Batch([(1, 6000), (1, 3000), (3, 900), (70, 2000)], 8, 2, 128, 16, F16, seed=1)
+    want, q = b.run(), b.q.cuda()
+    out = torch.zeros_like(q)
+    from gmlx_amd import _lib
+    need = _lib.lib().kq_sdpa_paged_workspace_bytes(b.T, 4, 8, 2, 128, b.T, 16 * b.table.shape[1], 0)
+    for stream in (torch.cuda.Stream(), torch.cuda.Stream()):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            before = torch.cuda.memory_allocated()
+            torch.cuda.reset_peak_memory_stats()
+            b.run(q=q, out=out)
+            assert torch.cuda.memory_allocated() == before
+            assert torch.cuda.max_memory_allocated() - before <= need + (2 << 20)  # (torch's blocks)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
