@@ -47,6 +47,7 @@ struct PagedArgs {
     // slots a token and query head, or 0: a row's slots follow those of the rows
     // before it (a chunk's tokens have fewer splits than a decode row's)
     int32_t slot_stride;
+    int32_t slots;       // of the workspace
     int32_t few_blocks;  // the most 16-column blocks of a row of few columns
     int32_t direct;    // the wave kernel's grid is (split, kv head, row), the merge's (token and head, row)
 };
@@ -180,6 +181,13 @@ __device__ __forceinline__ float wave_max(float v) {
 __device__ __forceinline__ int64_t slot_of(const PagedArgs &a, const Row &r, int slot0, int i, int hq) {
     if (a.slot_stride) return ((int64_t)(r.q0 + i) * a.Hq + hq) * a.slot_stride;
     return slot0 + (i * a.Hq + hq) * r.splits;
+}
+
+// Whether a row's partials lie in the workspace: its size counts every query row
+// once, and a cu_q that runs backwards may count some twice.  Such rows are left
+// out, by all kernels alike (the row is the same in a whole workgroup).
+__device__ __forceinline__ bool has_slots(const PagedArgs &a, const Row &r, int slot0) {
+    return a.slot_stride || r.splits <= 1 || (slot0 >= 0 && slot0 <= a.slots - row_slots(a, r));
 }
 
 // Row x of lane src, in scalar registers.
@@ -611,6 +619,7 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
         } else {
             int u = unit;
             if (!find_unit(a, [&](const Row &x) { return wave_units(a, x); }, u, b, row, slot0)) return;
+            if (!has_slots(a, row, slot0)) continue;
             const int head = u / row.blocks;
             blk = u - head * row.blocks;
             s = head / a.Hkv;
@@ -1097,6 +1106,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
         int u = unit, b, slot0;
         Row row;
         if (!find_unit(a, [&](const Row &x) { return chunk_units<D>(a, x); }, u, b, row, slot0)) return;
+        if (!has_slots(a, row, slot0)) continue;
         const int rest = u / a.Hkv, kvh = u - rest * a.Hkv;
         // the tiles with the most keys first
         const int back = rest / row.splits, s = rest - back * row.splits, blk = row.blocks - 1 - back;
@@ -1510,6 +1520,7 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
         int u = item, b, slot0;
         Row row;
         if (!find_unit(a, [&](const Row &x) { return merge_units(a, x); }, u, b, row, slot0)) return;
+        if (!has_slots(a, row, slot0)) continue;
         const int n = row.splits, items = merge_items(n), end = min((u + 1) * items, row.n * a.Hq);
         if (n <= 64) {
             int x = u * items + w;
@@ -1580,6 +1591,8 @@ SplitRule wave_rule(int Hq, int Hkv, int D, bool q8) {
 struct Plan {
     SplitRule rule;
     int few, many;    // the most splits of a row of few columns, of a chunk
+    int few_blocks;   // (PagedArgs)
+    bool direct;      // (PagedArgs)
     int64_t slots;    // of the workspace
     int slot_stride;  // (PagedArgs)
 };
@@ -1590,31 +1603,44 @@ Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max
     p.rule = wave_rule(Hq, Hkv, D, q8);
     p.few = chunk > 1 ? most_row_splits(p.rule, max_kv) : 1;
     p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, limit, group_columns(D, q8), group_slots(D, q8)) : 1;
-    const int most = p.few > p.many ? p.few : p.many;
-    if (most < 2) {
-        p.slots = p.slot_stride = 0;
-        return p;
-    }
-    // one slot a token, query head and split; and of a row, of few columns at
-    // most few_limit of them a kv head, a chunk's at most group_slots
-    // workgroups' columns (it has splits <= group_slots / workgroups)
+    const int64_t most = p.few > p.many ? p.few : p.many;
+    const int64_t columns = (int64_t)max_q * G < limit ? (int64_t)max_q * G : limit;
+    p.few_blocks = (int)(columns + 15) / 16;
+    // One slot a token, query head and split, where a token's place gives its
+    // slots (by_token); or, where slots follow those of the rows before, tokens of
+    // rows of few columns at their splits and the others at a chunk's (by_row).  A
+    // chunk has at most group_slots workgroups' columns (splits <= group_slots /
+    // workgroups), a row of few columns few_limit a kv head.
+    const int64_t tokens = T < B * max_q ? T : B * max_q, few_tokens = tokens < B * (limit / G) ? tokens : B * (limit / G);
+    const int64_t rest = p.few < p.many ? tokens : tokens - few_tokens;  // (the more of the two)
+    const int64_t chunk_row = (int64_t)group_slots(D, q8) * group_columns(D, q8);
+    const int64_t chunks = B < T / chunk ? B : T / chunk;
+    const int64_t chunk_slots = rest * Hq * p.many < chunks * chunk_row ? rest * Hq * p.many : chunks * chunk_row;
     const int64_t by_token = T * Hq * most;
-    const int64_t few_row = (int64_t)limit * Hkv * p.few, many_row = p.many > 1 ? group_slots(D, q8) * group_columns(D, q8) : 0;
-    const int64_t by_row = B * (few_row > many_row ? few_row : many_row);
-    p.slots = by_token < by_row ? by_token : by_row;
-    p.slot_stride = by_token <= by_row ? most : 0;
+    const int64_t by_row = (p.few > 1 ? few_tokens * Hq * p.few : 0) + (p.many > 1 ? chunk_slots : 0);
+    // Direct grids need the first; where padding makes it more than any rows could
+    // take, they are not worth its memory.
+    const int64_t few_row = (int64_t)limit * Hkv * p.few, many_row = p.many > 1 ? chunk_row : 0;
+    const int64_t waves = (int64_t)p.few * p.few_blocks * Hkv * B, items = (max_q < T ? max_q : T) * Hq;
+    p.direct = B < (1 << 16) && waves <= kDirect && items * B <= kDirect &&
+               (most < 2 || by_token <= B * (few_row > many_row ? few_row : many_row));
+    p.slots = most < 2 ? 0 : p.direct || by_token < by_row ? by_token : by_row;
+    p.slot_stride = most > 1 && p.slots == by_token ? (int)most : 0;
     return p;
 }
 
+// 31-bit numbers of tokens and heads, and of keys (a split past the last among them).
+bool sizes_fit(int64_t T, int64_t B, int Hq, int max_kv) { return T * Hq <= (1 << 30) && B <= (1 << 20) && max_kv <= (1 << 30); }
+
 size_t part_bytes(int64_t slots, int D) { return ((size_t)slots * D * 4 + 255) & ~(size_t)255; }
 
-// Whether 32-bit numbers count a call's tokens and heads, partials and units (a
-// grid's step past the last of them too).  Units of the two kernels apart, since
+// Whether 32-bit numbers count a call's partials and units (a grid's step past
+// the last of them too).  Units of the two kernels apart, since
 // a chunk of many columns has few splits however many keys it has: blocks and
 // splits of a row come to group_slots / Hkv, or to its blocks alone.
-bool numbers_fit(const Plan &p, int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max_kv, bool q8) {
+bool numbers_fit(const Plan &p, int64_t T, int64_t B, int Hq, int Hkv, int D, bool q8) {
     constexpr int64_t kMost = ((int64_t)1 << 31) - (1 << 17);
-    if (T * Hq > (1 << 30) || B > (1 << 20) || max_kv > (1 << 30) || p.slots >= (int64_t)1 << 31) return false;
+    if (p.slots >= (int64_t)1 << 31) return false;
     const int G = Hq / Hkv, limit = few_limit(q8), cols = group_columns(D, q8);
     const int64_t rows = T < B ? T : B;
     const int few_blocks = has_waves(D) ? (limit + 15) / 16 : 1;
@@ -1629,11 +1655,11 @@ extern "C" {
 
 size_t kq_sdpa_paged_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
                                      int32_t max_kv, int q8) {
-    if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_q <= 0 || max_kv <= 0 || max_kv > (1 << 30) ||
-        (int64_t)T * Hq > (1 << 30))
+    if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hkv > 1024 || D <= 0 || max_q <= 0 || max_kv <= 0 ||
+        !sizes_fit(T, B, Hq, max_kv))
         return 0;
     const Plan p = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, q8 != 0);
-    return p.slots && numbers_fit(p, T, B, Hq, Hkv, D, max_q, max_kv, q8 != 0) ? part_bytes(p.slots, D) + (size_t)p.slots * 8 : 0;
+    return p.slots && numbers_fit(p, T, B, Hq, Hkv, D, q8 != 0) ? part_bytes(p.slots, D) + (size_t)p.slots * 8 : 0;
 }
 
 int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int32_t *block_table,
@@ -1647,13 +1673,11 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     if (T < 0 || B < 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 64 || max_q < 1 || max_kv < 1 ||
         table_width < 1 || table_stride < table_width)
         return KQ_ERR_BAD_SHAPE;
-    // (31-bit key numbers, a split past the last key among them)
-    if ((int64_t)T * Hq > (1 << 30) || max_kv > (1 << 30) || q_stride < (int64_t)Hq * D || out_stride < (int64_t)Hq * D)
-        return KQ_ERR_BAD_SHAPE;
+    if (!sizes_fit(T, B, Hq, max_kv) || q_stride < (int64_t)Hq * D || out_stride < (int64_t)Hq * D) return KQ_ERR_BAD_SHAPE;
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_stride | out_stride) & 7)) return KQ_ERR_BAD_ALIGN;
     const Plan plan = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr);
     const int64_t most = plan.few > plan.many ? plan.few : plan.many;
-    if (!numbers_fit(plan, T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr)) return KQ_ERR_BAD_SHAPE;
+    if (!numbers_fit(plan, T, B, Hq, Hkv, D, pool->k_scales != nullptr)) return KQ_ERR_BAD_SHAPE;
     const size_t need = plan.slots ? part_bytes(plan.slots, D) + (size_t)plan.slots * 8 : 0;
     if (need && (!workspace || workspace_bytes < need)) return KQ_ERR_WORKSPACE_TOO_SMALL;
     if (need && ((uintptr_t)workspace & 255)) return KQ_ERR_BAD_ALIGN;
@@ -1694,16 +1718,15 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     a.ml = (float *)((char *)workspace + part_bytes(plan.slots, D));
     a.rule = plan.rule;
     a.slot_stride = plan.slot_stride;
+    a.slots = (int32_t)plan.slots;
+    a.few_blocks = plan.few_blocks;
+    a.direct = plan.direct;
     // Bounds of the units; past them the grids' waves and workgroups take the
     // rest in turn.  Where a wave or workgroup for every unit that the longest
     // rows would have is no large grid, each finds its own from its place there;
     // else they sum over the rows' units.
     Grid g;
-    a.few_blocks = (int)(((int64_t)max_q * a.G < a.few_limit ? (int64_t)max_q * a.G : a.few_limit) + 15) / 16;
-    const int64_t rows = T < B ? T : B, waves = (int64_t)plan.few * a.few_blocks * Hkv * B;
-    const int64_t items = (int64_t)(max_q < T ? max_q : T) * Hq;
-    a.direct = (plan.slot_stride || !plan.slots) && B < (1 << 16) && Hkv < (1 << 16) && waves <= kDirect &&
-               items * B <= kDirect;
+    const int64_t rows = T < B ? T : B, items = (int64_t)(max_q < T ? max_q : T) * Hq;
     g.waves = g.merge = dim3(0);
     const int64_t many = (((int64_t)T * a.G + a.group_cols - 1) / a.group_cols + rows) * Hkv *
                          (has_waves(D) ? plan.many : most);

@@ -964,3 +964,29 @@ def test_calls_keep_no_memory():
             assert torch.cuda.max_memory_allocated() - before <= need + (2 << 20)  # (torch's blocks)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_malformed_rows_stay_inside_the_workspace():
+    """A cu_q that counts tokens many times over, in a workspace that holds each
+    once: rows past its end are left out, and nothing behind it is written."""
+    from gmlx_amd import _lib
+    L, T, B, Hq, Hkv, D = _lib.lib(), 500, 300, 8, 2, 128
+    b = Batch([(1, 3000)], Hq, Hkv, D, 16, F16, seed=1)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cu = torch.zeros(B + 1, **i32)
+    cu[1::2], cu[2::4] = T, T - 3  # (500 tokens, none, 3, none again and again)
+    table = b.table.repeat(B, 1)
+    q = torch.randn(T, Hq, D, device="cuda").half()
+    out = torch.zeros_like(q)
+    need = L.kq_sdpa_paged_workspace_bytes(T, B, Hq, Hkv, D, T, 3000, 0)
+    ws = torch.full((need + (64 << 20),), 77, dtype=torch.uint8, device="cuda")
+    (k, v), n = b.pool, b.table.shape[1]
+    pool = _lib.PagedPool(k=k.data_ptr(), v=v.data_ptr(), page_stride=k.stride(0), head_stride=k.stride(1),
+                          token_stride=k.stride(2), n_pages=k.shape[0], page_size=16, Hkv=Hkv, D=D, dtype=_lib.DTYPE_F16)
+    _say("malformed rows", need)
+    import ctypes
+    rc = L.kq_sdpa_paged(q.data_ptr(), Hq * D, ctypes.byref(pool), table.data_ptr(), n, n,
+                         torch.full((B,), 3000, **i32).data_ptr(), cu.data_ptr(), T, B, Hq, T, 3000, D ** -0.5, out.data_ptr(),
+                         Hq * D, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0 and (ws[need:] == 77).all()

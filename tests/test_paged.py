@@ -232,3 +232,12 @@ def test_calls_past_31_bit_numbers_are_refused():
     # arguments that the call refuses by themselves need no workspace either
     assert L.kq_sdpa_paged_workspace_bytes(2 ** 31 - 1, 4, 2 ** 31 - 1, 1, 128, 4, 2 ** 31 - 1, 0) == 0
     assert L.kq_sdpa_paged_workspace_bytes(4, 4, 8, 8, 128, 4, (1 << 30) + 1, 0) == 0
+
+
+def test_workspace_counts_each_token_once():
+    """A step of 300 rows, a prompt among them: tokens of rows of few columns at
+    their splits, the rest at a chunk's (64 at most on 8 kv heads)."""
+    _, L = _lib()
+    T, B, Hq, few, many = 2348, 300, 32, 131072 // 512, 64
+    need = L.kq_sdpa_paged_workspace_bytes(T, B, Hq, 8, 128, 2048, 131072, 0)
+    assert 0 < need <= (4 * B * few + (T - 4 * B) * many) * Hq * (128 * 4 + 8) + 256
