@@ -1356,7 +1356,9 @@ __global__ __launch_bounds__(64 * chunk_waves(D, Q8), D > 256 ? 1 : 2) void kq_p
 }
 
 // Scale of a split of maximum ms beside the common maximum m; a split without
-// keys holds zeros and counts nothing, one of NaN scores has a NaN sum l.
+// keys holds zeros and counts nothing, one of NaN scores has a NaN sum l.  Splits
+// of scale 0 are added like any other: of a NaN or infinite value a token sees, 0
+// times it remains, as within a split.
 __device__ __forceinline__ float split_scale(float ms, float m) {
     return ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
 }
@@ -1397,7 +1399,6 @@ __device__ __forceinline__ void merge_group(const PagedArgs &a, int64_t slot, in
         float l = 0.f;
         const auto add = [&](float ms, float ls, const float4 &o) {
             const float f = split_scale(ms, m);
-            if (f == 0.f && ls == ls) return;
             l += f * ls;
             acc.x += f * o.x;
             acc.y += f * o.y;
@@ -1472,9 +1473,8 @@ struct WaveMerge {
 #pragma unroll
                 for (int k = 0; k < P; ++k) {
                     if (s0 + k >= n) break;
-                    const float fs = lane_of(f, s0 + k), lk = lane_of(ls, s0 + k);
-                    if (fs == 0.f && lk == lk) continue;
-                    l[k] += fs * lk;
+                    const float fs = lane_of(f, s0 + k);
+                    l[k] += fs * lane_of(ls, s0 + k);
 #pragma unroll
                     for (int x = 0; x < V; ++x) acc[k][x] += fs * o[r][k][x];
                 }

@@ -990,3 +990,38 @@ def test_malformed_rows_stay_inside_the_workspace():
                          Hq * D, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     assert rc == 0 and (ws[need:] == 77).all()
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,q8", [(128, 8, 2, False), (128, 8, 2, True), (64, 4, 1, False), (256, 4, 2, False)])
+@pytest.mark.parametrize("split", [None, "64"])
+def test_values_of_far_smaller_keys(D, Hq, Hkv, q8, split, monkeypatch):
+    """A NaN among the values that a token sees is in its output, though the whole
+    split's probabilities round to 0 beside another's."""
+    if split:
+        monkeypatch.setenv("GMLX_KQ_SDPA_SPLIT", split)  # (past 64 splits: the other merge)
+    from gmlx_amd import ops
+    rows = [(1, 5000), (40, 3000), (2, 900)]
+    b = Batch(rows, Hq, Hkv, D, 16, BF16, q8=q8, seed=D)
+    q = torch.ones(b.T, Hq, D, dtype=BF16, device="cuda")
+    k, v = b.pool
+    for r in range(len(rows)):  # the first 640 keys score 1000 below the others
+        for t in range(0, 640, 16):
+            page = int(b.table[r, t // 16])
+            if q8:
+                k[page], b.scales["k_scales"][page], b.scales["k_biases"][page] = 0, 0.0, -1000 * D ** -0.5
+            else:
+                k[page] = -1000 * D ** -0.5
+    clean = b.run(q=q)
+    assert torch.isfinite(clean).all()
+    for r in range(len(rows)):
+        page = int(b.table[r, 1])
+        if q8:
+            b.scales["v_biases"][page, 0, 3, 0] = float("nan")
+        else:
+            v[page, 0, 3, 5] = float("nan")
+    _say("far NaN", D, q8, split)
+    out = b.run(q=q)
+    G, dims = Hq // Hkv, slice(0, 64) if q8 else slice(5, 6)
+    assert torch.isnan(out[:, :G, dims]).all()
+    out[:, :G, dims] = clean[:, :G, dims]
+    assert torch.equal(out, clean)
