@@ -252,14 +252,16 @@ __global__ __launch_bounds__(256) void kq_paged_write_kernel(CopyArgs a) {
             odd += x[i] - x[i];  // NaN from an infinity or NaN (which fminf drops), else 0
         }
         group_range(lo, hi, odd);
+        // (bf16 values can be further apart than fp32's largest: halves of all then)
+        const float part = BF && !(hi - lo <= 3.4028235e38f) ? 0.5f : 1.f;
         // the scale as it is stored: the values are rounded against what is
         // read back; a bias of 16 bits holds lo exactly
-        const uint16_t s16 = from_f32<BF>((hi - lo) / 255.f + odd);
+        const uint16_t s16 = from_f32<BF>((hi * part - lo * part) / (255.f * part) + odd);
         const float s = f16bits_to_f32<BF>(s16);
         uint32_t q[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float v = s == 0.f ? 0.f : fminf(fmaxf(rintf((x[i] - lo) / s), 0.f), 255.f);
+            const float v = s == 0.f ? 0.f : fminf(fmaxf(rintf((x[i] * part - lo * part) / (s * part)), 0.f), 255.f);
             q[i >> 2] |= (uint32_t)v << (8 * (i & 3));
         }
         *(u32x2 *)((uint8_t *)(kv ? a.p.v : a.p.k) + to + 8 * c) = u32x2{q[0], q[1]};

@@ -1025,3 +1025,29 @@ def test_values_of_far_smaller_keys(D, Hq, Hkv, q8, split, monkeypatch):
     assert torch.isnan(out[:, :G, dims]).all()
     out[:, :G, dims] = clean[:, :G, dims]
     assert torch.equal(out, clean)
+
+
+def test_write_8bit_ranges_past_fp32():
+    """bf16 groups whose largest and smallest value are further apart than fp32's
+    largest: finite, and quantised as any other."""
+    from gmlx_amd import ops
+    (k, v), sc = _pool((2, 1, 16, 128), BF16, True, "head")
+    x = torch.rand(9, 1, 128, dtype=torch.float64, generator=torch.Generator().manual_seed(1)) * 6e38 - 3e38
+    x[:, :, 64:] /= 4  # (a range that fp32 holds)
+    x[:, :, 3], x[:, :, 7] = 3.2e38, -3.2e38
+    x = x.to(BF16)
+    slots = torch.arange(9, dtype=torch.int32, device="cuda")
+    _say("wide range")
+    ops.paged_write(x.cuda(), x.cuda(), k, v, slots, **sc)
+    got = ops.paged_read(k, v, slots, **sc)
+    _, want_s, want_b = _quantised(x, BF16)
+    for pool, name, back in ((k, "k", got[0]), (v, "v", got[1])):
+        q = pool[0, :, :9].transpose(0, 1).cpu().unflatten(-1, (-1, 64)).double()
+        s, b = (sc[name + t][0, :, :9].transpose(0, 1).cpu() for t in ("_scales", "_biases"))
+        assert torch.equal(b, want_b) and torch.isfinite(s.float()).all()
+        s, ws, b = s.double()[..., None], want_s.double()[..., None], b.double()[..., None]
+        assert ((s - ws).abs() <= ws * torch.finfo(BF16).eps).all()
+        ideal = ((x.double().unflatten(-1, (-1, 64)) - b) / s).clamp(0, 255)
+        assert ((q - ideal).abs() <= 0.5 + 255 * 2.0 ** -22).all()
+        val = (q * s + b).flatten(-2)
+        assert ((back.cpu().double() - val).abs() <= val.abs() * (HALF[BF16] + 2.0 ** -23)).all()
