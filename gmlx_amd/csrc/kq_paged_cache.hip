@@ -1,5 +1,7 @@
 // The paged KV cache's bookkeeping and copies (kq_capi.h): kq_paged_plan,
 // kq_paged_write, kq_paged_read.
+#include <algorithm>
+
 #include "kq_paged.h"
 
 int kq_pool_check(const kq_paged_pool *p) {
@@ -318,6 +320,26 @@ void launch_copy_d(const CopyArgs &a, bool write, hipStream_t s) {
     }
 }
 
+// Whether no two places of K and V lie on the same memory as far as the strides
+// and bases tell: each stride passes what the smaller ones reach (a page or head
+// that is repeated by a stride of 0 does not), and K is not V.  Rows written to
+// such places by different threads would be mixed.
+bool places_apart(const kq_paged_pool &p) {
+    struct { int64_t stride, n; } d[3] = {{p.token_stride, p.page_size}, {p.head_stride, p.Hkv}, {p.page_stride, p.n_pages}};
+    std::sort(d, d + 3, [](const auto &x, const auto &y) { return x.stride < y.stride; });
+    __int128 reach = p.D;
+    for (const auto &x : d) {
+        if (x.n == 1) continue;
+        if (x.stride < reach) return false;
+        reach += (__int128)x.stride * (x.n - 1);
+    }
+    const void *at[4] = {p.k_scales, p.k_biases, p.v_scales, p.v_biases};
+    for (int i = 0; p.k_scales && i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (at[i] == at[j]) return false;
+    return p.k != p.v;
+}
+
 int copy_rows(const CopyArgs &a, bool write, kq_stream_t stream) {
     // 32-bit item numbers
     if ((int64_t)a.T * a.p.Hkv * (a.p.D / 8) >= (int64_t)1 << 31) return KQ_ERR_BAD_SHAPE;
@@ -366,6 +388,7 @@ int kq_paged_write(const kq_paged_pool *pool, const void *k, int64_t k_token_str
     if (T == 0) return KQ_OK;
     if (!k || !v || !slots) return KQ_ERR_NULL_POINTER;
     if (T < 0) return KQ_ERR_BAD_SHAPE;
+    if (!places_apart(*pool)) return KQ_ERR_BAD_ARGUMENT;
     if ((((uintptr_t)k | (uintptr_t)v) & 15) || ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7))
         return KQ_ERR_BAD_ALIGN;
     const CopyArgs a{*pool,

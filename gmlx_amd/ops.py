@@ -1377,7 +1377,8 @@ def paged_write(k, v, k_cache, v_cache, slots, k_scales=None, k_biases=None, v_s
     64 values with an infinity or NaN among them read back as NaN.
     slots int32 [T] (PagedPlan.slots): page * page_size + place; a slot outside
     the pool (-1) writes nothing.  Slots are distinct: of two rows given the
-    same one, which values stay is not specified."""
+    same one, which values stay is not specified.  A pool that repeats pages or
+    heads (an expanded view), or whose K is its V, is refused here."""
     _fault("paged_write")
     lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
     dev, dt, shape = lay.device, lay.dtype, k.shape

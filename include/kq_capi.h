@@ -522,7 +522,9 @@ int kq_paged_plan(const int32_t *seq_lens, const int32_t *keep_lens, const int32
  * rounded to nearest even and clamped to 0..255 (0 where scale is 0); a group
  * that holds an infinity or NaN gets a NaN scale: all of it reads as NaN.  Slots
  * are distinct: of two rows given the same slot, which values stay there is
- * not specified. */
+ * not specified.  A pool whose places share memory (a page or head repeated by a
+ * stride below what it passes over, K that is V) can be read and attended but not
+ * written: KQ_ERR_BAD_ARGUMENT. */
 int kq_paged_write(const kq_paged_pool *pool, const void *k, int64_t k_token_stride, int64_t k_head_stride,
                    const void *v, int64_t v_token_stride, int64_t v_head_stride, const int32_t *slots,
                    int32_t T, kq_stream_t stream);

@@ -1051,3 +1051,24 @@ def test_write_8bit_ranges_past_fp32():
         assert ((q - ideal).abs() <= 0.5 + 255 * 2.0 ** -22).all()
         val = (q * s + b).flatten(-2)
         assert ((back.cpu().double() - val).abs() <= val.abs() * (HALF[BF16] + 2.0 ** -23)).all()
+
+
+def test_writes_to_pools_that_repeat_places_are_refused():
+    from gmlx_amd import KQError, ops
+    x = torch.ones(3, 2, 128, dtype=F16, device="cuda")
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    base = torch.zeros(2, 4, 1, 16, 128, dtype=F16, device="cuda")
+    one = torch.zeros(4, 2, 16, 128, dtype=F16, device="cuda")
+    for k, v in ((base[0].expand(4, 2, 16, 128), base[1].expand(4, 2, 16, 128)), (one, one)):
+        with pytest.raises(KQError):
+            ops.paged_write(x, x, k, v, slots)
+        assert not k.any()
+        ops.paged_read(k, v, slots)
+    # layouts that interleave without sharing are taken
+    for layout in ("head", "token", "mixed"):
+        (k, v), _ = _pool((4, 2, 16, 128), F16, False, layout)
+        ops.paged_write(x, x, k, v, slots)
+        assert int(k.sum()) == int(v.sum()) == 3 * 2 * 128
+    (k, v), _ = _pool((1, 1, 16, 64), F16, False, "token")
+    ops.paged_write(x[:, :1, :64], x[:, :1, :64], k, v, slots)
+    assert int(k.sum()) == 3 * 64

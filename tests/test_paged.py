@@ -241,3 +241,20 @@ def test_workspace_counts_each_token_once():
     T, B, Hq, few, many = 2348, 300, 32, 131072 // 512, 64
     need = L.kq_sdpa_paged_workspace_bytes(T, B, Hq, 8, 128, 2048, 131072, 0)
     assert 0 < need <= (4 * B * few + (T - 4 * B) * many) * Hq * (128 * 4 + 8) + 256
+
+
+def test_writes_to_places_that_share_memory_are_refused():
+    """Pools that repeat a page or a head (expanded views), or whose K is their V;
+    they can be read and attended."""
+    m, L = _lib()
+    x = 1 << 26
+
+    def write(**kw):
+        return L.kq_paged_write(ctypes.byref(_pool(**kw)), x, 1024, 128, x, 1024, 128, x, 4, None)
+    for kw in (dict(page_stride=0), dict(head_stride=0), dict(head_stride=128), dict(page_stride=16 * 128), dict(v=1 << 20),
+               dict(**{**Q8, "v_scales": Q8["k_scales"]})):
+        assert write(**kw) == m.KQ_ERR_BAD_ARGUMENT, kw
+    # one page, one head: their strides are never used
+    assert write(page_stride=0, n_pages=1, k=None) == m.KQ_ERR_NULL_POINTER
+    for kw in (dict(head_stride=0), dict(page_stride=0), dict(v=1 << 20)):
+        assert L.kq_paged_read(ctypes.byref(_pool(**kw)), x, 4, x + 8, x, None) == m.KQ_ERR_BAD_ALIGN
