@@ -1129,14 +1129,15 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
 
         State st;
         st.init();
-        // scores are products times |scale|
-        const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-        const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // (0 times a hidden key's -inf)
+        // scores are products of the queries with the scale's sign, times its size;
+        // of queries of 0 where it is 0, since 0 times a hidden key's -inf is NaN
+        const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.f ? 0u : ~0u;
+        const float scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
         const uint16_t *qp = a.q + (int64_t)(row.q0 + i) * a.q_stride + (int64_t)hq * D;
 #pragma unroll
         for (int d = 0; d < State::NQ; ++d) {
             const u32x4 v = *(const u32x4 *)(qp + State::qd(d));
-            st.qf[d] = __builtin_bit_cast(half8_t, live ? v ^ u32x4{flip, flip, flip, flip} : u32x4{0u, 0u, 0u, 0u});
+            st.qf[d] = __builtin_bit_cast(half8_t, live ? (v & keep) ^ flip : u32x4{0u, 0u, 0u, 0u});
         }
 
         if (t_end > t_begin) {

@@ -1072,3 +1072,13 @@ def test_writes_to_pools_that_repeat_places_are_refused():
     (k, v), _ = _pool((1, 1, 16, 64), F16, False, "token")
     ops.paged_write(x[:, :1, :64], x[:, :1, :64], k, v, slots)
     assert int(k.sum()) == 3 * 64
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,q8", [(64, 4, 2, False), (128, 8, 2, False), (128, 8, 2, True), (256, 4, 2, False)])
+def test_scale_of_zero_with_large_products(D, Hq, Hkv, q8):
+    """0 weighs all keys alike, products near fp32's largest too."""
+    b = Batch([(1, 300), (40, 333)], Hq, Hkv, D, 16, BF16, q8=q8, seed=D, spread=1e17)
+    q = b.q.cuda() * 1e17
+    b.scale = 0.0
+    _say("zero scale", D, q8)
+    assert torch.equal(b.run(q=q), b.run(q=torch.zeros_like(q)))
