@@ -1674,6 +1674,8 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     if (T < 0 || B < 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 64 || max_q < 1 || max_kv < 1 ||
         table_width < 1 || table_stride < table_width)
         return KQ_ERR_BAD_SHAPE;
+    // (in the kernels' log2 units, too)
+    if (!(fabsf(scale * 1.4426950408889634f) <= 3.4028235e38f)) return KQ_ERR_BAD_ARGUMENT;
     if (!sizes_fit(T, B, Hq, max_kv) || q_stride < (int64_t)Hq * D || out_stride < (int64_t)Hq * D) return KQ_ERR_BAD_SHAPE;
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_stride | out_stride) & 7)) return KQ_ERR_BAD_ALIGN;
     const Plan plan = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr);

@@ -1428,8 +1428,8 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     tokens are computed and only the first max_kv keys attended (token i sees
     those of them up to kv_lens[b] - n + i).  Entries of the table that are no
     page of the pool are not attended.  D in 64, 96, 128, 256, 512 (no 96 in 8
-    bits), Hq / Hkv up to 64.  A row's result is bitwise that of a call on the
-    row alone."""
+    bits), Hq / Hkv up to 64, scale any finite number up to 2.3e38.  A row's
+    result is bitwise that of a call on the row alone."""
     _fault("sdpa_paged")
     lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
     dev, dt, Hkv, D, B, shape = lay.device, lay.dtype, lay.Hkv, lay.D, kv_lens.numel(), q.shape

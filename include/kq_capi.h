@@ -554,7 +554,8 @@ int kq_paged_read(const kq_paged_pool *pool, const int32_t *slots, int32_t T, vo
  * Limits (KQ_ERR_BAD_SHAPE; the workspace's size is then 0): T * Hq <= 2^30, B <=
  * 2^20, fewer than 2^31 partials (a workspace of 8 + 4 D bytes each), and, rows of
  * few columns having at most max_kv / 512 splits past 32768 keys, min(T, B) * Hkv
- * splits below 2^30.
+ * splits below 2^30.  A scale that is NaN, infinite or past 2.3e38 is refused
+ * (KQ_ERR_BAD_ARGUMENT).
  * Workspace: fp32 split partials, no zero-fill needed; 256-byte aligned; calls
  * that share one are ordered.  A row's result is bitwise that of the call on
  * the row alone. */

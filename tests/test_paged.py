@@ -258,3 +258,10 @@ def test_writes_to_places_that_share_memory_are_refused():
     assert write(page_stride=0, n_pages=1, k=None) == m.KQ_ERR_NULL_POINTER
     for kw in (dict(head_stride=0), dict(page_stride=0), dict(v=1 << 20)):
         assert L.kq_paged_read(ctypes.byref(_pool(**kw)), x, 4, x + 8, x, None) == m.KQ_ERR_BAD_ALIGN
+
+
+def test_scales_that_are_no_numbers_are_refused():
+    """NaN, infinities, and what passes fp32 in the kernels' log2 units."""
+    m, _ = _lib()
+    for scale in (float("nan"), float("inf"), float("-inf"), 3e38, -3e38):
+        assert _sdpa(4, 2, 32, 64, scale=scale) == m.KQ_ERR_BAD_ARGUMENT, scale
