@@ -1082,3 +1082,13 @@ def test_scale_of_zero_with_large_products(D, Hq, Hkv, q8):
     b.scale = 0.0
     _say("zero scale", D, q8)
     assert torch.equal(b.run(q=q), b.run(q=torch.zeros_like(q)))
+
+
+def test_plan_sizes_past_32_bits_are_refused():
+    """And not cut to their low bits."""
+    from gmlx_amd import ops
+    i32 = dict(dtype=torch.int32, device="cuda")
+    one, table = torch.ones(1, **i32), torch.zeros(1, 4, **i32)
+    for page, tokens in ((2 ** 32 + 16, 4), (16, 2 ** 31), (16, 2 ** 32 + 4)):
+        with pytest.raises(ValueError, match="paged_plan"):
+            ops.paged_plan(one, one, table, one, one, page, tokens)
