@@ -25,6 +25,7 @@
 // dim 128, 236 GFLOP in 248 us, 950 TFLOP/s (1.19 PFLOP/s for a plain 8192^3
 // product on the same card): MFMA pipes busy 45 % of the cycles, LDS 35 %, a
 // third of that in bank conflicts.
+#include "kq_once.h"
 #include "kq_paged.h"
 
 namespace {
@@ -1551,9 +1552,13 @@ int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
     if (g.groups) {
         constexpr int lds = Chunk<D, Q8>::kLds + 16;  // (and a flag)
         static_assert(lds <= 160 << 10, "LDS of a CU");
-        static const bool ok = hipFuncSetAttribute((const void *)kq_paged_kernel<D, BF, Q8>,
-                                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
-        if (!ok) return KQ_ERR_LAUNCH_FAILED;
+        static OncePerDevice raised;
+        int device = -1;
+        if (hipGetDevice(&device) != hipSuccess || !raised(device, [] {
+                return hipFuncSetAttribute((const void *)kq_paged_kernel<D, BF, Q8>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           lds) == hipSuccess;
+            }))
+            return KQ_ERR_LAUNCH_FAILED;
         constexpr int NW = chunk_waves(D, Q8);
         const int beside = kBeside<D> ? (g.beside + NW - 1) / NW : 0;
         hipLaunchKernelGGL((kq_paged_kernel<D, BF, Q8>), dim3(beside + g.groups), dim3(64 * NW), lds, s, a, beside);

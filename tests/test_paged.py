@@ -265,3 +265,25 @@ def test_scales_that_are_no_numbers_are_refused():
     m, _ = _lib()
     for scale in (float("nan"), float("inf"), float("-inf"), 3e38, -3e38):
         assert _sdpa(4, 2, 32, 64, scale=scale) == m.KQ_ERR_BAD_ARGUMENT, scale
+
+
+def test_once_for_each_device(tmp_path):
+    """What launches need once is done on every device, and again after a failure."""
+    from gmlx_amd import build
+    (tmp_path / "t.cpp").write_text('''
+#include "kq_once.h"
+int main() {
+    OncePerDevice once;
+    int calls = 0;
+    const auto ok = [&] { return ++calls > 0; };
+    if (!once(0, ok) || !once(0, ok) || calls != 1) return 1;
+    if (!once(1, ok) || calls != 2 || !once(63, ok) || calls != 3) return 2;
+    if (once(2, [&] { ++calls; return false; }) || calls != 4) return 3;
+    if (!once(2, ok) || !once(2, ok) || calls != 5) return 4;
+    if (!once(64, ok) || !once(64, ok) || calls != 7) return 5;  // (past the table: at every call)
+    if (once(-1, ok) || calls != 7) return 6;
+    return 0;
+}
+''')
+    subprocess.run(["g++", "-std=c++17", "-I", build.CSRC, str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")], check=True)
+    assert subprocess.run([str(tmp_path / "t")]).returncode == 0
