@@ -1267,6 +1267,9 @@ class _PoolLayout:
                 raise ValueError("an 8-bit pool holds uint8 values in groups of 64")
             if dt not in (torch.float16, torch.bfloat16):
                 raise ValueError(f"scales and biases must be float16 or bfloat16, got {dt}")
+            if k.stride(2) != D:
+                raise ValueError(f"an 8-bit pool's tokens of a head and page must lie one after the other (a stride of {D}, "
+                                 f"got {k.stride(2)})")
             for t in scales:
                 if t.device != k.device or t.dtype != dt or t.shape != (n, H, ps, D // 64) or \
                         (D > 64 and t.stride(3) != 1) or \
@@ -1369,10 +1372,12 @@ def paged_write(k, v, k_cache, v_cache, slots, k_scales=None, k_biases=None, v_s
     """Write new tokens' K / V rows [T, Hkv, D] to their slots of a paged cache,
     in place.
 
-    k_cache / v_cache [n_pages, Hkv, page_size, D], any strides with D
-    contiguous (a [n_pages, page_size, Hkv, D] pool is passed permuted), of the
-    rows' dtype; or, with the four scale / bias tensors [n_pages, Hkv, page_size,
-    D / 64] in the rows' dtype, uint8: each 64 values are stored as
+    k_cache / v_cache [n_pages, Hkv, page_size, D], of the rows' dtype, D
+    contiguous, 16-byte aligned and of any strides that are multiples of 8 (a
+    [n_pages, page_size, Hkv, D] pool is passed permuted); or, with the four scale
+    / bias tensors [n_pages, Hkv, page_size, D / 64] in the rows' dtype, uint8, the
+    tokens of a head and page one after the other (so not permuted, but for one kv
+    head), page and head strides multiples of 64: each 64 values are stored as
     (x - bias) / scale rounded to 0..255, bias their smallest and scale a 255th
     of their range (the 8-bit affine cache of sdpa_decode_gqa's quantized form);
     64 values with an infinity or NaN among them read back as NaN.

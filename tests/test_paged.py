@@ -287,3 +287,17 @@ int main() {
 ''')
     subprocess.run(["g++", "-std=c++17", "-I", build.CSRC, str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")], check=True)
     assert subprocess.run([str(tmp_path / "t")]).returncode == 0
+
+
+def test_8bit_pools_of_tokens_before_heads_are_refused_by_name():
+    """Their scales lie a 64th of the way, but a head's tokens do not lie one after
+    the other; with one kv head they do."""
+    from gmlx_amd import ops
+
+    def layout(H):
+        k = torch.zeros(4, 16, H, 128, dtype=torch.uint8).permute(0, 2, 1, 3)
+        s = torch.zeros(4, 16, H, 2, dtype=torch.float16).permute(0, 2, 1, 3)
+        return ops._PoolLayout(k, k, (s, s, s, s))
+    with pytest.raises(ValueError, match="8-bit pool's tokens"):
+        layout(2)
+    assert layout(1).q8 == 1
