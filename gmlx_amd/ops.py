@@ -1339,9 +1339,17 @@ def paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_siz
     and free_count (or copies them over, inside a HIP graph).  Called again on
     the same inputs it gives the same.
 
-    The first row that the stack is too short for (or that would not fit the
-    table's width) and the later rows that need pages are refused: they stay as
-    they were, their tokens' slots are -1 and their attention is of no use.
+    A row whose pages would not fit the table's width is refused, and so are the
+    first row that the stack is too short for and the later rows that need pages:
+    they stay as they were, their tokens' slots are -1 and their attention is of
+    no use.
+
+    A page belongs to one row, or to the stack: nothing counts how many rows hold
+    one.  sdpa_paged takes tables whose rows share whole pages (a common prefix),
+    but each row that lets a page go here puts it on the stack, from which two
+    later rows would get it.  So a row that shares pages is ended in two steps:
+    keep its shared tokens, which gives back its own pages, then set its length
+    to 0 by hand; only the last holder keeps 0.
 
     seq_lens, new_lens, keep_lens int32 [B], B <= 2048; block_table int32
     [B, pages]; free_pages int32 [n] with n the pool's pages; free_count int32

@@ -492,9 +492,14 @@ typedef struct {
  * the request has ended), then get room for new_lens[b] more.  Pages that no
  * kept or new token needs go on the free stack (free_pages[0 .. *free_count),
  * of capacity n_stack) in row order; then new pages come off its top in row
- * order.  The first row that the stack is too short for, or one whose pages
- * would not fit table_width, is refused: it stays as it was, and so does every
- * later row that needs a page.
+ * order.  A row whose pages would not fit table_width is refused: it stays as it
+ * was and takes nothing from the others.  The first row that the stack is too
+ * short for is refused, and so is every later row that needs a page.
+ * A page belongs to one row or to the stack, and no count of its holders is kept:
+ * of rows that share whole pages (kq_sdpa_paged takes them) each that lets one go
+ * puts it on the stack, from which two later rows would get it.  Such a row keeps
+ * its shared tokens here, and its length is then set to 0 by the caller; only the
+ * last holder keeps 0.
  *   cu_q [B + 1]      running sum of new_lens (refused rows' tokens included)
  *   kv_lens [B]       kept + new (refused rows: seq_lens[b])
  *   slots [max_tokens], positions [max_tokens]  of every new token, in cu_q's

@@ -1092,3 +1092,17 @@ def test_plan_sizes_past_32_bits_are_refused():
     for page, tokens in ((2 ** 32 + 16, 4), (16, 2 ** 31), (16, 2 ** 32 + 4)):
         with pytest.raises(ValueError, match="paged_plan"):
             ops.paged_plan(one, one, table, one, one, page, tokens)
+
+
+def test_plan_of_rows_that_share_pages():
+    """Rows with a common prefix of whole pages: each ended by keeping the shared
+    tokens and a length of 0 by hand, the last one by keeping 0; every page is on
+    the stack once."""
+    table = np.array([[4, 2, 0, -1, -1], [4, 2, 3, 1, -1], [4, 2, 5, -1, -1]], np.int32)
+    stack, count, seq = np.full(6, -9, np.int32), 0, [40, 52, 33]
+    for keep, ended in (([40, 32, 33], 1), ([40, 0, 32], 2), ([0, 0, 0], 0)):
+        got = _check_plan(seq, [0, 0, 0], table, stack, count, 16, 3, keep)
+        seq, count, table, stack = got[1].tolist(), int(got[4][0]), got[6], got[7]
+        seq[ended] = 0
+        held = {int(p) for b, s in enumerate(seq) for p in table[b, :-(-s // 16)]}
+        assert sorted([*held, *stack[:count]]) == list(range(6))
