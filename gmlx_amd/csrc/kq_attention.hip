@@ -870,10 +870,7 @@ SplitRule split_rule(int B, int Hq, int Hkv, int D, int max_len, bool q8, bool w
     } else if ((int64_t)B * Hkv * (((int64_t)(max_len > 0 ? max_len : 1) + 1023) / 1024) >= 8 * (int64_t)device_cus()) {
         r.rest = 1024;
     } else if (!wide) {
-        if (D > 128) r = SplitRule{q8 || D > 256 ? 0 : 128, 1024, 8192, 32768, 512};
-        else if (q8) r = SplitRule{Hq > 8 * Hkv ? 256 : 0, 1024, 2048, 32768, 512};
-        else if (Hq > 8 * Hkv) r = SplitRule{512, 0, 1024, 8192, 512};
-        else r = SplitRule{256, 512, Hq > 4 * Hkv ? 1024 : 4096, 8192, 512};
+        r = row_split_rule(Hq, Hkv, D, q8);
     }
     return r;
 }

@@ -73,6 +73,16 @@ struct SplitRule {
     }
 };
 
+// Split lengths of decode rows, over contiguous caches and pages alike: short rows
+// one split, then 64, 128 and 256 tokens up to the lines, past them 512 (measured
+// beside split_rule in kq_attention.hip and wave_rule in kq_paged.hip).
+SplitRule row_split_rule(int Hq, int Hkv, int D, bool q8) {
+    if (D > 128) return SplitRule{q8 || D > 256 ? 0 : 128, 1024, 8192, 32768, 512};
+    if (q8) return SplitRule{Hq > 8 * Hkv ? 256 : 0, 1024, 2048, 32768, 512};
+    if (Hq > 8 * Hkv) return SplitRule{512, 0, 1024, 8192, 512};
+    return SplitRule{256, 512, Hq > 4 * Hkv ? 1024 : 4096, 8192, 512};
+}
+
 __host__ __device__ __forceinline__ int row_splits(const SplitRule &rule, int len) {
     const int split = rule.tokens(len);
     return len <= 0 ? 1 : (len + split - 1) / split;

@@ -1583,14 +1583,23 @@ int launch(const PagedArgs &a, bool q8, const Grid &g, hipStream_t s) {
     return launch_q8<D, BF, false>(a, g, s);
 }
 
-// Tokens per split of a row of few columns, by its own keys, as decode
-// attention over contiguous caches has them.
+// Tokens per split of a row of few columns, by its own keys: the lengths of
+// decode attention over contiguous caches, which suit pages as they do those.
+// Measured on pages of 64 (us; with the rule, and at 64 / 128 / 256 / 512 tokens),
+// where that rule's own sweep has no figures, fp16:
+//   16 query heads on 2, head dim 256
+//     1 row of  1600  13.4   11.7 / 13.5 / 18.9 / 29.8    16  19.4   19.9 / 17.6 / 22.0 / 33.8
+//     1 row of  6400  16.2   13.5 / 16.1 / 22.0 / 32.9    16  56.5   63.0 / 56.9 / 53.9 / 48.2
+//     1 of     32768  24.2   25.1 / 21.9 / 24.1 / 35.9    16   219    272 /  244 /  220 /  207
+//   the same in 8 bits
+//     1 row of  1600  17.4   13.7 / 17.7 / 26.7 / 44.4    16  20.8   18.6 / 20.4 / 28.7 / 47.3
+//     1 of     32768  30.7   23.3 / 23.4 / 30.7 / 49.5    16   144    210 /  167 /  142 /  120
+//   64 query heads on 4, head dim 128
+//     1 row of  1600  12.0    8.8 /  9.8 / 12.1 / 16.8    16  17.9   21.6 / 19.2 / 17.1 / 19.5
+//     1 of     32768  19.9   26.7 / 22.7 / 19.4 / 20.2    16   219    366 /  283 /  243 /  219
 SplitRule wave_rule(int Hq, int Hkv, int D, bool q8) {
     if (const int forced = env_int("GMLX_KQ_SDPA_SPLIT", 0)) return SplitRule{0, 0, 0, 0, (forced + 63) / 64 * 64};
-    if (D > 128) return SplitRule{q8 || D > 256 ? 0 : 128, 1024, 8192, 32768, 512};
-    if (q8) return SplitRule{Hq > 8 * Hkv ? 256 : 0, 1024, 2048, 32768, 512};
-    if (Hq > 8 * Hkv) return SplitRule{512, 0, 1024, 8192, 512};
-    return SplitRule{256, 512, Hq > 4 * Hkv ? 1024 : 4096, 8192, 512};
+    return row_split_rule(Hq, Hkv, D, q8);
 }
 
 // What a call's splits can come to, from the bounds that the host knows.

@@ -301,3 +301,14 @@ def test_8bit_pools_of_tokens_before_heads_are_refused_by_name():
     with pytest.raises(ValueError, match="8-bit pool's tokens"):
         layout(2)
     assert layout(1).q8 == 1
+
+
+def test_register_copies_of_the_decode_kernels(tmp_path):
+    """The same of the kernels over contiguous caches."""
+    from gmlx_amd import build
+    out = tmp_path / "kq_attention.s"
+    subprocess.run([build.HIPCC, *build.FLAGS, "-S", os.path.join(build.CSRC, "kq_attention.hip"), "-o", str(out),
+                    "--offload-device-only"], check=True, capture_output=True)
+    text = out.read_text()
+    assert "kq_sdpa_split_kernel" in text
+    assert not _before_exec(text)
