@@ -13,7 +13,7 @@
 //
 // Rounded to 16 bits are the probabilities (an MFMA operand: half a step each,
 // relative, averaged over the keys) and the output, nothing else; 8-bit pools
-// multiply integers, or hi + lo planes of 22 bits (fp16) or 16 (bf16; the lost
+// multiply integers, or hi + lo planes of 21 bits (fp16) or 16 (bf16; the lost
 // part is 2^-8 of half a step of the output).  Probabilities in hi + lo
 // too would double P.V's products and take the error (2-norm, bf16) from 0.0023 to
 // the 0.0017 of the output's own rounding.
@@ -792,7 +792,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2
 //
 // An 8-bit pool's tile is written to LDS as 16-bit values by the waves that
 // would copy it: value = hi + lo, each in the queries' type, hi the value
-// s q + b rounded and lo the rest, both multiplied (twice the MFMAs), so that
+// s q + b in 16 bits and lo the rest, both multiplied (twice the MFMAs), so that
 // no rounding of a dequantised value to 16 bits enters the result; dequantised
 // to hi alone, outputs were about twice as far from exact as the 16-bit pool's.
 // A value past the largest fp16 (255 steps from the least to 65504 end at 65535)
@@ -1086,11 +1086,12 @@ struct ChunkState16 {
     }
 };
 
-// The most that an 8-bit value's first half holds: past it the second takes the
-// rest (fp16; a bf16 half has fp32's range).
+// The first halves of two 8-bit values.  fp16's are cut, not rounded: past 65504
+// they stay there, and the second halves take the rest.
 template <bool BF>
-__device__ __forceinline__ float first_half(float v) {
-    return BF ? v : __builtin_amdgcn_fmed3f(v, -65504.f, 65504.f);
+__device__ __forceinline__ uint32_t first_halves(float a, float b) {
+    if constexpr (BF) return pack2<BF>(a, b);
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
 
 template <int D, bool BF, bool Q8>
@@ -1214,7 +1215,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
                             for (int i = 0; i < 4; ++i) {
                                 const uint32_t two = held[y][x][2 * half + (i >> 1)] >> (16 * (i & 1));
                                 const float u = fmaf((float)(two & 0xFFu), sc, bi), v = fmaf((float)((two >> 8) & 0xFFu), sc, bi);
-                                hi[i] = pack2<BF>(first_half<BF>(u), first_half<BF>(v));
+                                hi[i] = first_halves<BF>(u, v);
                                 lo[i] = pack2<BF>(u - f16bits_to_f32<BF>(hi[i] & 0xFFFFu), v - f16bits_to_f32<BF>(hi[i] >> 16));
                             }
                             const uint32_t to = stage + held_at[y] + (uint32_t)(t * C::kRow + 16 * ((pc + half) ^ turn));
@@ -1263,9 +1264,10 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
                             const float sc = f16bits_to_f32<BF>(a.vs[at >> 6]), bi = f16bits_to_f32<BF>(a.vb[at >> 6]);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                // (what `clean` took away: of fp16, the second half)
-                                const float v = fmaf((float)((const uint8_t *)a.v)[at + e], sc, bi);
-                                y[e] = t < lim ? odd_part<BF>(from_f32<BF>(BF ? v : v - first_half<BF>(v))) : 0.f;
+                                // (fp16: infinite from where the halves are, 2^17.  A comparison
+                                // with that in its place spilled 24 to 548 bytes a lane.)
+                                const float v = fmaf((float)((const uint8_t *)a.v)[at + e], sc, bi) * (BF ? 1.f : 0x1p111f);
+                                y[e] = t < lim && v - v != 0.f ? v : 0.f;
                             }
                         } else {
 #pragma unroll
