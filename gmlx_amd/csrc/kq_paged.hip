@@ -16,15 +16,18 @@
 // multiply integers, or hi + lo planes of 21 bits (fp16) or 16 (bf16; the lost
 // part is 2^-8 of half a step of the output).  Probabilities in hi + lo
 // too would double P.V's products and take the error (2-norm, bf16) from 0.0023 to
-// the 0.0017 of the output's own rounding.
+// the 0.0017 of the output's own rounding.  In 8-bit fp16 decode rows a probability
+// is rounded after its key's scale is on it: subnormal, so with fewer bits, where
+// scales are below 1e-5 or so (values of 3e-4 behind a first key of e^10 times the
+// others' weight: 7.6e-4 instead of the output rounding's 2.2e-4; of 1e-2: 2.1e-4).
 //
 // Few query columns (decode, verify): bound by HBM, one wave a unit streams its
 // keys through registers; 16 rows of 1 k to 131 k keys, head dim 128, 2.01 GB
 // in 371 us, 5.4 TB/s.  Chunks: bound by the MFMA, exp and LDS pipes together,
 // tiles in LDS shared by the workgroup's columns; 2048 tokens behind 6000, head
-// dim 128, 236 GFLOP in 248 us, 950 TFLOP/s (1.19 PFLOP/s for a plain 8192^3
-// product on the same card): MFMA pipes busy 45 % of the cycles, LDS 35 %, a
-// third of that in bank conflicts.
+// dim 128, 236 GFLOP in 247 to 255 us over runs, 925 to 950 TFLOP/s (1.19 PFLOP/s
+// for a plain 8192^3 product on the same card): MFMA pipes busy 45 % of the cycles,
+// LDS 35 %, a third of that in bank conflicts.
 #include "kq_once.h"
 #include "kq_paged.h"
 
@@ -80,7 +83,7 @@ __host__ __device__ __forceinline__ bool few_columns(int n, int G, int limit) { 
 constexpr bool has_waves(int D) { return D <= 256; }
 
 // A chunk's workgroup: its waves (eight share an 8-bit tile's conversion: 333
-// tokens over 4200 keys at head dim 256 142 us on four, 82 on eight; at 128 85 and
+// tokens over 4200 keys at head dim 256 142 us on four, 82 on eight, 77 since fp16 halves are cut; at 128 85 and
 // 73), query columns (32 a wave, 16 where 32 would take over 256 registers a lane
 // for the sums and the queries: at head dim 256 2048 tokens over 8048 keys 278 us,
 // with 32 400), and how many such workgroups the GPU holds at once, which

@@ -199,7 +199,9 @@ __global__ __launch_bounds__(kPlanThreads) void kq_paged_plan_kernel(PlanArgs a)
 // A thread moves 8 values (16 bytes of a 16-bit row); L = D / 8 threads a row
 // of a head, blockIdx.y K or V.  HBM-bound where rows are many: 4097 tokens of 8
 // heads, head dim 128 (33.6 MB each way a call), written in 7.6 us and read in 7.5,
-// 4.4 TB/s; 2048 tokens to 8 bits 7.1, back 5.1; 32 tokens 2.9 (the launch).
+// 4.4 TB/s; 32 tokens 2.7 (the launch).  2048 tokens (12.7 MB) to 8 bits 7.1, by
+// vector issue: 306 instructions a wave, about 85 of them the nine exact divisions,
+// fill 91 % of the busy cycles; back 5.2, its loads' latency in one round of waves.
 struct CopyArgs {
     kq_paged_pool p;
     const uint16_t *src[2];
