@@ -83,8 +83,8 @@ __host__ __device__ __forceinline__ bool few_columns(int n, int G, int limit) { 
 constexpr bool has_waves(int D) { return D <= 256; }
 
 // A chunk's workgroup: its waves (eight share an 8-bit tile's conversion: 333
-// tokens over 4200 keys at head dim 256 142 us on four, 82 on eight, 77 since fp16 halves are cut; at 128 85 and
-// 73), query columns (32 a wave, 16 where 32 would take over 256 registers a lane
+// tokens over 4200 keys at head dim 256 142 us on four, 82 on eight (77 since
+// fp16 halves are cut); at 128 85 and 73), query columns (32 a wave, 16 where 32 would take over 256 registers a lane
 // for the sums and the queries: at head dim 256 2048 tokens over 8048 keys 278 us,
 // with 32 400), and how many such workgroups the GPU holds at once, which
 // splitting a chunk aims at (512; half of it: 333 over 4200 50 -> 65).

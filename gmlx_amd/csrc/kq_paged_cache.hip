@@ -373,8 +373,8 @@ int kq_paged_plan(const int32_t *seq_lens, const int32_t *keep_lens, const int32
         return KQ_ERR_BAD_SHAPE;
     if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return KQ_ERR_BAD_SHAPE;
     if ((int64_t)table_width * page_size >= (int64_t)1 << 31) return KQ_ERR_BAD_SHAPE;
-    // 31-bit sums of pages
-    if ((int64_t)B * table_width >= 1 << 30 || n_stack >= 1 << 30) return KQ_ERR_BAD_SHAPE;
+    // 31-bit sums of pages, and numbers of tokens and pages a grid's step past the last
+    if ((int64_t)B * table_width >= 1 << 30 || n_stack >= 1 << 30 || max_tokens > 1 << 30) return KQ_ERR_BAD_SHAPE;
     const PlanArgs a{seq_lens,       keep_lens, new_lens,     free_count,  block_table, free_pages,
                      cu_q,           kv_lens,   slots,        positions,   free_count_out, refused,
                      table_stride,   B,         table_width,  n_stack,     __builtin_ctz(page_size), max_tokens};

@@ -1358,8 +1358,8 @@ def paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_siz
     _fault("paged_plan")
     _require_gpu(seq_lens)
     dev, B, T = seq_lens.device, seq_lens.numel(), int(max_tokens)
-    if not 1 <= B <= _lib.PAGED_MAX_ROWS or not 0 <= T < 1 << 31 or not 16 <= page_size <= 1024:
-        raise ValueError(f"paged_plan: 1 to {_lib.PAGED_MAX_ROWS} rows, max_tokens from 0 and below 2^31, a page_size of "
+    if not 1 <= B <= _lib.PAGED_MAX_ROWS or not 0 <= T <= 1 << 30 or not 16 <= page_size <= 1024:
+        raise ValueError(f"paged_plan: 1 to {_lib.PAGED_MAX_ROWS} rows, max_tokens from 0 to 2^30, a page_size of "
                          f"16 to 1024, got {B}, {T} and {page_size}")
     tab, tab_stride, width = _block_table(block_table, B, dev)
     seq, new = _ints(seq_lens, "seq_lens", B, dev), _ints(new_lens, "new_lens", B, dev)

@@ -511,7 +511,7 @@ typedef struct {
  * Outputs must not overlap inputs.  Negative lengths count as 0, seq_lens past
  * table_width * page_size as that; the new tokens of all rows are fewer than
  * 2^31 (of more, cu_q, slots and positions are of no use).  All int32 on the
- * device.  B * table_width and n_stack below 2^30. */
+ * device.  B * table_width and n_stack below 2^30, max_tokens up to 2^30. */
 #define KQ_PAGED_MAX_ROWS 2048
 int kq_paged_plan(const int32_t *seq_lens, const int32_t *keep_lens, const int32_t *new_lens, int32_t B,
                   int32_t *block_table, int64_t table_stride, int32_t table_width, int32_t *free_pages,

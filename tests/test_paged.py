@@ -312,3 +312,11 @@ def test_register_copies_of_the_decode_kernels(tmp_path):
     text = out.read_text()
     assert "kq_sdpa_split_kernel" in text
     assert not _before_exec(text)
+
+
+def test_plan_refuses_more_tokens_than_its_grid_counts():
+    """A grid's step past 2^31 - 1 tokens would be a negative number."""
+    m, L = _lib()
+    x = 1 << 26
+    for tokens in ((1 << 30) + 1, (1 << 31) - 1):
+        assert L.kq_paged_plan(x, None, x, 2, x, 4, 4, x, 8, x, 16, tokens, x, x, x, x, x, x, None) == m.KQ_ERR_BAD_SHAPE
