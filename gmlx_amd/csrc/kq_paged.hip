@@ -84,10 +84,11 @@ constexpr bool has_waves(int D) { return D <= 256; }
 
 // A chunk's workgroup: its waves (eight share an 8-bit tile's conversion: 333
 // tokens over 4200 keys at head dim 256 142 us on four, 82 on eight (77 since
-// fp16 halves are cut); at 128 85 and 73), query columns (32 a wave, 16 where 32 would take over 256 registers a lane
-// for the sums and the queries: at head dim 256 2048 tokens over 8048 keys 278 us,
-// with 32 400), and how many such workgroups the GPU holds at once, which
-// splitting a chunk aims at (512; half of it: 333 over 4200 50 -> 65).
+// fp16 halves are cut); at 128 85 and 73), query columns (32 a wave, 16 where 32
+// would take over 256 registers a lane for the sums and the queries: at head dim
+// 256 2048 tokens over 8048 keys 278 us, with 32 400), and how many such workgroups
+// the GPU holds at once, which splitting a chunk aims at (512; half of it: 333 over
+// 4200 50 -> 65).
 constexpr int chunk_waves(int D, bool q8) { return q8 && (D == 128 || D == 256) ? 8 : 4; }
 constexpr int group_columns(int D, bool q8) { return chunk_waves(D, q8) * (D > 128 ? 16 : 32); }
 constexpr int group_slots(int D, bool q8) { return D > 256 || chunk_waves(D, q8) > 4 ? 256 : 512; }
@@ -1135,14 +1136,15 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
         State st;
         st.init();
         // scores are products of the queries with the scale's sign, times its size;
-        // of queries of 0 where it is 0, since 0 times a hidden key's -inf is NaN
-        const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.f ? 0u : ~0u;
-        const float scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
+        // instead of 0, which makes a hidden key's -inf NaN, the least number of all
+        // (fp32 subnormals are kept here): no product passes 2^-20 with it
+        const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+        const float scale = fmaxf(fabsf(a.scale_log2), 0x1p-149f);
         const uint16_t *qp = a.q + (int64_t)(row.q0 + i) * a.q_stride + (int64_t)hq * D;
 #pragma unroll
         for (int d = 0; d < State::NQ; ++d) {
             const u32x4 v = *(const u32x4 *)(qp + State::qd(d));
-            st.qf[d] = __builtin_bit_cast(half8_t, live ? (v & keep) ^ flip : u32x4{0u, 0u, 0u, 0u});
+            st.qf[d] = __builtin_bit_cast(half8_t, live ? v ^ flip : u32x4{0u, 0u, 0u, 0u});
         }
 
         if (t_end > t_begin) {
@@ -1655,9 +1657,9 @@ bool sizes_fit(int64_t T, int64_t B, int Hq, int max_kv) { return T * Hq <= (1 <
 size_t part_bytes(int64_t slots, int D) { return ((size_t)slots * D * 4 + 255) & ~(size_t)255; }
 
 // Whether 32-bit numbers count a call's partials and units (a grid's step past
-// the last of them too).  Units of the two kernels apart, since
-// a chunk of many columns has few splits however many keys it has: blocks and
-// splits of a row come to group_slots / Hkv, or to its blocks alone.
+// the last of them too).  Units of the two kernels apart, since a chunk of many
+// columns has few splits however many keys it has: blocks times splits of a row
+// come to group_slots / Hkv, or to its blocks alone.
 bool numbers_fit(const Plan &p, int64_t T, int64_t B, int Hq, int Hkv, int D, bool q8) {
     constexpr int64_t kMost = ((int64_t)1 << 31) - (1 << 17);
     if (p.slots >= (int64_t)1 << 31) return false;

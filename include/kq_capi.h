@@ -473,7 +473,7 @@ int kq_sdpa_decode_gqa_cascade_q8(const void *q, const void *k_shared, const voi
  * bytes and multiples of 64, token_stride == D (a head's tokens of a page lie
  * one after the other), k / v 16-byte aligned, D in {64, 128, 256, 512}.  In an
  * f16 pool |scale * q + bias| up to 131008 (what kq_paged_write stores of finite
- * values ends at 65570); attention may take more for an infinity.
+ * values ends at 65570); with more, attention may not be finite.
  *
  * Token t of a row lies in page block_table[row][t / page_size], place t %
  * page_size; slot = page * page_size + place (n_pages * page_size < 2^31).
