@@ -1106,3 +1106,14 @@ def test_plan_of_rows_that_share_pages():
         seq[ended] = 0
         held = {int(p) for b, s in enumerate(seq) for p in table[b, :-(-s // 16)]}
         assert sorted([*held, *stack[:count]]) == list(range(6))
+
+
+@pytest.mark.parametrize("D,q8", [(64, False), (128, False), (128, True), (256, True), (512, False)])
+def test_sixty_four_query_heads_a_kv_head(D, q8):
+    """The most there are: rows of one token are chunks then, in 16 and 8 bits."""
+    b = Batch([(1, 1), (1, 700), (5, 90), (0, 3), (1, 2100)], 64, 1, D, 32, BF16, q8=q8, seed=D)
+    if q8:  # (chunks round a probability times the value, not the centred one)
+        b.err = [np.maximum(e, np.abs(v)) for e, v in zip(b.err, b.v)]
+    _say("64 heads", D, q8)
+    b.check(b.run())
+    b.check(b.run(max_q=5, max_kv=2100))
