@@ -50,6 +50,7 @@ EXPORTS = (
     "kq_sdpa_decode_gqa_q8", "kq_sdpa_decode_gqa_noalloc",
     "kq_sdpa_cascade_workspace_bytes", "kq_sdpa_decode_gqa_cascade", "kq_sdpa_decode_gqa_cascade_q8",
     "kq_paged_plan", "kq_paged_write", "kq_paged_read", "kq_sdpa_paged_workspace_bytes", "kq_sdpa_paged",
+    "kq_rope_qk", "kq_paged_write_rope", "kq_verify_workspace_bytes", "kq_verify_drafts",
     "kq_gguf_open", "kq_gguf_close", "kq_gguf_header", "kq_gguf_kv", "kq_gguf_tensor", "kq_gguf_type_size",
 )
 
@@ -129,6 +130,31 @@ class PagedPool(ctypes.Structure):
     ]
 
 
+class Rope(ctypes.Structure):
+    _fields_ = [
+        ("freqs", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("weight_dtype", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("factor", ctypes.c_float),
+    ]
+
+
+class RopeRows(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -184,6 +210,11 @@ _SIGS = {
     "kq_sdpa_paged_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _int], _sz),
     "kq_sdpa_paged": ([_vp, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
                        _f32, _vp, _i64, _vp, _sz, _vp], _int),
+    "kq_rope_qk": ([_vp, _vp, _i32, _i32, _int, _vp, _vp, _vp], _int),
+    "kq_paged_write_rope": ([_vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp], _int),
+    "kq_verify_workspace_bytes": ([_i32, _i32, _i32, _int, _int], _sz),
+    "kq_verify_drafts": ([_vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _int, _i64, _vp, _f32, _vp, _i32, _i32, _i32, _vp,
+                          _vp, _vp, _vp, _sz, _vp], _int),
     "kq_gguf_open": ([ctypes.c_char_p, ctypes.POINTER(_vp)], _int),
     "kq_gguf_close": ([_vp], None),
     "kq_gguf_header": ([_vp, ctypes.POINTER(ctypes.c_uint32)] + [ctypes.POINTER(_i64)] * 6, _int),

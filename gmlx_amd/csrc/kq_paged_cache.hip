@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "kq_paged.h"
+#include "kq_paged_store.h"
 
 int kq_pool_check(const kq_paged_pool *p) {
     if (!p || !p->k || !p->v) return KQ_ERR_NULL_POINTER;
@@ -26,6 +27,26 @@ int kq_pool_check(const kq_paged_pool *p) {
             return KQ_ERR_BAD_ALIGN;
     }
     return KQ_OK;
+}
+
+// Whether no two places of K and V lie on the same memory as far as the strides
+// and bases tell: each stride passes what the smaller ones reach (a page or head
+// that is repeated by a stride of 0 does not), and K is not V.  Rows written to
+// such places by different threads would be mixed.
+bool kq_pool_places_apart(const kq_paged_pool &p) {
+    struct { int64_t stride, n; } d[3] = {{p.token_stride, p.page_size}, {p.head_stride, p.Hkv}, {p.page_stride, p.n_pages}};
+    std::sort(d, d + 3, [](const auto &x, const auto &y) { return x.stride < y.stride; });
+    __int128 reach = p.D;
+    for (const auto &x : d) {
+        if (x.n == 1) continue;
+        if (x.stride < reach) return false;
+        reach += (__int128)x.stride * (x.n - 1);
+    }
+    const void *at[4] = {p.k_scales, p.k_biases, p.v_scales, p.v_biases};
+    for (int i = 0; p.k_scales && i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (at[i] == at[j]) return false;
+    return p.k != p.v;
 }
 
 namespace {
@@ -212,23 +233,6 @@ struct CopyArgs {
     uint32_t rows;  // T * Hkv
 };
 
-// Element (byte, 8-bit pool) offset of a slot's row of head h; -1 outside the pool.
-__device__ __forceinline__ int64_t slot_offset(const CopyArgs &a, int slot, int h) {
-    const int page = slot >> a.lps;
-    if (slot < 0 || page >= a.p.n_pages) return -1;
-    return page * a.p.page_stride + h * a.p.head_stride + (slot & ((1 << a.lps) - 1)) * a.p.token_stride;
-}
-
-// Smallest, largest and sum of what a group's 8 threads hold.
-__device__ __forceinline__ void group_range(float &lo, float &hi, float &odd) {
-#pragma unroll
-    for (int off = 1; off < 8; off <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, off));
-        hi = fmaxf(hi, __shfl_xor(hi, off));
-        odd += __shfl_xor(odd, off);
-    }
-}
-
 template <int D, bool BF, bool Q8>
 __global__ __launch_bounds__(256) void kq_paged_write_kernel(CopyArgs a) {
     constexpr int L = D / 8;
@@ -236,45 +240,10 @@ __global__ __launch_bounds__(256) void kq_paged_write_kernel(CopyArgs a) {
     if (row >= a.rows) return;
     const int kv = blockIdx.y;
     const uint32_t t = row / (uint32_t)a.p.Hkv, h = row - t * a.p.Hkv;
-    const int64_t to = slot_offset(a, a.slots[t], h);
+    const int64_t to = slot_offset(a.p, a.lps, a.slots[t], h);
     if (to < 0) return;  // uniform over a row's threads
     const u32x4 w = *(const u32x4 *)(a.src[kv] + t * a.token_stride[kv] + h * a.head_stride[kv] + 8 * c);
-    if constexpr (!Q8) {
-        *(u32x4 *)((uint16_t *)(kv ? a.p.v : a.p.k) + to + 8 * c) = w;
-    } else {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = f16bits_to_f32<BF>(w[i] & 0xFFFFu);
-            x[2 * i + 1] = f16bits_to_f32<BF>(w[i] >> 16);
-        }
-        float lo = x[0], hi = x[0], odd = x[0] - x[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) {
-            lo = fminf(lo, x[i]);
-            hi = fmaxf(hi, x[i]);
-            odd += x[i] - x[i];  // NaN from an infinity or NaN (which fminf drops), else 0
-        }
-        group_range(lo, hi, odd);
-        // (bf16 values can be further apart than fp32's largest: halves of all then)
-        const float part = BF && !(hi - lo <= 3.4028235e38f) ? 0.5f : 1.f;
-        // the scale as it is stored: the values are rounded against what is
-        // read back; a bias of 16 bits holds lo exactly
-        const uint16_t s16 = from_f32<BF>((hi * part - lo * part) / (255.f * part) + odd);
-        const float s = f16bits_to_f32<BF>(s16);
-        uint32_t q[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = s == 0.f ? 0.f : fminf(fmaxf(rintf((x[i] * part - lo * part) / (s * part)), 0.f), 255.f);
-            q[i >> 2] |= (uint32_t)v << (8 * (i & 3));
-        }
-        *(u32x2 *)((uint8_t *)(kv ? a.p.v : a.p.k) + to + 8 * c) = u32x2{q[0], q[1]};
-        if ((c & 7) == 0) {
-            const int64_t g = (to + 8 * c) >> 6;
-            ((uint16_t *)(kv ? a.p.v_scales : a.p.k_scales))[g] = s16;
-            ((uint16_t *)(kv ? a.p.v_biases : a.p.k_biases))[g] = from_f32<BF>(lo);
-        }
-    }
+    store_values<BF, Q8>(a.p, kv, to, c, w);
 }
 
 template <int D, bool BF, bool Q8>
@@ -284,7 +253,7 @@ __global__ __launch_bounds__(256) void kq_paged_read_kernel(CopyArgs a) {
     if (row >= a.rows) return;
     const int kv = blockIdx.y;
     const uint32_t t = row / (uint32_t)a.p.Hkv, h = row - t * a.p.Hkv;
-    const int64_t from = slot_offset(a, a.slots[t], h);
+    const int64_t from = slot_offset(a.p, a.lps, a.slots[t], h);
     u32x4 w = {0, 0, 0, 0};
     if (from >= 0) {
         if constexpr (!Q8) {
@@ -320,26 +289,6 @@ void launch_copy_d(const CopyArgs &a, bool write, hipStream_t s) {
         // a 16-bit row moves as bits whatever its type
         launch_copy<D, false, false>(a, write, s);
     }
-}
-
-// Whether no two places of K and V lie on the same memory as far as the strides
-// and bases tell: each stride passes what the smaller ones reach (a page or head
-// that is repeated by a stride of 0 does not), and K is not V.  Rows written to
-// such places by different threads would be mixed.
-bool places_apart(const kq_paged_pool &p) {
-    struct { int64_t stride, n; } d[3] = {{p.token_stride, p.page_size}, {p.head_stride, p.Hkv}, {p.page_stride, p.n_pages}};
-    std::sort(d, d + 3, [](const auto &x, const auto &y) { return x.stride < y.stride; });
-    __int128 reach = p.D;
-    for (const auto &x : d) {
-        if (x.n == 1) continue;
-        if (x.stride < reach) return false;
-        reach += (__int128)x.stride * (x.n - 1);
-    }
-    const void *at[4] = {p.k_scales, p.k_biases, p.v_scales, p.v_biases};
-    for (int i = 0; p.k_scales && i < 4; ++i)
-        for (int j = 0; j < i; ++j)
-            if (at[i] == at[j]) return false;
-    return p.k != p.v;
 }
 
 int copy_rows(const CopyArgs &a, bool write, kq_stream_t stream) {
@@ -390,7 +339,7 @@ int kq_paged_write(const kq_paged_pool *pool, const void *k, int64_t k_token_str
     if (T == 0) return KQ_OK;
     if (!k || !v || !slots) return KQ_ERR_NULL_POINTER;
     if (T < 0) return KQ_ERR_BAD_SHAPE;
-    if (!places_apart(*pool)) return KQ_ERR_BAD_ARGUMENT;
+    if (!kq_pool_places_apart(*pool)) return KQ_ERR_BAD_ARGUMENT;
     if ((((uintptr_t)k | (uintptr_t)v) & 15) || ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7))
         return KQ_ERR_BAD_ALIGN;
     const CopyArgs a{*pool,

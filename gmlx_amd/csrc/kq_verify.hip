@@ -1,0 +1,570 @@
+// Drafted tokens checked against the target's logits (kq_verify_drafts).
+//
+// Row t of the logits at temperature c has the weights
+//   e_v = exp((x_v - max x) / c), p_v = e_v / Z, Z = sum of e_v.
+// The draft d behind it stands where u q_d Z < e_d (u q_d < p_d), q the
+// probabilities that it was drawn from, or 1 for d alone.  Behind the first draft of
+// a row that does not stand, or behind all of them, comes the token v at which
+// the running sum of w passes r times the whole: w = max(e - q Z, 0) (e without e_d
+// where d alone was proposed) behind a refused draft, e behind the last.
+//
+// A running sum over V tokens has V borders that r may fall next to, so weights
+// and sums are fp64: 2 10^-16 each, where fp32's 10^-7 would put one draw in a
+// hundred on the other side of some border at V = 10^5.
+#include "kq_attn.h"
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+// What a slice of a logits row comes to.
+struct Part {
+    float m;     // its largest value, -infinity: none
+    int32_t at;  // the lowest token that has it
+    double sum;  // of exp((x - m) / c)
+};
+
+struct VerifyArgs {
+    const void *logits, *probs;
+    int64_t stride, probs_stride;
+    const int32_t *tokens, *cu, *kv;
+    const float *u, *draws, *temps;
+    float temp;
+    int32_t T, B, V, S;  // S: slices a row
+    int32_t probs_type;
+    Part *part;    // [T][S]
+    double *rest;  // [B][S]: sums of max(e - q Z, 0)
+    int32_t *accepted, *next, *keep;
+};
+
+// 2^y for y <= 0 (NaN: 0) by the series of exp(f ln 2) on |f| <= 1/2: its next term
+// is below 2 10^-16.
+__device__ __forceinline__ double exp2_64(double y) {
+    y = fmax(y, -1100.0);
+    const double n = rint(y), f = (y - n) * 0.69314718055994530942;
+    double p = 1.0 / 479001600;
+    p = fma(p, f, 1.0 / 39916800);
+    p = fma(p, f, 1.0 / 3628800);
+    p = fma(p, f, 1.0 / 362880);
+    p = fma(p, f, 1.0 / 40320);
+    p = fma(p, f, 1.0 / 5040);
+    p = fma(p, f, 1.0 / 720);
+    p = fma(p, f, 1.0 / 120);
+    p = fma(p, f, 1.0 / 24);
+    p = fma(p, f, 1.0 / 6);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.0);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n);
+}
+
+// Values of 16 bytes of logits.
+template <int DT>
+constexpr int kValues = DT == KQ_DTYPE_F32 ? 4 : 8;
+
+template <int DT>
+__device__ __forceinline__ float value(const void *p, int64_t i) {
+    if constexpr (DT == KQ_DTYPE_F32) return ((const float *)p)[i];
+    else return f16bits_to_f32<DT == KQ_DTYPE_BF16>(((const uint16_t *)p)[i]);
+}
+
+// Values i .. i + N - 1 of a row of V (rows start at any multiple of a value's
+// size); `past` for those behind its end.
+template <int DT, int N>
+__device__ __forceinline__ void values(const void *row, int i, int V, float past, float (&x)[N]) {
+    if (i <= V - N) {
+        if constexpr (DT == KQ_DTYPE_F32) {
+            typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const vec w = *(const vec *)((const float *)row + i + j);
+                x[j] = w.x, x[j + 1] = w.y, x[j + 2] = w.z, x[j + 3] = w.w;
+            }
+        } else {
+            typedef uint32_t vec __attribute__((ext_vector_type(N / 2), aligned(2)));
+            const vec w = *(const vec *)((const uint16_t *)row + i);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                x[j] = f16bits_to_f32<DT == KQ_DTYPE_BF16>((w[j >> 1] >> (16 * (j & 1))) & 0xFFFFu);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = i < V - j ? value<DT>(row, i + j) : past;
+    }
+}
+
+// A logit as it counts: NaN as -infinity, +infinity as the largest number.
+__device__ __forceinline__ float counted(float x) { return x != x ? -INFINITY : fminf(x, 3.4028235e38f); }
+
+// log2(e) / c of row b, 0: greedy.
+__device__ __forceinline__ double rate_of(const VerifyArgs &a, int b) {
+    const float c = a.temps ? a.temps[b] : a.temp;
+    return c > 0.f ? 1.4426950408889634074 / (double)c : 0.0;
+}
+__device__ __forceinline__ bool greedy(const VerifyArgs &a, int b) { return !((a.temps ? a.temps[b] : a.temp) > 0.f); }
+
+__device__ __forceinline__ double weight(float x, float m, double rate) { return exp2_64(((double)x - (double)m) * rate); }
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
+    return v;
+}
+
+// The larger of two (value, token), the lower token of equal values.
+__device__ __forceinline__ void take_larger(float &m, int &at, float m2, int at2) {
+    const bool other = m2 > m || (m2 == m && at2 < at);
+    m = other ? m2 : m;
+    at = other ? at2 : at;
+}
+__device__ __forceinline__ void wave_largest(float &m, int &at) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const float m2 = __shfl_xor(m, off);
+        const int at2 = __shfl_xor(at, off);
+        take_larger(m, at, m2, at2);
+    }
+}
+
+// The row b that logits row t belongs to: the last whose first row is at or before
+// t (rows without logits are passed over).
+__device__ __forceinline__ int row_at(const int32_t *cu, int B, int t) {
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cu[mid] <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// One slice of one logits row a workgroup: CH chunks of 16 bytes a thread, held in
+// registers between the maximum and the sum, so the logits are read once.
+template <int DT, int CH>
+__global__ __launch_bounds__(kThreads) void kq_verify_rows_kernel(VerifyArgs a) {
+    constexpr int N = kValues<DT>;
+    __shared__ float red_m[kWaves];
+    __shared__ int red_at[kWaves];
+    __shared__ double red_sum[kWaves];
+    const int t = blockIdx.x / a.S, s = blockIdx.x - t * a.S;
+    if (t >= a.cu[a.B]) return;
+    const uint8_t *row = (const uint8_t *)a.logits + (int64_t)t * a.stride * (16 / N);
+    const int lane = kq_lane(), w = threadIdx.x >> 6;
+    float x[CH][N];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N;
+        values<DT, N>(row, min(i, a.V), a.V, -INFINITY, x[c]);
+    }
+    float m = -INFINITY;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            x[c][j] = counted(x[c][j]);
+            if (x[c][j] > m) {
+                m = x[c][j];
+                at = i + j;
+            }
+        }
+    }
+    wave_largest(m, at);
+    if (lane == 0) {
+        red_m[w] = m;
+        red_at[w] = at;
+    }
+    __syncthreads();
+    m = red_m[0];
+    at = red_at[0];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) take_larger(m, at, red_m[k], red_at[k]);
+    const int b = a.temps ? row_at(a.cu, a.B, t) : 0;
+    double sum = 0.0;
+    if (!greedy(a, b) && m > -INFINITY) {
+        const double rate = rate_of(a, b);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum += weight(x[c][j], m, rate);
+        sum = wave_sum(sum);
+    }
+    if (lane == 0) red_sum[w] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double all = red_sum[0];
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k) all += red_sum[k];
+        a.part[(int64_t)t * a.S + s] = Part{m, at, all};
+    }
+}
+
+// Where row b ends, the same in every thread.
+struct Verdict {
+    int t;         // the logits row whose token follows
+    int accepted;  // drafts that stand
+    int draft;     // the refused one, -1: none was
+    float m;       // its largest logit, -infinity: none
+    int top;       // the lowest token that has it
+    double Z;
+};
+
+template <int PT>
+__device__ __forceinline__ double prob(const void *probs, int64_t at) {
+    return fmax((double)value<PT>(probs, at), 0.0);  // (NaN: 0)
+}
+
+__device__ __forceinline__ double prob_at(const VerifyArgs &a, int t, int v) {
+    const int64_t at = (int64_t)t * a.probs_stride + v;
+    return a.probs_type == KQ_DTYPE_F32    ? prob<KQ_DTYPE_F32>(a.probs, at)
+           : a.probs_type == KQ_DTYPE_BF16 ? prob<KQ_DTYPE_BF16>(a.probs, at)
+                                           : prob<KQ_DTYPE_F16>(a.probs, at);
+}
+
+// A wave a draft, kWaves of them at a time until one does not stand.  n > 0.
+template <int DT>
+__device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, int n) {
+    __shared__ float s_m[kWaves];
+    __shared__ int s_top[kWaves], s_ok[kWaves];
+    __shared__ double s_z[kWaves];
+    const int lane = kq_lane(), w = threadIdx.x >> 6;
+    const bool pick_top = greedy(a, b);
+    const double rate = rate_of(a, b);
+    for (int i0 = 0;; i0 += kWaves) {
+        const int i = min(i0 + w, n - 1), t = q0 + i;
+        const Part *part = a.part + (int64_t)t * a.S;
+        const bool last = i == n - 1;
+        const int d = last ? -1 : a.tokens[t + 1];
+        const bool known = d >= 0 && d < a.V;
+        const float x = known ? counted(value<DT>(a.logits, (int64_t)t * a.stride + d)) : -INFINITY;
+        const double q = known && !pick_top && a.probs ? prob_at(a, t, d) : 1.0;
+        float m = -INFINITY;
+        int at = 0x7fffffff;
+        for (int s = lane; s < a.S; s += 64) take_larger(m, at, part[s].m, part[s].at);
+        wave_largest(m, at);
+        double z = 0.0;
+        bool ok;
+        if (pick_top) {
+            ok = known && d == at;
+        } else {
+            if (m > -INFINITY)
+                for (int s = lane; s < a.S; s += 64) z += part[s].sum * weight(part[s].m, m, rate);
+            z = wave_sum(z);
+            ok = known && x > -INFINITY && (double)a.u[t] * q * z < weight(x, m, rate);
+        }
+        __syncthreads();  // the last round's reads
+        if (lane == 0) {
+            s_m[w] = m;
+            s_top[w] = at;
+            s_z[w] = z;
+            s_ok[w] = ok && !last;
+        }
+        __syncthreads();
+        int k = 0;
+        while (k < kWaves && s_ok[k]) ++k;
+        if (k < kWaves) {
+            // (waves past the row's end repeat its last row, which is never a draft)
+            const int j = min(i0 + k, n - 1), refused = j == n - 1 ? -1 : a.tokens[q0 + j + 1];
+            const float mj = s_m[k];
+            return Verdict{q0 + j, j, refused, mj, mj > -INFINITY ? s_top[k] : -1, s_z[k]};
+        }
+    }
+}
+
+__device__ __forceinline__ bool row_of(const VerifyArgs &a, int b, int &q0, int &n) {
+    q0 = min(max(a.cu[b], 0), a.T);
+    n = min(max(a.cu[b + 1], q0), a.T) - q0;
+    return n > 0;
+}
+
+// max(e - q Z, 0) of N tokens from i on; 0 past the end.
+template <int DT, int PT, int N>
+__device__ __forceinline__ void rest_of(const VerifyArgs &a, const Verdict &r, double rate, int i, double (&w)[N]) {
+    float x[N], q[N];
+    values<DT, N>((const uint8_t *)a.logits + (int64_t)r.t * a.stride * (DT == KQ_DTYPE_F32 ? 4 : 2), i, a.V, -INFINITY, x);
+    values<PT, N>((const uint8_t *)a.probs + (int64_t)r.t * a.probs_stride * (PT == KQ_DTYPE_F32 ? 4 : 2), i, a.V, 0.f, q);
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = fmax(weight(counted(x[j]), r.m, rate) - fmax((double)q[j], 0.0) * r.Z, 0.0);
+}
+
+// Sums of max(e - q Z, 0) over one slice a workgroup, of rows whose draft was
+// refused.
+template <int DT, int PT, int CH>
+__global__ __launch_bounds__(kThreads) void kq_verify_rest_kernel(VerifyArgs a) {
+    constexpr int N = kValues<DT>;
+    __shared__ double red[kWaves];
+    const int s = blockIdx.x, b = blockIdx.y;
+    int q0, n;
+    if (!row_of(a, b, q0, n) || n < 2 || greedy(a, b)) return;
+    const Verdict r = decide<DT>(a, b, q0, n);
+    if (r.accepted == n - 1 || !(r.m > -INFINITY)) return;
+    const double rate = rate_of(a, b);
+    double sum = 0.0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N;
+        double w[N];
+        rest_of<DT, PT, N>(a, r, rate, min(i, a.V), w);
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum += w[j];
+    }
+    sum = wave_sum(sum);
+    if (kq_lane() == 0) red[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double all = red[0];
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k) all += red[k];
+        a.rest[(int64_t)b * a.S + s] = all;
+    }
+}
+
+// The token that follows, one workgroup a row: the slice whose running sum passes
+// r times the whole, then the token within it.
+template <int DT, int PT, int CH>
+__global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) {
+    constexpr int N = kValues<DT>;
+    __shared__ double red[kWaves];
+    __shared__ double s_target;
+    __shared__ int s_how, s_slice, s_first, s_last;
+    const int b = blockIdx.x, lane = kq_lane(), wv = threadIdx.x >> 6;
+    int q0, n;
+    if (!row_of(a, b, q0, n)) {
+        if (threadIdx.x == 0) {
+            a.accepted[b] = 0;
+            a.next[b] = -1;
+            if (a.keep) a.keep[b] = max(a.kv[b], 0);
+        }
+        return;
+    }
+    const Verdict r = decide<DT>(a, b, q0, n);
+    const auto finish = [&](int token) {
+        a.accepted[b] = r.accepted;
+        a.next[b] = token;
+        if (a.keep) a.keep[b] = max(a.kv[b] - (n - 1 - r.accepted), 0);
+    };
+    if (greedy(a, b) || r.top < 0) {
+        if (threadIdx.x == 0) finish(r.top);
+        return;
+    }
+    const double rate = rate_of(a, b);
+    const Part *part = a.part + (int64_t)r.t * a.S;
+    const bool refused = r.accepted < n - 1, lone = refused && !a.probs && r.draft >= 0 && r.draft < a.V;
+    // weights of a slice's chunk c: how 0 as they are, 1 without the draft, 2 beside q
+    const auto weights = [&](int how, int s, int c, double(&w)[N]) {
+        const int i = min(((s * CH + c) * kThreads + (int)threadIdx.x) * N, a.V);
+        if (how == 2) {
+            rest_of<DT, PT, N>(a, r, rate, i, w);
+        } else {
+            float x[N];
+            values<DT, N>((const uint8_t *)a.logits + (int64_t)r.t * a.stride * (16 / N), i, a.V, -INFINITY, x);
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = how == 1 && i + j == r.draft ? 0.0 : weight(counted(x[j]), r.m, rate);
+        }
+    };
+    // the slice of a lone draft again without it (taken off its sum, a draft of
+    // nearly all the weight would leave a rest of few digits)
+    double without = 0.0;
+    const int own = lone ? r.draft / (CH * kThreads * N) : -1;
+    if (lone) {
+        double sum = 0.0;
+        for (int c = 0; c < CH; ++c) {
+            double w[N];
+            weights(1, own, c, w);
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum += w[j];
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) red[wv] = sum;
+        __syncthreads();
+        for (int k = 0; k < kWaves; ++k) without += red[k];
+    }
+    // wave 0: the slices' running sums
+    int how = lone ? 1 : refused && a.probs ? 2 : 0;
+    const auto slice_sum = [&](int s) {
+        return how == 2   ? a.rest[(int64_t)b * a.S + s]
+               : s == own && how == 1 ? without
+                          : part[s].sum * weight(part[s].m, r.m, rate);
+    };
+    if (wv == 0) {
+        double all = 0.0;
+        for (int pass = 0; pass < 2; ++pass) {
+            for (int s = lane; s < a.S; s += 64) all += slice_sum(s);
+            all = wave_sum(all);
+            if (all > 0.0) break;
+            how = 0;  // nothing is left beside q: the target's own
+        }
+        const float draw = a.draws[b];
+        const double target = (draw > 0.f ? (double)draw : 0.0) * all;
+        double before = 0.0, at_before = 0.0;
+        int slice = -1;
+        for (int s0 = 0; s0 < a.S; s0 += 64) {
+            const double mine = s0 + lane < a.S ? slice_sum(s0 + lane) : 0.0;
+            double run = mine;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const double v = __shfl_up(run, off);
+                if (lane >= off) run += v;
+            }
+            const uint64_t over = __ballot(mine > 0.0 && before + run > target), some = __ballot(mine > 0.0);
+            // (none passes a draw of 1: the last slice that has any weight)
+            const int pick = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
+            if (pick >= 0) {
+                slice = s0 + pick;
+                at_before = before + __shfl(run, pick) - __shfl(mine, pick);
+            }
+            if (over) break;
+            before += __shfl(run, 63);
+        }
+        if (lane == 0) {
+            s_how = how;
+            s_slice = slice;
+            s_target = target - at_before;
+            s_first = 0x7fffffff;
+            s_last = -1;
+        }
+    }
+    __syncthreads();
+    how = s_how;
+    const int slice = s_slice;
+    const double target = s_target;
+    double before = 0.0;
+    for (int c = 0; c < CH; ++c) {
+        double w[N], run[N];
+        weights(how, slice, c, w);
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) run[j] = sum += w[j];
+        double up = sum;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const double v = __shfl_up(up, off);
+            if (lane >= off) up += v;
+        }
+        __syncthreads();  // the last reads of red
+        if (lane == 63) red[wv] = up;
+        __syncthreads();
+        double mine = before + up - sum;
+        for (int k = 0; k < wv; ++k) mine += red[k];
+        const int i = ((slice * CH + c) * kThreads + (int)threadIdx.x) * N;
+        int first = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (w[j] > 0.0) {
+                last = i + j;
+                if (first == 0x7fffffff && mine + run[j] > target) first = i + j;
+            }
+        }
+        if (first != 0x7fffffff) atomicMin(&s_first, first);
+        if (last >= 0) atomicMax(&s_last, last);
+        for (int k = 0; k < kWaves; ++k) before += red[k];
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) finish(s_first != 0x7fffffff ? s_first : s_last);
+}
+
+// Chunks of 16 bytes a thread: the longest slices (fewest partials, most bytes in
+// flight a wave) that still give every CU four workgroups.
+int chunks(int64_t T, int V, int dtype) {
+    const int n = dtype == KQ_DTYPE_F32 ? 4 : 8;
+    for (int ch = 4; ch > 1; ch /= 2)
+        if (T * ((V + kThreads * n * ch - 1) / (kThreads * n * ch)) >= 1024) return ch;
+    return 1;
+}
+int slices(int V, int dtype, int ch) {
+    const int64_t len = (int64_t)kThreads * (dtype == KQ_DTYPE_F32 ? 4 : 8) * ch;
+    return (int)((V + len - 1) / len);
+}
+size_t part_bytes(int64_t T, int S) { return ((size_t)T * S * sizeof(Part) + 255) & ~(size_t)255; }
+size_t need_bytes(int64_t T, int64_t B, int S, bool probs) { return part_bytes(T, S) + (probs ? (size_t)B * S * sizeof(double) : 0); }
+
+// Grids of fewer than 2^32 threads, and 31-bit numbers of tokens a slice past the last.
+bool sizes_fit(int64_t T, int64_t B, int V, int S) {
+    return T <= 1 << 22 && B < 1 << 16 && V <= 1 << 28 && T * S < 1 << 23;
+}
+
+template <int DT, int PT, int CH>
+void launch(const VerifyArgs &a, hipStream_t s) {
+    if (a.T) hipLaunchKernelGGL((kq_verify_rows_kernel<DT, CH>), dim3(a.T * a.S), dim3(kThreads), 0, s, a);
+    if (a.T && a.probs && (a.temps || a.temp > 0.f))
+        hipLaunchKernelGGL((kq_verify_rest_kernel<DT, PT, CH>), dim3(a.S, a.B), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((kq_verify_pick_kernel<DT, PT, CH>), dim3(a.B), dim3(kThreads), 0, s, a);
+}
+
+template <int DT, int PT>
+void launch_chunks(const VerifyArgs &a, int ch, hipStream_t s) {
+    if (ch == 4) launch<DT, PT, 4>(a, s);
+    else if (ch == 2) launch<DT, PT, 2>(a, s);
+    else launch<DT, PT, 1>(a, s);
+}
+
+template <int DT>
+void launch_probs(const VerifyArgs &a, int ch, hipStream_t s) {
+    if (!a.probs || a.probs_type == KQ_DTYPE_F32) launch_chunks<DT, KQ_DTYPE_F32>(a, ch, s);
+    else if (a.probs_type == KQ_DTYPE_BF16) launch_chunks<DT, KQ_DTYPE_BF16>(a, ch, s);
+    else launch_chunks<DT, KQ_DTYPE_F16>(a, ch, s);
+}
+
+bool a_type(int dtype) { return dtype == KQ_DTYPE_F32 || dtype == KQ_DTYPE_F16 || dtype == KQ_DTYPE_BF16; }
+
+}  // namespace
+
+extern "C" {
+
+size_t kq_verify_workspace_bytes(int32_t T, int32_t B, int32_t V, int dtype, int with_probs) {
+    if (T < 1 || B < 1 || V < 1 || !a_type(dtype)) return 0;
+    const int S = slices(V, dtype, chunks(T, V, dtype));
+    return sizes_fit(T, B, V, S) ? need_bytes(T, B, S, with_probs != 0) : 0;
+}
+
+int kq_verify_drafts(const void *logits, int dtype, int64_t row_stride, const int32_t *tokens, const int32_t *cu_rows,
+                     const float *uniforms, const float *draws, const void *draft_probs, int probs_dtype,
+                     int64_t probs_row_stride, const float *temperatures, float temperature, const int32_t *kv_lens,
+                     int32_t T, int32_t B, int32_t V, int32_t *accepted, int32_t *next_tokens, int32_t *keep_lens,
+                     void *workspace, size_t workspace_bytes, kq_stream_t stream) {
+    if (B == 0) return KQ_OK;
+    const bool greedy_all = !temperatures && temperature == 0.f;
+    if (!cu_rows || !accepted || !next_tokens || (keep_lens && !kv_lens) || (T > 0 && (!logits || !tokens)) ||
+        (!greedy_all && ((T > 0 && !uniforms) || !draws)))
+        return KQ_ERR_NULL_POINTER;
+    if (!a_type(dtype) || (draft_probs && !a_type(probs_dtype))) return KQ_ERR_UNSUPPORTED_DTYPE;
+    if (T < 0 || B < 0 || V < 1 || row_stride < 0 || (draft_probs && probs_row_stride < 0)) return KQ_ERR_BAD_SHAPE;
+    if (!temperatures && !(temperature >= 0.f && temperature <= 3.4028235e38f)) return KQ_ERR_BAD_ARGUMENT;
+    if (((uintptr_t)logits & (dtype == KQ_DTYPE_F32 ? 3 : 1)) ||
+        (draft_probs && ((uintptr_t)draft_probs & (probs_dtype == KQ_DTYPE_F32 ? 3 : 1))))
+        return KQ_ERR_BAD_ALIGN;
+    const int ch = chunks(T, V, dtype), S = slices(V, dtype, ch);
+    if (!sizes_fit(T, B, V, S)) return KQ_ERR_BAD_SHAPE;
+    if (T && (!workspace || workspace_bytes < need_bytes(T, B, S, draft_probs != nullptr))) return KQ_ERR_WORKSPACE_TOO_SMALL;
+    if ((uintptr_t)workspace & 255) return KQ_ERR_BAD_ALIGN;
+    VerifyArgs a;
+    a.logits = logits;
+    a.probs = draft_probs;
+    a.stride = row_stride;
+    a.probs_stride = probs_row_stride;
+    a.tokens = tokens;
+    a.cu = cu_rows;
+    a.kv = kv_lens;
+    a.u = uniforms;
+    a.draws = draws;
+    a.temps = temperatures;
+    a.temp = temperature;
+    a.T = T;
+    a.B = B;
+    a.V = V;
+    a.S = S;
+    a.probs_type = probs_dtype;
+    a.part = (Part *)workspace;
+    a.rest = (double *)((char *)workspace + part_bytes(T, S));
+    a.accepted = accepted;
+    a.next = next_tokens;
+    a.keep = keep_lens;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == KQ_DTYPE_F32) launch_probs<KQ_DTYPE_F32>(a, ch, s);
+    else if (dtype == KQ_DTYPE_BF16) launch_probs<KQ_DTYPE_BF16>(a, ch, s);
+    else launch_probs<KQ_DTYPE_F16>(a, ch, s);
+    return hipGetLastError() == hipSuccess ? KQ_OK : KQ_ERR_LAUNCH_FAILED;
+}
+
+}  // extern "C"

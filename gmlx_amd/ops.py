@@ -34,6 +34,7 @@ copied over in place, as here):
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import struct
 from collections import OrderedDict
@@ -53,6 +54,7 @@ __all__ = [
     "quantized_matmul_grouped", "fused_mlp", "fused_mlp_status", "counts", "moe_route", "gather_qmm", "moe_glu_gather_kq", "gather_qmv_kq",
     "gather_qmv_mix_ns_kq", "moe_router_topk", "sdpa_decode_ragged", "sdpa_decode_gqa",
     "ragged_decode_attention", "wire_k", "PagedPlan", "paged_plan", "paged_write", "paged_read", "sdpa_paged",
+    "rope_frequencies", "rope_qk", "paged_write_rope", "DraftVerdict", "verify_drafts",
 ]
 
 
@@ -1493,3 +1495,276 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     _paged_call("kq_sdpa_paged", dev, q.data_ptr(), qt, pool, tab, tab_stride, width, lens, cu, T, B, Hq, mq, mkv,
                 float(scale), out.data_ptr(), ot, ws_ptr, ws_len, s)
     return out
+
+
+# ------------------------------------------------ positions and head norms
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling=None, device="cuda"):
+    """(freqs, factor) of a rotation by position: freqs float64 [rotary_dim / 2] on
+    `device`, radians a position, base ** (-2 j / rotary_dim) for pair j unless
+    `scaling` stretches them for contexts longer than the trained one; factor (a
+    number) scales the rotated values.
+
+    scaling: None, or a dict with "type" and "factor" (how many times longer, >= 1):
+      "linear"  every frequency divided by factor;
+      "ntk"     the base times factor ** (rotary_dim / (rotary_dim - 2)), which
+                divides the lowest frequency by factor and leaves the highest;
+      "bands"   by turns over the trained context ("original" positions): fewer than
+                "low" (1) divided by factor, more than "high" (4) as they are,
+                between them the two blended linearly in the turns;
+      "yarn"    the same blend, linear in the pair's number between those of
+                "high" (32) and "low" (1) turns (rounded outwards), and the
+                rotated values times 0.1 ln(factor) + 1 (or "attention")."""
+    R = int(rotary_dim)
+    if R < 2 or R % 2 or not base > 1 or math.isinf(base):
+        raise ValueError(f"rope_frequencies: an even rotary_dim and a base above 1, got {rotary_dim} and {base}")
+    pair = torch.arange(R // 2, dtype=torch.float64)
+    freqs, out = float(base) ** (-2 * pair / R), 1.0
+    if scaling is not None:
+        kind, by = scaling.get("type"), float(scaling.get("factor", 1.0))
+        if kind not in ("linear", "ntk", "bands", "yarn") or not 1 <= by < math.inf:
+            raise ValueError(f"rope_frequencies: scaling of type linear, ntk, bands or yarn and factor >= 1, got {scaling}")
+        if kind == "linear":
+            freqs = freqs / by
+        elif kind == "ntk":
+            if R < 4:
+                raise ValueError("rope_frequencies: ntk scaling needs a rotary_dim of 4 or more")
+            freqs = (float(base) * by ** (R / (R - 2))) ** (-2 * pair / R)
+        else:
+            original = float(scaling.get("original", 0))
+            low, high = float(scaling.get("low", 1)), float(scaling.get("high", 4 if kind == "bands" else 32))
+            if not original > 0 or not 0 < low < high or math.isinf(original + high):
+                raise ValueError(f"rope_frequencies: {kind} scaling needs original > 0 and 0 < low < high, got {scaling}")
+            if kind == "bands":
+                kept = ((original * freqs / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+            else:
+                # the pair (a real number) that makes `turns` turns over the trained context
+                at = lambda turns: R * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))  # noqa: E731
+                first, last = max(math.floor(at(high)), 0), min(math.ceil(at(low)), R - 1)
+                kept = 1 - ((pair - first) / max(last - first, 1e-3)).clamp(0, 1)
+                out = float(scaling.get("attention", 0.1 * math.log(by) + 1))
+            freqs = freqs / by * (1 - kept) + freqs * kept
+    return freqs.to(device), out
+
+
+def _rope(op, x, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor):
+    """The packed kq_rope and the positions' address, checked; x: the rows' tensor."""
+    dev, dt, T = x.device, x.dtype, x.shape[0]
+    if not isinstance(freqs, torch.Tensor) or freqs.dtype is not torch.float64 or freqs.dim() != 1 or \
+            freqs.device != dev or not freqs.is_contiguous():
+        raise ValueError(f"{op}: freqs must be a contiguous float64 tensor [rotary_dim / 2] on {dev}")
+    R = 2 * freqs.numel()
+    if R < 16 or R % 16 or R > D:
+        raise ValueError(f"{op}: the rotated part must be a multiple of 16 values, at most {D}, got {R}")
+    wdt, ptrs = None, []
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            ptrs.append(None)
+            continue
+        if not isinstance(w, torch.Tensor) or w.shape != (D,) or w.device != dev or w.dtype not in (dt, torch.float32) or \
+                not w.is_contiguous() or w.data_ptr() % 16 or wdt not in (None, w.dtype):
+            raise ValueError(f"{op}: {name} must be a contiguous 16-byte aligned tensor [{D}] of {dt} or float32 on "
+                             f"{dev} (both weights of one dtype)")
+        wdt = w.dtype
+        ptrs.append(w.data_ptr())
+    eps, factor = float(eps), float(factor)
+    if not 0 <= eps < 3.4e38 or not abs(factor) < 3.4e38:
+        raise ValueError(f"{op}: eps must be finite and not negative, factor finite, got {eps} and {factor}")
+    pos = _ints(positions, "positions", T, dev)
+    return _lib.Rope(freqs.data_ptr(), ptrs[0], ptrs[1], _TORCH_DTYPE[wdt or dt], R, int(bool(interleaved)), eps,
+                     factor), pos
+
+
+def _rope_rows(op, name, x, out):
+    """(x, out, the kq_rope_rows of the two): x [T, H, D], copied only where its
+    layout needs it, and its output, made where none is given."""
+    given = x
+    x, t, h = _token_rows(x)
+    T, H, D = x.shape
+    if out is None:
+        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+        ot, oh = H * D, D
+    else:
+        if not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+            raise ValueError(f"{op}: {name}_out must be like {name}")
+        ot, oh, one = out.stride()
+        ot, oh = ot if T > 1 else H * D, oh if H > 1 else D
+        if one != 1 or ot % 8 or oh % 8 or out.data_ptr() % 16 or not _apart(T, ot, H, oh, D):
+            raise ValueError(f"{op}: {name}_out must have contiguous rows at strides in multiples of 8, none on "
+                             "another, and be 16-byte aligned")
+        if out.data_ptr() == given.data_ptr() and out.stride() != given.stride():
+            raise ValueError(f"{op}: {name}_out at {name}'s address must have its strides")
+    return x, out, _lib.RopeRows(x.data_ptr(), out.data_ptr(), t, h, ot, oh, H)
+
+
+def _apart(T, t, H, h, D):
+    """Whether no two rows of D values at strides t (of T tokens) and h (of H heads) overlap."""
+    reach = D
+    for stride, n in sorted(((t, T), (h, H))):
+        if n > 1 and stride < reach:
+            return False
+        reach += stride * (n - 1)
+    return True
+
+
+def rope_qk(q, k, positions, freqs, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, factor=1.0, q_out=None,
+            k_out=None):
+    """Queries [T, Hq, D] and keys [T, Hkv, D] rotated by their positions, each
+    head normed before where it has a weight, in one pass: (q, k) rotated, in their
+    dtype.
+
+    Of a head's row x: y = x * w / sqrt(mean(x ** 2) + eps) with w = q_weight or
+    k_weight [D] (None: no norm; the rows' dtype or float32), and the pairs (a, b) of
+    its first 2 * len(freqs) values become (a cos - b sin, b cos + a sin) * factor of
+    the angle positions[t] * freqs[j]: pair j is values j and j + len(freqs), or with
+    `interleaved` 2 j and 2 j + 1.  The rest of the row is normed only.  Computed in
+    fp32 (the angle in 64 bits) and rounded once.
+
+    freqs float64 [rotary_dim / 2] (rope_frequencies), rotary_dim a multiple of 16 up
+    to D; positions int32 [T] on the device (PagedPlan.positions).  A token of
+    negative position is left out: its rows of q_out and k_out stay as they were
+    (unspecified where they are not given).  float16 or bfloat16, D in 64, 96, 128,
+    256, 512; q and k may be views of a packed q|k|v (strides of 8 values).  q_out /
+    k_out: where the results go, also q and k themselves (their own views), else no
+    part of an input."""
+    _fault("rope_qk")
+    _require_gpu(q, k)
+    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype != q.dtype or \
+            k.device != q.device or q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("rope_qk: q [T, Hq, D] and k [T, Hkv, D] must be float16 or bfloat16, of one dtype and device")
+    T, Hq, D = q.shape
+    if D not in (64, 96, 128, 256, 512):
+        raise ValueError(f"rope_qk: head dims 64, 96, 128, 256 and 512, got {D}")
+    rope, pos = _rope("rope_qk", q, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor)
+    q, q_out, qr = _rope_rows("rope_qk", "q", q, q_out)
+    k, k_out, kr = _rope_rows("rope_qk", "k", k, k_out)
+    if T and Hq + k.shape[1]:
+        _paged_call("kq_rope_qk", q.device, ctypes.byref(rope), pos, T, D, _TORCH_DTYPE[q.dtype], ctypes.byref(qr),
+                    ctypes.byref(kr), _stream(q))
+    return q_out, k_out
+
+
+def paged_write_rope(q, k, v, k_cache, v_cache, slots, positions, freqs, q_weight=None, k_weight=None, eps=1e-6,
+                     interleaved=False, factor=1.0, k_scales=None, k_biases=None, v_scales=None, v_biases=None, q_out=None):
+    """rope_qk and paged_write in one launch: the queries [T, Hq, D] normed and
+    rotated are returned, the keys [T, Hkv, D] go normed and rotated to their slots of
+    a paged cache, the values beside them as they are.  Bit for bit what the two
+    calls give.
+
+    Arguments as rope_qk and paged_write have them.  A token of negative position
+    (PagedPlan marks refused rows' so) is left out: its query row stays as it was in
+    q_out (unspecified where that is not given) and its slot is not written; one whose
+    slot lies outside the pool has its queries rotated all the same."""
+    _fault("paged_write_rope")
+    lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
+    dev, dt, shape, D = lay.device, lay.dtype, k.shape, lay.D
+    if k.dtype is not dt or v.dtype is not dt or k.device != dev or v.device != dev or len(shape) != 3 or \
+            v.shape != shape or shape[1] != lay.Hkv or shape[2] != D:
+        raise ValueError(f"paged_write_rope: k and v must be [T, {lay.Hkv}, {D}] of dtype {dt} on the cache's device")
+    T = shape[0]
+    if q.dtype is not dt or q.device != dev or q.dim() != 3 or q.shape[0] != T or q.shape[2] != D:
+        raise ValueError(f"paged_write_rope: q must be [{T}, Hq, {D}] of dtype {dt} on the cache's device")
+    rope, pos = _rope("paged_write_rope", q, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor)
+    sl = _ints(slots, "slots", T, dev)
+    q, q_out, qr = _rope_rows("paged_write_rope", "q", q, q_out)
+    k, kt, kh = _token_rows(k)
+    v, vt, vh = _token_rows(v)
+    if T:
+        _paged_call("kq_paged_write_rope", dev, pool, ctypes.byref(rope), pos, sl, T, ctypes.byref(qr), k.data_ptr(), kt,
+                    kh, v.data_ptr(), vt, vh, _stream(q))
+    return q_out
+
+
+# -------------------------------------------------------------- drafted tokens
+
+class DraftVerdict(NamedTuple):
+    """What verify_drafts says of each row; int32 tensors on the device."""
+    accepted: torch.Tensor    # [B] drafts that stand
+    tokens: torch.Tensor      # [B] the token after them, -1: none
+    keep_lens: torch.Tensor   # [B] cached tokens to keep (None without kv_lens)
+
+
+def _floats(t, name, n, device):
+    """The address of a contiguous float32 device tensor of n values."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.shape != (n,) or t.device != device or \
+            not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor of {n} values on {device}")
+    return t.data_ptr()
+
+
+def verify_drafts(logits, tokens, cu, uniforms=None, draws=None, draft_probs=None, temperature=1.0, kv_lens=None):
+    """How many drafted tokens of each row stand against the target's logits, and
+    the token after them, from given random numbers: speculative sampling, in which
+    the tokens kept are distributed as the target's own.
+
+    logits [T, V] (float32, float16 or bfloat16): row b's are cu[b] .. cu[b + 1] (n of
+    them), of the tokens the step was fed, tokens int32 [T]; tokens[t + 1] is the draft
+    that row t is asked about, for all but the row's last.  With p the softmax of row
+    t's logits / temperature and q the distribution that draft d was drawn from
+    (draft_probs[t], [T, V] of any of the types; None: d alone was proposed, q_d = 1), d
+    stands where uniforms[t] * q_d < p_d.  Behind the first draft that does not stand
+    the token is drawn from max(p - q, 0) (None: from p without d), behind the last
+    one from p: the least token at which the running sum passes draws[b] times the
+    whole.  A temperature of 0 takes the largest logit (the lowest of equal ones) and
+    the drafts that are it.
+
+    uniforms float32 [T] and draws float32 [B] in [0, 1), not needed where the
+    temperature is 0; temperature a number, or float32 [B] on the device (0 or below:
+    greedy); cu int32 [B + 1]; kv_lens int32 [B] (PagedPlan.kv_lens, all n tokens of
+    the row counted) for keep_lens, which paged_plan takes.  Returns a DraftVerdict.
+
+    Computed in 64 bits.  NaN logits count as -inf, +inf as the largest float32,
+    probabilities below 0 or NaN as 0; a draft outside the vocabulary does not stand.
+    A row without logits gives 0 and -1; where nothing is above -inf the row ends,
+    with -1.  Logits behind cu[B] are not read."""
+    _fault("verify_drafts")
+    _require_gpu(logits)
+    dev = logits.device
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("verify_drafts: logits must be [T, V]")
+    T, V = logits.shape
+    dt = _dt(logits.dtype)
+    B = cu.numel() - 1
+    if B < 0:
+        raise ValueError("verify_drafts: cu must be int32 [B + 1]")
+    cu_p, tok = _ints(cu, "cu", B + 1, dev), _ints(tokens, "tokens", T, dev)
+    logits, stride = _logit_rows(logits, "logits")
+    temps, temp = None, 1.0
+    if isinstance(temperature, torch.Tensor):
+        temps = _floats(temperature, "temperature", B, dev)
+    else:
+        temp = float(temperature)
+        if not 0 <= temp < 3.4e38:
+            raise ValueError(f"verify_drafts: a temperature of 0 or more, got {temperature}")
+        temp = max(temp, 1e-45) if temp else 0.0  # (not 0 in float32)
+    if (uniforms is None or draws is None) and not (temps is None and temp == 0):
+        raise ValueError("verify_drafts: uniforms and draws are needed unless the temperature is 0")
+    u = None if uniforms is None else _floats(uniforms, "uniforms", T, dev)
+    r = None if draws is None else _floats(draws, "draws", B, dev)
+    probs, pdt, pstride = None, 0, 0
+    if draft_probs is not None:
+        if not isinstance(draft_probs, torch.Tensor) or draft_probs.shape != (T, V) or draft_probs.device != dev:
+            raise ValueError(f"verify_drafts: draft_probs must be [{T}, {V}] on {dev}")
+        pdt = _dt(draft_probs.dtype)
+        draft_probs, pstride = _logit_rows(draft_probs, "draft_probs")
+        probs = draft_probs.data_ptr()
+    kv = None if kv_lens is None else _ints(kv_lens, "kv_lens", B, dev)
+    out = torch.empty((2 if kv is None else 3, B), dtype=_I32, device=dev)
+    got = out.unbind(0)
+    if B:
+        need = lib().kq_verify_workspace_bytes(T, B, V, dt, int(probs is not None))
+        # (the call's own, as sdpa_paged's)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        at = out.data_ptr()
+        _paged_call("kq_verify_drafts", dev, logits.data_ptr(), dt, stride, tok, cu_p, u, r, probs, pdt, pstride, temps,
+                    temp, kv, T, B, V, at, at + 4 * B, None if kv is None else at + 8 * B,
+                    None if ws is None else ws.data_ptr(), need, _stream(logits))
+    return DraftVerdict(got[0], got[1], None if kv is None else got[2])
+
+
+def _logit_rows(x, name):
+    """x [T, V] with its rows contiguous and apart by 0 or more values (copied only
+    where they are not): (x, row stride)."""
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]

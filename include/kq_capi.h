@@ -571,6 +571,91 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
                   int32_t T, int32_t B, int32_t Hq, int32_t max_q, int32_t max_kv, float scale, void *out,
                   int64_t out_stride, void *workspace, size_t workspace_bytes, kq_stream_t stream);
 
+/* ---- positions and head norms ----------------------------------------------- */
+/* The rotation of queries and keys by their positions, and the norm of each head
+ * before it.  Of a head's row x of D values, with a weight w [D] (NULL: no norm),
+ *   y = x * w / sqrt(mean(x^2) + eps),
+ * and of its first rotary_dim values the pairs (a, b) at position p become
+ *   (a cos(p f) - b sin(p f)) factor, (b cos(p f) + a sin(p f)) factor,
+ * pair j < rotary_dim / 2 being values j and j + rotary_dim / 2, or with
+ * `interleaved` 2 j and 2 j + 1, and f = freqs[j] (radians a position, fp64 on the
+ * device).  fp32 throughout, p f in 64 bits; one rounding.  A stretched context is
+ * in the frequencies and the factor. */
+typedef struct {
+    const double *freqs;               /* [rotary_dim / 2], 8-byte aligned */
+    const void *q_weight, *k_weight;   /* [D], 16-byte aligned, or NULL */
+    int32_t weight_dtype;              /* the rows' dtype or fp32 */
+    int32_t rotary_dim, interleaved;   /* rotary_dim: a multiple of 16, 16 .. D */
+    float eps, factor;                 /* eps >= 0; both finite */
+} kq_rope;
+
+/* Rows [T][heads][D] of 16-bit values, D contiguous: strides in elements,
+ * multiples of 8, addresses 16-byte aligned.  out may be x itself (with its
+ * strides), and overlaps no other input otherwise. */
+typedef struct {
+    const void *x;
+    void *out;
+    int64_t token_stride, head_stride, out_token_stride, out_head_stride;
+    int32_t heads; /* 0 .. 65536; 0: none, x and out may be NULL */
+} kq_rope_rows;
+
+/* q and k at positions[t] (int32 on the device).  A token of negative position (as
+ * kq_paged_plan marks those without one) is left out: its output stays as it was.
+ * dtype f16 or bf16, D in {64, 96, 128, 256, 512}, T up to 2^23. */
+int kq_rope_qk(const kq_rope *rope, const int32_t *positions, int32_t T, int32_t D, int dtype, const kq_rope_rows *q,
+               const kq_rope_rows *k, kq_stream_t stream);
+
+/* kq_rope_qk whose keys go to slots[t] of the pool, v [T][Hkv][D] beside them: bit
+ * for bit kq_rope_qk followed by kq_paged_write, in one launch.  A token of
+ * negative position is left out, its slot too; one whose slot lies outside the pool
+ * has its queries rotated and writes nothing.  Slots and pools as kq_paged_write
+ * has them; q as above. */
+int kq_paged_write_rope(const kq_paged_pool *pool, const kq_rope *rope, const int32_t *positions, const int32_t *slots,
+                        int32_t T, const kq_rope_rows *q, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void *v, int64_t v_token_stride, int64_t v_head_stride, kq_stream_t stream);
+
+/* ---- drafted tokens --------------------------------------------------------- */
+/* How many drafted tokens of each row stand against the target's logits, and the
+ * token after them, from given random numbers (speculative sampling: the tokens
+ * kept are distributed as the target's).  No counterpart in the reference's call
+ * sites.
+ *
+ * Row b's logits are rows t = cu_rows[b] .. cu_rows[b + 1] of logits [T][V]
+ * (row_stride values apart; fp32, fp16 or bf16), n of them, of the tokens that the
+ * step was fed: tokens[t] (int32 [T]); tokens[t + 1] is the draft that row t is
+ * asked about, for all but a row's last, n - 1 drafts.  With e_v = exp((x_v - max x)
+ * / c) at temperature c and Z their sum, draft d stands where
+ *   uniforms[t] * q_d * Z < e_d  (u q < p),
+ * q = draft_probs[t][d], the distribution that it was drawn from (rows as the
+ * logits', their strides and type apart), or 1 with draft_probs NULL (the draft alone
+ * was proposed).  accepted[b]: drafts before the first that does not stand.
+ * next_tokens[b]: the least v at which the running sum of w passes draws[b] times
+ * the whole, over the row behind the accepted ones, w_v = max(e_v - q_v Z, 0) (e_v
+ * without e_d, draft_probs NULL) where a draft was refused there, or e_v (also where
+ * the other is 0 throughout); for a draw of 1 or more the last with any weight.
+ * Temperature 0 (or below): drafts stand where they are the largest logit, which
+ * else is the next token; of equal ones the lowest.
+ * keep_lens[b] (may be NULL): kv_lens[b] less the refused drafts, what
+ * kq_paged_plan keeps of a row whose kv_lens count all n tokens.
+ *
+ * Weights and sums in fp64.  NaN counts as -infinity, +infinity as the largest
+ * fp32; probabilities below 0 and NaN as 0; drafts outside 0 .. V - 1 do not stand.
+ * A row without logits has 0 and -1; one of nothing above -infinity ends there,
+ * with -1.
+ *
+ * temperatures: fp32 [B] on the device, or NULL and `temperature` (finite, >= 0) for
+ * all.  uniforms [T] and draws [B] fp32 in [0, 1) (may be NULL where temperature is
+ * 0 for all).  T up to 2^22, B below 2^16, V up to 2^28, and fewer than 2^23 slices
+ * of a row (of 4096 to 32768 bytes).  Workspace: kq_verify_workspace_bytes, no
+ * zero-fill needed, 256-byte aligned; calls that share one are ordered.  Nothing
+ * is read of logits past cu_rows[B]. */
+size_t kq_verify_workspace_bytes(int32_t T, int32_t B, int32_t V, int dtype, int with_probs);
+int kq_verify_drafts(const void *logits, int dtype, int64_t row_stride, const int32_t *tokens, const int32_t *cu_rows,
+                     const float *uniforms, const float *draws, const void *draft_probs, int probs_dtype,
+                     int64_t probs_row_stride, const float *temperatures, float temperature, const int32_t *kv_lens,
+                     int32_t T, int32_t B, int32_t V, int32_t *accepted, int32_t *next_tokens, int32_t *keep_lens,
+                     void *workspace, size_t workspace_bytes, kq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,249 @@
+"""Drafted tokens verified on the GPU against fp64 numpy: whole numbers, so equal.
+(Two fp64 computations disagree where a border of the running sum and the draw are
+within some 10^-13 of each other: inputs are random, or sums exact.)"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import step as ref
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def _say(*a):
+    print(*a, flush=True)
+
+
+def _case(ns, V, dt, pt, seed, spread=3.0, near=0.5, temp=1.0):
+    """Logits of ragged rows, drafts drawn from a model near the target's."""
+    rng = np.random.default_rng(seed)
+    T, B = int(sum(ns)), len(ns)
+    logits = torch.from_numpy(rng.normal(0, spread, (T, V))).to(dt)
+    other = logits.double().numpy() + rng.normal(0, near, (T, V))
+    other = other / (temp if temp > 0 else 1.0)
+    p = np.exp(other - other.max(1, keepdims=True)) if T else other
+    p = p / p.sum(1, keepdims=True)
+    tokens = np.zeros(T, np.int64)
+    for t in range(T - 1):
+        tokens[t + 1] = np.searchsorted(np.cumsum(p[t]), rng.random() * 0.999999)
+    return dict(logits=logits.cuda(), tokens=torch.tensor(np.minimum(tokens, V - 1), dtype=torch.int32, device="cuda"),
+                cu=torch.tensor(np.concatenate([[0], np.cumsum(ns)]), dtype=torch.int32, device="cuda"),
+                uniforms=torch.from_numpy(rng.random(T).astype(np.float32)).cuda(),
+                draws=torch.from_numpy(rng.random(B).astype(np.float32)).cuda(),
+                draft_probs=None if pt is None else torch.from_numpy(p).to(pt).cuda(), temperature=temp,
+                kv_lens=torch.tensor([n + 3 for n in ns], dtype=torch.int32, device="cuda"))
+
+
+def _want(c):
+    at = lambda x: None if x is None else x.double().cpu().numpy() if x.is_floating_point() else x.cpu().numpy()  # noqa: E731
+    temp = c["temperature"]
+    return ref.verify(at(c["logits"]), at(c["tokens"]), at(c["cu"]), at(c["uniforms"]), at(c["draws"]),
+                      at(c["draft_probs"]), temp if not isinstance(temp, torch.Tensor) else at(temp), at(c["kv_lens"]))
+
+
+def _check(c):
+    from gmlx_amd import ops
+    got = ops.verify_drafts(**c)
+    want = _want(c)
+    assert got.accepted.tolist() == want[0]
+    assert got.tokens.tolist() == want[1]
+    assert (got.keep_lens is None and want[2] is None) or got.keep_lens.tolist() == want[2]
+    return got
+
+
+@pytest.mark.parametrize("dt,pt", [(F16, None), (BF16, F32), (F32, F32), (F16, F16), (BF16, BF16), (F32, BF16), (F16, F32)])
+@pytest.mark.parametrize("V", [1, 2, 7, 33, 1000, 2047, 2049, 8193, 50001])
+def test_verify(V, dt, pt):
+    rng = np.random.default_rng(V)
+    ns = [1, 5, 0, 3, 9, 2, 1, 4, 0] + rng.integers(0, 7, 5 if V > 9000 else 40).tolist()
+    _say("verify", V, dt, pt)
+    for temp in (1.0, 0.0, 0.6, 2.5):
+        _check(_case(ns, V, dt, pt, V + int(10 * temp), temp=temp))
+
+
+def test_a_large_batch_takes_long_slices():
+    for V, B, dt, pt in ((32000, 300, BF16, None), (9001, 500, F32, F16)):
+        rng = np.random.default_rng(B)
+        _say("large", V, B)
+        _check(_case(rng.integers(1, 4, B).tolist(), V, dt, pt, B))
+
+
+def test_drafts_of_all_kinds_of_agreement():
+    """Models that agree (all stand) and that do not (the first falls), long drafts."""
+    for near, spread in ((0.0, 4.0), (8.0, 4.0), (0.1, 0.0)):
+        _say("near", near)
+        got = _check(_case([70, 1, 130, 6], 300, F32, F32, 5, spread=spread, near=near))
+        if near == 0.0:
+            assert got.accepted.tolist() == [69, 0, 129, 5]
+
+
+def test_temperatures_by_row():
+    c = _case([4, 3, 1, 5, 2, 6], 5000, BF16, F32, 11)
+    c["temperature"] = torch.tensor([1.0, 0.0, -1.0, 0.3, float("nan"), 1e-30], device="cuda")
+    _check(c)
+
+
+def test_equal_logits_go_to_the_lowest_and_exact_sums():
+    """Equal weights sum exactly: the draw of k / V starts token k."""
+    from gmlx_amd import ops
+    V = 4096
+    B = 64
+    x = torch.zeros(B, V, device="cuda")
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    k = torch.arange(B, device="cuda") * 63
+    r = ops.verify_drafts(x, torch.zeros(B, dtype=torch.int32, device="cuda"), cu, torch.zeros(B, device="cuda"),
+                          (k.double() / V).float())
+    assert r.tokens.tolist() == k.tolist() and r.accepted.tolist() == [0] * B and r.keep_lens is None
+    x[:, 7] = x[:, 4000] = 2.0
+    r = ops.verify_drafts(x.bfloat16(), torch.zeros(B, dtype=torch.int32, device="cuda"), cu, temperature=0)
+    assert r.tokens.tolist() == [7] * B
+
+
+@pytest.mark.parametrize("pt", [None, F32])
+def test_draws_at_the_ends(pt):
+    c = _case([3, 1, 4, 2, 5], 2500, F16, pt, 21)
+    for u in (0.0, 1.0 - 2.0 ** -24, 1.0):
+        for r in (0.0, 1.0 - 2.0 ** -24, 1.0, 1.5, -1.0):
+            c["uniforms"].fill_(u)
+            c["draws"].fill_(r)
+            _say("ends", u, r)
+            if pt is None and r < 1:
+                _check(c)
+            elif r < 1 - 2.0 ** -23:
+                _check(c)
+            else:  # (a border within 10^-13 of the whole is any of the last tokens': one with weight)
+                from gmlx_amd import ops
+                got = ops.verify_drafts(**c)
+                assert got.accepted.tolist() == _want(c)[0] and all(0 <= t < 2500 for t in got.tokens.tolist())
+
+
+def test_logits_and_probabilities_that_are_not_finite():
+    nan, inf = float("nan"), float("inf")
+    for temp in (1.0, 0.0, 0.5):
+        for dt in (F32, F16, BF16):
+            c = _case([3, 3, 2, 4, 1, 2, 3], 3000, dt, F32, 31, temp=temp)
+            x, p = c["logits"], c["draft_probs"]
+            x[0, ::2] = -inf
+            x[1, 5] = nan
+            x[3] = -inf                     # nothing to take
+            x[6, :] = nan
+            x[8, 77] = inf
+            x[9, [3, 2999]] = inf
+            x[12] = -inf
+            x[12, 1234] = -5.0              # one token only
+            x[13, :2999] = -inf
+            p[1, 4:900] = nan
+            p[4] = -1.0
+            p[9] = 0.0
+            p[10, 7] = inf
+            c["tokens"][2], c["tokens"][10] = 3000, -5  # no tokens
+            _say("odd", temp, dt)
+            _check(c)
+            c["draft_probs"] = None
+            _check(c)
+
+
+def test_probabilities_equal_to_the_targets_leave_no_rest():
+    """Nothing is left beside q: the target's own."""
+    from gmlx_amd import ops
+    V = 1024
+    x = torch.zeros(2, V, device="cuda")
+    p = torch.full((2, V), 1.0 / V, device="cuda")  # exact
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    r = ops.verify_drafts(x, i32(0, 9), i32(0, 2), torch.ones(2, device="cuda"), torch.tensor([0.5], device="cuda"), p)
+    assert (r.accepted.tolist(), r.tokens.tolist()) == ([0], [512])
+
+
+def test_kept_tokens_follow_the_target():
+    """The first token after a step (a draft that stands, or the token in its
+    place) has the target's distribution: 40000 rows, five deviations."""
+    from gmlx_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    B, V = 40000, 6
+    p = torch.tensor([0.4, 0.05, 0.25, 0.0, 0.2, 0.1], device="cuda")
+    q = torch.tensor([0.1, 0.5, 0.15, 0.05, 0.0, 0.2], device="cuda")
+    x = p.log().repeat(2 * B, 1)
+    drafts = torch.multinomial(q, B, replacement=True, generator=gen).int()
+    tokens = torch.stack([torch.zeros_like(drafts), drafts], 1).reshape(-1).contiguous()
+    cu = torch.arange(0, 2 * B + 1, 2, dtype=torch.int32, device="cuda")
+    u, r = torch.rand(2 * B, device="cuda", generator=gen), torch.rand(B, device="cuda", generator=gen)
+    for probs in (q.expand(2 * B, V), None):
+        d = tokens if probs is not None else torch.where(torch.arange(2 * B, device="cuda") % 2 == 1, 2, 0).int()
+        got = ops.verify_drafts(x, d, cu, u, r, draft_probs=probs)
+        first = torch.where(got.accepted == 1, d[1::2], got.tokens).long()
+        share = torch.bincount(first, minlength=V).double() / B
+        room = 5 * (p.double() * (1 - p.double()) / B).sqrt() + 1e-9
+        assert ((share - p.double()).abs() <= room).all(), share
+
+
+def test_padding_strides_and_the_same_bits_again():
+    """Rows behind the last sequence are not read; rows of a wider matrix, rows at
+    odd addresses, one row for all."""
+    from gmlx_amd import ops
+    c = _case([2, 4, 1, 3], 1003, BF16, F32, 41)
+    want = _check(c)
+    wide = torch.full((14, 1009), float("nan"), dtype=BF16, device="cuda")
+    wide[:10, 3:1006] = c["logits"]
+    probs = torch.full((14, 1007), float("nan"), device="cuda")
+    probs[:10, 1:1004] = c["draft_probs"]
+    pad = lambda x, v: torch.cat([x, torch.full((4,), v, dtype=x.dtype, device="cuda")])  # noqa: E731
+    got = ops.verify_drafts(wide[:, 3:1006], pad(c["tokens"], -1), c["cu"], pad(c["uniforms"], float("nan")), c["draws"],
+                            probs[:, 1:1004], kv_lens=c["kv_lens"])
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    one = c["logits"][:1].expand(10, 1003)
+    c["logits"] = one
+    _check(c)
+    c["logits"] = c["logits"].t().contiguous().t()  # columns together: copied
+    _check(c)
+
+
+def test_no_rows():
+    from gmlx_amd import ops
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    f = lambda n: torch.zeros(n, device="cuda")  # noqa: E731
+    r = ops.verify_drafts(torch.zeros(0, 50, device="cuda"), z(0), z(4), f(0), f(3), kv_lens=z(3) + 5)
+    assert (r.accepted.tolist(), r.tokens.tolist(), r.keep_lens.tolist()) == ([0] * 3, [-1] * 3, [5] * 3)
+    r = ops.verify_drafts(torch.zeros(4, 50, device="cuda"), z(4), z(1), f(4), f(0))
+    assert r.accepted.numel() == 0 and r.tokens.numel() == 0
+
+
+def test_captured_and_replayed():
+    """Two graphs captured on one stream, replayed in turn beside eager calls."""
+    from gmlx_amd import ops
+    cs = [_case([3, 5, 1], 9000, BF16, F32, 51), _case([2] * 9, 3001, F32, None, 52, temp=0.7)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(s):
+        for c in cs:
+            ops.verify_drafts(**c)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                outs.append(ops.verify_drafts(**c))
+            graphs.append(g)
+    torch.cuda.current_stream().wait_stream(s)
+    for _ in range(4):
+        for c, g, o in zip(cs, graphs, outs):
+            c["draws"].copy_(torch.rand_like(c["draws"]))
+            c["uniforms"].copy_(torch.rand_like(c["uniforms"]))
+            g.replay()
+            torch.cuda.synchronize()
+            want = _check(c)
+            for a, b in zip(o, want):
+                assert torch.equal(a, b)
+
+
+def test_refusals():
+    from gmlx_amd import ops
+    base = _case([2, 3], 100, F16, F32, 61)
+    for bad in (dict(logits=base["logits"][0]), dict(logits=base["logits"].cpu()), dict(logits=base["logits"].double()),
+                dict(tokens=base["tokens"][:3]), dict(tokens=base["tokens"].long()), dict(cu=base["cu"].long()),
+                dict(uniforms=None), dict(draws=None), dict(uniforms=base["uniforms"].double()), dict(draws=base["draws"][:1]),
+                dict(draft_probs=base["draft_probs"][:, :99]), dict(draft_probs=base["draft_probs"].double()),
+                dict(temperature=-0.5), dict(temperature=float("nan")), dict(temperature=float("inf")),
+                dict(temperature=torch.ones(3, device="cuda")), dict(kv_lens=base["kv_lens"][:1])):
+        with pytest.raises(ValueError):
+            ops.verify_drafts(**{**base, **bad})
