@@ -50,6 +50,7 @@ EXPORTS = (
     "kq_sdpa_decode_gqa_q8", "kq_sdpa_decode_gqa_noalloc",
     "kq_sdpa_cascade_workspace_bytes", "kq_sdpa_decode_gqa_cascade", "kq_sdpa_decode_gqa_cascade_q8",
     "kq_paged_plan", "kq_paged_write", "kq_paged_read", "kq_sdpa_paged_workspace_bytes", "kq_sdpa_paged",
+    "kq_sdpa_paged_window_workspace_bytes", "kq_sdpa_paged_window",
     "kq_rope_qk", "kq_paged_write_rope", "kq_verify_workspace_bytes", "kq_verify_drafts",
     "kq_gguf_open", "kq_gguf_close", "kq_gguf_header", "kq_gguf_kv", "kq_gguf_tensor", "kq_gguf_type_size",
 )
@@ -210,6 +211,9 @@ _SIGS = {
     "kq_sdpa_paged_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _int], _sz),
     "kq_sdpa_paged": ([_vp, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
                        _f32, _vp, _i64, _vp, _sz, _vp], _int),
+    "kq_sdpa_paged_window_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _int, _i32, _i32], _sz),
+    "kq_sdpa_paged_window": ([_vp, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                              _f32, _vp, _i64, _vp, _sz, _vp], _int),
     "kq_rope_qk": ([_vp, _vp, _i32, _i32, _int, _vp, _vp, _vp], _int),
     "kq_paged_write_rope": ([_vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp], _int),
     "kq_verify_workspace_bytes": ([_i32, _i32, _i32, _int, _int], _sz),

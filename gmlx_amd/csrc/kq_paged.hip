@@ -54,6 +54,7 @@ struct PagedArgs {
     int32_t slots;       // of the workspace
     int32_t few_blocks;  // the most 16-column blocks of a row of few columns
     int32_t direct;    // the wave kernel's grid is (split, kv head, row), the merge's (token and head, row)
+    int32_t window, sinks;  // (Window)
 };
 
 // Least keys of a chunk's split, where the GPU has room for more workgroups: 512
@@ -111,10 +112,43 @@ struct Row {
     int q0;      // first query row
     int n;       // tokens computed
     int kv;      // keys attended: the row's, cut by max_kv and the table's width
+    int span;    // keys that its splits divide: all, or the most that a block sees through its window
     int before;  // cached tokens before the new ones, uncut (below 0: more new ones than cached)
     int blocks, splits;
 };
 
+// A window: the token that sees keys 0 .. p alone sees the last `window` of them and
+// the row's first `sinks`.  The keys that some column of a block sees are then its
+// first `head` pieces of 16 (the sinks') and those from the first column's window
+// on; the block numbers these keys on, as if the `skip` pieces between were not
+// there, and everything that goes by key numbers (splits, tiles, ends) goes by
+// these; only a table's entry and a key's place in its page go by the key itself.
+// So what is read and multiplied is the window, whatever lies behind it.
+struct Window {
+    int head, skip;  // pieces of 16 keys
+
+    // of a block whose first column sees `first` keys
+    __device__ __forceinline__ Window(const PagedArgs &a, int first) {
+        head = (a.sinks + 15) >> 4;
+        skip = max((max(first - a.window, 0) >> 4) - head, 0);
+    }
+    // piece of the row that the block's piece c is
+    __device__ __forceinline__ int piece(int c) const { return c < head ? c : c + skip; }
+    // how many of the block's keys are among the row's first x
+    __device__ __forceinline__ int keys(int x) const { return x <= 16 * head ? x : max(16 * head, x - 16 * skip); }
+    // the first key of the block in the window of a token that sees `seen` keys
+    __device__ __forceinline__ int low(const PagedArgs &a, int seen) const { return keys(max(seen - a.window, 0)); }
+};
+
+// The most keys that a block of `cols` columns of up to n tokens sees through a
+// window (its tokens' windows together, with what completes the pieces at the ends).
+__host__ __device__ __forceinline__ int window_span(int kv, int window, int sinks, int n, int G, int cols) {
+    const int tokens = (cols + G - 2) / G + 1;
+    const int64_t span = (int64_t)((sinks + 15) & ~15) + window + (n < tokens ? n : tokens) + 14;
+    return (int)(span < kv ? span : kv);
+}
+
+template <bool WIN>
 __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     Row r;
     r.q0 = min(max(a.cu_q[b], 0), a.T);
@@ -123,8 +157,15 @@ __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
     r.kv = (int)min((int64_t)min(kv, a.max_kv), (int64_t)a.width << a.lps);
     // what a token sees goes by the row as it is, of which a cut leaves keys out
     r.before = kv - n;
-    r.blocks = row_blocks(r.n, a.G, few_columns(r.n, a.G, a.few_limit) ? a.few_cols : a.group_cols);
-    r.splits = paged_splits(a.rule, r.n, r.kv, a.G, a.Hkv, a.few_limit, a.group_cols, a.group_slots);
+    const int cols = few_columns(r.n, a.G, a.few_limit) ? a.few_cols : a.group_cols;
+    r.blocks = row_blocks(r.n, a.G, cols);
+    r.span = r.kv;
+    if constexpr (WIN) {
+        // (keys that only tokens past max_q see are nobody's)
+        r.kv = min(r.kv, max(r.before + r.n, 0));
+        r.span = window_span(r.kv, a.window, a.sinks, r.n, a.G, cols);
+    }
+    r.splits = paged_splits(a.rule, r.n, r.span, a.G, a.Hkv, a.few_limit, a.group_cols, a.group_slots);
     return r;
 }
 
@@ -201,6 +242,7 @@ __device__ __forceinline__ Row lane_row(const Row &x, int src) {
     r.q0 = __builtin_amdgcn_readlane(x.q0, src);
     r.n = __builtin_amdgcn_readlane(x.n, src);
     r.kv = __builtin_amdgcn_readlane(x.kv, src);
+    r.span = __builtin_amdgcn_readlane(x.span, src);
     r.before = __builtin_amdgcn_readlane(x.before, src);
     r.blocks = __builtin_amdgcn_readlane(x.blocks, src);
     r.splits = __builtin_amdgcn_readlane(x.splits, src);
@@ -210,7 +252,7 @@ __device__ __forceinline__ Row lane_row(const Row &x, int src) {
 // The row b that unit u belongs to, with u made its number within the row, and
 // the row's first partial slot; false past the last unit.  units(row) is summed
 // over the rows, 64 at a time, by every wave that asks.
-template <class Units>
+template <bool WIN, class Units>
 __device__ __forceinline__ bool find_unit(const PagedArgs &a, Units &&units, int &u, int &b, Row &row, int &slot0) {
     const int lane = kq_lane();
     int slots = 0;
@@ -218,7 +260,7 @@ __device__ __forceinline__ bool find_unit(const PagedArgs &a, Units &&units, int
         int mu = 0, ms = 0;
         Row x{};
         if (c0 + lane < a.B) {
-            x = row_at(a, c0 + lane);
+            x = row_at<WIN>(a, c0 + lane);
             mu = units(x);
             ms = row_slots(a, x);
         }
@@ -241,6 +283,21 @@ __device__ __forceinline__ bool find_unit(const PagedArgs &a, Units &&units, int
 // 64 entries of a block table row in a register; at(p) takes rising p.
 struct PageIds {
     int first, ids;
+
+    // Whether the entries first .. last all are pages of the pool.
+    __device__ __forceinline__ static bool all_pages(const PagedArgs &a, const int32_t *tab, int first, int last) {
+        bool bad = false;
+        for (int i = first; i <= last; i += 64) bad |= (uint32_t)tab[min(i + kq_lane(), last)] >= (uint32_t)a.n_pages;
+        return __builtin_amdgcn_ballot_w64(bad) == 0;
+    }
+
+    // Whether those of pieces c0 .. c1 of 16 keys (1 << sh a page) through a window
+    // are; loads the first 64.
+    __device__ __forceinline__ bool start(const PagedArgs &a, const int32_t *tab, const Window &win, int c0, int c1, int sh) {
+        load(tab, win.piece(c0) >> sh, win.piece(c1) >> sh);
+        return (c0 >= win.head || all_pages(a, tab, c0 >> sh, min(c1, win.head - 1) >> sh)) &&
+               (c1 < win.head || all_pages(a, tab, win.piece(max(c0, win.head)) >> sh, win.piece(c1) >> sh));
+    }
 
     // Whether entries p .. last all are pages of the pool; loads the first 64.
     __device__ __forceinline__ bool start(const PagedArgs &a, const int32_t *tab, int p, int last) {
@@ -603,7 +660,7 @@ struct State {
 // Rows of few columns: one wave a unit = (row, split, kv head), the kv heads
 // fastest.  The wave takes the units `first`, `first` + `step`, ..., or with
 // DIRECT the one of its place in the grid.
-template <int D, bool BF, bool Q8, bool DIRECT>
+template <int D, bool BF, bool Q8, bool DIRECT, bool WIN>
 __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int step) {
     using Tile = std::conditional_t<Q8, Tile8<D, BF>, Tile16<D, BF>>;
     constexpr int TT = Geo<D>::TT, CH = Geo<D>::CH, NC = Geo<D>::NC;
@@ -619,11 +676,11 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
             blk = a.few_blocks > 1 ? unit / 8 % 2 : 0;
             h = blockIdx.y;
             b = blockIdx.z;
-            row = lane_row(row_at(a, b), 0);
+            row = lane_row(row_at<WIN>(a, b), 0);
             if (!few_columns(row.n, a.G, a.few_limit) || blk >= row.blocks || s >= row.splits) return;
         } else {
             int u = unit;
-            if (!find_unit(a, [&](const Row &x) { return wave_units(a, x); }, u, b, row, slot0)) return;
+            if (!find_unit<WIN>(a, [&](const Row &x) { return wave_units(a, x); }, u, b, row, slot0)) return;
             if (!has_slots(a, row, slot0)) continue;
             const int head = u / row.blocks;
             blk = u - head * row.blocks;
@@ -639,10 +696,22 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
         st.init();
         // keys seen: the column's, the block's least and most
         const int first = row.before + 1;
-        const int seen = live ? max(first + i, 0) : 0x7fffffff;
-        const int least = max(first + 16 * blk / a.G, 0);
-        const int most = min(max(first + min((16 * blk + 15) / a.G, row.n - 1), 0), row.kv);
-        const int per = a.rule.tokens(row.kv);
+        int seen = live ? max(first + i, 0) : 0x7fffffff;
+        int least = max(first + 16 * blk / a.G, 0);
+        int most = min(max(first + min((16 * blk + 15) / a.G, row.n - 1), 0), row.kv);
+        // with a window, by the block's numbers: the column's first key behind the
+        // sinks, and the block's last such (a dead column may see any)
+        const Window win(a, WIN ? least : 0);
+        int low = 0, low_all = 0;
+        if constexpr (WIN) {
+            low = live ? win.low(a, seen) : 0;
+            low_all = __builtin_amdgcn_readfirstlane(win.low(a, max(first + min((16 * blk + 15) / a.G, row.n - 1), 0)));
+            seen = live ? win.keys(min(seen, row.kv)) : seen;
+            least = win.keys(min(least, row.kv));
+            most = win.keys(most);
+        }
+        const auto in_window = [&](int t) { return !WIN || t < a.sinks || t >= low; };
+        const int per = a.rule.tokens(row.span);
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
         const int t_end = __builtin_amdgcn_readfirstlane(min(most, t_begin + per));
         const uint16_t *qp = a.q + (int64_t)(row.q0 + i) * a.q_stride + (int64_t)hq * D;
@@ -671,9 +740,11 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
             // the row's block table, 64 entries at a time in a register
             const int32_t *tab = a.table + (int64_t)b * a.table_stride;
             const int sh = a.lps - 4;  // log2 of a page's chunks
-            const int c_last = (t_end - 1) >> 4, p_last = c_last >> sh;
+            const int c_last = (t_end - 1) >> 4, p_last = (WIN ? win.piece(c_last) : c_last) >> sh;
             PageIds ids;
-            const bool all_ok = ids.start(a, tab, (t_begin >> 4) >> sh, p_last);
+            bool all_ok;
+            if constexpr (WIN) all_ok = ids.start(a, tab, win, t_begin >> 4, c_last, sh);
+            else all_ok = ids.start(a, tab, (t_begin >> 4) >> sh, p_last);
             const int64_t h_off = (int64_t)h * a.head_stride;
             auto at_tile = [&](int t0) {
                 TileAt<D> x;
@@ -681,7 +752,7 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
 #pragma unroll
                 for (int ch = 0; ch < CH; ++ch) {
                     // (chunks past the end repeat the last: their keys are hidden)
-                    const int c = min((t0 >> 4) + ch, c_last), p = c >> sh;
+                    const int cb = min((t0 >> 4) + ch, c_last), c = WIN ? win.piece(cb) : cb, p = c >> sh;
                     const int id = ids.at(tab, p, p_last);
                     const bool in = (uint32_t)id < (uint32_t)a.n_pages;
                     x.ok |= in ? 1u << ch : 0u;
@@ -695,36 +766,53 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
             // by one before them, so that their code is there once.
             int whole = min(least, t_end);
             whole = whole <= t_begin || !all_ok ? t_begin : whole - (whole - t_begin) % TT;
+            // With a window only those below `sunk` (sinks) and from `from` on are whole.
+            int sunk = t_begin, from = t_begin;
+            if constexpr (WIN) {
+                const int head = min(a.sinks, whole), all = min(low_all, whole);
+                sunk += max(head - t_begin, 0) / TT * TT;
+                from = max(sunk, t_begin + (max(all - t_begin, 0) + TT - 1) / TT * TT);
+            }
+            const int n_sunk = (sunk - t_begin) / TT;
+            // (tile k of the whole ones)
+            const auto whole_at = [&](int k) { return !WIN || k < n_sunk ? t_begin + TT * k : from + TT * (k - n_sunk); };
+            const int n_whole = WIN ? n_sunk + (whole - from) / TT : (whole - t_begin) / TT;
             Tile ring[NBUF];
 #pragma unroll 1
-            for (int t = whole; t < t_end; t += TT) {
+            for (int t = WIN && sunk < from ? sunk : whole; t < t_end; t += TT) {
+                if constexpr (WIN) {
+                    if (t == from && t < whole) t = whole;
+                    if (t >= t_end) break;
+                }
                 const TileAt<D> at = at_tile(t);
                 ring[0].load(a, at);
                 const int lim = min(seen, t_end);
                 uint32_t vis = 0, odd = 0;
 #pragma unroll
                 for (int x = 0; x < 4 * CH; ++x)
-                    if (((at.ok >> (x >> 2)) & 1) && t + 16 * (x >> 2) + 4 * g + (x & 3) < lim) vis |= 1u << x;
+                    if (((at.ok >> (x >> 2)) & 1) && t + 16 * (x >> 2) + 4 * g + (x & 3) < lim &&
+                        in_window(t + 16 * (x >> 2) + 4 * g + (x & 3)))
+                        vis |= 1u << x;
                 st.template tile<true>(ring[0], a.scale_log2, vis, odd);
                 if constexpr (!Q8) {
                     if (__builtin_amdgcn_ballot_w64(odd != 0)) {
 #pragma unroll 1
                         for (int k = 0; k < TT; ++k)
                             st.add_odd((const uint16_t *)a.v + (k < 16 ? at.off[0] : at.off[1]) + (k & 15) * a.tok_stride,
-                                       ((at.ok >> (k >> 4)) & 1) && t + k < lim);
+                                       ((at.ok >> (k >> 4)) & 1) && t + k < lim && in_window(t + k));
                     }
                 }
             }
-            if (whole > t_begin) {
+            if (n_whole > 0) {
                 uint32_t odd;
 #pragma unroll
-                for (int j = 0; j < NBUF - 1; ++j) ring[j].load(a, at_tile(t_begin + TT * j));
-                for (int t0 = t_begin; t0 < whole; t0 += TT * NBUF) {
+                for (int j = 0; j < NBUF - 1; ++j) ring[j].load(a, at_tile(whole_at(j)));
+                for (int k = 0; k < n_whole; k += NBUF) {
 #pragma unroll
                     for (int j = 0; j < NBUF; ++j) {
-                        ring[(j + NBUF - 1) % NBUF].load(a, at_tile(t0 + TT * (j + NBUF - 1)));
+                        ring[(j + NBUF - 1) % NBUF].load(a, at_tile(whole_at(k + j + NBUF - 1)));
                         __builtin_amdgcn_sched_barrier(0);
-                        if (t0 + TT * j < whole) st.template tile<false>(ring[j], a.scale_log2, 0, odd);
+                        if (k + j < n_whole) st.template tile<false>(ring[j], a.scale_log2, 0, odd);
                     }
                 }
             }
@@ -777,10 +865,10 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
     }
 }
 
-template <int D, bool BF, bool Q8, bool DIRECT>
+template <int D, bool BF, bool Q8, bool DIRECT, bool WIN>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void kq_paged_wave_kernel(
     PagedArgs a) {
-    wave_work<D, BF, Q8, DIRECT>(a, blockIdx.x, gridDim.x);
+    wave_work<D, BF, Q8, DIRECT, WIN>(a, blockIdx.x, gridDim.x);
 }
 
 // ---- prompt chunks --------------------------------------------------------
@@ -933,8 +1021,11 @@ struct ChunkState {
     }
 
     // masked: some key of the tile is hidden from a column (lim: the column's
-    // first unseen key; okbits: the 16-token pieces that lie in the pool).
-    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, bool masked, int t0, int lim, uint32_t okbits) {
+    // first unseen key; with a window, it sees below `sinks` and from `low` on; okbits:
+    // the 16-token pieces that lie in the pool).
+    template <bool WIN>
+    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, bool masked, int t0, int lim, int sinks, int low,
+                                         uint32_t okbits) {
         const int lane = kq_lane(), c = lane & 31, h = lane >> 5;
         floatx16 s[C::NT];
         // rows t and t + 32 have the same order of pieces
@@ -957,7 +1048,7 @@ struct ChunkState {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int t = 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                    s[b][i] = t0 + t < lim && ((okbits >> (2 * b + (i >> 3))) & 1) ? s[b][i] : -INFINITY;
+                    s[b][i] = t0 + t < lim && (!WIN || t0 + t < sinks || t0 + t >= low) && ((okbits >> (2 * b + (i >> 3))) & 1) ? s[b][i] : -INFINITY;
                 }
         }
         float tmax = s[0][0];
@@ -1038,7 +1129,9 @@ struct ChunkState16 {
     __device__ __forceinline__ floatx4 run(int k) const { return o[k]; }
     __device__ __forceinline__ void add(int k, const floatx4 &y) { o[k] = o[k] + y; }
 
-    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, bool masked, int t0, int lim, uint32_t okbits) {
+    template <bool WIN>
+    __device__ __forceinline__ void tile(uint32_t stage, float scale_log2, bool masked, int t0, int lim, int sinks, int low,
+                                         uint32_t okbits) {
         const int lane = kq_lane(), c = lane & 15, g = lane >> 4;
         floatx4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         const uint32_t ka = stage + (uint32_t)(c * C::kRow) + 16u * (uint32_t)(C::kswz(c) ^ g);
@@ -1053,8 +1146,10 @@ struct ChunkState16 {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[b][i] = t0 + 16 * b + 4 * g + i < lim && ((okbits >> b) & 1) ? s[b][i] : -INFINITY;
+                for (int i = 0; i < 4; ++i) {
+                    const int t = t0 + 16 * b + 4 * g + i;
+                    s[b][i] = t < lim && (!WIN || t < sinks || t >= low) && ((okbits >> b) & 1) ? s[b][i] : -INFINITY;
+                }
         }
         float tmax = max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
         tmax = max_over_groups(max3(max3(tmax, s[1][1], s[1][2]), s[1][3], s[1][3])) * scale_log2;
@@ -1098,7 +1193,7 @@ __device__ __forceinline__ uint32_t first_halves(float a, float b) {
     else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
 
-template <int D, bool BF, bool Q8>
+template <int D, bool BF, bool Q8, bool WIN>
 __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, int first, int step) {
     using C = Chunk<D, Q8>;
     using State = std::conditional_t<(D > 128), ChunkState16<D, BF, Q8>, ChunkState<D, BF, Q8>>;
@@ -1111,7 +1206,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
     for (int unit = first;; unit += step) {
         int u = unit, b, slot0;
         Row row;
-        if (!find_unit(a, [&](const Row &x) { return chunk_units<D>(a, x); }, u, b, row, slot0)) return;
+        if (!find_unit<WIN>(a, [&](const Row &x) { return chunk_units<D>(a, x); }, u, b, row, slot0)) return;
         if (!has_slots(a, row, slot0)) continue;
         const int rest = u / a.Hkv, kvh = u - rest * a.Hkv;
         // the tiles with the most keys first
@@ -1123,13 +1218,27 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
         const bool live = col < cols;
         const int i = live ? col / a.G : row.n - 1, hq = kvh * a.G + (live ? col - i * a.G : 0);
         const auto seen_by = [&](int cl) { return max(row.before + 1 + min(cl, cols - 1) / a.G, 0); };
-        const int seen = live ? min(seen_by(col), row.kv) : 0x7fffffff;
-        const int least = __builtin_amdgcn_readfirstlane(seen_by(col0));
-        const int most = __builtin_amdgcn_readfirstlane(col0 < cols ? min(seen_by(col0 + COLS - 1), row.kv) : 0);
-        const int least_all = __builtin_amdgcn_readfirstlane(seen_by(blk * C::NW * COLS));
-        const int most_all = __builtin_amdgcn_readfirstlane(min(seen_by((blk + 1) * C::NW * COLS - 1), row.kv));
-        const int per = few_columns(row.n, a.G, a.few_limit) ? a.rule.tokens(row.kv)
-                                                : ((row.kv + row.splits - 1) / row.splits + C::BN - 1) / C::BN * C::BN;
+        const Window win(a, WIN ? seen_by(blk * C::NW * COLS) : 0);
+        // keys by number: the row's, or with a window the block's
+        const auto keys = [&](int x) { return WIN ? win.keys(min(x, row.kv)) : x; };
+        const int seen = live ? keys(min(seen_by(col), row.kv)) : 0x7fffffff;
+        const int least = __builtin_amdgcn_readfirstlane(keys(seen_by(col0)));
+        const int most = __builtin_amdgcn_readfirstlane(col0 < cols ? keys(min(seen_by(col0 + COLS - 1), row.kv)) : 0);
+        const int least_all = __builtin_amdgcn_readfirstlane(keys(seen_by(blk * C::NW * COLS)));
+        const int most_all = __builtin_amdgcn_readfirstlane(keys(min(seen_by((blk + 1) * C::NW * COLS - 1), row.kv)));
+        // the first key behind the sinks that is in the window of this lane's column, of
+        // the wave's first and last, and of the workgroup's last
+        int low = 0, low_first = 0, low_last = 0, low_all = 0;
+        if constexpr (WIN) {
+            low = live ? win.low(a, seen_by(col)) : 0;
+            low_first = __builtin_amdgcn_readfirstlane(win.low(a, seen_by(col0)));
+            low_last = __builtin_amdgcn_readfirstlane(win.low(a, seen_by(col0 + COLS - 1)));
+            low_all = __builtin_amdgcn_readfirstlane(win.low(a, seen_by((blk + 1) * C::NW * COLS - 1)));
+        }
+        // whether a tile lies between the sinks and a window's first key in part or whole
+        const auto left_out = [&](int t0, int first) { return WIN && t0 < first && t0 + C::BN > a.sinks; };
+        const int per = few_columns(row.n, a.G, a.few_limit) ? a.rule.tokens(row.span)
+                                                : ((row.span + row.splits - 1) / row.splits + C::BN - 1) / C::BN * C::BN;
         const int t_begin = __builtin_amdgcn_readfirstlane(s * per);
         const int t_end = __builtin_amdgcn_readfirstlane(min(most_all, t_begin + per));
 
@@ -1150,9 +1259,11 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
         if (t_end > t_begin) {
             const int32_t *tab = a.table + (int64_t)b * a.table_stride;
             const int sh = a.lps - 4;
-            const int c_last = (t_end - 1) >> 4, p_last = c_last >> sh;
+            const int c_last = (t_end - 1) >> 4, p_last = (WIN ? win.piece(c_last) : c_last) >> sh;
             PageIds ids;
-            const bool all_ok = ids.start(a, tab, (t_begin >> 4) >> sh, p_last);
+            bool all_ok;
+            if constexpr (WIN) all_ok = ids.start(a, tab, win, t_begin >> 4, c_last, sh);
+            else all_ok = ids.start(a, tab, (t_begin >> 4) >> sh, p_last);
             const int64_t h_off = (int64_t)kvh * a.head_stride;
             // Piece y of the RT tokens at a time of the tile at t0 that this
             // wave copies, of K (even waves) or V (odd waves): where it starts
@@ -1162,7 +1273,7 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
             auto piece = [&](int t0, int y, uint32_t &dst) {
                 const int t = RT * (C::NW / 2 * y + (w >> 1));
                 // (16 tokens past the end are the last ones again: their keys are hidden)
-                const int ch = min((t0 + t) >> 4, c_last), p = ch >> sh;
+                const int cb = min((t0 + t) >> 4, c_last), ch = WIN ? win.piece(cb) : cb, p = ch >> sh;
                 const int id = ids.at(tab, p, p_last);
                 dst = (uint32_t)((w & 1) * C::kHalf + t * C::kRow);
                 return (int64_t)((uint32_t)id < (uint32_t)a.n_pages ? id : 0) * a.page_stride + h_off +
@@ -1234,7 +1345,9 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
                 uint32_t ok = (1u << (C::BN / 16)) - 1;
                 if (!all_ok)
                     for (int j = 0; j < C::BN / 16; ++j)
-                        if ((uint32_t)tab[min((t0 >> 4) + j, c_last) >> sh] >= (uint32_t)a.n_pages) ok &= ~(1u << j);
+                        if ((uint32_t)tab[(WIN ? win.piece(min((t0 >> 4) + j, c_last)) : min((t0 >> 4) + j, c_last)) >> sh] >=
+                            (uint32_t)a.n_pages)
+                            ok &= ~(1u << j);
                 return ok;
             };
             // In a tile with hidden keys, the product of a hidden key's value
@@ -1258,9 +1371,11 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
             auto add_odd = [&](int t0, int lim) {
 #pragma unroll 1
                 for (int t = t0; t < min(t0 + C::BN, t_end); ++t) {
-                    const int id = __builtin_amdgcn_readfirstlane(tab[t >> a.lps]);
+                    const int key = WIN ? 16 * win.piece(t >> 4) + (t & 15) : t;
+                    const int id = __builtin_amdgcn_readfirstlane(tab[key >> a.lps]);
                     if ((uint32_t)id >= (uint32_t)a.n_pages) continue;
-                    const int64_t off = (int64_t)id * a.page_stride + h_off + (int64_t)(t & ((1 << a.lps) - 1)) * a.tok_stride;
+                    const bool sees = t < lim && (!WIN || t < a.sinks || t >= low);
+                    const int64_t off = (int64_t)id * a.page_stride + h_off + (int64_t)(key & ((1 << a.lps) - 1)) * a.tok_stride;
 #pragma unroll
                     for (int k = 0; k < State::NR; ++k) {
                         const int64_t at = off + State::run_d(k);
@@ -1272,11 +1387,11 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
                                 // (fp16: infinite from where the halves are, 2^17.  A comparison
                                 // with that in its place spilled 24 to 548 bytes a lane.)
                                 const float v = fmaf((float)((const uint8_t *)a.v)[at + e], sc, bi) * (BF ? 1.f : 0x1p111f);
-                                y[e] = t < lim && v - v != 0.f ? v : 0.f;
+                                y[e] = sees && v - v != 0.f ? v : 0.f;
                             }
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) y[e] = t < lim ? odd_part<BF>(((const uint16_t *)a.v)[at + e]) : 0.f;
+                            for (int e = 0; e < 4; ++e) y[e] = sees ? odd_part<BF>(((const uint16_t *)a.v)[at + e]) : 0.f;
                         }
                         st.add(k, y);
                         __builtin_amdgcn_sched_barrier(0);  // (few loads at a time: registers)
@@ -1302,12 +1417,14 @@ __device__ __forceinline__ void chunk_work(const PagedArgs &a, uint8_t *smem, in
                     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                     if (more) copy(t0 + C::BN, other);
                 }
-                const bool hidden = !all_ok || t0 + C::BN > min(least_all, t_end);  // uniform over the workgroup
+                // uniform over the workgroup
+                const bool hidden = !all_ok || t0 + C::BN > min(least_all, t_end) || left_out(t0, low_all);
                 if (hidden) clean(stage, t0);
-                if (t0 < most) {
+                // (tiles that no column of the wave sees are passed over)
+                if (t0 < most && !(WIN && t0 + C::BN <= low_first && t0 >= a.sinks)) {
                     const int lim = min(seen, t_end);
-                    const bool masked = !all_ok || t0 + C::BN > min(least, t_end);
-                    st.tile(stage, scale, masked, t0, lim, masked ? pages_ok(t0) : 0u);
+                    const bool masked = !all_ok || t0 + C::BN > min(least, t_end) || left_out(t0, low_last);
+                    st.template tile<WIN>(stage, scale, masked, t0, lim, a.sinks, low, masked ? pages_ok(t0) : 0u);
                     if (hidden && *odd_flag == t0 + 1) add_odd(t0, lim);
                 }
                 if constexpr (Q8) {
@@ -1350,18 +1467,18 @@ constexpr bool kBeside = D <= 128;
 // The first `wave_groups` workgroups take rows of few columns, a wave a unit, the
 // others chunks: decode rows, which wait for memory, run beside a prompt
 // chunk's products.  (Eight of each kind in turn instead: 68 -> 81 us.)
-template <int D, bool BF, bool Q8>
+template <int D, bool BF, bool Q8, bool WIN>
 __global__ __launch_bounds__(64 * chunk_waves(D, Q8), D > 256 ? 1 : 2) void kq_paged_kernel(PagedArgs a, int wave_groups) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     if constexpr (kBeside<D>) {
         if ((int)blockIdx.x < wave_groups) {
             constexpr int NW = chunk_waves(D, Q8);
             const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-            wave_work<D, BF, Q8, false>(a, NW * (int)blockIdx.x + w, NW * wave_groups);
+            wave_work<D, BF, Q8, false, WIN>(a, NW * (int)blockIdx.x + w, NW * wave_groups);
             return;
         }
     }
-    chunk_work<D, BF, Q8>(a, smem, (int)blockIdx.x - wave_groups, (int)gridDim.x - wave_groups);
+    chunk_work<D, BF, Q8, WIN>(a, smem, (int)blockIdx.x - wave_groups, (int)gridDim.x - wave_groups);
 }
 
 // Scale of a split of maximum ms beside the common maximum m; a split without
@@ -1506,7 +1623,7 @@ struct WaveMerge {
 
 // Workgroups take a token and query head each (direct), or merge_items of a
 // row's at a time.
-template <int D, bool BF, bool DIRECT>
+template <int D, bool BF, bool DIRECT, bool WIN>
 __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
     const auto out = [&](const Row &r, int x) {
         const int i = x / a.Hq;
@@ -1517,7 +1634,7 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
         return slot_of(a, r, slot0, i, x - i * a.Hq);
     };
     if constexpr (DIRECT) {
-        const Row row = lane_row(row_at(a, blockIdx.y), 0);
+        const Row row = lane_row(row_at<WIN>(a, blockIdx.y), 0);
         const int x = blockIdx.x;
         if (row.splits <= 1 || x >= row.n * a.Hq) return;
         if (row.splits > 64) merge_group<D, BF, kSlices>(a, slot(row, 0, x), row.splits, blockIdx.z, out(row, x));
@@ -1528,7 +1645,7 @@ __global__ __launch_bounds__(256) void kq_paged_merge_kernel(PagedArgs a) {
     for (int item = blockIdx.x;; item += gridDim.x) {
         int u = item, b, slot0;
         Row row;
-        if (!find_unit(a, [&](const Row &x) { return merge_units(a, x); }, u, b, row, slot0)) return;
+        if (!find_unit<WIN>(a, [&](const Row &x) { return merge_units(a, x); }, u, b, row, slot0)) return;
         if (!has_slots(a, row, slot0)) continue;
         const int n = row.splits, items = merge_items(n), end = min((u + 1) * items, row.n * a.Hq);
         if (n <= 64) {
@@ -1554,31 +1671,31 @@ struct Grid {
     int beside;          // waves of rows of few columns beside them
 };
 
-template <int D, bool BF, bool Q8>
-int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
+template <int D, bool BF, bool Q8, bool WIN>
+int launch_form(const PagedArgs &a, const Grid &g, hipStream_t s) {
     if (g.groups) {
         constexpr int lds = Chunk<D, Q8>::kLds + 16;  // (and a flag)
         static_assert(lds <= 160 << 10, "LDS of a CU");
         static OncePerDevice raised;
         int device = -1;
         if (hipGetDevice(&device) != hipSuccess || !raised(device, [] {
-                return hipFuncSetAttribute((const void *)kq_paged_kernel<D, BF, Q8>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                return hipFuncSetAttribute((const void *)kq_paged_kernel<D, BF, Q8, WIN>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                            lds) == hipSuccess;
             }))
             return KQ_ERR_LAUNCH_FAILED;
         constexpr int NW = chunk_waves(D, Q8);
         const int beside = kBeside<D> ? (g.beside + NW - 1) / NW : 0;
-        hipLaunchKernelGGL((kq_paged_kernel<D, BF, Q8>), dim3(beside + g.groups), dim3(64 * NW), lds, s, a, beside);
+        hipLaunchKernelGGL((kq_paged_kernel<D, BF, Q8, WIN>), dim3(beside + g.groups), dim3(64 * NW), lds, s, a, beside);
     }
     if constexpr (has_waves(D)) {
         if (g.waves.x && !(kBeside<D> && g.groups)) {
-            if (a.direct) hipLaunchKernelGGL((kq_paged_wave_kernel<D, BF, Q8, true>), g.waves, dim3(64), 0, s, a);
-            else hipLaunchKernelGGL((kq_paged_wave_kernel<D, BF, Q8, false>), g.waves, dim3(64), 0, s, a);
+            if (a.direct) hipLaunchKernelGGL((kq_paged_wave_kernel<D, BF, Q8, true, WIN>), g.waves, dim3(64), 0, s, a);
+            else hipLaunchKernelGGL((kq_paged_wave_kernel<D, BF, Q8, false, WIN>), g.waves, dim3(64), 0, s, a);
         }
     }
     if (g.merge.x) {
-        if (a.direct) hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF, true>), g.merge, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF, false>), g.merge, dim3(256), 0, s, a);
+        if (a.direct) hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF, true, WIN>), g.merge, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((kq_paged_merge_kernel<D, BF, false, WIN>), g.merge, dim3(256), 0, s, a);
     }
     return hipGetLastError() == hipSuccess ? KQ_OK : KQ_ERR_LAUNCH_FAILED;
 }
@@ -1586,8 +1703,8 @@ int launch_q8(const PagedArgs &a, const Grid &g, hipStream_t s) {
 template <int D, bool BF>
 int launch(const PagedArgs &a, bool q8, const Grid &g, hipStream_t s) {
     if constexpr (D % 64 == 0)
-        if (q8) return launch_q8<D, BF, true>(a, g, s);
-    return launch_q8<D, BF, false>(a, g, s);
+        if (q8) return a.window ? launch_form<D, BF, true, true>(a, g, s) : launch_form<D, BF, true, false>(a, g, s);
+    return a.window ? launch_form<D, BF, false, true>(a, g, s) : launch_form<D, BF, false, false>(a, g, s);
 }
 
 // Tokens per split of a row of few columns, by its own keys: the lengths of
@@ -1671,23 +1788,30 @@ bool numbers_fit(const Plan &p, int64_t T, int64_t B, int Hq, int Hkv, int D, bo
     return has_waves(D) ? few < kMost && many < kMost : few + many < kMost;
 }
 
-}  // namespace
+// (31-bit numbers of keys)
+bool window_fits(int32_t window, int32_t sinks) {
+    return window >= 1 && window <= (1 << 30) && sinks >= 0 && sinks <= (1 << 30);
+}
 
-extern "C" {
+// The most keys that a row's splits divide (window 0: none).
+int most_span(int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q, int32_t max_kv, bool q8, int32_t window, int32_t sinks) {
+    return window ? window_span(max_kv, window, sinks, max_q, Hq / Hkv, group_columns(D, q8)) : max_kv;
+}
 
-size_t kq_sdpa_paged_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
-                                     int32_t max_kv, int q8) {
+size_t workspace_bytes_of(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q, int32_t max_kv, int q8,
+                          int32_t window, int32_t sinks) {
     if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hkv > 1024 || D <= 0 || max_q <= 0 || max_kv <= 0 ||
         !sizes_fit(T, B, Hq, max_kv))
         return 0;
-    const Plan p = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, q8 != 0);
+    const int span = most_span(Hq, Hkv, D, max_q, max_kv, q8 != 0, window, sinks);
+    const Plan p = paged_plan(T, B, Hq, Hkv, D, max_q, span, q8 != 0);
     return p.slots && numbers_fit(p, T, B, Hq, Hkv, D, q8 != 0) ? part_bytes(p.slots, D) + (size_t)p.slots * 8 : 0;
 }
 
-int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int32_t *block_table,
-                  int64_t table_stride, int32_t table_width, const int32_t *kv_lens, const int32_t *cu_q, int32_t T,
-                  int32_t B, int32_t Hq, int32_t max_q, int32_t max_kv, float scale, void *out, int64_t out_stride,
-                  void *workspace, size_t workspace_bytes, kq_stream_t stream) {
+int attend(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int32_t *block_table, int64_t table_stride,
+           int32_t table_width, const int32_t *kv_lens, const int32_t *cu_q, int32_t T, int32_t B, int32_t Hq, int32_t max_q,
+           int32_t max_kv, int32_t window, int32_t sinks, float scale, void *out, int64_t out_stride, void *workspace,
+           size_t workspace_bytes, kq_stream_t stream) {
     if (const int rc = kq_pool_check(pool)) return rc;
     if (T == 0 || B == 0) return KQ_OK;
     if (!q || !block_table || !kv_lens || !cu_q || !out) return KQ_ERR_NULL_POINTER;
@@ -1699,7 +1823,8 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     if (!(fabsf(scale * 1.4426950408889634f) <= 3.4028235e38f)) return KQ_ERR_BAD_ARGUMENT;
     if (!sizes_fit(T, B, Hq, max_kv) || q_stride < (int64_t)Hq * D || out_stride < (int64_t)Hq * D) return KQ_ERR_BAD_SHAPE;
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_stride | out_stride) & 7)) return KQ_ERR_BAD_ALIGN;
-    const Plan plan = paged_plan(T, B, Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr);
+    const int span = most_span(Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr, window, sinks);
+    const Plan plan = paged_plan(T, B, Hq, Hkv, D, max_q, span, pool->k_scales != nullptr);
     const int64_t most = plan.few > plan.many ? plan.few : plan.many;
     if (!numbers_fit(plan, T, B, Hq, Hkv, D, pool->k_scales != nullptr)) return KQ_ERR_BAD_SHAPE;
     const size_t need = plan.slots ? part_bytes(plan.slots, D) + (size_t)plan.slots * 8 : 0;
@@ -1737,6 +1862,8 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     a.few_cols = has_waves(D) ? 16 : a.group_cols;
     a.max_q = max_q;
     a.max_kv = max_kv;
+    a.window = window;
+    a.sinks = sinks;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.part = (float *)workspace;
     a.ml = (float *)((char *)workspace + part_bytes(plan.slots, D));
@@ -1775,6 +1902,38 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
     case 256: return bf ? launch<256, true>(a, q8, g, s) : launch<256, false>(a, q8, g, s);
     default: return bf ? launch<512, true>(a, q8, g, s) : launch<512, false>(a, q8, g, s);
     }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t kq_sdpa_paged_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
+                                     int32_t max_kv, int q8) {
+    return workspace_bytes_of(T, B, Hq, Hkv, D, max_q, max_kv, q8, 0, 0);
+}
+
+int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int32_t *block_table,
+                  int64_t table_stride, int32_t table_width, const int32_t *kv_lens, const int32_t *cu_q, int32_t T,
+                  int32_t B, int32_t Hq, int32_t max_q, int32_t max_kv, float scale, void *out, int64_t out_stride,
+                  void *workspace, size_t workspace_bytes, kq_stream_t stream) {
+    return attend(q, q_stride, pool, block_table, table_stride, table_width, kv_lens, cu_q, T, B, Hq, max_q, max_kv, 0, 0,
+                  scale, out, out_stride, workspace, workspace_bytes, stream);
+}
+
+size_t kq_sdpa_paged_window_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
+                                            int32_t max_kv, int q8, int32_t window, int32_t sinks) {
+    if (!window_fits(window, sinks)) return 0;
+    return workspace_bytes_of(T, B, Hq, Hkv, D, max_q, max_kv, q8, window, sinks);
+}
+
+int kq_sdpa_paged_window(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int32_t *block_table,
+                         int64_t table_stride, int32_t table_width, const int32_t *kv_lens, const int32_t *cu_q, int32_t T,
+                         int32_t B, int32_t Hq, int32_t max_q, int32_t max_kv, int32_t window, int32_t sinks, float scale,
+                         void *out, int64_t out_stride, void *workspace, size_t workspace_bytes, kq_stream_t stream) {
+    if (!window_fits(window, sinks)) return KQ_ERR_BAD_SHAPE;
+    return attend(q, q_stride, pool, block_table, table_stride, table_width, kv_lens, cu_q, T, B, Hq, max_q, max_kv, window,
+                  sinks, scale, out, out_stride, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -1425,7 +1425,7 @@ def paged_read(k_cache, v_cache, slots, k_scales=None, k_biases=None, v_scales=N
 
 
 def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=None, max_kv=None, k_scales=None,
-               k_biases=None, v_scales=None, v_biases=None, out=None):
+               k_biases=None, v_scales=None, v_biases=None, out=None, window=None, sinks=0):
     """Attention of each row's new tokens over its pages of a paged cache: decode
     rows, verify blocks and prompt chunks in one call, causal at the end.
 
@@ -1445,7 +1445,12 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     those of them up to kv_lens[b] - n + i).  Entries of the table that are no
     page of the pool are not attended.  D in 64, 96, 128, 256, 512 (no 96 in 8
     bits), Hq / Hkv up to 64, scale any finite number up to 2.3e38.  A row's
-    result is bitwise that of a call on the row alone."""
+    result is bitwise that of a call on the row alone.
+
+    window (1 to 2^30; None: none): of the keys up to its own, a token sees the last
+    `window` and the row's first `sinks` (0 to 2^30).  Only their pages are read, and
+    time goes by them: table entries between the sinks and the window of the row's
+    first new token may be anything."""
     _fault("sdpa_paged")
     lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
     dev, dt, Hkv, D, B, shape = lay.device, lay.dtype, lay.Hkv, lay.D, kv_lens.numel(), q.shape
@@ -1482,7 +1487,15 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
         mkv = min(mkv, int(max_kv))
     if mq < 1 or mkv < 1:
         raise ValueError("sdpa_paged: max_q and max_kv must be positive")
-    need = lib().kq_sdpa_paged_workspace_bytes(T, B, Hq, Hkv, D, mq, mkv, lay.q8)
+    if window is None:
+        if sinks:
+            raise ValueError("sdpa_paged: sinks go with a window")
+        need = lib().kq_sdpa_paged_workspace_bytes(T, B, Hq, Hkv, D, mq, mkv, lay.q8)
+    else:
+        window, sinks = int(window), int(sinks)
+        if not 1 <= window <= 1 << 30 or not 0 <= sinks <= 1 << 30:
+            raise ValueError(f"sdpa_paged: a window of 1 to 2^30 keys and 0 to 2^30 sinks, got {window} and {sinks}")
+        need = lib().kq_sdpa_paged_window_workspace_bytes(T, B, Hq, Hkv, D, mq, mkv, lay.q8, window, sinks)
     s = _stream(q)
     ws_ptr, ws_len = None, 0
     if need:
@@ -1492,8 +1505,12 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
         # replayed on two at once)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         ws_ptr, ws_len = ws.data_ptr(), need
-    _paged_call("kq_sdpa_paged", dev, q.data_ptr(), qt, pool, tab, tab_stride, width, lens, cu, T, B, Hq, mq, mkv,
-                float(scale), out.data_ptr(), ot, ws_ptr, ws_len, s)
+    if window is None:
+        _paged_call("kq_sdpa_paged", dev, q.data_ptr(), qt, pool, tab, tab_stride, width, lens, cu, T, B, Hq, mq, mkv,
+                    float(scale), out.data_ptr(), ot, ws_ptr, ws_len, s)
+    else:
+        _paged_call("kq_sdpa_paged_window", dev, q.data_ptr(), qt, pool, tab, tab_stride, width, lens, cu, T, B, Hq, mq,
+                    mkv, window, sinks, float(scale), out.data_ptr(), ot, ws_ptr, ws_len, s)
     return out
 
 

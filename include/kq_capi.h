@@ -571,6 +571,20 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
                   int32_t T, int32_t B, int32_t Hq, int32_t max_q, int32_t max_kv, float scale, void *out,
                   int64_t out_stride, void *workspace, size_t workspace_bytes, kq_stream_t stream);
 
+/* kq_sdpa_paged through a window: a token that sees keys 0 .. p there sees of them
+ * those past p - window, the last `window`, and the row's first `sinks` (window 1 ..
+ * 2^30, sinks 0 .. 2^30; window 1: itself and the sinks).  Only these keys' pages are
+ * read: table entries between the sinks and the first new token's window may be
+ * anything (their pages given back).  Splits follow the window's length, not the
+ * row's; with a window that no row passes, what kq_sdpa_paged gives to its rounding.
+ * Everything else as kq_sdpa_paged has it, the workspace's size apart. */
+size_t kq_sdpa_paged_window_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
+                                            int32_t max_kv, int q8, int32_t window, int32_t sinks);
+int kq_sdpa_paged_window(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int32_t *block_table,
+                         int64_t table_stride, int32_t table_width, const int32_t *kv_lens, const int32_t *cu_q, int32_t T,
+                         int32_t B, int32_t Hq, int32_t max_q, int32_t max_kv, int32_t window, int32_t sinks, float scale,
+                         void *out, int64_t out_stride, void *workspace, size_t workspace_bytes, kq_stream_t stream);
+
 /* ---- positions and head norms ----------------------------------------------- */
 /* The rotation of queries and keys by their positions, and the norm of each head
  * before it.  Of a head's row x of D values, with a weight w [D] (NULL: no norm),

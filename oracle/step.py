@@ -82,3 +82,30 @@ def verify(logits, tokens, cu, uniforms, draws, probs=None, temperature=1.0, kv_
         if kv_lens is not None:
             keep.append(max(int(kv_lens[b]) - (max(hi - lo, 1) - 1 - a), 0))
     return acc, out, keep if kv_lens is not None else None
+
+
+def window_attention(q, k, v, n, scale, window, sinks, err=None, kv=None):
+    """The last n of a row's kv keys (default: all of k) are its new tokens; token i
+    sees the last `window` keys up to its own and the first `sinks`, of those that k
+    holds: q (n, Hq, D), k / v (Hkv, keys, D) -> out (n, Hq, D) and the weighted
+    mean of `err` (Hkv, keys, D; default |v|)."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    err = np.abs(v) if err is None else np.asarray(err, np.float64)
+    Hq, D = q.shape[1:]
+    Hkv, have = k.shape[:2]
+    kv = have if kv is None else kv
+    out, far = np.zeros((len(q), Hq, D)), np.zeros((len(q), Hq, D))
+    t = np.arange(have)
+    for i in range(len(q)):
+        me = kv - n + i
+        see = (t <= me) & ((t > me - window) | (t < sinks))
+        if not see.any():
+            continue
+        for h in range(Hkv):
+            g = slice(h * (Hq // Hkv), (h + 1) * (Hq // Hkv))
+            s = q[i, g] @ k[h, see].T * scale
+            p = np.exp(s - s.max(-1, keepdims=True))
+            p /= p.sum(-1, keepdims=True)
+            out[i, g] = p @ v[h, see]
+            far[i, g] = p @ err[h, see]
+    return out, far

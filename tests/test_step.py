@@ -159,3 +159,35 @@ def test_verify_reference():
     assert ref.verify_row(x, [0, 2], [0, 0, 0], 0, None, 0.0) == (2, 0)
     assert ref.verify_row(x, [1, 2], [0, 0, 0], 0, None, 0.0) == (0, 0)
     assert ref.verify_row(x[:0], [], [], 0.5, None, 1.0) == (0, -1)
+
+
+def test_window_calls_are_refused_and_sized():
+    m, L = _lib()
+    pool = _pool(m)
+
+    def call(window=64, sinks=4, **kw):
+        d = dict(T=4, B=2, Hq=32, mq=4, mkv=64, q=X, ws=None, n=0)
+        d.update(kw)
+        return L.kq_sdpa_paged_window(d["q"], 4096, pool, X, 4, 4, X, X, d["T"], d["B"], d["Hq"], d["mq"], d["mkv"], window,
+                                      sinks, 0.1, X, 4096, d["ws"], d["n"], None)
+    for bad in (dict(window=0), dict(window=-1), dict(window=(1 << 30) + 1), dict(sinks=-1), dict(sinks=(1 << 30) + 1),
+                dict(Hq=12), dict(mq=0), dict(T=-1)):
+        assert call(**bad) == m.KQ_ERR_BAD_SHAPE, bad
+    assert call(q=None) == m.KQ_ERR_NULL_POINTER and call(T=0) == m.KQ_OK
+    size = lambda mkv, w, s, mq=4: L.kq_sdpa_paged_window_workspace_bytes(4, 2, 32, 8, 128, mq, mkv, 0, w, s)  # noqa: E731
+    whole = L.kq_sdpa_paged_workspace_bytes(4, 2, 32, 8, 128, 4, 1 << 20, 0)
+    # by the window, not the rows: the same at any length, and never more than without
+    assert 0 < size(1 << 20, 4096, 4) == size(1 << 30, 4096, 4) < whole
+    assert size(1 << 20, 1 << 30, 0) == size(1 << 20, 64, 1 << 30) == whole
+    assert size(1 << 20, 0, 0) == size(1 << 20, 4, -1) == 0
+    assert call(window=4096, mkv=1 << 20) == m.KQ_ERR_WORKSPACE_TOO_SMALL
+
+
+def test_window_reference():
+    rng = np.random.default_rng(2)
+    q, k, v = rng.normal(size=(3, 2, 8)), rng.normal(size=(1, 20, 8)), rng.normal(size=(1, 20, 8))
+    out, _ = ref.window_attention(q, k, v, 3, 0.3, 4, 2)
+    # token 1 is key 18: it sees 0, 1, 15 .. 18
+    see = [0, 1, 15, 16, 17, 18]
+    p = np.exp(q[1, 1] @ k[0, see].T * 0.3)
+    assert np.allclose(out[1, 1], p @ v[0, see] / p.sum())
