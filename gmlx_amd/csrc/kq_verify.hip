@@ -34,28 +34,33 @@ struct VerifyArgs {
     int32_t probs_type;
     Part *part;    // [T][S]
     double *rest;  // [B][S]: sums of max(e - q Z, 0)
+    struct Verdict *verdict;  // [B], NULL: found by the last kernel
     int32_t *accepted, *next, *keep;
 };
 
-// 2^y for y <= 0 (NaN: 0) by the series of exp(f ln 2) on |f| <= 1/2: its next term
-// is below 2 10^-16.
-__device__ __forceinline__ double exp2_64(double y) {
-    y = fmax(y, -1100.0);
-    const double n = rint(y), f = (y - n) * 0.69314718055994530942;
-    double p = 1.0 / 479001600;
-    p = fma(p, f, 1.0 / 39916800);
-    p = fma(p, f, 1.0 / 3628800);
-    p = fma(p, f, 1.0 / 362880);
-    p = fma(p, f, 1.0 / 40320);
-    p = fma(p, f, 1.0 / 5040);
-    p = fma(p, f, 1.0 / 720);
-    p = fma(p, f, 1.0 / 120);
-    p = fma(p, f, 1.0 / 24);
-    p = fma(p, f, 1.0 / 6);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+// 2^y for y <= 0 as 2^(j / 64) from a table in LDS, times 2^r for |r| <= 1/128, times
+// a power of two added to the exponent: within 5 10^-15, exact at 0.  The table's
+// part saves nine of a lone polynomial's fifteen steps; 397 rows of 152064 values
+// kROWS us, with an exponential series to the 12th power 74.  Below 2^-1000 (and of
+// NaN) 2^-1000, which no sum beside a largest weight of 1 notices.
+constexpr int kTable = 64;
+
+__device__ __forceinline__ void fill_table(double *table) {
+    if (threadIdx.x < kTable) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / kTable));
+}
+
+__device__ __forceinline__ double exp2_64(double y, const double *table) {
+    constexpr double kRound = 0x1.8p52;  // its unit is 1: adding it rounds, the integer in the low bits
+    y = fmin(fmax(y, -1000.0), 0.0) * kTable;
+    const double t = y + kRound, r = y - (t - kRound);
+    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+    // least maximum of the error in sixty-fourths, the constant term 1
+    double p = fma(r, 0.009618138509201629 / 0x1p24, 0.05550419004645178 / 0x1p18);
+    p = fma(r, p, 0.24022650695902897 / 0x1p12);
+    p = fma(r, p, 0.6931471805593244 / 0x1p6);
+    p = fma(r, p, 1.0);
+    const uint64_t e = __builtin_bit_cast(uint64_t, table[n & (kTable - 1)] * p);
+    return __builtin_bit_cast(double, e + ((uint64_t)(uint32_t)((n >> 6) << 20) << 32));
 }
 
 // Values of 16 bytes of logits.
@@ -93,18 +98,30 @@ __device__ __forceinline__ void values(const void *row, int i, int V, float past
     }
 }
 
-// A logit as it counts: NaN as -infinity, +infinity as the largest number.
+// A logit as it counts: NaN as -infinity, +infinity as the largest number.  (A
+// weight of either is right as it is.)
 __device__ __forceinline__ float counted(float x) { return x != x ? -INFINITY : fminf(x, 3.4028235e38f); }
 
 // log2(e) / c of row b, 0: greedy.
 __device__ __forceinline__ double rate_of(const VerifyArgs &a, int b) {
-    const float c = a.temps ? a.temps[b] : a.temp;
+    const float c = fminf(a.temps ? a.temps[b] : a.temp, 3.4028235e38f);
     return c > 0.f ? 1.4426950408889634074 / (double)c : 0.0;
 }
 __device__ __forceinline__ bool greedy(const VerifyArgs &a, int b) { return !((a.temps ? a.temps[b] : a.temp) > 0.f); }
 
-__device__ __forceinline__ double weight(float x, float m, double rate) { return exp2_64(((double)x - (double)m) * rate); }
+__device__ __forceinline__ double weight(float x, float m, double rate, const double *table) {
+    return exp2_64(((double)x - (double)m) * rate, table);
+}
+// The same, 0 below 2^-1000.
+__device__ __forceinline__ double weight0(float x, float m, double rate, const double *table) {
+    return weight(x, m, rate, table) - 0x1p-1000;
+}
 
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v = fmaxf(v, __shfl_xor(v, off));
+    return v;
+}
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
@@ -145,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void kq_verify_rows_kernel(VerifyArgs a) 
     constexpr int N = kValues<DT>;
     __shared__ float red_m[kWaves];
     __shared__ int red_at[kWaves];
-    __shared__ double red_sum[kWaves];
+    __shared__ double red_sum[kWaves], table[kTable];
     const int t = blockIdx.x / a.S, s = blockIdx.x - t * a.S;
     if (t >= a.cu[a.B]) return;
     const uint8_t *row = (const uint8_t *)a.logits + (int64_t)t * a.stride * (16 / N);
@@ -156,38 +173,46 @@ __global__ __launch_bounds__(kThreads) void kq_verify_rows_kernel(VerifyArgs a) 
         const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N;
         values<DT, N>(row, min(i, a.V), a.V, -INFINITY, x[c]);
     }
+    fill_table(table);
+    const int b = a.temps ? row_at(a.cu, a.B, t) : 0;
+    const bool pick_top = greedy(a, b);
     float m = -INFINITY;
     int at = 0x7fffffff;
+    if (pick_top) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N;
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            x[c][j] = counted(x[c][j]);
-            if (x[c][j] > m) {
-                m = x[c][j];
-                at = i + j;
+            for (int j = 0; j < N; ++j) {
+                const float v = counted(x[c][j]);
+                if (v > m) {
+                    m = v;
+                    at = ((s * CH + c) * kThreads + (int)threadIdx.x) * N + j;
+                }
             }
-        }
+        wave_largest(m, at);
+    } else {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int j = 0; j < N; ++j) m = fmaxf(m, x[c][j]);  // (drops NaN)
+        m = fminf(wave_max(m), 3.4028235e38f);
     }
-    wave_largest(m, at);
     if (lane == 0) {
         red_m[w] = m;
         red_at[w] = at;
     }
-    __syncthreads();
+    __syncthreads();  // (the table too)
     m = red_m[0];
     at = red_at[0];
 #pragma unroll
     for (int k = 1; k < kWaves; ++k) take_larger(m, at, red_m[k], red_at[k]);
-    const int b = a.temps ? row_at(a.cu, a.B, t) : 0;
     double sum = 0.0;
-    if (!greedy(a, b) && m > -INFINITY) {
+    if (!pick_top && m > -INFINITY) {
         const double rate = rate_of(a, b);
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int j = 0; j < N; ++j) sum += weight(x[c][j], m, rate);
+            for (int j = 0; j < N; ++j) sum += weight(x[c][j], m, rate, table);
         sum = wave_sum(sum);
     }
     if (lane == 0) red_sum[w] = sum;
@@ -202,12 +227,12 @@ __global__ __launch_bounds__(kThreads) void kq_verify_rows_kernel(VerifyArgs a) 
 
 // Where row b ends, the same in every thread.
 struct Verdict {
+    double Z;
     int t;         // the logits row whose token follows
     int accepted;  // drafts that stand
     int draft;     // the refused one, -1: none was
     float m;       // its largest logit, -infinity: none
-    int top;       // the lowest token that has it
-    double Z;
+    int top;       // the lowest token that has it (greedy)
 };
 
 template <int PT>
@@ -224,7 +249,7 @@ __device__ __forceinline__ double prob_at(const VerifyArgs &a, int t, int v) {
 
 // A wave a draft, kWaves of them at a time until one does not stand.  n > 0.
 template <int DT>
-__device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, int n) {
+__device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, int n, const double *table) {
     __shared__ float s_m[kWaves];
     __shared__ int s_top[kWaves], s_ok[kWaves];
     __shared__ double s_z[kWaves];
@@ -241,17 +266,25 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, in
         const double q = known && !pick_top && a.probs ? prob_at(a, t, d) : 1.0;
         float m = -INFINITY;
         int at = 0x7fffffff;
-        for (int s = lane; s < a.S; s += 64) take_larger(m, at, part[s].m, part[s].at);
-        wave_largest(m, at);
         double z = 0.0;
         bool ok;
         if (pick_top) {
+            for (int s = lane; s < a.S; s += 64) take_larger(m, at, part[s].m, part[s].at);
+            wave_largest(m, at);
             ok = known && d == at;
         } else {
-            if (m > -INFINITY)
-                for (int s = lane; s < a.S; s += 64) z += part[s].sum * weight(part[s].m, m, rate);
+            const float u = last ? 0.f : a.u[t];
+            const Part first = lane < a.S ? part[lane] : Part{-INFINITY, 0, 0.0};
+            m = first.m;
+            for (int s = lane + 64; s < a.S; s += 64) m = fmaxf(m, part[s].m);
+            m = wave_max(m);
+            __syncthreads();  // (the table)
+            if (m > -INFINITY) {
+                z = first.sum * weight(first.m, m, rate, table);
+                for (int s = lane + 64; s < a.S; s += 64) z += part[s].sum * weight(part[s].m, m, rate, table);
+            }
             z = wave_sum(z);
-            ok = known && x > -INFINITY && (double)a.u[t] * q * z < weight(x, m, rate);
+            ok = known && x > -INFINITY && (double)u * q * z < weight0(x, m, rate, table);
         }
         __syncthreads();  // the last round's reads
         if (lane == 0) {
@@ -267,7 +300,7 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, in
             // (waves past the row's end repeat its last row, which is never a draft)
             const int j = min(i0 + k, n - 1), refused = j == n - 1 ? -1 : a.tokens[q0 + j + 1];
             const float mj = s_m[k];
-            return Verdict{q0 + j, j, refused, mj, mj > -INFINITY ? s_top[k] : -1, s_z[k]};
+            return Verdict{s_z[k], q0 + j, j, refused, mj, pick_top ? s_top[k] : 0};
         }
     }
 }
@@ -280,32 +313,35 @@ __device__ __forceinline__ bool row_of(const VerifyArgs &a, int b, int &q0, int 
 
 // max(e - q Z, 0) of N tokens from i on; 0 past the end.
 template <int DT, int PT, int N>
-__device__ __forceinline__ void rest_of(const VerifyArgs &a, const Verdict &r, double rate, int i, double (&w)[N]) {
+__device__ __forceinline__ void rest_of(const VerifyArgs &a, const Verdict &r, double rate, int i, const double *table,
+                                        double (&w)[N]) {
     float x[N], q[N];
     values<DT, N>((const uint8_t *)a.logits + (int64_t)r.t * a.stride * (DT == KQ_DTYPE_F32 ? 4 : 2), i, a.V, -INFINITY, x);
     values<PT, N>((const uint8_t *)a.probs + (int64_t)r.t * a.probs_stride * (PT == KQ_DTYPE_F32 ? 4 : 2), i, a.V, 0.f, q);
 #pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = fmax(weight(counted(x[j]), r.m, rate) - fmax((double)q[j], 0.0) * r.Z, 0.0);
+    for (int j = 0; j < N; ++j) w[j] = fmax(weight0(x[j], r.m, rate, table) - fmax((double)q[j], 0.0) * r.Z, 0.0);
 }
 
-// Sums of max(e - q Z, 0) over one slice a workgroup, of rows whose draft was
-// refused.
+// Where each row ends, and the sums of max(e - q Z, 0) over one slice a workgroup of
+// rows whose draft was refused.
 template <int DT, int PT, int CH>
 __global__ __launch_bounds__(kThreads) void kq_verify_rest_kernel(VerifyArgs a) {
     constexpr int N = kValues<DT>;
-    __shared__ double red[kWaves];
+    __shared__ double red[kWaves], table[kTable];
     const int s = blockIdx.x, b = blockIdx.y;
     int q0, n;
-    if (!row_of(a, b, q0, n) || n < 2 || greedy(a, b)) return;
-    const Verdict r = decide<DT>(a, b, q0, n);
-    if (r.accepted == n - 1 || !(r.m > -INFINITY)) return;
+    if (!row_of(a, b, q0, n)) return;
+    fill_table(table);
+    const Verdict r = decide<DT>(a, b, q0, n, table);
+    if (s == 0 && threadIdx.x == 0) a.verdict[b] = r;
+    if (r.accepted == n - 1 || greedy(a, b) || !(r.m > -INFINITY)) return;
     const double rate = rate_of(a, b);
     double sum = 0.0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N;
         double w[N];
-        rest_of<DT, PT, N>(a, r, rate, min(i, a.V), w);
+        rest_of<DT, PT, N>(a, r, rate, min(i, a.V), table, w);
 #pragma unroll
         for (int j = 0; j < N; ++j) sum += w[j];
     }
@@ -325,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void kq_verify_rest_kernel(VerifyArgs a) 
 template <int DT, int PT, int CH>
 __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) {
     constexpr int N = kValues<DT>;
-    __shared__ double red[kWaves];
+    __shared__ double red[CH][kWaves], table[kTable];
     __shared__ double s_target;
     __shared__ int s_how, s_slice, s_first, s_last;
     const int b = blockIdx.x, lane = kq_lane(), wv = threadIdx.x >> 6;
@@ -338,59 +374,75 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
         }
         return;
     }
-    const Verdict r = decide<DT>(a, b, q0, n);
+    fill_table(table);
+    __syncthreads();
+    const Verdict r = a.verdict ? a.verdict[b] : decide<DT>(a, b, q0, n, table);
     const auto finish = [&](int token) {
         a.accepted[b] = r.accepted;
         a.next[b] = token;
         if (a.keep) a.keep[b] = max(a.kv[b] - (n - 1 - r.accepted), 0);
     };
-    if (greedy(a, b) || r.top < 0) {
-        if (threadIdx.x == 0) finish(r.top);
+    const bool none = !(r.m > -INFINITY);
+    if (greedy(a, b) || none) {
+        if (threadIdx.x == 0) finish(none ? -1 : r.top);
         return;
     }
     const double rate = rate_of(a, b);
     const Part *part = a.part + (int64_t)r.t * a.S;
     const bool refused = r.accepted < n - 1, lone = refused && !a.probs && r.draft >= 0 && r.draft < a.V;
-    // weights of a slice's chunk c: how 0 as they are, 1 without the draft, 2 beside q
-    const auto weights = [&](int how, int s, int c, double(&w)[N]) {
-        const int i = min(((s * CH + c) * kThreads + (int)threadIdx.x) * N, a.V);
-        if (how == 2) {
-            rest_of<DT, PT, N>(a, r, rate, i, w);
-        } else {
-            float x[N];
-            values<DT, N>((const uint8_t *)a.logits + (int64_t)r.t * a.stride * (16 / N), i, a.V, -INFINITY, x);
+    // a thread's weights in a slice: how 0 as they are, 1 without the draft, 2 beside q
+    double w[CH][N];
+    const auto weigh = [&](int how, int s) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) w[j] = how == 1 && i + j == r.draft ? 0.0 : weight(counted(x[j]), r.m, rate);
+        for (int c = 0; c < CH; ++c) {
+            const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N, from = min(i, a.V);
+            if (how == 2) {
+                rest_of<DT, PT, N>(a, r, rate, from, table, w[c]);
+            } else {
+                float x[N];
+                values<DT, N>((const uint8_t *)a.logits + (int64_t)r.t * a.stride * (16 / N), from, a.V, -INFINITY, x);
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    w[c][j] = how == 1 && i + j == r.draft ? 0.0 : weight0(x[j], r.m, rate, table);
+            }
         }
     };
-    // the slice of a lone draft again without it (taken off its sum, a draft of
-    // nearly all the weight would leave a rest of few digits)
-    double without = 0.0;
+    // A lone draft's slice without it: taken off the slice's sum, and where that leaves
+    // less than a millionth of it (few digits), summed again.
     const int own = lone ? r.draft / (CH * kThreads * N) : -1;
+    double without = 0.0;
     if (lone) {
-        double sum = 0.0;
-        for (int c = 0; c < CH; ++c) {
-            double w[N];
-            weights(1, own, c, w);
+        const float x = counted(value<DT>(a.logits, (int64_t)r.t * a.stride + r.draft));
+        const double all = part[own].sum * weight(part[own].m, r.m, rate, table);
+        without = all - weight0(x, r.m, rate, table);
+        if (!(without > 0x1p-20 * all)) {
+            weigh(1, own);
+            double sum = 0.0;
 #pragma unroll
-            for (int j = 0; j < N; ++j) sum += w[j];
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum += w[c][j];
+            sum = wave_sum(sum);
+            if (lane == 0) red[0][wv] = sum;
+            __syncthreads();
+            without = 0.0;
+            for (int k = 0; k < kWaves; ++k) without += red[0][k];
+            __syncthreads();
         }
-        sum = wave_sum(sum);
-        if (lane == 0) red[wv] = sum;
-        __syncthreads();
-        for (int k = 0; k < kWaves; ++k) without += red[k];
     }
     // wave 0: the slices' running sums
     int how = lone ? 1 : refused && a.probs ? 2 : 0;
-    const auto slice_sum = [&](int s) {
-        return how == 2   ? a.rest[(int64_t)b * a.S + s]
-               : s == own && how == 1 ? without
-                          : part[s].sum * weight(part[s].m, r.m, rate);
-    };
     if (wv == 0) {
-        double all = 0.0;
+        const auto slice_sum = [&](int s) {
+            if (s >= a.S) return 0.0;
+            return how == 2 ? a.rest[(int64_t)b * a.S + s]
+                   : s == own && how == 1 ? without
+                                          : part[s].sum * weight0(part[s].m, r.m, rate, table);
+        };
+        double all = 0.0, first = 0.0;  // (first: this lane's of the first 64)
         for (int pass = 0; pass < 2; ++pass) {
-            for (int s = lane; s < a.S; s += 64) all += slice_sum(s);
+            first = all = slice_sum(lane);
+            for (int s = lane + 64; s < a.S; s += 64) all += slice_sum(s);
             all = wave_sum(all);
             if (all > 0.0) break;
             how = 0;  // nothing is left beside q: the target's own
@@ -398,9 +450,9 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
         const float draw = a.draws[b];
         const double target = (draw > 0.f ? (double)draw : 0.0) * all;
         double before = 0.0, at_before = 0.0;
-        int slice = -1;
+        int slice = 0;
         for (int s0 = 0; s0 < a.S; s0 += 64) {
-            const double mine = s0 + lane < a.S ? slice_sum(s0 + lane) : 0.0;
+            const double mine = s0 ? slice_sum(s0 + lane) : first;
             double run = mine;
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
@@ -426,40 +478,48 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
         }
     }
     __syncthreads();
-    how = s_how;
     const int slice = s_slice;
     const double target = s_target;
-    double before = 0.0;
+    weigh(s_how, slice);
+    double sum[CH], up[CH];
+#pragma unroll
     for (int c = 0; c < CH; ++c) {
-        double w[N], run[N];
-        weights(how, slice, c, w);
-        double sum = 0.0;
+        sum[c] = 0.0;
 #pragma unroll
-        for (int j = 0; j < N; ++j) run[j] = sum += w[j];
-        double up = sum;
+        for (int j = 0; j < N; ++j) sum[c] += w[c][j];
+        up[c] = sum[c];
+    }
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const double v = __shfl_up(up, off);
-            if (lane >= off) up += v;
+    for (int off = 1; off < 64; off <<= 1)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const double v = __shfl_up(up[c], off);
+            if (lane >= off) up[c] += v;
         }
-        __syncthreads();  // the last reads of red
-        if (lane == 63) red[wv] = up;
-        __syncthreads();
-        double mine = before + up - sum;
-        for (int k = 0; k < wv; ++k) mine += red[k];
-        const int i = ((slice * CH + c) * kThreads + (int)threadIdx.x) * N;
-        int first = 0x7fffffff, last = -1;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        if (lane == 63) red[c][wv] = up[c];
+    __syncthreads();
+    double before = 0.0;
+    int first = 0x7fffffff, last = -1;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        double run = before + up[c] - sum[c];
+        for (int k = 0; k < kWaves; ++k) {
+            if (k < wv) run += red[c][k];
+            before += red[c][k];
+        }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            if (w[j] > 0.0) {
-                last = i + j;
-                if (first == 0x7fffffff && mine + run[j] > target) first = i + j;
+            run += w[c][j];
+            if (w[c][j] > 0.0) {
+                last = ((slice * CH + c) * kThreads + (int)threadIdx.x) * N + j;
+                if (first == 0x7fffffff && run > target) first = last;
             }
         }
-        if (first != 0x7fffffff) atomicMin(&s_first, first);
-        if (last >= 0) atomicMax(&s_last, last);
-        for (int k = 0; k < kWaves; ++k) before += red[k];
     }
+    if (first != 0x7fffffff) atomicMin(&s_first, first);
+    if (last >= 0) atomicMax(&s_last, last);
     __syncthreads();
     if (threadIdx.x == 0) finish(s_first != 0x7fffffff ? s_first : s_last);
 }
@@ -477,7 +537,9 @@ int slices(int V, int dtype, int ch) {
     return (int)((V + len - 1) / len);
 }
 size_t part_bytes(int64_t T, int S) { return ((size_t)T * S * sizeof(Part) + 255) & ~(size_t)255; }
-size_t need_bytes(int64_t T, int64_t B, int S, bool probs) { return part_bytes(T, S) + (probs ? (size_t)B * S * sizeof(double) : 0); }
+size_t need_bytes(int64_t T, int64_t B, int S, bool probs) {
+    return part_bytes(T, S) + (probs ? (size_t)B * (S * sizeof(double) + sizeof(Verdict)) : 0);
+}
 
 // Grids of fewer than 2^32 threads, and 31-bit numbers of tokens a slice past the last.
 bool sizes_fit(int64_t T, int64_t B, int V, int S) {
@@ -487,7 +549,7 @@ bool sizes_fit(int64_t T, int64_t B, int V, int S) {
 template <int DT, int PT, int CH>
 void launch(const VerifyArgs &a, hipStream_t s) {
     if (a.T) hipLaunchKernelGGL((kq_verify_rows_kernel<DT, CH>), dim3(a.T * a.S), dim3(kThreads), 0, s, a);
-    if (a.T && a.probs && (a.temps || a.temp > 0.f))
+    if (a.verdict)
         hipLaunchKernelGGL((kq_verify_rest_kernel<DT, PT, CH>), dim3(a.S, a.B), dim3(kThreads), 0, s, a);
     hipLaunchKernelGGL((kq_verify_pick_kernel<DT, PT, CH>), dim3(a.B), dim3(kThreads), 0, s, a);
 }
@@ -556,7 +618,9 @@ int kq_verify_drafts(const void *logits, int dtype, int64_t row_stride, const in
     a.S = S;
     a.probs_type = probs_dtype;
     a.part = (Part *)workspace;
-    a.rest = (double *)((char *)workspace + part_bytes(T, S));
+    const bool with_rest = draft_probs && T && !greedy_all;
+    a.verdict = with_rest ? (Verdict *)((char *)workspace + part_bytes(T, S)) : nullptr;
+    a.rest = with_rest ? (double *)(a.verdict + B) : nullptr;
     a.accepted = accepted;
     a.next = next_tokens;
     a.keep = keep_lens;

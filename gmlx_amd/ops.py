@@ -1564,54 +1564,61 @@ def rope_frequencies(rotary_dim, base=10000.0, scaling=None, device="cuda"):
     return freqs.to(device), out
 
 
-def _rope(op, x, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor):
-    """The packed kq_rope and the positions' address, checked; x: the rows' tensor."""
-    dev, dt, T = x.device, x.dtype, x.shape[0]
+_ROPE_PACK = struct.Struct("3P3i2f4x").pack       # kq_rope
+_ROPE_ROWS_PACK = struct.Struct("2P4qi4x").pack   # kq_rope_rows
+
+
+def _rope(op, dev, dt, T, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor):
+    """The bytes of a kq_rope and the positions' address, checked."""
     if not isinstance(freqs, torch.Tensor) or freqs.dtype is not torch.float64 or freqs.dim() != 1 or \
             freqs.device != dev or not freqs.is_contiguous():
         raise ValueError(f"{op}: freqs must be a contiguous float64 tensor [rotary_dim / 2] on {dev}")
     R = 2 * freqs.numel()
     if R < 16 or R % 16 or R > D:
         raise ValueError(f"{op}: the rotated part must be a multiple of 16 values, at most {D}, got {R}")
-    wdt, ptrs = None, []
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is None:
-            ptrs.append(None)
-            continue
-        if not isinstance(w, torch.Tensor) or w.shape != (D,) or w.device != dev or w.dtype not in (dt, torch.float32) or \
-                not w.is_contiguous() or w.data_ptr() % 16 or wdt not in (None, w.dtype):
-            raise ValueError(f"{op}: {name} must be a contiguous 16-byte aligned tensor [{D}] of {dt} or float32 on "
-                             f"{dev} (both weights of one dtype)")
-        wdt = w.dtype
-        ptrs.append(w.data_ptr())
-    eps, factor = float(eps), float(factor)
-    if not 0 <= eps < 3.4e38 or not abs(factor) < 3.4e38:
+    wq = wk = 0
+    wdt = dt
+    if q_weight is not None or k_weight is not None:
+        wdt = (k_weight if q_weight is None else q_weight).dtype
+        if q_weight is not None:
+            wq = _rope_weight(op, "q_weight", q_weight, D, dt, wdt, dev)
+        if k_weight is not None:
+            wk = _rope_weight(op, "k_weight", k_weight, D, dt, wdt, dev)
+    if not 0 <= eps < 3.4e38 or not -3.4e38 < factor < 3.4e38:
         raise ValueError(f"{op}: eps must be finite and not negative, factor finite, got {eps} and {factor}")
-    pos = _ints(positions, "positions", T, dev)
-    return _lib.Rope(freqs.data_ptr(), ptrs[0], ptrs[1], _TORCH_DTYPE[wdt or dt], R, int(bool(interleaved)), eps,
-                     factor), pos
+    return _ROPE_PACK(freqs.data_ptr(), wq, wk, _TORCH_DTYPE[wdt], R, 1 if interleaved else 0, eps, factor), \
+        _ints(positions, "positions", T, dev)
+
+
+def _rope_weight(op, name, w, D, dt, wdt, dev):
+    """The address of a norm's weight."""
+    at = w.data_ptr()
+    if w.dtype is not wdt or (wdt is not dt and wdt is not torch.float32) or w.shape != (D,) or w.device != dev or \
+            not w.is_contiguous() or at % 16:
+        raise ValueError(f"{op}: {name} must be a contiguous 16-byte aligned tensor [{D}] of {dt} or float32 on {dev} "
+                         "(both weights of one dtype)")
+    return at
 
 
 def _rope_rows(op, name, x, out):
-    """(x, out, the kq_rope_rows of the two): x [T, H, D], copied only where its
-    layout needs it, and its output, made where none is given."""
+    """(x, out, the bytes of a kq_rope_rows of the two): x [T, H, D], copied only
+    where its layout needs it, and its output, made where none is given."""
     given = x
     x, t, h = _token_rows(x)
     T, H, D = x.shape
     if out is None:
         out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
-        ot, oh = H * D, D
-    else:
-        if not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-            raise ValueError(f"{op}: {name}_out must be like {name}")
-        ot, oh, one = out.stride()
-        ot, oh = ot if T > 1 else H * D, oh if H > 1 else D
-        if one != 1 or ot % 8 or oh % 8 or out.data_ptr() % 16 or not _apart(T, ot, H, oh, D):
-            raise ValueError(f"{op}: {name}_out must have contiguous rows at strides in multiples of 8, none on "
-                             "another, and be 16-byte aligned")
-        if out.data_ptr() == given.data_ptr() and out.stride() != given.stride():
-            raise ValueError(f"{op}: {name}_out at {name}'s address must have its strides")
-    return x, out, _lib.RopeRows(x.data_ptr(), out.data_ptr(), t, h, ot, oh, H)
+        return x, out, _ROPE_ROWS_PACK(x.data_ptr(), out.data_ptr(), t, h, H * D, D, H)
+    if not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{op}: {name}_out must be like {name}")
+    ot, oh, one = out.stride()
+    ot, oh = ot if T > 1 else H * D, oh if H > 1 else D
+    if one != 1 or ot % 8 or oh % 8 or out.data_ptr() % 16 or not _apart(T, ot, H, oh, D):
+        raise ValueError(f"{op}: {name}_out must have contiguous rows at strides in multiples of 8, none on "
+                         "another, and be 16-byte aligned")
+    if out.data_ptr() == given.data_ptr() and out.stride() != given.stride():
+        raise ValueError(f"{op}: {name}_out at {name}'s address must have its strides")
+    return x, out, _ROPE_ROWS_PACK(x.data_ptr(), out.data_ptr(), t, h, ot, oh, H)
 
 
 def _apart(T, t, H, h, D):
@@ -1652,12 +1659,11 @@ def rope_qk(q, k, positions, freqs, q_weight=None, k_weight=None, eps=1e-6, inte
     T, Hq, D = q.shape
     if D not in (64, 96, 128, 256, 512):
         raise ValueError(f"rope_qk: head dims 64, 96, 128, 256 and 512, got {D}")
-    rope, pos = _rope("rope_qk", q, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor)
+    rope, pos = _rope("rope_qk", q.device, q.dtype, T, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor)
     q, q_out, qr = _rope_rows("rope_qk", "q", q, q_out)
     k, k_out, kr = _rope_rows("rope_qk", "k", k, k_out)
     if T and Hq + k.shape[1]:
-        _paged_call("kq_rope_qk", q.device, ctypes.byref(rope), pos, T, D, _TORCH_DTYPE[q.dtype], ctypes.byref(qr),
-                    ctypes.byref(kr), _stream(q))
+        _paged_call("kq_rope_qk", q.device, rope, pos, T, D, _TORCH_DTYPE[q.dtype], qr, kr, _stream(q))
     return q_out, k_out
 
 
@@ -1681,14 +1687,14 @@ def paged_write_rope(q, k, v, k_cache, v_cache, slots, positions, freqs, q_weigh
     T = shape[0]
     if q.dtype is not dt or q.device != dev or q.dim() != 3 or q.shape[0] != T or q.shape[2] != D:
         raise ValueError(f"paged_write_rope: q must be [{T}, Hq, {D}] of dtype {dt} on the cache's device")
-    rope, pos = _rope("paged_write_rope", q, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor)
+    rope, pos = _rope("paged_write_rope", dev, dt, T, D, positions, freqs, q_weight, k_weight, eps, interleaved, factor)
     sl = _ints(slots, "slots", T, dev)
     q, q_out, qr = _rope_rows("paged_write_rope", "q", q, q_out)
     k, kt, kh = _token_rows(k)
     v, vt, vh = _token_rows(v)
     if T:
-        _paged_call("kq_paged_write_rope", dev, pool, ctypes.byref(rope), pos, sl, T, ctypes.byref(qr), k.data_ptr(), kt,
-                    kh, v.data_ptr(), vt, vh, _stream(q))
+        _paged_call("kq_paged_write_rope", dev, pool, rope, pos, sl, T, qr, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+                    _stream(q))
     return q_out
 
 
