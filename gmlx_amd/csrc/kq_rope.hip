@@ -27,41 +27,59 @@ struct RopeArgs {
     int32_t R, interleaved, weight_f32, lps;
 };
 
-// 8 weights.
-template <bool BF>
-__device__ __forceinline__ void weights8(const void *p, bool f32, int d, float (&w)[8]) {
-    if (f32) {
-        const float4 a = ((const float4 *)p)[d / 4], b = ((const float4 *)p)[d / 4 + 1];
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-    } else {
-        const u32x4 v = ((const u32x4 *)p)[d / 8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = f16bits_to_f32<BF>((v[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-    }
-}
-
 template <bool BF>
 __device__ __forceinline__ void unpack8(const u32x4 &v, float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = f16bits_to_f32<BF>((v[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
 }
 
+// Sum over the LG lanes of a head's row, in all of them: row operations inside the
+// VALU up to 16 lanes, swaps of rows and halves past them.
+template <int CTRL>
+__device__ __forceinline__ float add_lane(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+template <int LG>
+__device__ __forceinline__ float row_sum(float v) {
+    if constexpr (LG == 8) {
+        v = add_lane<0xB1>(v);   // neighbours, pairs, then halves of eight (mirrored)
+        v = add_lane<0x4E>(v);
+        return add_lane<0x141>(v);
+    }
+    v = add_lane<0x128>(v);  // row_ror:8, 4, 2, 1
+    v = add_lane<0x124>(v);
+    v = add_lane<0x122>(v);
+    v = add_lane<0x121>(v);
+    if constexpr (LG >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto w = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        v = __builtin_bit_cast(float, (uint32_t)w[0]) + __builtin_bit_cast(float, (uint32_t)w[1]);
+    }
+    if constexpr (LG == 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        v = __builtin_bit_cast(float, (uint32_t)w[0]) + __builtin_bit_cast(float, (uint32_t)w[1]);
+    }
+    return v;
+}
+
 // A workgroup takes PASSES times 256 / LG heads' rows of one token, LG lanes a
 // row and 8 values a lane.  The token's sines and cosines are made once, a pair a
-// thread, and shared through LDS.  A lane loads its pairs' other halves itself,
+// thread, and shared through LDS, and so are the weights (loaded where they are
+// used, behind the barrier, 8192 tokens took 40.5 us in place of 35.6).  A lane loads its pairs' other halves itself,
 // from the lines that its row's lanes have just asked for.  Rows are loaded before
 // any is stored, by the same wave, so outputs may be the inputs.
 template <int D, bool BF, bool Q8, bool WRITE, int PASSES>
 __global__ __launch_bounds__(256) void kq_rope_kernel(RopeArgs a) {
     constexpr int L = D / 8, LG = L <= 8 ? 8 : L <= 16 ? 16 : L <= 32 ? 32 : 64, RP = 256 / LG;
-    __shared__ __attribute__((aligned(16))) float cs[D / 2], sn[D / 2];
+    __shared__ __attribute__((aligned(16))) float cs[D / 2], sn[D / 2], weight[2][D];
     const int t = blockIdx.x, pos = a.positions[t];
     if (pos < 0) return;
     const int c = threadIdx.x % LG, row0 = blockIdx.y * (RP * PASSES) + threadIdx.x / LG;
     const int half = a.R / 2;
     // where this lane's pairs' other halves lie: in itself, or half the rotated part away
-    const bool turned = 8 * c < a.R;
-    const int other = a.interleaved || !turned ? c : 8 * c < half ? c + half / 8 : c - half / 8;
+    const bool turned = 8 * c < a.R, apart = turned && !a.interleaved, low = 8 * c < half;
+    const int other = !apart ? c : low ? c + half / 8 : c - half / 8;
     u32x4 v[PASSES], vo[PASSES];
     int which[PASSES], head[PASSES];
 #pragma unroll
@@ -75,8 +93,14 @@ __global__ __launch_bounds__(256) void kq_rope_kernel(RopeArgs a) {
                                 : which[p] == 1 ? a.src[1] + t * a.token_stride[1] + head[p] * a.head_stride[1]
                                                 : a.src[2] + t * a.token_stride[2] + head[p] * a.head_stride[2];
             v[p] = *(const u32x4 *)(x + 8 * c);
-            if (which[p] < 2) vo[p] = *(const u32x4 *)(x + 8 * other);
+            if (which[p] < 2 && apart) vo[p] = *(const u32x4 *)(x + 8 * other);
         }
+    }
+#pragma unroll
+    for (int i = threadIdx.x; i < 2 * D; i += 256) {
+        const int d = i % D;
+        if (const void *w = i < D ? a.weight[0] : a.weight[1])
+            weight[i / D][d] = a.weight_f32 ? ((const float *)w)[d] : f16bits_to_f32<BF>(((const uint16_t *)w)[d]);
     }
     if ((int)threadIdx.x < half) {
         const double turns = (double)pos * a.freqs[threadIdx.x] * 0.15915494309189533577;
@@ -86,6 +110,17 @@ __global__ __launch_bounds__(256) void kq_rope_kernel(RopeArgs a) {
         sn[threadIdx.x] = s * a.factor;
     }
     __syncthreads();
+    // a value becomes itself times its cosine plus its pair's other times +-its sine
+    float co[8], si[8];
+    if (turned) {
+        const int j = a.interleaved ? 4 * c : low ? 8 * c : 8 * c - half;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int k = j + (a.interleaved ? i / 2 : i);
+            co[i] = cs[k];
+            si[i] = (a.interleaved ? i % 2 == 0 : low) ? -sn[k] : sn[k];
+        }
+    }
     const int slot = WRITE ? a.slots[t] : 0;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
@@ -96,31 +131,26 @@ __global__ __launch_bounds__(256) void kq_rope_kernel(RopeArgs a) {
             float x[8], xo[8];
             unpack8<BF>(v[p], x);
             unpack8<BF>(vo[p], xo);
-            if (const void *w = which[p] == 0 ? a.weight[0] : a.weight[1]) {
-                float sum = 0.f;
+            if (which[p] == 0 ? a.weight[0] : a.weight[1]) {
+                const float *wx = weight[which[p]] + 8 * min(c, L - 1), *wo = weight[which[p]] + 8 * min(other, L - 1);
+                const auto mean = [&](float eps) {
+                    float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-                for (int off = 1; off < LG; off <<= 1) sum += __shfl_xor(sum, off);
-                float inv;
-                if (BF && !(sum <= 3.4028235e38f)) {
-                    // squares past fp32's largest: of 2^-70 times the values
-                    sum = 0.f;
+                    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+                    return fmaf(row_sum<LG>(sum), 1.f / D, eps);
+                };
+                float m = mean(a.eps);
+                if (BF && !(m >= 0x1p-100f && m <= 3.4028235e38f)) {
+                    // squares past the ends of fp32: of the values times a power of two
+                    const float by = m < 1.f ? 0x1p70f : 0x1p-70f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        x[i] *= 0x1p-70f;
-                        xo[i] *= 0x1p-70f;
-                        sum = fmaf(x[i], x[i], sum);
+                        x[i] *= by;
+                        xo[i] *= by;
                     }
-#pragma unroll
-                    for (int off = 1; off < LG; off <<= 1) sum += __shfl_xor(sum, off);
-                    inv = 1.f / sqrtf(sum * (1.f / D));
-                } else {
-                    inv = 1.f / sqrtf(sum * (1.f / D) + a.eps);
+                    m = mean(a.eps * by * by);
                 }
-                float wx[8], wo[8];
-                weights8<BF>(w, a.weight_f32, 8 * min(c, L - 1), wx);
-                weights8<BF>(w, a.weight_f32, 8 * min(other, L - 1), wo);
+                const float inv = rsqrtf(m);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     x[i] = x[i] * inv * wx[i];
@@ -128,22 +158,11 @@ __global__ __launch_bounds__(256) void kq_rope_kernel(RopeArgs a) {
                 }
             }
             if (turned) {
-                if (a.interleaved) {
+                float y[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const float co = cs[4 * c + i / 2], s = sn[4 * c + i / 2], u = x[i], w = x[i + 1];
-                        x[i] = fmaf(u, co, -(w * s));
-                        x[i + 1] = fmaf(w, co, u * s);
-                    }
-                } else {
-                    const bool low = 8 * c < half;
-                    const int j = low ? 8 * c : 8 * c - half;
+                for (int i = 0; i < 8; ++i) y[i] = fmaf(x[i], co[i], (a.interleaved ? x[i ^ 1] : xo[i]) * si[i]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float s = sn[j + i];
-                        x[i] = fmaf(x[i], cs[j + i], xo[i] * (low ? -s : s));
-                    }
-                }
+                for (int i = 0; i < 8; ++i) x[i] = y[i];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) out[i] = pack2<BF>(x[2 * i], x[2 * i + 1]);
@@ -169,7 +188,12 @@ void launch_passes(const RopeArgs &a, hipStream_t s) {
 
 template <int D, bool BF, bool Q8, bool WRITE>
 void launch(const RopeArgs &a, hipStream_t s) {
-    if (a.T < 512) launch_passes<D, BF, Q8, WRITE, 1>(a, s);
+    // Three passes where one would give the GPU four workgroups a CU (us with 1 / 2 / 3
+    // passes, 32 + 8 heads of 128: 33 tokens 4.9 / 5.0 / 5.1, 128 4.8 / 5.1 / 5.2, 512 5.7 /
+    // 5.7 / 5.8, 1024 9.1 / 7.8 / 8.0, 2048 14.1 / 13.4 / 12.9, 8192 45.5 / 42.3 / 35.6; a
+    // copy of 2048 tokens' bytes 7.6, of 8192 33.7)
+    constexpr int L = D / 8, LG = L <= 8 ? 8 : L <= 16 ? 16 : L <= 32 ? 32 : 64, RP = 256 / LG;
+    if ((int64_t)a.T * ((a.rows + RP - 1) / RP) < 1024) launch_passes<D, BF, Q8, WRITE, 1>(a, s);
     else launch_passes<D, BF, Q8, WRITE, 3>(a, s);
 }
 

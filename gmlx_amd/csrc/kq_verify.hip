@@ -38,29 +38,31 @@ struct VerifyArgs {
     int32_t *accepted, *next, *keep;
 };
 
-// 2^y for y <= 0 as 2^(j / 64) from a table in LDS, times 2^r for |r| <= 1/128, times
-// a power of two added to the exponent: within 5 10^-15, exact at 0.  The table's
-// part saves nine of a lone polynomial's fifteen steps; 397 rows of 152064 values
-// kROWS us, with an exponential series to the 12th power 74.  Below 2^-1000 (and of
-// NaN) 2^-1000, which no sum beside a largest weight of 1 notices.
-constexpr int kTable = 64;
-
-__device__ __forceinline__ void fill_table(double *table) {
-    if (threadIdx.x < kTable) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / kTable));
-}
-
-__device__ __forceinline__ double exp2_64(double y, const double *table) {
+// 2^y for y <= 0 as p 2^n: a polynomial of y's distance to the nearest whole number,
+// within 4 10^-14 and exact at 0, with n put in the exponent of 1.  (From a table of
+// 64 or 256 powers in LDS and a polynomial of the fourth or third power, 397 rows of
+// 152064 values took 58 and 62 us, with this one 56: the table's bank conflicts
+// cost more than five fp64 steps.)  Below 2^-1000 (and of NaN) 2^-1000, which no sum
+// beside a largest weight of 1 notices.
+struct Power {
+    double scale, p;  // their product
+};
+__device__ __forceinline__ Power power(double y) {
     constexpr double kRound = 0x1.8p52;  // its unit is 1: adding it rounds, the integer in the low bits
-    y = fmin(fmax(y, -1000.0), 0.0) * kTable;
+    y = fmax(y, -1000.0);
     const double t = y + kRound, r = y - (t - kRound);
-    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
-    // least maximum of the error in sixty-fourths, the constant term 1
-    double p = fma(r, 0.009618138509201629 / 0x1p24, 0.05550419004645178 / 0x1p18);
-    p = fma(r, p, 0.24022650695902897 / 0x1p12);
-    p = fma(r, p, 0.6931471805593244 / 0x1p6);
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
+    // least maximum of the error, the constant term 1
+    double p = fma(r, 1.0203121063391729e-07, 1.3255224878668817e-06);
+    p = fma(r, p, 1.525268684626772e-05);
+    p = fma(r, p, 0.00015403455852453838);
+    p = fma(r, p, 0.0013333558179043112);
+    p = fma(r, p, 0.009618129159402558);
+    p = fma(r, p, 0.055504108664760424);
+    p = fma(r, p, 0.2402265069581299);
+    p = fma(r, p, 0.6931471805599453);
     p = fma(r, p, 1.0);
-    const uint64_t e = __builtin_bit_cast(uint64_t, table[n & (kTable - 1)] * p);
-    return __builtin_bit_cast(double, e + ((uint64_t)(uint32_t)((n >> 6) << 20) << 32));
+    return Power{__builtin_bit_cast(double, (uint64_t)((n + 1023u) << 20) << 32), p};
 }
 
 // Values of 16 bytes of logits.
@@ -102,31 +104,71 @@ __device__ __forceinline__ void values(const void *row, int i, int V, float past
 // weight of either is right as it is.)
 __device__ __forceinline__ float counted(float x) { return x != x ? -INFINITY : fminf(x, 3.4028235e38f); }
 
-// log2(e) / c of row b, 0: greedy.
-__device__ __forceinline__ double rate_of(const VerifyArgs &a, int b) {
-    const float c = fminf(a.temps ? a.temps[b] : a.temp, 3.4028235e38f);
-    return c > 0.f ? 1.4426950408889634074 / (double)c : 0.0;
-}
 __device__ __forceinline__ bool greedy(const VerifyArgs &a, int b) { return !((a.temps ? a.temps[b] : a.temp) > 0.f); }
 
-__device__ __forceinline__ double weight(float x, float m, double rate, const double *table) {
-    return exp2_64(((double)x - (double)m) * rate, table);
+// log2(e) / c of row b.
+__device__ __forceinline__ double rate_of(const VerifyArgs &a, int b) {
+    return 1.4426950408889634074 / (double)fminf(a.temps ? a.temps[b] : a.temp, 3.4028235e38f);
 }
-// The same, 0 below 2^-1000.
-__device__ __forceinline__ double weight0(float x, float m, double rate, const double *table) {
-    return weight(x, m, rate, table) - 0x1p-1000;
+
+// The weight of x <= m (both fp64 steps are exact for x = m), and the same, 0 below 2^-1000.
+__device__ __forceinline__ double weight(float x, float m, double rate) {
+    const Power e = power(((double)x - (double)m) * rate);
+    return e.scale * e.p;
+}
+__device__ __forceinline__ double weight0(float x, float m, double rate) {
+    return weight(x, m, rate) - 0x1p-1000;
+}
+
+// Infinities among a thread's values as the largest number, where that is m (NaN
+// stays, and weighs nothing).
+template <int N>
+__device__ __forceinline__ void cap(float m, float (&x)[N]) {
+    if (m < 3.4028235e38f) return;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = x[j] > 3.4028235e38f ? 3.4028235e38f : x[j];
+}
+
+// v of another lane of the wave (a DPP pattern), or `none` where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float from_lane(float v, float none) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL,
+                                                                 ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lane(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double of_lane(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) v = fmaxf(v, __shfl_xor(v, off));
+    v = fmaxf(v, from_lane<0x111, 0xf>(v, -INFINITY));  // row_shr:1, 2, 4, 8
+    v = fmaxf(v, from_lane<0x112, 0xf>(v, -INFINITY));
+    v = fmaxf(v, from_lane<0x114, 0xf>(v, -INFINITY));
+    v = fmaxf(v, from_lane<0x118, 0xf>(v, -INFINITY));
+    v = fmaxf(v, from_lane<0x142, 0xa>(v, -INFINITY));  // row_bcast:15, 31
+    v = fmaxf(v, from_lane<0x143, 0xc>(v, -INFINITY));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+// Inclusive running sum over the wave's lanes, and the whole sum.
+__device__ __forceinline__ double wave_scan(double v) {
+    v += from_lane<0x111, 0xf>(v);
+    v += from_lane<0x112, 0xf>(v);
+    v += from_lane<0x114, 0xf>(v);
+    v += from_lane<0x118, 0xf>(v);
+    v += from_lane<0x142, 0xa>(v);
+    v += from_lane<0x143, 0xc>(v);
     return v;
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
-    return v;
-}
+__device__ __forceinline__ double wave_sum(double v) { return of_lane(wave_scan(v), 63); }
 
 // The larger of two (value, token), the lower token of equal values.
 __device__ __forceinline__ void take_larger(float &m, int &at, float m2, int at2) {
@@ -155,74 +197,62 @@ __device__ __forceinline__ int row_at(const int32_t *cu, int B, int t) {
     return lo;
 }
 
-// One slice of one logits row a workgroup: CH chunks of 16 bytes a thread, held in
-// registers between the maximum and the sum, so the logits are read once.
-template <int DT, int CH>
+// A slice: 256 times 16 bytes of a row, kChunks of them a lane to the wave that sums
+// it, one a thread to the workgroup that looks for a token in it.
+constexpr int kChunks = kThreads / 64;
+
+// One slice of one logits row a wave, held in registers between the maximum and the
+// sum, so the logits are read once; waves share nothing, so that some load while
+// others calculate (a slice four times as long by a workgroup together:
+// 57 us; the next kernels look through four times as many tokens then).
+template <int DT>
 __global__ __launch_bounds__(kThreads) void kq_verify_rows_kernel(VerifyArgs a) {
     constexpr int N = kValues<DT>;
-    __shared__ float red_m[kWaves];
-    __shared__ int red_at[kWaves];
-    __shared__ double red_sum[kWaves], table[kTable];
-    const int t = blockIdx.x / a.S, s = blockIdx.x - t * a.S;
-    if (t >= a.cu[a.B]) return;
+    const int lane = kq_lane(), unit = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+    const int t = unit / a.S, s = unit - t * a.S;
+    if (t >= min(a.cu[a.B], a.T)) return;
     const uint8_t *row = (const uint8_t *)a.logits + (int64_t)t * a.stride * (16 / N);
-    const int lane = kq_lane(), w = threadIdx.x >> 6;
-    float x[CH][N];
+    float x[kChunks][N];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N;
-        values<DT, N>(row, min(i, a.V), a.V, -INFINITY, x[c]);
-    }
-    fill_table(table);
+    for (int c = 0; c < kChunks; ++c)
+        values<DT, N>(row, min(((s * kChunks + c) * 64 + lane) * N, a.V), a.V, -INFINITY, x[c]);
     const int b = a.temps ? row_at(a.cu, a.B, t) : 0;
-    const bool pick_top = greedy(a, b);
     float m = -INFINITY;
     int at = 0x7fffffff;
-    if (pick_top) {
+    double sum = 0.0;
+    if (greedy(a, b)) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float v = counted(x[c][j]);
                 if (v > m) {
                     m = v;
-                    at = ((s * CH + c) * kThreads + (int)threadIdx.x) * N + j;
+                    at = ((s * kChunks + c) * 64 + lane) * N + j;
                 }
             }
         wave_largest(m, at);
     } else {
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int j = 0; j < N; ++j) m = fmaxf(m, x[c][j]);  // (drops NaN)
         m = fminf(wave_max(m), 3.4028235e38f);
-    }
-    if (lane == 0) {
-        red_m[w] = m;
-        red_at[w] = at;
-    }
-    __syncthreads();  // (the table too)
-    m = red_m[0];
-    at = red_at[0];
+        if (m > -INFINITY) {
+            const double rate = rate_of(a, b);
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) take_larger(m, at, red_m[k], red_at[k]);
-    double sum = 0.0;
-    if (!pick_top && m > -INFINITY) {
-        const double rate = rate_of(a, b);
+            for (int c = 0; c < kChunks; ++c) {
+                cap(m, x[c]);
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int j = 0; j < N; ++j) sum += weight(x[c][j], m, rate, table);
-        sum = wave_sum(sum);
+                for (int j = 0; j < N; ++j) {
+                    const Power e = power(((double)x[c][j] - (double)m) * rate);
+                    sum = fma(e.scale, e.p, sum);
+                }
+            }
+            sum = wave_sum(sum);
+        }
     }
-    if (lane == 0) red_sum[w] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double all = red_sum[0];
-#pragma unroll
-        for (int k = 1; k < kWaves; ++k) all += red_sum[k];
-        a.part[(int64_t)t * a.S + s] = Part{m, at, all};
-    }
+    if (lane == 0) a.part[(int64_t)t * a.S + s] = Part{m, at, sum};
 }
 
 // Where row b ends, the same in every thread.
@@ -230,8 +260,9 @@ struct Verdict {
     double Z;
     int t;         // the logits row whose token follows
     int accepted;  // drafts that stand
-    int draft;     // the refused one, -1: none was
+    int draft;     // the refused one, -1: none was, or it is no token
     float m;       // its largest logit, -infinity: none
+    float x;       // the draft's
     int top;       // the lowest token that has it (greedy)
 };
 
@@ -249,9 +280,9 @@ __device__ __forceinline__ double prob_at(const VerifyArgs &a, int t, int v) {
 
 // A wave a draft, kWaves of them at a time until one does not stand.  n > 0.
 template <int DT>
-__device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, int n, const double *table) {
-    __shared__ float s_m[kWaves];
-    __shared__ int s_top[kWaves], s_ok[kWaves];
+__device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, int n) {
+    __shared__ float s_m[kWaves], s_x[kWaves];
+    __shared__ int s_top[kWaves], s_ok[kWaves], s_d[kWaves];
     __shared__ double s_z[kWaves];
     const int lane = kq_lane(), w = threadIdx.x >> 6;
     const bool pick_top = greedy(a, b);
@@ -278,17 +309,18 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, in
             m = first.m;
             for (int s = lane + 64; s < a.S; s += 64) m = fmaxf(m, part[s].m);
             m = wave_max(m);
-            __syncthreads();  // (the table)
             if (m > -INFINITY) {
-                z = first.sum * weight(first.m, m, rate, table);
-                for (int s = lane + 64; s < a.S; s += 64) z += part[s].sum * weight(part[s].m, m, rate, table);
+                z = first.sum * weight(first.m, m, rate);
+                for (int s = lane + 64; s < a.S; s += 64) z += part[s].sum * weight(part[s].m, m, rate);
             }
             z = wave_sum(z);
-            ok = known && x > -INFINITY && (double)u * q * z < weight0(x, m, rate, table);
+            ok = known && x > -INFINITY && (double)u * q * z < weight0(x, m, rate);
         }
         __syncthreads();  // the last round's reads
         if (lane == 0) {
             s_m[w] = m;
+            s_x[w] = x;
+            s_d[w] = known ? d : -1;
             s_top[w] = at;
             s_z[w] = z;
             s_ok[w] = ok && !last;
@@ -298,9 +330,8 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs &a, int b, int q0, in
         while (k < kWaves && s_ok[k]) ++k;
         if (k < kWaves) {
             // (waves past the row's end repeat its last row, which is never a draft)
-            const int j = min(i0 + k, n - 1), refused = j == n - 1 ? -1 : a.tokens[q0 + j + 1];
-            const float mj = s_m[k];
-            return Verdict{s_z[k], q0 + j, j, refused, mj, pick_top ? s_top[k] : 0};
+            const int j = min(i0 + k, n - 1);
+            return Verdict{s_z[k], q0 + j, j, s_d[k], s_m[k], s_x[k], pick_top ? s_top[k] : 0};
         }
     }
 }
@@ -313,55 +344,55 @@ __device__ __forceinline__ bool row_of(const VerifyArgs &a, int b, int &q0, int 
 
 // max(e - q Z, 0) of N tokens from i on; 0 past the end.
 template <int DT, int PT, int N>
-__device__ __forceinline__ void rest_of(const VerifyArgs &a, const Verdict &r, double rate, int i, const double *table,
+__device__ __forceinline__ void rest_of(const VerifyArgs &a, const Verdict &r, double rate, int i,
                                         double (&w)[N]) {
     float x[N], q[N];
     values<DT, N>((const uint8_t *)a.logits + (int64_t)r.t * a.stride * (DT == KQ_DTYPE_F32 ? 4 : 2), i, a.V, -INFINITY, x);
     values<PT, N>((const uint8_t *)a.probs + (int64_t)r.t * a.probs_stride * (PT == KQ_DTYPE_F32 ? 4 : 2), i, a.V, 0.f, q);
+    cap(r.m, x);
 #pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = fmax(weight0(x[j], r.m, rate, table) - fmax((double)q[j], 0.0) * r.Z, 0.0);
+    for (int j = 0; j < N; ++j) w[j] = fmax(weight0(x[j], r.m, rate) - fmax((double)q[j], 0.0) * r.Z, 0.0);
 }
 
-// Where each row ends, and the sums of max(e - q Z, 0) over one slice a workgroup of
-// rows whose draft was refused.
-template <int DT, int PT, int CH>
-__global__ __launch_bounds__(kThreads) void kq_verify_rest_kernel(VerifyArgs a) {
-    constexpr int N = kValues<DT>;
-    __shared__ double red[kWaves], table[kTable];
-    const int s = blockIdx.x, b = blockIdx.y;
+// Where each row ends, one workgroup a row.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void kq_verify_decide_kernel(VerifyArgs a) {
+    const int b = blockIdx.x;
     int q0, n;
     if (!row_of(a, b, q0, n)) return;
-    fill_table(table);
-    const Verdict r = decide<DT>(a, b, q0, n, table);
-    if (s == 0 && threadIdx.x == 0) a.verdict[b] = r;
+    const Verdict r = decide<DT>(a, b, q0, n);
+    if (threadIdx.x == 0) a.verdict[b] = r;
+}
+
+// Sums of max(e - q Z, 0) over one slice a wave, of rows whose draft was refused.
+template <int DT, int PT>
+__global__ __launch_bounds__(kThreads) void kq_verify_rest_kernel(VerifyArgs a) {
+    constexpr int N = kValues<DT>;
+    const int lane = kq_lane(), b = blockIdx.y;
+    const int s = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+    int q0, n;
+    if (s >= a.S || !row_of(a, b, q0, n) || n < 2) return;
+    const Verdict r = a.verdict[b];
     if (r.accepted == n - 1 || greedy(a, b) || !(r.m > -INFINITY)) return;
     const double rate = rate_of(a, b);
     double sum = 0.0;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N;
+    for (int c = 0; c < kChunks; ++c) {
         double w[N];
-        rest_of<DT, PT, N>(a, r, rate, min(i, a.V), table, w);
+        rest_of<DT, PT, N>(a, r, rate, min(((s * kChunks + c) * 64 + lane) * N, a.V), w);
 #pragma unroll
         for (int j = 0; j < N; ++j) sum += w[j];
     }
     sum = wave_sum(sum);
-    if (kq_lane() == 0) red[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double all = red[0];
-#pragma unroll
-        for (int k = 1; k < kWaves; ++k) all += red[k];
-        a.rest[(int64_t)b * a.S + s] = all;
-    }
+    if (lane == 0) a.rest[(int64_t)b * a.S + s] = sum;
 }
 
 // The token that follows, one workgroup a row: the slice whose running sum passes
 // r times the whole, then the token within it.
-template <int DT, int PT, int CH>
+template <int DT, int PT>
 __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) {
     constexpr int N = kValues<DT>;
-    __shared__ double red[CH][kWaves], table[kTable];
+    __shared__ double red[kWaves];
     __shared__ double s_target;
     __shared__ int s_how, s_slice, s_first, s_last;
     const int b = blockIdx.x, lane = kq_lane(), wv = threadIdx.x >> 6;
@@ -374,9 +405,7 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
         }
         return;
     }
-    fill_table(table);
-    __syncthreads();
-    const Verdict r = a.verdict ? a.verdict[b] : decide<DT>(a, b, q0, n, table);
+    const Verdict r = a.verdict ? a.verdict[b] : decide<DT>(a, b, q0, n);
     const auto finish = [&](int token) {
         a.accepted[b] = r.accepted;
         a.next[b] = token;
@@ -389,44 +418,38 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
     }
     const double rate = rate_of(a, b);
     const Part *part = a.part + (int64_t)r.t * a.S;
-    const bool refused = r.accepted < n - 1, lone = refused && !a.probs && r.draft >= 0 && r.draft < a.V;
+    const bool refused = r.accepted < n - 1, lone = refused && !a.probs && r.draft >= 0;
     // a thread's weights in a slice: how 0 as they are, 1 without the draft, 2 beside q
-    double w[CH][N];
+    double w[N];
     const auto weigh = [&](int how, int s) {
+        const int i = (s * kThreads + (int)threadIdx.x) * N, from = min(i, a.V);
+        if (how == 2) {
+            rest_of<DT, PT, N>(a, r, rate, from, w);
+        } else {
+            float x[N];
+            values<DT, N>((const uint8_t *)a.logits + (int64_t)r.t * a.stride * (16 / N), from, a.V, -INFINITY, x);
+            cap(r.m, x);
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int i = ((s * CH + c) * kThreads + (int)threadIdx.x) * N, from = min(i, a.V);
-            if (how == 2) {
-                rest_of<DT, PT, N>(a, r, rate, from, table, w[c]);
-            } else {
-                float x[N];
-                values<DT, N>((const uint8_t *)a.logits + (int64_t)r.t * a.stride * (16 / N), from, a.V, -INFINITY, x);
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                    w[c][j] = how == 1 && i + j == r.draft ? 0.0 : weight0(x[j], r.m, rate, table);
-            }
+            for (int j = 0; j < N; ++j) w[j] = how == 1 && i + j == r.draft ? 0.0 : weight0(x[j], r.m, rate);
         }
     };
     // A lone draft's slice without it: taken off the slice's sum, and where that leaves
     // less than a millionth of it (few digits), summed again.
-    const int own = lone ? r.draft / (CH * kThreads * N) : -1;
+    const int own = lone ? r.draft / (kThreads * N) : -1;
     double without = 0.0;
     if (lone) {
-        const float x = counted(value<DT>(a.logits, (int64_t)r.t * a.stride + r.draft));
-        const double all = part[own].sum * weight(part[own].m, r.m, rate, table);
-        without = all - weight0(x, r.m, rate, table);
+        const double all = part[own].sum * weight(part[own].m, r.m, rate);
+        without = all - weight0(r.x, r.m, rate);
         if (!(without > 0x1p-20 * all)) {
             weigh(1, own);
             double sum = 0.0;
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum += w[c][j];
+            for (int j = 0; j < N; ++j) sum += w[j];
             sum = wave_sum(sum);
-            if (lane == 0) red[0][wv] = sum;
+            if (lane == 0) red[wv] = sum;
             __syncthreads();
             without = 0.0;
-            for (int k = 0; k < kWaves; ++k) without += red[0][k];
+            for (int k = 0; k < kWaves; ++k) without += red[k];
             __syncthreads();
         }
     }
@@ -437,7 +460,7 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
             if (s >= a.S) return 0.0;
             return how == 2 ? a.rest[(int64_t)b * a.S + s]
                    : s == own && how == 1 ? without
-                                          : part[s].sum * weight0(part[s].m, r.m, rate, table);
+                                          : part[s].sum * weight0(part[s].m, r.m, rate);
         };
         double all = 0.0, first = 0.0;  // (first: this lane's of the first 64)
         for (int pass = 0; pass < 2; ++pass) {
@@ -453,21 +476,16 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
         int slice = 0;
         for (int s0 = 0; s0 < a.S; s0 += 64) {
             const double mine = s0 ? slice_sum(s0 + lane) : first;
-            double run = mine;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const double v = __shfl_up(run, off);
-                if (lane >= off) run += v;
-            }
+            const double run = wave_scan(mine);
             const uint64_t over = __ballot(mine > 0.0 && before + run > target), some = __ballot(mine > 0.0);
             // (none passes a draw of 1: the last slice that has any weight)
             const int pick = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
             if (pick >= 0) {
                 slice = s0 + pick;
-                at_before = before + __shfl(run, pick) - __shfl(mine, pick);
+                at_before = before + of_lane(run, pick) - of_lane(mine, pick);
             }
             if (over) break;
-            before += __shfl(run, 63);
+            before += of_lane(run, 63);
         }
         if (lane == 0) {
             s_how = how;
@@ -481,41 +499,21 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
     const int slice = s_slice;
     const double target = s_target;
     weigh(s_how, slice);
-    double sum[CH], up[CH];
+    double sum = 0.0;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        sum[c] = 0.0;
-#pragma unroll
-        for (int j = 0; j < N; ++j) sum[c] += w[c][j];
-        up[c] = sum[c];
-    }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1)
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const double v = __shfl_up(up[c], off);
-            if (lane >= off) up[c] += v;
-        }
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-        if (lane == 63) red[c][wv] = up[c];
+    for (int j = 0; j < N; ++j) sum += w[j];
+    const double up = wave_scan(sum);
+    if (lane == 63) red[wv] = up;
     __syncthreads();
-    double before = 0.0;
+    double run = up - sum;
+    for (int k = 0; k < wv; ++k) run += red[k];
     int first = 0x7fffffff, last = -1;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        double run = before + up[c] - sum[c];
-        for (int k = 0; k < kWaves; ++k) {
-            if (k < wv) run += red[c][k];
-            before += red[c][k];
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            run += w[c][j];
-            if (w[c][j] > 0.0) {
-                last = ((slice * CH + c) * kThreads + (int)threadIdx.x) * N + j;
-                if (first == 0x7fffffff && run > target) first = last;
-            }
+    for (int j = 0; j < N; ++j) {
+        run += w[j];
+        if (w[j] > 0.0) {
+            last = (slice * kThreads + (int)threadIdx.x) * N + j;
+            if (first == 0x7fffffff && run > target) first = last;
         }
     }
     if (first != 0x7fffffff) atomicMin(&s_first, first);
@@ -524,17 +522,9 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
     if (threadIdx.x == 0) finish(s_first != 0x7fffffff ? s_first : s_last);
 }
 
-// Chunks of 16 bytes a thread: the longest slices (fewest partials, most bytes in
-// flight a wave) that still give every CU four workgroups.
-int chunks(int64_t T, int V, int dtype) {
-    const int n = dtype == KQ_DTYPE_F32 ? 4 : 8;
-    for (int ch = 4; ch > 1; ch /= 2)
-        if (T * ((V + kThreads * n * ch - 1) / (kThreads * n * ch)) >= 1024) return ch;
-    return 1;
-}
-int slices(int V, int dtype, int ch) {
-    const int64_t len = (int64_t)kThreads * (dtype == KQ_DTYPE_F32 ? 4 : 8) * ch;
-    return (int)((V + len - 1) / len);
+int slices(int V, int dtype) {
+    const int len = kThreads * (dtype == KQ_DTYPE_F32 ? 4 : 8);
+    return (int)(((int64_t)V + len - 1) / len);
 }
 size_t part_bytes(int64_t T, int S) { return ((size_t)T * S * sizeof(Part) + 255) & ~(size_t)255; }
 size_t need_bytes(int64_t T, int64_t B, int S, bool probs) {
@@ -543,29 +533,24 @@ size_t need_bytes(int64_t T, int64_t B, int S, bool probs) {
 
 // Grids of fewer than 2^32 threads, and 31-bit numbers of tokens a slice past the last.
 bool sizes_fit(int64_t T, int64_t B, int V, int S) {
-    return T <= 1 << 22 && B < 1 << 16 && V <= 1 << 28 && T * S < 1 << 23;
-}
-
-template <int DT, int PT, int CH>
-void launch(const VerifyArgs &a, hipStream_t s) {
-    if (a.T) hipLaunchKernelGGL((kq_verify_rows_kernel<DT, CH>), dim3(a.T * a.S), dim3(kThreads), 0, s, a);
-    if (a.verdict)
-        hipLaunchKernelGGL((kq_verify_rest_kernel<DT, PT, CH>), dim3(a.S, a.B), dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL((kq_verify_pick_kernel<DT, PT, CH>), dim3(a.B), dim3(kThreads), 0, s, a);
+    return T <= 1 << 22 && B < 1 << 16 && V <= 1 << 28 && T * S <= 1 << 24;
 }
 
 template <int DT, int PT>
-void launch_chunks(const VerifyArgs &a, int ch, hipStream_t s) {
-    if (ch == 4) launch<DT, PT, 4>(a, s);
-    else if (ch == 2) launch<DT, PT, 2>(a, s);
-    else launch<DT, PT, 1>(a, s);
+void launch(const VerifyArgs &a, hipStream_t s) {
+    if (a.T) hipLaunchKernelGGL((kq_verify_rows_kernel<DT>), dim3((a.T * a.S + kWaves - 1) / kWaves), dim3(kThreads), 0, s, a);
+    if (a.verdict) {
+        hipLaunchKernelGGL((kq_verify_decide_kernel<DT>), dim3(a.B), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((kq_verify_rest_kernel<DT, PT>), dim3((a.S + kWaves - 1) / kWaves, a.B), dim3(kThreads), 0, s, a);
+    }
+    hipLaunchKernelGGL((kq_verify_pick_kernel<DT, PT>), dim3(a.B), dim3(kThreads), 0, s, a);
 }
 
 template <int DT>
-void launch_probs(const VerifyArgs &a, int ch, hipStream_t s) {
-    if (!a.probs || a.probs_type == KQ_DTYPE_F32) launch_chunks<DT, KQ_DTYPE_F32>(a, ch, s);
-    else if (a.probs_type == KQ_DTYPE_BF16) launch_chunks<DT, KQ_DTYPE_BF16>(a, ch, s);
-    else launch_chunks<DT, KQ_DTYPE_F16>(a, ch, s);
+void launch_probs(const VerifyArgs &a, hipStream_t s) {
+    if (!a.probs || a.probs_type == KQ_DTYPE_F32) launch<DT, KQ_DTYPE_F32>(a, s);
+    else if (a.probs_type == KQ_DTYPE_BF16) launch<DT, KQ_DTYPE_BF16>(a, s);
+    else launch<DT, KQ_DTYPE_F16>(a, s);
 }
 
 bool a_type(int dtype) { return dtype == KQ_DTYPE_F32 || dtype == KQ_DTYPE_F16 || dtype == KQ_DTYPE_BF16; }
@@ -576,7 +561,7 @@ extern "C" {
 
 size_t kq_verify_workspace_bytes(int32_t T, int32_t B, int32_t V, int dtype, int with_probs) {
     if (T < 1 || B < 1 || V < 1 || !a_type(dtype)) return 0;
-    const int S = slices(V, dtype, chunks(T, V, dtype));
+    const int S = slices(V, dtype);
     return sizes_fit(T, B, V, S) ? need_bytes(T, B, S, with_probs != 0) : 0;
 }
 
@@ -596,7 +581,7 @@ int kq_verify_drafts(const void *logits, int dtype, int64_t row_stride, const in
     if (((uintptr_t)logits & (dtype == KQ_DTYPE_F32 ? 3 : 1)) ||
         (draft_probs && ((uintptr_t)draft_probs & (probs_dtype == KQ_DTYPE_F32 ? 3 : 1))))
         return KQ_ERR_BAD_ALIGN;
-    const int ch = chunks(T, V, dtype), S = slices(V, dtype, ch);
+    const int S = slices(V, dtype);
     if (!sizes_fit(T, B, V, S)) return KQ_ERR_BAD_SHAPE;
     if (T && (!workspace || workspace_bytes < need_bytes(T, B, S, draft_probs != nullptr))) return KQ_ERR_WORKSPACE_TOO_SMALL;
     if ((uintptr_t)workspace & 255) return KQ_ERR_BAD_ALIGN;
@@ -625,9 +610,9 @@ int kq_verify_drafts(const void *logits, int dtype, int64_t row_stride, const in
     a.next = next_tokens;
     a.keep = keep_lens;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == KQ_DTYPE_F32) launch_probs<KQ_DTYPE_F32>(a, ch, s);
-    else if (dtype == KQ_DTYPE_BF16) launch_probs<KQ_DTYPE_BF16>(a, ch, s);
-    else launch_probs<KQ_DTYPE_F16>(a, ch, s);
+    if (dtype == KQ_DTYPE_F32) launch_probs<KQ_DTYPE_F32>(a, s);
+    else if (dtype == KQ_DTYPE_BF16) launch_probs<KQ_DTYPE_BF16>(a, s);
+    else launch_probs<KQ_DTYPE_F16>(a, s);
     return hipGetLastError() == hipSuccess ? KQ_OK : KQ_ERR_LAUNCH_FAILED;
 }
 

@@ -659,8 +659,8 @@ int kq_paged_write_rope(const kq_paged_pool *pool, const kq_rope *rope, const in
  *
  * temperatures: fp32 [B] on the device, or NULL and `temperature` (finite, >= 0) for
  * all.  uniforms [T] and draws [B] fp32 in [0, 1) (may be NULL where temperature is
- * 0 for all).  T up to 2^22, B below 2^16, V up to 2^28, and fewer than 2^23 slices
- * of a row (of 4096 to 32768 bytes).  Workspace: kq_verify_workspace_bytes, no
+ * 0 for all).  T up to 2^22, B below 2^16, V up to 2^28, and at most 2^24 slices
+ * of 4096 bytes in the rows together.  Workspace: kq_verify_workspace_bytes, no
  * zero-fill needed, 256-byte aligned; calls that share one are ordered.  Nothing
  * is read of logits past cu_rows[B]. */
 size_t kq_verify_workspace_bytes(int32_t T, int32_t B, int32_t V, int dtype, int with_probs);
