@@ -62,6 +62,12 @@ struct PagedArgs {
 // over 4000 24 / 19 / 40, four of 100 over 1000 34 / 43 / 34, 8 rows of 8 over 2 k
 // to 6 k 43 / 51 / 49, two chunks beside 14 decode rows 147 / 170 / 145.
 constexpr int kSplitTokens = 512;
+// Through a window, which has few splits of 512 (us with the merge, 512 against 256):
+// rows of so few units that half the GPU is idle split at 256.  500 tokens through 777
+// keys at head dim 256 49 / 43, 100 through 1000 at 128 33 / 29, 64 through 4000 35 / 31,
+// 300 through 1000 in 8 bits at 256 67 / 52; but 1000 tokens through 500, 256 units, 33
+// / 46.
+constexpr int kLeastUnits = 128;
 // Most waves, and merged tokens and heads, of grids in which each finds its place
 // without a sum over the rows: three rows of 400 to 1700 keys 10.8 us (16.5 with
 // the sum), 8 rows of 4 tokens 43.9 (45), four of 4000 at head dim 512 30 (38);
@@ -102,10 +108,10 @@ __host__ __device__ __forceinline__ int row_blocks(int n, int G, int cols) {
 // Splits of a row of n tokens and kv keys: from the row and the head counts
 // alone, so that a row of a batch has the bits of the row alone.
 __host__ __device__ __forceinline__ int paged_splits(const SplitRule &rule, int n, int kv, int G, int Hkv, int few_limit,
-                                                            int group_cols, int group_slots) {
+                                                     int group_cols, int group_slots, int least_units) {
     if (few_columns(n, G, few_limit)) return row_splits(rule, kv);
     const int units = row_blocks(n, G, group_cols) * Hkv;
-    return max(1, min(group_slots / units, kv / kSplitTokens));
+    return max(1, min(group_slots / units, kv / (units <= least_units ? kSplitTokens / 2 : kSplitTokens)));
 }
 
 struct Row {
@@ -165,7 +171,7 @@ __device__ __forceinline__ Row row_at(const PagedArgs &a, int b) {
         r.kv = min(r.kv, max(r.before + r.n, 0));
         r.span = window_span(r.kv, a.window, a.sinks, r.n, a.G, cols);
     }
-    r.splits = paged_splits(a.rule, r.n, r.span, a.G, a.Hkv, a.few_limit, a.group_cols, a.group_slots);
+    r.splits = paged_splits(a.rule, r.n, r.span, a.G, a.Hkv, a.few_limit, a.group_cols, a.group_slots, WIN ? kLeastUnits : 0);
     return r;
 }
 
@@ -672,10 +678,17 @@ __device__ __forceinline__ void wave_work(const PagedArgs &a, int first, int ste
         int b, h, s, blk, slot0 = 0;
         Row row;
         if constexpr (DIRECT) {
+            if (unit >= step) return;  // (one unit a wave)
             s = a.few_blocks > 1 ? unit / 16 * 8 + unit % 8 : unit;
             blk = a.few_blocks > 1 ? unit / 8 % 2 : 0;
             h = blockIdx.y;
             b = blockIdx.z;
+            // Rows with fewer splits than the grid has leave its last places idle: turned
+            // by row and head, these fall on all XCDs alike (64 rows of 5 splits in a grid
+            // of 8, the XCD's number in place of the split's: 39 us, unturned 49)
+            const int most = a.few_blocks > 1 ? gridDim.x / 2 : gridDim.x;
+            s += (h + b * a.Hkv) & 7;
+            while (s >= most) s -= most;
             row = lane_row(row_at<WIN>(a, b), 0);
             if (!few_columns(row.n, a.G, a.few_limit) || blk >= row.blocks || s >= row.splits) return;
         } else {
@@ -1736,12 +1749,23 @@ struct Plan {
     int slot_stride;  // (PagedArgs)
 };
 
-Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max_kv, bool q8) {
+Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max_kv, bool q8, int window, int sinks) {
     Plan p;
     const int G = Hq / Hkv, limit = few_limit(q8), chunk = limit / G + 1;  // tokens of the shortest chunk
     p.rule = wave_rule(Hq, Hkv, D, q8);
+    if (window) {
+        // One length for the call's rows, by what its window shows at most: then no row
+        // has more splits than a full window, and no grid's waves are left without work
+        // (us, at lengths by row / this: 64 rows of 512 keys 39 / 37, 48 of 4096 202 / 168,
+        // in 8 bits 48 of 1024 49 / 36).  Not by the windows past 4096, behind which many
+        // rows are shorter: one of 1500 keys would wait for 256 at a time.
+        const int span = window_span(4096, window, sinks, 1, G, 16);
+        p.rule = SplitRule{0, 0, 0, 0, p.rule.tokens(span)};
+    }
     p.few = chunk > 1 ? most_row_splits(p.rule, max_kv) : 1;
-    p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, limit, group_columns(D, q8), group_slots(D, q8)) : 1;
+    p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, limit, group_columns(D, q8), group_slots(D, q8),
+                                           window ? kLeastUnits : 0)
+                            : 1;
     const int64_t most = p.few > p.many ? p.few : p.many;
     const int64_t columns = (int64_t)max_q * G < limit ? (int64_t)max_q * G : limit;
     p.few_blocks = (int)(columns + 15) / 16;
@@ -1804,7 +1828,7 @@ size_t workspace_bytes_of(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t
         !sizes_fit(T, B, Hq, max_kv))
         return 0;
     const int span = most_span(Hq, Hkv, D, max_q, max_kv, q8 != 0, window, sinks);
-    const Plan p = paged_plan(T, B, Hq, Hkv, D, max_q, span, q8 != 0);
+    const Plan p = paged_plan(T, B, Hq, Hkv, D, max_q, span, q8 != 0, window, sinks);
     return p.slots && numbers_fit(p, T, B, Hq, Hkv, D, q8 != 0) ? part_bytes(p.slots, D) + (size_t)p.slots * 8 : 0;
 }
 
@@ -1824,7 +1848,7 @@ int attend(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int
     if (!sizes_fit(T, B, Hq, max_kv) || q_stride < (int64_t)Hq * D || out_stride < (int64_t)Hq * D) return KQ_ERR_BAD_SHAPE;
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_stride | out_stride) & 7)) return KQ_ERR_BAD_ALIGN;
     const int span = most_span(Hq, Hkv, D, max_q, max_kv, pool->k_scales != nullptr, window, sinks);
-    const Plan plan = paged_plan(T, B, Hq, Hkv, D, max_q, span, pool->k_scales != nullptr);
+    const Plan plan = paged_plan(T, B, Hq, Hkv, D, max_q, span, pool->k_scales != nullptr, window, sinks);
     const int64_t most = plan.few > plan.many ? plan.few : plan.many;
     if (!numbers_fit(plan, T, B, Hq, Hkv, D, pool->k_scales != nullptr)) return KQ_ERR_BAD_SHAPE;
     const size_t need = plan.slots ? part_bytes(plan.slots, D) + (size_t)plan.slots * 8 : 0;

@@ -1223,7 +1223,7 @@ def _paged_call(fn, device, *args):
     """One library call with `device` current (a launch goes to the current
     device, whichever the stream's is)."""
     f = getattr(lib(), fn)
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == device.index:  # (a tensor there has initialised CUDA)
         rc = f(*args)
     else:
         with torch.cuda.device(device):
