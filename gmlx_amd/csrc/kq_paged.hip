@@ -1757,10 +1757,10 @@ Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max
         // One length for the call's rows, by what its window shows at most: then no row
         // has more splits than a full window, and no grid's waves are left without work
         // (us, at lengths by row / this: 64 rows of 512 keys 39 / 37, 48 of 4096 202 / 168,
-        // in 8 bits 48 of 1024 49 / 36).  Not by the windows past 4096, behind which many
-        // rows are shorter: one of 1500 keys would wait for 256 at a time.
-        const int span = window_span(4096, window, sinks, 1, G, 16);
-        p.rule = SplitRule{0, 0, 0, 0, p.rule.tokens(span)};
+        // in 8 bits 48 of 1024 49 / 36).  Windows of up to 16384 keys as those of 4096, for
+        // many rows are shorter: one of 1500 keys would wait for 256 at a time.
+        const int span = window_span(1 << 30, window, sinks, 1, G, 16);
+        p.rule = SplitRule{0, 0, 0, 0, p.rule.tokens(span <= 16384 && span > 4096 ? 4096 : span)};
     }
     p.few = chunk > 1 ? most_row_splits(p.rule, max_kv) : 1;
     p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, limit, group_columns(D, q8), group_slots(D, q8),

@@ -184,6 +184,37 @@ def test_values_outside_the_window(n, kv, Hq, D, window, sinks, dt):
                 assert torch.equal(got[..., rest], clean[:n, half:][sees][..., rest])
 
 
+@pytest.mark.parametrize("D,q8", [(128, False), (128, True), (256, False), (512, False)])
+def test_pages_missing_in_the_window_and_among_the_sinks(D, q8):
+    """Their keys are not seen; where none is left, zeros."""
+    P, window, sinks = 16, 100, 40
+    b = Windowed([(1, 700), (3, 90), (60, 500), (1, 17)], 8, 2, D, P, F16, window, sinks, q8=q8, seed=D)
+    holes = {0: (0, 40), 1: (1, 3), 2: (2, 27, 30), 3: (0, 1)}
+    tab = b.table.cpu().numpy()
+    for row, pages in holes.items():
+        for p in pages:
+            tab[row, p] = -1 if p % 2 else 10 ** 6
+    b.table = torch.from_numpy(tab).cuda()
+    _say("holes", D, q8)
+    out = b.run().double().cpu().numpy()
+    for row, (n, kv) in enumerate(b.rows):
+        keep = np.array([t // P not in holes[row] for t in range(kv)])
+        for i in range(n):
+            me = kv - n + i
+            t = np.arange(kv)
+            see = keep & (t <= me) & ((t > me - window) | (t < sinks))
+            q = b.q[b.cu[row] + i:b.cu[row] + i + 1].double().numpy()
+            got = out[b.cu[row] + i]
+            if not see.any():
+                assert (got == 0).all()
+                continue
+            k, v = b.k[row][:, see], b.v[row][:, see]
+            err = np.maximum(b.err[row], np.abs(b.v[row]))[:, see]
+            want, far = ref.window_attention(q, k, v, 1, b.scale, 10 ** 6, 0, err)
+            # the output's and the probabilities' roundings, and 2^-16 for the 32-bit work of 140 keys
+            assert (np.abs(got - want[0]) <= HALF[F16] * (np.abs(want[0]) + 1.01 * far[0]) + 2.0 ** -16 * far[0] + 1e-7).all()
+
+
 def test_captured_steps_through_a_window():
     b = Windowed([(1, 900), (5, 400), (60, 300)], 8, 2, 128, 16, BF16, 100, 4, seed=4)
     q = b.q.cuda()
