@@ -1003,6 +1003,17 @@ __device__ __forceinline__ void pipelined(Read &&read, Use &&use) {
 template <bool BF>
 constexpr float slack() { return BF ? 8.f : 4.f; }
 
+// Which keys of a tile a lane's column sees, by their distance from the lane's
+// first key t: below lim, and through a window below sinks or from low on.
+struct Shown {
+    int end, sunk, from;
+    __device__ __forceinline__ Shown(int t, int lim, int sinks, int low) : end(lim - t), sunk(sinks - t), from(low - t) {}
+    template <bool WIN>
+    __device__ __forceinline__ bool at(int d) const {
+        return d < end && (!WIN || d < sunk || d >= from);
+    }
+};
+
 template <int D, bool BF, bool Q8>
 struct ChunkState {
     using C = Chunk<D, Q8>;
@@ -1056,13 +1067,18 @@ struct ChunkState {
             },
             [&](int x, const half8_t &f) { s[x % C::NT] = mfma32<BF>(f, qf[x / (C::NT * C::NP)], s[x % C::NT]); });
         if (masked) {
+            const Shown shown(t0 + 4 * h, lim, sinks, low);
 #pragma unroll
             for (int b = 0; b < C::NT; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int t = 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                    s[b][i] = t0 + t < lim && (!WIN || t0 + t < sinks || t0 + t >= low) && ((okbits >> (2 * b + (i >> 3))) & 1) ? s[b][i] : -INFINITY;
-                }
+                for (int i = 0; i < 16; ++i)
+                    s[b][i] = shown.template at<WIN>(32 * b + 8 * (i >> 2) + (i & 3)) ? s[b][i] : -INFINITY;
+            if (okbits != (1u << 2 * C::NT) - 1) {
+#pragma unroll
+                for (int b = 0; b < C::NT; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[b][i] = (okbits >> (2 * b + (i >> 3))) & 1 ? s[b][i] : -INFINITY;
+            }
         }
         float tmax = s[0][0];
 #pragma unroll
@@ -1156,13 +1172,12 @@ struct ChunkState16 {
             },
             [&](int x, const half8_t &f) { s[x % 2] = mfma<BF>(f, qf[x / (2 * C::NP)], s[x % 2]); });
         if (masked) {
+            const Shown shown(t0 + 4 * g, lim, sinks, low);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = t0 + 16 * b + 4 * g + i;
-                    s[b][i] = t < lim && (!WIN || t < sinks || t >= low) && ((okbits >> b) & 1) ? s[b][i] : -INFINITY;
-                }
+                for (int i = 0; i < 4; ++i)
+                    s[b][i] = shown.template at<WIN>(16 * b + i) && ((okbits >> b) & 1) ? s[b][i] : -INFINITY;
         }
         float tmax = max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
         tmax = max_over_groups(max3(max3(tmax, s[1][1], s[1][2]), s[1][3], s[1][3])) * scale_log2;
