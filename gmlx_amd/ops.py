@@ -28,8 +28,11 @@ blocks and prompt chunks over it.  A step, eager or captured (the state is then
 copied over in place, as here):
   p = paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_size, T, keep_lens=kept)
   seq_lens.copy_(p.kv_lens); free_count.copy_(p.free_count)
-  for each layer: paged_write(k, v, k_cache, v_cache, p.slots)
-                  o = sdpa_paged(q, k_cache, v_cache, block_table, p.kv_lens, p.cu_q, scale, max_q=, max_kv=)
+  for each layer: q = paged_write_rope(q, k, v, k_cache, v_cache, p.slots, p.positions, freqs, q_weight=, k_weight=)
+                  o = sdpa_paged(q, k_cache, v_cache, block_table, p.kv_lens, p.cu_q, scale, max_q=, max_kv=, window=)
+  r = verify_drafts(logits, tokens, p.cu_q, uniforms, draws, kv_lens=p.kv_lens)    # kept = r.keep_lens
+paged_write_rope is rope_qk (head norms and rotary positions) and paged_write in one
+launch; verify_drafts judges drafted tokens and draws the next one.
 """
 from __future__ import annotations
 
