@@ -10,6 +10,8 @@
 // pair j being y[j], y[j + R / 2], or with `interleaved` y[2 j], y[2 j + 1].  All
 // in fp32, rounded once; p f in 64 bits, of which the whole turns are taken off
 // before the 32-bit sine: a position of 10^6 in fp32 would be off by 0.03 radians.
+#include <algorithm>
+
 #include "kq_paged_store.h"
 
 namespace {
@@ -25,7 +27,11 @@ struct RopeArgs {
     float eps, factor;
     int32_t T, Hq, Hkv, rows;  // rows: heads of q, k and, where they are stored, v
     int32_t R, interleaved, weight_f32, lps;
+    int32_t tokens;  // of a workgroup that takes several
 };
+
+// The most tokens of a workgroup: 8 KB of sines and cosines.
+constexpr int most_tokens(int D) { return 2048 / D; }
 
 template <bool BF>
 __device__ __forceinline__ void unpack8(const u32x4 &v, float (&x)[8]) {
@@ -68,27 +74,33 @@ __device__ __forceinline__ float row_sum(float v) {
 // thread, and shared through LDS, and so are the weights (loaded where they are
 // used, behind the barrier, 8192 tokens took 40.5 us in place of 35.6).  A lane loads its pairs' other halves itself,
 // from the lines that its row's lanes have just asked for.  Rows are loaded before
-// any is stored, by the same wave, so outputs may be the inputs.
-template <int D, bool BF, bool Q8, bool WRITE, int PASSES>
+// any is stored, by the same wave, so outputs may be the inputs.  MANY: a.tokens
+// tokens of few heads share a workgroup (66425 tokens of 2 + 1 heads of 64 83 us
+// with one each, 21 so).
+template <int D, bool BF, bool Q8, bool WRITE, int PASSES, bool MANY>
 __global__ __launch_bounds__(256) void kq_rope_kernel(RopeArgs a) {
     constexpr int L = D / 8, LG = L <= 8 ? 8 : L <= 16 ? 16 : L <= 32 ? 32 : 64, RP = 256 / LG;
-    __shared__ __attribute__((aligned(16))) float cs[D / 2], sn[D / 2], weight[2][D];
-    const int t = blockIdx.x, pos = a.positions[t];
-    if (pos < 0) return;
+    constexpr int TOKENS = MANY ? most_tokens(D) : 1;
+    __shared__ __attribute__((aligned(16))) float cs[TOKENS * (D / 2)], sn[TOKENS * (D / 2)], weight[2][D];
+    const int t0 = MANY ? blockIdx.x * a.tokens : blockIdx.x;
+    const int tokens = MANY ? min(a.tokens, a.T - t0) : 1;
+    if (!MANY && a.positions[t0] < 0) return;
     const int c = threadIdx.x % LG, row0 = blockIdx.y * (RP * PASSES) + threadIdx.x / LG;
     const int half = a.R / 2;
     // where this lane's pairs' other halves lie: in itself, or half the rotated part away
     const bool turned = 8 * c < a.R, apart = turned && !a.interleaved, low = 8 * c < half;
     const int other = !apart ? c : low ? c + half / 8 : c - half / 8;
     u32x4 v[PASSES], vo[PASSES];
-    int which[PASSES], head[PASSES];
+    int which[PASSES], head[PASSES], at[PASSES];  // at: the token's number in the workgroup, -1: no row
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-        const int row = row0 + p * RP;
+        const int item = row0 + p * RP, nth = MANY ? item / a.rows : 0, row = item - nth * a.rows;
+        const int t = t0 + nth;
+        at[p] = !MANY || (nth < tokens && a.positions[t] >= 0) ? nth : -1;
         which[p] = row < a.Hq ? 0 : row < a.Hq + a.Hkv ? 1 : 2;
         head[p] = row - (which[p] == 0 ? 0 : which[p] == 1 ? a.Hq : a.Hq + a.Hkv);
         v[p] = vo[p] = u32x4{0u, 0u, 0u, 0u};
-        if (row < a.rows && c < L) {
+        if ((MANY ? at[p] >= 0 : row < a.rows) && c < L) {
             const uint16_t *x = which[p] == 0   ? a.src[0] + t * a.token_stride[0] + head[p] * a.head_stride[0]
                                 : which[p] == 1 ? a.src[1] + t * a.token_stride[1] + head[p] * a.head_stride[1]
                                                 : a.src[2] + t * a.token_stride[2] + head[p] * a.head_stride[2];
@@ -102,30 +114,38 @@ __global__ __launch_bounds__(256) void kq_rope_kernel(RopeArgs a) {
         if (const void *w = i < D ? a.weight[0] : a.weight[1])
             weight[i / D][d] = a.weight_f32 ? ((const float *)w)[d] : f16bits_to_f32<BF>(((const uint16_t *)w)[d]);
     }
-    if ((int)threadIdx.x < half) {
-        const double turns = (double)pos * a.freqs[threadIdx.x] * 0.15915494309189533577;
+    for (int i = threadIdx.x; i < tokens * half; i += 256) {
+        const int nth = MANY ? i / half : 0;
+        const double turns = (double)a.positions[t0 + nth] * a.freqs[i - nth * half] * 0.15915494309189533577;
         float s, co;
         sincospif(2.f * (float)(turns - rint(turns)), &s, &co);
-        cs[threadIdx.x] = co * a.factor;
-        sn[threadIdx.x] = s * a.factor;
+        cs[i] = co * a.factor;
+        sn[i] = s * a.factor;
     }
     __syncthreads();
     // a value becomes itself times its cosine plus its pair's other times +-its sine
     float co[8], si[8];
-    if (turned) {
-        const int j = a.interleaved ? 4 * c : low ? 8 * c : 8 * c - half;
+    const auto turn = [&](int nth) {
+        if (!turned) return;
+        const int j = nth * half + (a.interleaved ? 4 * c : low ? 8 * c : 8 * c - half);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int k = j + (a.interleaved ? i / 2 : i);
             co[i] = cs[k];
             si[i] = (a.interleaved ? i % 2 == 0 : low) ? -sn[k] : sn[k];
         }
-    }
-    const int slot = WRITE ? a.slots[t] : 0;
+    };
+    if constexpr (!MANY) turn(0);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-        const int row = row0 + p * RP;
-        if (row >= a.rows) break;  // (uniform over a row's lanes, as all below is)
+        // (uniform over a row's lanes, as all below is)
+        if constexpr (MANY) {
+            if (at[p] < 0) continue;
+        } else {
+            if (row0 + p * RP >= a.rows) break;
+        }
+        const int t = t0 + at[p];
+        if constexpr (MANY) turn(at[p]);
         u32x4 out = v[p];
         if (which[p] < 2) {
             float x[8], xo[8];
@@ -174,27 +194,32 @@ __global__ __launch_bounds__(256) void kq_rope_kernel(RopeArgs a) {
                 *(u32x4 *)(y + 8 * c) = out;
             }
         } else {
-            const int64_t to = slot_offset(a.pool, a.lps, slot, head[p]);
+            const int64_t to = slot_offset(a.pool, a.lps, a.slots[t], head[p]);
             if (to >= 0 && c < L) store_values<BF, Q8>(a.pool, which[p] - 1, to, c, out);
         }
     }
 }
 
-template <int D, bool BF, bool Q8, bool WRITE, int PASSES>
-void launch_passes(const RopeArgs &a, hipStream_t s) {
-    constexpr int L = D / 8, LG = L <= 8 ? 8 : L <= 16 ? 16 : L <= 32 ? 32 : 64, RP = 256 / LG * PASSES;
-    hipLaunchKernelGGL((kq_rope_kernel<D, BF, Q8, WRITE, PASSES>), dim3(a.T, (a.rows + RP - 1) / RP), dim3(256), 0, s, a);
-}
-
 template <int D, bool BF, bool Q8, bool WRITE>
-void launch(const RopeArgs &a, hipStream_t s) {
+void launch(RopeArgs a, hipStream_t s) {
+    constexpr int L = D / 8, LG = L <= 8 ? 8 : L <= 16 ? 16 : L <= 32 ? 32 : 64, RP = 256 / LG;
+    const int groups = (a.rows + RP - 1) / RP, groups3 = (a.rows + 3 * RP - 1) / (3 * RP);
     // Three passes where one would give the GPU four workgroups a CU (us with 1 / 2 / 3
     // passes, 32 + 8 heads of 128: 33 tokens 4.9 / 5.0 / 5.1, 128 4.8 / 5.1 / 5.2, 512 5.7 /
     // 5.7 / 5.8, 1024 9.1 / 7.8 / 8.0, 2048 14.1 / 13.4 / 12.9, 8192 45.5 / 42.3 / 35.6; a
-    // copy of 2048 tokens' bytes 7.6, of 8192 33.7)
-    constexpr int L = D / 8, LG = L <= 8 ? 8 : L <= 16 ? 16 : L <= 32 ? 32 : 64, RP = 256 / LG;
-    if ((int64_t)a.T * ((a.rows + RP - 1) / RP) < 1024) launch_passes<D, BF, Q8, WRITE, 1>(a, s);
-    else launch_passes<D, BF, Q8, WRITE, 3>(a, s);
+    // copy of 2048 tokens' bytes 7.6, of 8192 33.7).  Three tokens or more a workgroup
+    // where they fit these passes and leave 1024 workgroups (one / several, 20000
+    // tokens of 4 + 1 heads of 128 36 / 20, 10000 of 8 + 1 22 / 16; but two each, 4097 of 16
+    // + 4 14.1 / 15.0, and 1100 of 4 + 4 of 64, which 92 would take, 5.4 / 5.9).
+    if ((int64_t)a.T * groups < 1024) {
+        hipLaunchKernelGGL((kq_rope_kernel<D, BF, Q8, WRITE, 1, false>), dim3(a.T, groups), dim3(256), 0, s, a);
+        return;
+    }
+    a.tokens = std::min({3 * RP / a.rows, most_tokens(D), a.T / 1024});
+    if (a.tokens > 2)
+        hipLaunchKernelGGL((kq_rope_kernel<D, BF, Q8, WRITE, 3, true>), dim3((a.T + a.tokens - 1) / a.tokens), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((kq_rope_kernel<D, BF, Q8, WRITE, 3, false>), dim3(a.T, groups3), dim3(256), 0, s, a);
 }
 
 template <int D, bool BF>

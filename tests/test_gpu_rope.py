@@ -38,7 +38,10 @@ CASES = [  # T, Hq, Hkv, D, R, interleaved, norm
     (5, 3, 1, 96, 96, True, False), (33, 16, 2, 256, 64, False, True), (2, 5, 5, 512, 512, False, True),
     (9, 8, 1, 512, 16, True, True), (130, 7, 2, 128, 112, False, False), (515, 6, 2, 128, 128, False, True),
     (777, 9, 4, 64, 32, True, True), (600, 4, 2, 256, 256, True, True), (513, 3, 1, 512, 256, False, True),
-    (514, 20, 4, 96, 96, False, True)]
+    (514, 20, 4, 96, 96, False, True),
+    # several tokens a workgroup: a last one of few, a lone head, one token too many for the passes
+    (9001, 2, 1, 64, 64, False, True), (7003, 1, 0, 128, 128, True, True), (4099, 5, 1, 256, 128, False, False),
+    (3085, 2, 1, 512, 512, False, True), (4100, 7, 1, 96, 64, True, True), (4111, 16, 8, 128, 128, False, True)]
 
 
 @pytest.mark.parametrize("dt", [F16, BF16])
@@ -140,7 +143,8 @@ def _pool(n, H, P, D, dt, q8, token_layout):
     (1, 32, 8, 128, 128, False, 16, False, False), (37, 16, 2, 256, 64, True, 32, True, False),
     (520, 6, 3, 96, 32, False, 64, False, True), (600, 4, 1, 64, 64, False, 128, True, False),
     (19, 3, 1, 512, 512, True, 16, True, False), (700, 8, 2, 128, 128, False, 1024, True, False),
-    (5, 0, 2, 128, 64, False, 16, False, False)])
+    (5, 0, 2, 128, 64, False, 16, False, False), (6500, 2, 1, 64, 64, False, 32, False, False),
+    (4201, 4, 2, 128, 128, True, 16, True, False), (3077, 1, 1, 512, 256, False, 64, False, True)])
 def test_write_rope_is_the_two_calls(T, Hq, Hkv, D, R, interleaved, P, q8, token_layout, dt):
     from gmlx_amd import ops
     gen = torch.Generator(device="cuda").manual_seed(T + D)
