@@ -35,6 +35,7 @@ struct VerifyArgs {
     Part *part;    // [T][S]
     double *rest;  // [B][S]: sums of max(e - q Z, 0)
     struct Verdict *verdict;  // [B], NULL: found by the last kernel
+    int32_t decides;  // the rest's kernel finds the verdicts
     int32_t *accepted, *next, *keep;
 };
 
@@ -364,35 +365,50 @@ __global__ __launch_bounds__(kThreads) void kq_verify_decide_kernel(VerifyArgs a
     if (threadIdx.x == 0) a.verdict[b] = r;
 }
 
-// Sums of max(e - q Z, 0) over one slice a wave, of rows whose draft was refused.
+// The sum of max(e - q Z, 0) over a slice, by a wave.
 template <int DT, int PT>
-__global__ __launch_bounds__(kThreads) void kq_verify_rest_kernel(VerifyArgs a) {
+__device__ __forceinline__ double rest_sum(const VerifyArgs &a, const Verdict &r, double rate, int s) {
     constexpr int N = kValues<DT>;
-    const int lane = kq_lane(), b = blockIdx.y;
-    const int s = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-    int q0, n;
-    if (s >= a.S || !row_of(a, b, q0, n) || n < 2) return;
-    const Verdict r = a.verdict[b];
-    if (r.accepted == n - 1 || greedy(a, b) || !(r.m > -INFINITY)) return;
-    const double rate = rate_of(a, b);
     double sum = 0.0;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
         double w[N];
-        rest_of<DT, PT, N>(a, r, rate, min(((s * kChunks + c) * 64 + lane) * N, a.V), w);
+        rest_of<DT, PT, N>(a, r, rate, min(((s * kChunks + c) * 64 + kq_lane()) * N, a.V), w);
 #pragma unroll
         for (int j = 0; j < N; ++j) sum += w[j];
     }
-    sum = wave_sum(sum);
-    if (lane == 0) a.rest[(int64_t)b * a.S + s] = sum;
+    return wave_sum(sum);
 }
+
+// These sums of every slice, a wave each, of rows whose draft was refused.  decides:
+// every workgroup finds for itself where its row ends.
+template <int DT, int PT>
+__global__ __launch_bounds__(kThreads) void kq_verify_rest_kernel(VerifyArgs a) {
+    const int b = blockIdx.y, s = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+    int q0, n;
+    if (!row_of(a, b, q0, n)) return;
+    const Verdict r = a.decides ? decide<DT>(a, b, q0, n) : a.verdict[b];
+    if (a.decides && blockIdx.x == 0 && threadIdx.x == 0) a.verdict[b] = r;
+    if (s >= a.S || r.accepted == n - 1 || greedy(a, b) || !(r.m > -INFINITY)) return;
+    const double sum = rest_sum<DT, PT>(a, r, rate_of(a, b), s);
+    if (kq_lane() == 0) a.rest[(int64_t)b * a.S + s] = sum;
+}
+
+// The most slices of a row whose last kernel sums the rest beside q itself, two
+// rounds of its waves, in place of two launches before it (us of the kernels: 4
+// slices 12 in place of 17, 8 20 in place of 20, 16 27 in place of 19).
+constexpr int kFewSlices = 8;
+// The most workgroups of the rest's kernel that find their rows' ends each, in
+// place of a launch (one row of 64 slices 8 us in place of 5 and 6, eight 11 in place
+// of 5 and 9; 96 rows of 75 30 in place of 6 and 16).
+constexpr int kDecide = 512;
 
 // The token that follows, one workgroup a row: the slice whose running sum passes
 // r times the whole, then the token within it.
 template <int DT, int PT>
 __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) {
     constexpr int N = kValues<DT>;
-    __shared__ double red[kWaves];
+    __shared__ double red[kWaves], s_rest[kFewSlices];
     __shared__ double s_target;
     __shared__ int s_how, s_slice, s_first, s_last;
     const int b = blockIdx.x, lane = kq_lane(), wv = threadIdx.x >> 6;
@@ -455,10 +471,17 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
     }
     // wave 0: the slices' running sums
     int how = lone ? 1 : refused && a.probs ? 2 : 0;
+    if (how == 2 && !a.verdict) {
+        for (int s = wv; s < a.S; s += kWaves) {
+            const double sum = rest_sum<DT, PT>(a, r, rate, s);
+            if (lane == 0) s_rest[s] = sum;
+        }
+        __syncthreads();
+    }
     if (wv == 0) {
         const auto slice_sum = [&](int s) {
             if (s >= a.S) return 0.0;
-            return how == 2 ? a.rest[(int64_t)b * a.S + s]
+            return how == 2 ? (a.verdict ? a.rest[(int64_t)b * a.S + s] : s_rest[s])
                    : s == own && how == 1 ? without
                                           : part[s].sum * weight0(part[s].m, r.m, rate);
         };
@@ -540,7 +563,7 @@ template <int DT, int PT>
 void launch(const VerifyArgs &a, hipStream_t s) {
     if (a.T) hipLaunchKernelGGL((kq_verify_rows_kernel<DT>), dim3((a.T * a.S + kWaves - 1) / kWaves), dim3(kThreads), 0, s, a);
     if (a.verdict) {
-        hipLaunchKernelGGL((kq_verify_decide_kernel<DT>), dim3(a.B), dim3(kThreads), 0, s, a);
+        if (!a.decides) hipLaunchKernelGGL((kq_verify_decide_kernel<DT>), dim3(a.B), dim3(kThreads), 0, s, a);
         hipLaunchKernelGGL((kq_verify_rest_kernel<DT, PT>), dim3((a.S + kWaves - 1) / kWaves, a.B), dim3(kThreads), 0, s, a);
     }
     hipLaunchKernelGGL((kq_verify_pick_kernel<DT, PT>), dim3(a.B), dim3(kThreads), 0, s, a);
@@ -603,7 +626,8 @@ int kq_verify_drafts(const void *logits, int dtype, int64_t row_stride, const in
     a.S = S;
     a.probs_type = probs_dtype;
     a.part = (Part *)workspace;
-    const bool with_rest = draft_probs && T && !greedy_all;
+    const bool with_rest = draft_probs && T && !greedy_all && S > kFewSlices;
+    a.decides = (int64_t)B * ((S + kWaves - 1) / kWaves) <= kDecide;
     a.verdict = with_rest ? (Verdict *)((char *)workspace + part_bytes(T, S)) : nullptr;
     a.rest = with_rest ? (double *)(a.verdict + B) : nullptr;
     a.accepted = accepted;
