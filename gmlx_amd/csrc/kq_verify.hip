@@ -9,7 +9,7 @@
 // where d alone was proposed) behind a refused draft, e behind the last.
 //
 // A running sum over V tokens has V borders that r may fall next to, so weights
-// and sums are fp64: 2 10^-16 each, where fp32's 10^-7 would put one draw in a
+// (good to 4 10^-14) and sums are fp64, where fp32's 10^-7 would put one draw in a
 // hundred on the other side of some border at V = 10^5.
 #include "kq_attn.h"
 
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
     const int own = lone ? r.draft / (kThreads * N) : -1;
     double without = 0.0;
     if (lone) {
-        const double all = part[own].sum * weight(part[own].m, r.m, rate);
+        const double all = part[own].sum * weight0(part[own].m, r.m, rate);
         without = all - weight0(r.x, r.m, rate);
         if (!(without > 0x1p-20 * all)) {
             weigh(1, own);

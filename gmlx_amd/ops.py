@@ -1651,7 +1651,7 @@ def rope_qk(q, k, positions, freqs, q_weight=None, k_weight=None, eps=1e-6, inte
     to D; positions int32 [T] on the device (PagedPlan.positions).  A token of
     negative position is left out: its rows of q_out and k_out stay as they were
     (unspecified where they are not given).  float16 or bfloat16, D in 64, 96, 128,
-    256, 512; q and k may be views of a packed q|k|v (strides of 8 values).  q_out /
+    256, 512, up to 2^23 tokens; q and k may be views of a packed q|k|v (strides of 8 values).  q_out /
     k_out: where the results go, also q and k themselves (their own views), else no
     part of an input."""
     _fault("rope_qk")

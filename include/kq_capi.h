@@ -652,7 +652,7 @@ int kq_paged_write_rope(const kq_paged_pool *pool, const kq_rope *rope, const in
  * keep_lens[b] (may be NULL): kv_lens[b] less the refused drafts, what
  * kq_paged_plan keeps of a row whose kv_lens count all n tokens.
  *
- * Weights and sums in fp64.  NaN counts as -infinity, +infinity as the largest
+ * Weights (good to 4 10^-14) and sums in fp64.  NaN counts as -infinity, +infinity as the largest
  * fp32; probabilities below 0 and NaN as 0; drafts outside 0 .. V - 1 do not stand.
  * A row without logits has 0 and -1; one of nothing above -infinity ends there,
  * with -1.

@@ -174,6 +174,26 @@ def test_write_rope_is_the_two_calls(T, Hq, Hkv, D, R, interleaved, P, q8, token
         assert torch.equal(bits(a), bits(b))
 
 
+@pytest.mark.parametrize("T", [3, 2000, 9001])
+def test_write_rope_in_place(T):
+    """The queries rotated where they lie, beside the keys and values that are read."""
+    from gmlx_amd import ops
+    torch.manual_seed(T)
+    Hq, Hkv, D, P = (32, 8, 128, 16) if T < 9000 else (2, 1, 64, 16)
+    packed = torch.randn(T, Hq + 2 * Hkv, D, device="cuda").half()
+    q, k, v = packed[:, :Hq], packed[:, Hq:Hq + Hkv], packed[:, Hq + Hkv:]
+    kv = packed[:, Hq:].clone()
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    slots, w = pos.clone(), torch.randn(D, device="cuda")
+    freqs = _freqs(D)
+    (a, b), _ = _pool(-(-T // P), Hkv, P, D, F16, False, True)
+    (c, d), _ = _pool(-(-T // P), Hkv, P, D, F16, False, True)
+    want = ops.paged_write_rope(q, k, v, a, b, slots, pos, freqs, q_weight=w, k_weight=w)
+    got = ops.paged_write_rope(q, k, v, c, d, slots, pos, freqs, q_weight=w, k_weight=w, q_out=q)
+    assert got is q and torch.equal(q, want) and torch.equal(a, c) and torch.equal(b, d)
+    assert torch.equal(packed[:, Hq:], kv)
+
+
 def test_captured_and_on_another_stream():
     from gmlx_amd import ops
     torch.manual_seed(3)

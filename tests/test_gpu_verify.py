@@ -119,6 +119,18 @@ def test_draws_at_the_ends(pt):
                 assert got.accepted.tolist() == _want(c)[0] and all(0 <= t < 2500 for t in got.tokens.tolist())
 
 
+def test_a_refused_draft_without_weight_takes_none_along():
+    """A draft, and all its slice, below any weight: a draw of 1 ends before them."""
+    from gmlx_amd import ops
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    x = torch.zeros(2, 5000, device="cuda").bfloat16()
+    x[:, 4096:] = -10000.0
+    f = lambda *v: torch.tensor(v, device="cuda")  # noqa: E731
+    for draw, want in ((1.0, 4095), (0.5, 2048), (2.0, 4095)):
+        r = ops.verify_drafts(x, i32(0, 4500), i32(0, 2), f(0.0, 0.0), f(draw))
+        assert (r.accepted.tolist(), r.tokens.tolist()) == ([0], [want])
+
+
 def test_logits_and_probabilities_that_are_not_finite():
     nan, inf = float("nan"), float("inf")
     for temp in (1.0, 0.0, 0.5):
@@ -198,6 +210,23 @@ def test_padding_strides_and_the_same_bits_again():
     _check(c)
     c["logits"] = c["logits"].t().contiguous().t()  # columns together: copied
     _check(c)
+
+
+def test_logits_past_32_bits_of_bytes():
+    """Rows whose byte offsets pass 2^32, many of them."""
+    from gmlx_amd import ops
+    T, V = 15000, 152064
+    x = torch.zeros(T, V, dtype=F16, device="cuda")
+    at = (torch.arange(T, device="cuda") * 7919) % V
+    x[torch.arange(T, device="cuda"), at] = 30.0
+    cu = torch.arange(T + 1, dtype=torch.int32, device="cuda")
+    tokens = torch.zeros(T, dtype=torch.int32, device="cuda")
+    _say("past 32 bits")
+    r = ops.verify_drafts(x, tokens, cu, temperature=0)
+    assert torch.equal(r.tokens.long(), at)
+    # (30 above the rest of V: 1 - V e^-30 of the weight)
+    r = ops.verify_drafts(x, tokens, cu, torch.zeros(T, device="cuda"), torch.full((T,), 0.5, device="cuda"))
+    assert torch.equal(r.tokens.long(), at)
 
 
 def test_no_rows():

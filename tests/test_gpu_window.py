@@ -215,6 +215,26 @@ def test_pages_missing_in_the_window_and_among_the_sinks(D, q8):
             assert (np.abs(got - want[0]) <= HALF[F16] * (np.abs(want[0]) + 1.01 * far[0]) + 2.0 ** -16 * far[0] + 1e-7).all()
 
 
+@pytest.mark.parametrize("D,q8", [(128, False), (128, True), (256, False), (512, False)])
+def test_output_in_place_and_rows_behind_the_last(D, q8):
+    """The output may be the queries; rows behind the last sequence stay as they were."""
+    b = Windowed([(1, 700), (0, 30), (70, 500), (2, 64), (0, 0)], 8, 2, D, 16, BF16, 90, 4, q8=q8, seed=D, pad=3)
+    q = b.q.cuda()
+    q[b.T:] = float("nan")
+    want = b.run(q=q.clone(), out=torch.full_like(q, 7.0))
+    assert (want[b.T:] == 7).all()
+    b.check(want)
+    got = b.run(q=q, out=q)
+    assert got is q and torch.equal(q[:b.T], want[:b.T]) and torch.isnan(q[b.T:]).all()
+    # strided queries and output
+    wide = torch.full((b.T + 3, 8 * D + 64), 5.0, device="cuda").to(BF16)
+    src = torch.zeros(b.T + 3, 8 * D + 8, device="cuda").to(BF16)
+    src[:, :8 * D] = b.q.cuda().view(b.T + 3, -1)
+    out = wide[:, 64:].view(b.T + 3, 8, D)
+    b.run(q=src[:, :8 * D].view(b.T + 3, 8, D), out=out)
+    assert torch.equal(out[:b.T], want[:b.T]) and (wide[:, :64] == 5).all() and (out[b.T:] == 5).all()
+
+
 def test_captured_steps_through_a_window():
     b = Windowed([(1, 900), (5, 400), (60, 300)], 8, 2, 128, 16, BF16, 100, 4, seed=4)
     q = b.q.cuda()
