@@ -395,13 +395,15 @@ __global__ __launch_bounds__(kThreads) void kq_verify_rest_kernel(VerifyArgs a) 
 }
 
 // The most slices of a row whose last kernel sums the rest beside q itself, two
-// rounds of its waves, in place of two launches before it (us of the kernels: 4
-// slices 12 in place of 17, 8 20 in place of 20, 16 27 in place of 19).
+// rounds of its waves, in place of a launch before it (us behind the rows' kernel,
+// 128 rows of 4 drafts: 4 slices 15 in place of 18, 8 19.5 in place of 18.5 and that
+// launch, 12 23 in place of 19, 15 27 in place of 19).
 constexpr int kFewSlices = 8;
 // The most workgroups of the rest's kernel that find their rows' ends each, in
-// place of a launch (one row of 64 slices 8 us in place of 5 and 6, eight 11 in place
-// of 5 and 9; 96 rows of 75 30 in place of 6 and 16).
-constexpr int kDecide = 512;
+// place of a launch (us, rows of 64 slices, 4 drafts: 1 row 4.7 in place of 3.7 and
+// 2.3, 48 11.7 in place of 4.9 and 9.5, 96 16.5 in place of 5.3 and 12.7; 128, 2048
+// workgroups, 20.6 in place of 5.2 and 15.0, 160 24.7 in place of 5.2 and 16.6).
+constexpr int kDecide = 1536;
 
 // The token that follows, one workgroup a row: the slice whose running sum passes
 // r times the whole, then the token within it.

@@ -70,6 +70,14 @@ def test_a_large_batch_takes_long_slices():
         _check(_case(rng.integers(1, 4, B).tolist(), V, dt, pt, B))
 
 
+@pytest.mark.parametrize("B", [512, 513])
+def test_rows_at_the_border_of_a_launch(B):
+    """9 slices, 3 workgroups a row: 1536 find their rows' ends themselves, 1539 do not."""
+    ns = np.random.default_rng(B).integers(0, 4, B).tolist()
+    _say("border", B)
+    _check(_case(ns, 9001, F32, F32, B, near=2.0))
+
+
 def test_drafts_of_all_kinds_of_agreement():
     """Models that agree (all stand) and that do not (the first falls), long drafts."""
     for near, spread in ((0.0, 4.0), (8.0, 4.0), (0.1, 0.0)):
