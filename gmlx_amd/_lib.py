@@ -217,7 +217,7 @@ _SIGS = {
     "kq_rope_qk": ([_vp, _vp, _i32, _i32, _int, _vp, _vp, _vp], _int),
     "kq_paged_write_rope": ([_vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp], _int),
     "kq_verify_workspace_bytes": ([_i32, _i32, _i32, _int, _int], _sz),
-    "kq_verify_drafts": ([_vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _int, _i64, _vp, _f32, _vp, _i32, _i32, _i32, _vp,
+    "kq_verify_drafts": ([_vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _int, _i64, _vp, ctypes.c_double, _vp, _i32, _i32, _i32, _vp,
                           _vp, _vp, _vp, _sz, _vp], _int),
     "kq_gguf_open": ([ctypes.c_char_p, ctypes.POINTER(_vp)], _int),
     "kq_gguf_close": ([_vp], None),

@@ -1735,8 +1735,8 @@ def verify_drafts(logits, tokens, cu, uniforms=None, draws=None, draft_probs=Non
     the drafts that are it.
 
     uniforms float32 [T] and draws float32 [B] in [0, 1), not needed where the
-    temperature is 0; temperature a number, or float32 [B] on the device (0 or below:
-    greedy); cu int32 [B + 1]; kv_lens int32 [B] (PagedPlan.kv_lens, all n tokens of
+    temperature is 0; temperature a number (taken in 64 bits), or float32 [B] on the
+    device (0 or below: greedy); cu int32 [B + 1]; kv_lens int32 [B] (PagedPlan.kv_lens, all n tokens of
     the row counted) for keep_lens, which paged_plan takes.  Returns a DraftVerdict.
 
     Computed in 64 bits.  NaN logits count as -inf, +inf as the largest float32,
@@ -1760,9 +1760,8 @@ def verify_drafts(logits, tokens, cu, uniforms=None, draws=None, draft_probs=Non
         temps = _floats(temperature, "temperature", B, dev)
     else:
         temp = float(temperature)
-        if not 0 <= temp < 3.4e38:
+        if not 0 <= temp < math.inf:
             raise ValueError(f"verify_drafts: a temperature of 0 or more, got {temperature}")
-        temp = max(temp, 1e-45) if temp else 0.0  # (not 0 in float32)
     if (uniforms is None or draws is None) and not (temps is None and temp == 0):
         raise ValueError("verify_drafts: uniforms and draws are needed unless the temperature is 0")
     u = None if uniforms is None else _floats(uniforms, "uniforms", T, dev)

@@ -652,21 +652,22 @@ int kq_paged_write_rope(const kq_paged_pool *pool, const kq_rope *rope, const in
  * keep_lens[b] (may be NULL): kv_lens[b] less the refused drafts, what
  * kq_paged_plan keeps of a row whose kv_lens count all n tokens.
  *
- * Weights (good to 4 10^-14) and sums in fp64.  NaN counts as -infinity, +infinity as the largest
- * fp32; probabilities below 0 and NaN as 0; drafts outside 0 .. V - 1 do not stand.
+ * Weights (good to 4 10^-14; below 2^-1000 none) and sums in fp64.  NaN counts as
+ * -infinity, +infinity as the largest fp32; probabilities below 0 and NaN as 0; drafts
+ * outside 0 .. V - 1 do not stand.
  * A row without logits has 0 and -1; one of nothing above -infinity ends there,
  * with -1.
  *
- * temperatures: fp32 [B] on the device, or NULL and `temperature` (finite, >= 0) for
- * all.  uniforms [T] and draws [B] fp32 in [0, 1) (may be NULL where temperature is
- * 0 for all).  T up to 2^22, B below 2^16, V up to 2^28, and at most 2^24 slices
- * of 4096 bytes in the rows together.  Workspace: kq_verify_workspace_bytes, no
- * zero-fill needed, 256-byte aligned; calls that share one are ordered.  Nothing
- * is read of logits past cu_rows[B]. */
+ * temperatures: fp32 [B] on the device, or NULL and `temperature` (finite, >= 0; taken
+ * in fp64, as 0.7 is no fp32 number) for all.  uniforms [T] and draws [B] fp32 in
+ * [0, 1) (may be NULL where temperature is 0 for all).  T up to 2^22, B below 2^16, V
+ * up to 2^28, and at most 2^24 slices of 4096 bytes in the rows together.
+ * Workspace: kq_verify_workspace_bytes, no zero-fill needed, 256-byte aligned; calls
+ * that share one are ordered.  Nothing is read of logits past cu_rows[B]. */
 size_t kq_verify_workspace_bytes(int32_t T, int32_t B, int32_t V, int dtype, int with_probs);
 int kq_verify_drafts(const void *logits, int dtype, int64_t row_stride, const int32_t *tokens, const int32_t *cu_rows,
                      const float *uniforms, const float *draws, const void *draft_probs, int probs_dtype,
-                     int64_t probs_row_stride, const float *temperatures, float temperature, const int32_t *kv_lens,
+                     int64_t probs_row_stride, const float *temperatures, double temperature, const int32_t *kv_lens,
                      int32_t T, int32_t B, int32_t V, int32_t *accepted, int32_t *next_tokens, int32_t *keep_lens,
                      void *workspace, size_t workspace_bytes, kq_stream_t stream);
 

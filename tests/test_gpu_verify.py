@@ -87,6 +87,67 @@ def test_drafts_of_all_kinds_of_agreement():
             assert got.accepted.tolist() == [69, 0, 129, 5]
 
 
+# A border and a draw that is further than this from it (of the whole): weights good to 4e-14, two of them in a quotient,
+# and some 200 roundings of 2^-53 in a running sum of the kernel's come to 1.1e-13; the references below are in 80 bits.
+_APART = np.longdouble(1e-12)
+
+
+@pytest.mark.parametrize("temp", [0.7, 0.8])
+def test_draws_at_a_temperature_that_32_bits_do_not_hold(temp):
+    """60000 draws from one flat row: with the temperature rounded to 32 bits, off by 1.7e-8 and 1.5e-8 of itself, weights
+    are off by that times their distance from the largest, and some ten draws fall on another side of some border."""
+    from gmlx_amd import ops
+    B, V = 60000, 152064
+    rng = np.random.default_rng(int(10 * temp))
+    x = torch.from_numpy(rng.normal(0, 3, V)).half()
+    draws = rng.random(B).astype(np.float32)
+    w = x.numpy().astype(np.longdouble)
+    w = np.exp((w - w.max()) / np.longdouble(temp))
+    run = np.cumsum(w)
+    at = draws.astype(np.longdouble) * run[-1]
+    want = np.searchsorted(run, at, side="right")
+    near = np.minimum(np.abs(run[want] - at), np.abs(run[np.maximum(want - 1, 0)] - at)) < _APART * run[-1]
+    assert near.sum() < 10
+    _say("draws", temp, int(near.sum()), "left out")
+    r = ops.verify_drafts(x.cuda()[None].expand(B, V), torch.zeros(B, dtype=torch.int32, device="cuda"),
+                          torch.arange(B + 1, dtype=torch.int32, device="cuda"), torch.zeros(B, device="cuda"),
+                          torch.from_numpy(draws).cuda(), temperature=temp)
+    got = r.tokens.cpu().numpy()
+    assert np.array_equal(got[~near], want[~near]), int((got != want).sum())
+
+
+@pytest.mark.parametrize("temp", [0.6, 0.7, 0.8, 1.0])
+def test_drafts_whose_uniform_is_the_nearest_number_to_their_border(temp):
+    """u is p_d rounded to 32 bits, above or below it by up to 6e-8 of it; weights off by 2e-8 times a distance of some
+    ten logits would judge many of them the other way."""
+    from gmlx_amd import ops
+    n, V = 400, 1000
+    rng = np.random.default_rng(7)
+    x = torch.from_numpy(rng.normal(0, 3, (n, V))).half()
+    d = rng.integers(0, V, n)
+    w = x.numpy().astype(np.longdouble)
+    w = np.exp((w - w.max(1, keepdims=True)) / np.longdouble(temp))
+    p = w[np.arange(n), d] / w.sum(1)
+    u = p.astype(np.float32)
+    kept = (np.abs(u - p) > _APART * p) & (u > 1e-30)
+    assert kept.sum() > 0.9 * n
+    tokens, uniforms = np.zeros((n, 2), np.int32), np.zeros((n, 2), np.float32)
+    tokens[:, 1], uniforms[:, 0] = d, u
+    r = ops.verify_drafts(x.cuda().repeat_interleave(2, 0), torch.from_numpy(tokens.reshape(-1)).cuda(),
+                          torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device="cuda"),
+                          torch.from_numpy(uniforms.reshape(-1)).cuda(), torch.full((n,), 0.5, device="cuda"), temperature=temp)
+    got = r.accepted.cpu().numpy()
+    assert np.array_equal(got[kept], (u < p).astype(np.int32)[kept]), int((got != (u < p)).sum())
+
+
+@pytest.mark.parametrize("temp", [1e-310, 1e-60, 1e-40, 1e39, 1e60, 1e308])
+def test_temperatures_past_the_ends_of_32_bits(temp):
+    for dt, pt, near in ((F16, None, 0.5), (F32, F32, 0.01)):
+        c = _case([4, 3, 1, 5, 2, 6], 5000, dt, pt, 12, near=near)
+        c["temperature"] = temp
+        _check(c)
+
+
 def test_temperatures_by_row():
     c = _case([4, 3, 1, 5, 2, 6], 5000, BF16, F32, 11)
     c["temperature"] = torch.tensor([1.0, 0.0, -1.0, 0.3, float("nan"), 1e-30], device="cuda")

@@ -102,6 +102,17 @@ def test_verify_calls_are_refused():
         assert L.kq_verify_workspace_bytes(*bad, 1) == 0, bad
 
 
+def test_a_temperature_crosses_the_c_abi_in_64_bits():
+    m, L = _lib()
+    args = dict(x=X, dt=m.DTYPE_F16, stride=100, tok=X, cu=X, u=None, r=None, p=None, pt=0, ps=0, temps=None, temp=0.0, kv=X,
+                T=4, B=2, V=100, acc=X, nxt=X, keep=X, ws=None, n=0)
+    call = lambda temp: L.kq_verify_drafts(*{**args, "temp": temp}.values(), None)  # noqa: E731
+    # 0 needs no random numbers; one that 32 bits would round to 0 or to infinity is as any other
+    assert call(0.0) == m.KQ_ERR_WORKSPACE_TOO_SMALL
+    for temp in (1e-60, 0.7, 1e60):
+        assert call(temp) == m.KQ_ERR_NULL_POINTER, temp
+
+
 def test_frequencies():
     from gmlx_amd import ops
     f, by = ops.rope_frequencies(64, 10000.0, device="cpu")
