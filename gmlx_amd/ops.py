@@ -1619,7 +1619,8 @@ def _rope_rows(op, name, x, out):
     if one != 1 or ot % 8 or oh % 8 or out.data_ptr() % 16 or not _apart(T, ot, H, oh, D):
         raise ValueError(f"{op}: {name}_out must have contiguous rows at strides in multiples of 8, none on "
                          "another, and be 16-byte aligned")
-    if out.data_ptr() == given.data_ptr() and out.stride() != given.stride():
+    gt, gh, _ = given.stride()
+    if T and out.data_ptr() == given.data_ptr() and ((T > 1 and gt != ot) or (H > 1 and gh != oh)):
         raise ValueError(f"{op}: {name}_out at {name}'s address must have its strides")
     return x, out, _ROPE_ROWS_PACK(x.data_ptr(), out.data_ptr(), t, h, ot, oh, H)
 
@@ -1651,9 +1652,9 @@ def rope_qk(q, k, positions, freqs, q_weight=None, k_weight=None, eps=1e-6, inte
     to D; positions int32 [T] on the device (PagedPlan.positions).  A token of
     negative position is left out: its rows of q_out and k_out stay as they were
     (unspecified where they are not given).  float16 or bfloat16, D in 64, 96, 128,
-    256, 512, up to 2^23 tokens; q and k may be views of a packed q|k|v (strides of 8 values).  q_out /
-    k_out: where the results go, also q and k themselves (their own views), else no
-    part of an input."""
+    256, 512, up to 2^23 tokens; q and k may be views of a packed q|k|v (strides of 8
+    values).  q_out / k_out: where the results go, also q and k themselves (their own
+    views), else no part of an input or of the other."""
     _fault("rope_qk")
     _require_gpu(q, k)
     if q.dim() != 3 or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype != q.dtype or \

@@ -605,7 +605,7 @@ typedef struct {
 
 /* Rows [T][heads][D] of 16-bit values, D contiguous: strides in elements,
  * multiples of 8, addresses 16-byte aligned.  out may be x itself (with its
- * strides), and overlaps no other input otherwise. */
+ * strides); it overlaps no other input and no other output. */
 typedef struct {
     const void *x;
     void *out;

@@ -194,6 +194,20 @@ def test_write_rope_in_place(T):
     assert torch.equal(packed[:, Hq:], kv)
 
 
+@pytest.mark.parametrize("T,Hq", [(1, 8), (5, 1), (1, 1)])
+def test_in_place_where_a_dimension_is_one(T, Hq):
+    """A view of one token, or of one head, whose stride there is another than the output's."""
+    from gmlx_amd import ops
+    torch.manual_seed(T)
+    buf, k = torch.randn(T * Hq * 128, device="cuda").half(), torch.randn(T, 2, 128, device="cuda").half()
+    at = lambda odd: buf.as_strided((T, Hq, 128), (Hq * 128 if T > 1 else odd, 128 if Hq > 1 else odd, 1))  # noqa: E731
+    pos = torch.arange(T, dtype=torch.int32, device="cuda") + 7
+    want = ops.rope_qk(at(128), k, pos, _freqs(128))
+    out = at(4096)
+    got = ops.rope_qk(at(128), k, pos, _freqs(128), q_out=out)
+    assert got[0] is out and torch.equal(out, want[0]) and torch.equal(got[1], want[1])
+
+
 def test_captured_and_on_another_stream():
     from gmlx_amd import ops
     torch.manual_seed(3)

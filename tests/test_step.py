@@ -74,6 +74,21 @@ def test_rope_calls_are_refused():
     assert call(q=none, k=none) == m.KQ_OK  # no heads: nothing to do
 
 
+def test_outputs_at_an_inputs_address():
+    """Strides of a dimension of one say nothing of where its rows lie."""
+    from gmlx_amd import ops
+    buf = torch.zeros(6 * 12 * 64, dtype=torch.float16)
+    at = lambda T, H, t, h: buf.as_strided((T, H, 64), (t, h, 1))  # noqa: E731
+    for x, out in ((at(1, 8, 768, 64), at(1, 8, 512, 64)), (at(5, 1, 768, 64), at(5, 1, 768, 768)),
+                   (at(1, 1, 768, 64), at(1, 1, 64, 768)), (at(5, 8, 768, 64), at(5, 8, 768, 64)),
+                   (at(0, 8, 768, 64), at(0, 8, 512, 128))):
+        assert ops._rope_rows("rope_qk", "q", x, out)[1] is out
+    for x, out in ((at(2, 8, 768, 64), at(2, 8, 512, 64)), (at(1, 5, 768, 64), at(1, 5, 768, 128)),
+                   (at(5, 8, 768, 64), at(5, 8, 64, 320))):
+        with pytest.raises(ValueError):
+            ops._rope_rows("rope_qk", "q", x, out)
+
+
 def test_verify_calls_are_refused():
     m, L = _lib()
 
