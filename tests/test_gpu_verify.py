@@ -78,6 +78,96 @@ def test_rows_at_the_border_of_a_launch(B):
     _check(_case(ns, 9001, F32, F32, B, near=2.0))
 
 
+def _late_case(ns, V, dt, pt, seed, temp=1.0):
+    """Rows whose likely tokens lie in the slices past the 64th (of 4 KB of logits), with about as many drafts that
+    stand there as are refused there."""
+    rng = np.random.default_rng(seed)
+    T, B, late = int(sum(ns)), len(ns), 64 * 4096 // dt.itemsize
+    assert V > late
+    x = rng.normal(0, 1, (T, V)).astype(np.float32)
+    likely = np.stack([late + rng.permutation(V - late)[:min(24, V - late)] for _ in range(T)])
+    at = np.arange(T)[:, None]
+    x[at, likely] = 10 + rng.normal(0, 1, likely.shape)
+    x[np.arange(T), rng.integers(0, late, T)] = 11  # and one before
+    logits = torch.from_numpy(x).to(dt)
+    other = logits.double().numpy()
+    other[at, likely] += rng.normal(0, 1.0, likely.shape)
+    other = np.exp((other - other.max(1, keepdims=True)) / (temp if temp > 0 else 1.0))
+    p = other / other.sum(1, keepdims=True)
+    tokens = np.zeros(T, np.int64)
+    for t in range(T - 1):
+        tokens[t + 1] = logits[t].argmax() if temp == 0 and t % 2 else np.searchsorted(np.cumsum(p[t]), rng.random() * 0.999999)
+    return dict(logits=logits.cuda(), tokens=torch.tensor(tokens, dtype=torch.int32, device="cuda"),
+                cu=torch.tensor(np.concatenate([[0], np.cumsum(ns)]), dtype=torch.int32, device="cuda"),
+                uniforms=torch.from_numpy(rng.random(T).astype(np.float32)).cuda(),
+                draws=torch.from_numpy(rng.random(B).astype(np.float32)).cuda(),
+                draft_probs=None if pt is None else torch.from_numpy(p).to(pt).cuda(), temperature=temp,
+                kv_lens=torch.tensor([n + 3 for n in ns], dtype=torch.int32, device="cuda"))
+
+
+# slices: 65 and 69 of 1024 values, 65 and 75 of 2048 (one value in the last of the first of each)
+@pytest.mark.parametrize("V,dt", [(65537, F32), (70001, F32), (131073, F16), (152064, BF16)])
+@pytest.mark.parametrize("pt", [None, F32, F16])
+@pytest.mark.parametrize("temp", [1.0, 0.7, 0.0])
+def test_drafts_past_the_64th_slice(V, dt, pt, temp):
+    _say("late", V, dt, pt, temp)
+    ns = [2, 3, 1, 5, 4, 2, 2, 3, 6, 2, 2, 1, 3, 2]
+    c = _late_case(ns, V, dt, pt, V + int(10 * temp), temp)
+    got = _check(c)
+    late = 64 * 4096 // dt.itemsize
+    cu, tokens, acc = (x.tolist() for x in (c["cu"], c["tokens"], got.accepted))
+    fell = sum(tokens[cu[b] + 1 + acc[b]] >= late for b in range(len(ns)) if acc[b] < ns[b] - 1)
+    stood = lambda acc: sum(tokens[cu[b] + 1 + i] >= late for b in range(len(ns)) for i in range(acc[b]))  # noqa: E731
+    if V in (65537, 131073):  # (whose last slice is one token)
+        return
+    assert fell >= 2 and sum(t >= late for t in got.tokens.tolist()) >= 5
+    if pt is None and temp:  # (of 24 likely tokens a lone draft stands once in some 24 times: with smaller numbers too)
+        c["uniforms"] *= 0.05
+        got = _check(c)
+    assert stood(got.accepted.tolist()) >= 3
+
+
+@pytest.mark.parametrize("B", [90, 91])
+def test_many_rows_of_drafts_past_the_64th_slice(B):
+    """17 workgroups a row: 1530 find their rows' ends themselves, 1547 do not."""
+    _say("late", B)
+    ns = np.random.default_rng(B).integers(1, 4, B).tolist()
+    _check(_late_case(ns, 66000, F32, F32, B, 0.7))
+
+
+def test_equal_logits_in_slices_of_one_lane():
+    """The largest logit in slices 3, 67 and 131 (one lane's), 130 (an earlier lane's) and within a slice twice."""
+    from gmlx_amd import ops
+    V = 140 * 1024
+    spots = [[3, 67, 131], [67, 131], [130, 131], [66, 67], [131], [64, 2 + 64], [139]]
+    x = torch.randn(len(spots), V, device="cuda")
+    for t, where in enumerate(spots):
+        for s in where:
+            x[t, [s * 1024 + 77, s * 1024 + 900]] = 9.0
+    want = [w[0] * 1024 + 77 for w in spots]
+    n = len(spots)
+    r = ops.verify_drafts(x, torch.tensor([0] + want[:-1], dtype=torch.int32, device="cuda"),
+                          torch.tensor([0, n], dtype=torch.int32, device="cuda"), temperature=0)
+    assert r.accepted.tolist() == [n - 1] and r.tokens.tolist() == [want[-1]]
+
+
+def test_a_lone_draft_holds_its_late_slice():
+    """A refused draft with all but a millionth of the weight of a slice past the 64th, or all of the row's."""
+    from gmlx_amd import ops
+    V, d = 70001, 66 * 1024 + 5
+    for others in (-20.0, -60.0, -float("inf")):
+        x = torch.full((2, V), others, device="cuda")
+        x[0, d], x[0, 3] = 4.0, -12.0
+        x[0, d + 1] = -18.0
+        kw = dict(tokens=torch.tensor([0, d], dtype=torch.int32, device="cuda"), uniforms=torch.ones(2, device="cuda"))
+        for draw in (0.0, 0.3, 0.9, 0.99999, 0.9999999):
+            c = dict(logits=x, cu=torch.tensor([0, 2], dtype=torch.int32, device="cuda"),
+                     draws=torch.tensor([draw], device="cuda"), draft_probs=None, temperature=1.0,
+                     kv_lens=torch.tensor([9], dtype=torch.int32, device="cuda"), **kw)
+            got = _check(c)
+            assert got.accepted.tolist() == [0] and got.tokens.tolist() != [d]
+
+
 def test_drafts_of_all_kinds_of_agreement():
     """Models that agree (all stand) and that do not (the first falls), long drafts."""
     for near, spread in ((0.0, 4.0), (8.0, 4.0), (0.1, 0.0)):
