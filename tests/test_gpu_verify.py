@@ -168,6 +168,38 @@ def test_a_lone_draft_holds_its_late_slice():
             assert got.accepted.tolist() == [0] and got.tokens.tolist() != [d]
 
 
+@pytest.mark.parametrize("V,share", [(1500, 2e-6), (1500, 1e-4), (1500, 0.05), (9000, 3e-6), (150000, 2e-4)])
+def test_draws_behind_a_refused_draft_of_nearly_all_the_weight(V, share):
+    """The rest of a row whose lone draft holds all but `share` of the weight is summed by itself: taken off the whole,
+    it would keep the whole's error, 10^-16 and more of it.  Draws are the numbers nearest to a border of the rest, of
+    which they are 10^-8 apart at most."""
+    from gmlx_amd import ops
+    n = 300
+    rng = np.random.default_rng(V)
+    x = rng.normal(0, 1, V)
+    x = torch.from_numpy(x - np.log(np.exp(x).sum() / share)).float()  # (a sum of `share` beside the draft's 1)
+    d = V // 3
+    x[d] = 0.0
+    w = np.exp(x.numpy().astype(np.longdouble))
+    w[d] = 0
+    run = np.cumsum(w)
+    border = run / run[-1]
+    draw = border.astype(np.float32)
+    gap = np.abs(draw - border)
+    ok = np.nonzero((gap > _APART) & (draw < 1) & (w > 0))[0]
+    ok = ok[np.argsort(gap[ok])[:n]]  # the nearest
+    n = len(ok)
+    draws = draw[ok]
+    want = np.searchsorted(run, draws.astype(np.longdouble) * run[-1], side="right")
+    tokens = torch.tensor([0, d] * n, dtype=torch.int32, device="cuda")
+    r = ops.verify_drafts(x.cuda()[None].expand(2 * n, V), tokens, torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device="cuda"),
+                          torch.ones(2 * n, device="cuda"), torch.from_numpy(draws).cuda())
+    assert r.accepted.tolist() == [0] * n
+    got = r.tokens.cpu().numpy()
+    _say("rest", V, share, float(gap[ok].min()), float(gap[ok].max()), int((got != want).sum()), "of", n)
+    assert np.array_equal(got, want)
+
+
 def test_drafts_of_all_kinds_of_agreement():
     """Models that agree (all stand) and that do not (the first falls), long drafts."""
     for near, spread in ((0.0, 4.0), (8.0, 4.0), (0.1, 0.0)):
