@@ -31,6 +31,8 @@ copied over in place, as here):
   for each layer: q = paged_write_rope(q, k, v, k_cache, v_cache, p.slots, p.positions, freqs, q_weight=, k_weight=)
                   o = sdpa_paged(q, k_cache, v_cache, block_table, p.kv_lens, p.cu_q, scale, max_q=, max_kv=, window=)
   r = verify_drafts(logits, tokens, p.cu_q, uniforms, draws, kv_lens=p.kv_lens)    # kept = r.keep_lens
+(A row ends with kept = 0; one whose pages behind a window were given back by hand does
+not: paged_plan says how.)
 paged_write_rope is rope_qk (head norms and rotary positions) and paged_write in one
 launch; verify_drafts judges drafted tokens and draws the next one.
 """
@@ -1356,6 +1358,14 @@ def paged_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_siz
     keep its shared tokens, which gives back its own pages, then set its length
     to 0 by hand; only the last holder keeps 0.
 
+    Every entry of a row below its length is held for a page of the row's,
+    whatever is there.  Of a row whose pages behind a window were put on the stack by
+    hand (between two calls), those entries must never be let go here, or they are
+    handed out to later rows: keep_lens[b] stays at or past the first page still held
+    behind them, and the row is ended in two steps too: keep the tokens before that
+    page, which gives back the pages from there on, then by hand put its first pages
+    (the sinks') on the stack and set its length to 0.
+
     seq_lens, new_lens, keep_lens int32 [B], B <= 2048; block_table int32
     [B, pages]; free_pages int32 [n] with n the pool's pages; free_count int32
     [1]; page_size a power of two from 16 to 1024; max_tokens >= the new tokens
@@ -1453,7 +1463,8 @@ def sdpa_paged(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, max_q=Non
     window (1 to 2^30; None: none): of the keys up to its own, a token sees the last
     `window` and the row's first `sinks` (0 to 2^30).  Only their pages are read, and
     time goes by them: table entries between the sinks and the window of the row's
-    first new token may be anything."""
+    first new token may be anything.  Their pages may be put on the free stack by hand
+    between two plans; paged_plan says how such a row is then ended."""
     _fault("sdpa_paged")
     lay, pool = _paged_pool(k_cache, v_cache, (k_scales, k_biases, v_scales, v_biases))
     dev, dt, Hkv, D, B, shape = lay.device, lay.dtype, lay.Hkv, lay.D, kv_lens.numel(), q.shape

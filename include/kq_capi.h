@@ -500,6 +500,13 @@ typedef struct {
  * puts it on the stack, from which two later rows would get it.  Such a row keeps
  * its shared tokens here, and its length is then set to 0 by the caller; only the
  * last holder keeps 0.
+ * Every entry of a row below its length is held for a page of the row's, whatever
+ * is there.  A row whose pages behind a window the caller has put on the stack
+ * (kq_sdpa_paged_window) therefore never lets those entries go here: keep_lens[b]
+ * stays at or past the first page still held behind them, and the row is ended in
+ * two steps, kept up to that page here, then its first pages put on the stack and its
+ * length set to 0 by the caller.  (Let go here, such entries would be handed out:
+ * later rows' tokens would get no slot without being refused, or share one.)
  *   cu_q [B + 1]      running sum of new_lens (refused rows' tokens included)
  *   kv_lens [B]       kept + new (refused rows: seq_lens[b])
  *   slots [max_tokens], positions [max_tokens]  of every new token, in cu_q's
@@ -575,7 +582,8 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
  * those past p - window, the last `window`, and the row's first `sinks` (window 1 ..
  * 2^30, sinks 0 .. 2^30; window 1: itself and the sinks).  Only these keys' pages are
  * read: table entries between the sinks and the first new token's window may be
- * anything (their pages given back).  Splits follow the window's length, not the
+ * anything.  Their pages may be put on the free stack between two plans; such a row is
+ * then ended as kq_paged_plan says.  Splits follow the window's length, not the
  * row's; with a window that no row passes, what kq_sdpa_paged gives to its rounding.
  * Everything else as kq_sdpa_paged has it, the workspace's size apart. */
 size_t kq_sdpa_paged_window_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,

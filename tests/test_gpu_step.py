@@ -162,3 +162,80 @@ def test_steps(q8, dt):
     used = [int(eager.table[b, i]) for b in range(5) for i in range(-(-int(eager.seq[b]) // P))]
     free = eager.free[:int(eager.count)].tolist()
     assert sorted(used + free) == list(range(5 * 16))
+
+
+@pytest.mark.parametrize("sinks", [0, 3, 40])
+def test_pages_behind_the_window_given_back_and_rows_ended(sinks):
+    """Pages that no later token sees go on the stack by hand between two plans, and their rows are ended in two steps:
+    what lies from the first page held behind them on by the plan, the sinks' pages by hand.  Outputs are those of a
+    cache that holds everything, in a pool too small for that, and no page is ever in two places."""
+    from gmlx_amd import ops
+    B, n, steps, width = 3, 20, 40, 64
+    rng = np.random.default_rng(sinks)
+    gen = torch.Generator(device="cuda").manual_seed(sinks)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    class Cache:
+        def __init__(self, n_pages):
+            self.n = n_pages
+            self.k, self.v = (torch.full((n_pages, HKV, P, D), float("nan"), dtype=torch.float16, device="cuda") for _ in range(2))
+            self.table, self.free, self.count = i32([[-1] * width] * B), i32(list(range(n_pages))), i32([n_pages])
+            self.seq, self.hole = i32([0] * B), [(0, 0)] * B
+
+        def step(self, new, keep, q, k, v):
+            p = ops.paged_plan(self.seq, i32(new), self.table, self.free, self.count, P, sum(new), keep_lens=i32(keep))
+            ops.paged_write(k, v, self.k, self.v, p.slots)
+            self.seq.copy_(p.kv_lens)
+            self.count.copy_(p.free_count)
+            assert p.refused.sum() == 0
+            return ops.sdpa_paged(q, self.k, self.v, self.table, p.kv_lens, p.cu_q, D ** -0.5, max_q=max(new), window=WINDOW,
+                                  sinks=sinks)
+
+        def push(self, b, pages):
+            c = int(self.count)
+            for j in pages:
+                self.free[c], c = int(self.table[b, j]), c + 1
+                self.table[b, j] = -1
+            self.count.fill_(c)
+
+        def give_back(self, b, kept):
+            """Pages between the sinks and the window of the next new token, at position `kept`."""
+            first, end = self.hole[b][1] or -(-sinks // P), max(kept + 1 - WINDOW, 0) // P
+            if end > first:
+                self.push(b, range(first, end))
+                self.hole[b] = (-(-sinks // P), end)
+
+        def held(self):
+            return [int(x) for b in range(B) for x in self.table[b, :-(-int(self.seq[b]) // P)] if x >= 0]
+
+        def whole(self):
+            assert sorted(self.held() + self.free[:int(self.count)].tolist()) == list(range(self.n))
+
+    # a row holds the sinks', the window's and the new tokens' pages, and what the last one had
+    small, large = Cache(B * (-(-sinks // P) + (WINDOW + 2 * n) // P + 3)), Cache(B * width)
+    kept, most = [0] * B, 0
+    for step in range(steps):
+        new = rng.integers(1, n + 1, B).tolist()
+        if step % 13 == 12:
+            b = step // 13 % B  # the row ends, and a new request takes its place
+            if small.hole[b][1]:
+                keep = [small.hole[b][1] * P if i == b else kept[i] for i in range(B)]
+                assert keep[b] <= int(small.seq[b])
+                p = ops.paged_plan(small.seq, i32([0] * B), small.table, small.free, small.count, P, 0, keep_lens=i32(keep))
+                small.seq.copy_(p.kv_lens)
+                small.count.copy_(p.free_count)
+                small.push(b, range(small.hole[b][0]))
+                small.seq[b], small.hole[b] = 0, (0, 0)
+                small.whole()
+            kept[b] = 0
+        x = torch.randn(sum(new), HQ + 2 * HKV, D, device="cuda", generator=gen).half()
+        a, b = (c.step(new, kept, x[:, :HQ], x[:, HQ:HQ + HKV], x[:, HQ + HKV:]) for c in (small, large))
+        assert torch.equal(a, b), step
+        assert not a.isnan().any()
+        small.whole()
+        large.whole()
+        most = max(most, len(large.held()))
+        kept = [max(k, k + m - int(r)) for k, m, r in zip(kept, new, rng.integers(0, 3, B))]  # some drafts fall
+        for r in range(B):
+            small.give_back(r, kept[r])
+    assert most > small.n
