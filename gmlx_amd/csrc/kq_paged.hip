@@ -1768,14 +1768,27 @@ Plan paged_plan(int64_t T, int64_t B, int Hq, int Hkv, int D, int max_q, int max
     Plan p;
     const int G = Hq / Hkv, limit = few_limit(q8), chunk = limit / G + 1;  // tokens of the shortest chunk
     p.rule = wave_rule(Hq, Hkv, D, q8);
+    // Through a window of up to kOneLength keys one length for the call's rows, by what
+    // it shows at most: then no row has more splits than a full window, and no grid's
+    // waves are left without work.  That of 4096 keys past them, since the longer one by
+    // the window leaves a few rows to a few long splits.  Wider windows are filled by few
+    // rows: each row's own length there, as without one.  us, lengths by row / one by
+    // the window / this, 32 query heads on 8, head dim 128, rows of the window or
+    // more, then rows of a tenth to half of it:
+    //    1024 keys     1 row  11.6 / 11.6 / 11.6,  9.9 / 10.5 / 10.4    64    70 /   70 /   70,  39 /  29 /  29
+    //    4100                 16.0 / 15.9 / 14.2, 11.2 / 14.0 / 11.3         276 /  215 /  232,  81 /  68 /  80
+    //    8196                 21.7 / 21.4 / 16.2, 11.9 / 19.9 / 11.9         505 /  399 /  463, 155 / 118 / 155
+    //   16004                 22.3 / 22.4 / 20.1, 15.1 / 20.3 / 13.9         772 /  773 /  886, 242 / 245 / 234
+    //   20004 (this: by row)  23.9 / 23.7 / 23.9, 15.3 / 20.5 / 15.3         971 /  974 /  971, 299 / 284 / 299
+    //   32772 (this: by row)  38.7 / 39.0 / 38.7, 20.8 / 20.9 / 20.8        1591 / 1591 / 1591, 452 / 516 / 452
+    // and one row of 1800 keys through 32768 or more 12.5 / 19.9 / 12.5, at head dim 256 15.1
+    // / 31.6 / 15.1.  Over four head counts and types, 1, 16 and 64 rows, in the geometric
+    // mean: up to 3000 keys by row 1.02 of this; 4100 to 16004 by row 1.04, one by the window
+    // 1.03; 20004 one 1.00 of this, 32772 1.06.
+    constexpr int kOneLength = 16384;
     if (window) {
-        // One length for the call's rows, by what its window shows at most: then no row
-        // has more splits than a full window, and no grid's waves are left without work
-        // (us, at lengths by row / this: 64 rows of 512 keys 39 / 37, 48 of 4096 202 / 168,
-        // in 8 bits 48 of 1024 49 / 36).  Windows of up to 16384 keys as those of 4096, for
-        // many rows are shorter: one of 1500 keys would wait for 256 at a time.
         const int span = window_span(1 << 30, window, sinks, 1, G, 16);
-        p.rule = SplitRule{0, 0, 0, 0, p.rule.tokens(span <= 16384 && span > 4096 ? 4096 : span)};
+        if (span <= kOneLength) p.rule = SplitRule{0, 0, 0, 0, p.rule.tokens(span < 4096 ? span : 4096)};
     }
     p.few = chunk > 1 ? most_row_splits(p.rule, max_kv) : 1;
     p.many = max_q >= chunk ? paged_splits(p.rule, chunk, max_kv, G, Hkv, limit, group_columns(D, q8), group_slots(D, q8),

@@ -100,6 +100,24 @@ def test_long_rows(P, layout, q8):
         b.check(b.run())
 
 
+@pytest.mark.parametrize("window,sinks", [(16382, 1), (16384, 0), (16385, 0), (16300, 200), (20000, 4)])
+@pytest.mark.parametrize("Hq,Hkv,D,q8", [(8, 2, 128, False), (8, 2, 64, True), (4, 1, 256, False)])
+def test_wide_windows(window, sinks, Hq, Hkv, D, q8):
+    """On both sides of the line behind which splits go by the row: rows shorter than the window, at its end and past it."""
+    rows = [(1, 1700), (1, window + 3), (3, 25000), (1, 600), (1, window - 1), (20, 16400), (1, 4097)]
+    b = Windowed(rows, Hq, Hkv, D, 64, F16, window, sinks, q8=q8, seed=window)
+    _say("wide", window, sinks, Hq, D, q8)
+    out = b.run()
+    b.check(out)
+    from gmlx_amd import ops
+    for i in (0, 2, 4):  # a row alone has its bits
+        lo, hi = int(b.cu[i]), int(b.cu[i + 1])
+        one = ops.sdpa_paged(b.q[lo:hi].cuda(), *b.pool, b.table[i:i + 1], b.kv_lens[i:i + 1],
+                             torch.tensor([0, hi - lo], dtype=torch.int32, device="cuda"), b.scale, max_q=hi - lo,
+                             max_kv=rows[i][1], window=window, sinks=sinks, **b.scales)
+        assert torch.equal(one, out[lo:hi]), rows[i]
+
+
 def test_a_window_past_every_row_is_none():
     for q8 in (False, True):
         rows = [(1, 700), (40, 333), (5, 2), (1, 5000), (130, 2100)]

@@ -209,6 +209,16 @@ def test_window_calls_are_refused_and_sized():
     assert call(window=4096, mkv=1 << 20) == m.KQ_ERR_WORKSPACE_TOO_SMALL
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,q8", [(32, 8, 128, 0), (32, 8, 128, 1), (64, 4, 128, 0), (16, 2, 256, 0), (16, 2, 256, 1)])
+def test_a_window_far_past_the_rows_keeps_their_splits(Hq, Hkv, D, q8):
+    """The workspace counts a call's splits: those of the rows, not of a window that none of them fills."""
+    L = _lib()[1]
+    for keys in (1600, 2000, 6000, 8000, 12000):
+        whole = L.kq_sdpa_paged_workspace_bytes(4, 4, Hq, Hkv, D, 1, keys, q8)
+        for window, sinks in ((16385, 0), (16320, 65), (32768, 4), (1 << 18, 0), (1 << 30, 1 << 30), (64, 1 << 20)):
+            assert L.kq_sdpa_paged_window_workspace_bytes(4, 4, Hq, Hkv, D, 1, keys, q8, window, sinks) == whole
+
+
 def test_window_reference():
     rng = np.random.default_rng(2)
     q, k, v = rng.normal(size=(3, 2, 8)), rng.normal(size=(1, 20, 8)), rng.normal(size=(1, 20, 8))
