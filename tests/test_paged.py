@@ -314,6 +314,36 @@ def test_register_copies_of_the_decode_kernels(tmp_path):
     assert not _before_exec(text)
 
 
+def _vector_registers(lib):
+    """{kernel: (vector registers, bytes spilled)} of the library's gfx950 code, from its objects' own notes."""
+    import struct
+    data, magic, at, found = open(lib, "rb").read(), b"__CLANG_OFFLOAD_BUNDLE__", 0, {}
+    while (at := data.find(magic, at)) >= 0:
+        n, = struct.unpack_from("<Q", data, at + len(magic))
+        p = at + len(magic) + 8
+        for _ in range(n):
+            off, size, name = struct.unpack_from("<QQQ", data, p)
+            if b"gfx950" in data[p + 24:p + 24 + name]:
+                notes = subprocess.run(["/opt/rocm/llvm/bin/llvm-readelf", "--notes", "-"], input=data[at + off:at + off + size],
+                                       capture_output=True, check=True).stdout.decode()
+                for k in notes.split("  - .agpr_count:")[1:]:
+                    get = lambda key: re.search(rf"\.{key}: *(\S+)", k).group(1)  # noqa: E731
+                    found[get("name")] = int(get("vgpr_count")), int(get("vgpr_spill_count"))
+            p += 24 + name
+        at += len(magic)
+    return found
+
+
+def test_merges_leave_room_for_three_and_four_waves():
+    """512 vector registers a SIMD lane: at head dim 64 the merge of many rows holds sixteen splits ahead and takes a third
+    of them; one more and 22928 tokens and heads take 24 us in place of 20."""
+    from gmlx_amd import build
+    merges = {k: v for k, v in _vector_registers(build.LIB).items() if "kq_paged_merge_kernel" in k}
+    assert len(merges) == 5 * 2 * 2 * 2  # head dims, types, grids, with a window and without
+    for name, (registers, spilled) in merges.items():
+        assert registers <= (168 if "ILi64E" in name else 128) and spilled == 0, (name, registers, spilled)
+
+
 def test_plan_refuses_more_tokens_than_its_grid_counts():
     """A grid's step past 2^31 - 1 tokens would be a negative number."""
     m, L = _lib()
