@@ -30,9 +30,11 @@ copied over in place, as here):
   seq_lens.copy_(p.kv_lens); free_count.copy_(p.free_count)
   for each layer: q = paged_write_rope(q, k, v, k_cache, v_cache, p.slots, p.positions, freqs, q_weight=, k_weight=)
                   o = sdpa_paged(q, k_cache, v_cache, block_table, p.kv_lens, p.cu_q, scale, max_q=, max_kv=, window=)
-  r = verify_drafts(logits, tokens, p.cu_q, uniforms, draws, kv_lens=p.kv_lens)    # kept = r.keep_lens
-(A row ends with kept = 0; one whose pages behind a window were given back by hand does
-not: paged_plan says how.)
+  r = verify_drafts(logits, tokens, p.cu_q, uniforms, draws, kv_lens=p.kv_lens)
+  kept.copy_(torch.where(p.refused > 0, kept, r.keep_lens))
+(A row that the plan refused stays as it was, the drafts of the step before still at its
+end, and keeps what it kept.  A row ends with kept = 0; one whose pages behind a window
+were given back by hand does not: paged_plan says how.)
 paged_write_rope is rope_qk (head norms and rotary positions) and paged_write in one
 launch; verify_drafts judges drafted tokens and draws the next one.
 """
@@ -1749,7 +1751,9 @@ def verify_drafts(logits, tokens, cu, uniforms=None, draws=None, draft_probs=Non
     uniforms float32 [T] and draws float32 [B] in [0, 1), not needed where the
     temperature is 0; temperature a number (taken in 64 bits), or float32 [B] on the
     device (0 or below: greedy); cu int32 [B + 1]; kv_lens int32 [B] (PagedPlan.kv_lens, all n tokens of
-    the row counted) for keep_lens, which paged_plan takes.  Returns a DraftVerdict.
+    the row counted) for keep_lens, which paged_plan takes.  Of a row that the plan
+    refused kv_lens counts none of them: its verdict is of no use, and it keeps what it
+    kept (PagedPlan.refused).  Returns a DraftVerdict.
 
     Computed in 64 bits.  NaN logits count as -inf, +inf as the largest float32,
     probabilities below 0 or NaN as 0; a draft outside the vocabulary does not stand.

@@ -659,7 +659,8 @@ int kq_paged_write_rope(const kq_paged_pool *pool, const kq_rope *rope, const in
  * Temperature 0 (or below): drafts stand where they are the largest logit, which
  * else is the next token; of equal ones the lowest.
  * keep_lens[b] (may be NULL): kv_lens[b] less the refused drafts, what
- * kq_paged_plan keeps of a row whose kv_lens count all n tokens.
+ * kq_paged_plan keeps of a row whose kv_lens count all n tokens.  Those of a row that
+ * the plan refused count none: its verdict is of no use, and it keeps what it kept.
  *
  * Weights (good to 4 10^-14; below 2^-1000 none) and sums in fp64.  NaN counts as
  * -infinity, +infinity as the largest fp32; probabilities below 0 and NaN as 0; drafts

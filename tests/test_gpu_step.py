@@ -239,3 +239,60 @@ def test_pages_behind_the_window_given_back_and_rows_ended(sinks):
         for r in range(B):
             small.give_back(r, kept[r])
     assert most > small.n
+
+
+def test_a_row_that_the_plan_refuses_keeps_what_it_kept():
+    """A row without pages for its new tokens stays as it was, with the drafts of the step before still at its end: its
+    verdict is of no use, and what it keeps is what it kept.  It goes on when pages come free, its cache whole."""
+    from gmlx_amd import ops
+    dt, n, width = torch.float16, 4, 8
+    rng = np.random.default_rng(5)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    packed = torch.randn(V, HQ + 2 * HKV, D, device="cuda", generator=gen).to(dt)
+    freqs, _ = ops.rope_frequencies(D)
+    n_pages = 7
+    kc, vc = (torch.zeros(n_pages, HKV, P, D, dtype=dt, device="cuda") for _ in range(2))
+    table, free, count = i32([[-1] * width] * 3), i32(list(range(n_pages))), i32([n_pages])
+    rows = [rng.integers(0, V, m).tolist() for m in (30, 20, 40)]
+    seq, kept = i32([0, 0, 0]), i32([0, 0, 0])
+
+    def step(new, toks):
+        p = ops.paged_plan(seq, i32(new), table, free, count, P, len(toks), keep_lens=kept)
+        x = packed[torch.tensor(toks, device="cuda")]
+        ops.paged_write_rope(x[:, :HQ], x[:, HQ:HQ + HKV], x[:, HQ + HKV:], kc, vc, p.slots, p.positions, freqs)
+        seq.copy_(p.kv_lens)
+        count.copy_(p.free_count)
+        return p
+    p = step([30, 20, 40], sum(rows, []))  # 2 + 2 + 3 pages: none left
+    assert p.refused.sum() == 0 and int(p.free_count) == 0
+    kept.copy_(p.kv_lens)
+    refusals = went_on = 0
+    for t in range(12):
+        if t == 7:  # the third row ends
+            kept[2], rows[2] = 0, []
+        toks = [rng.integers(0, V, n).tolist() for _ in range(3)]
+        before = kept.tolist()
+        assert before == [len(r) for r in rows]
+        p = step([n, n, n if t < 7 else 0], sum(toks[:3 if t < 7 else 2], []))
+        T = 3 * n if t < 7 else 2 * n
+        logits = torch.randn(T, V, device="cuda", generator=gen)
+        r = ops.verify_drafts(logits, i32(sum(toks, [])[:T]), p.cu_q, torch.rand(T, device="cuda", generator=gen) * 0.02,
+                              torch.rand(3, device="cuda", generator=gen), kv_lens=p.kv_lens)
+        # a row without new tokens keeps all, a refused one what it kept
+        kept.copy_(torch.where(p.refused > 0, kept, r.keep_lens))
+        for b in range(3):
+            if p.refused[b]:
+                refusals += 1
+                assert int(kept[b]) == before[b] <= int(seq[b]) == int(p.kv_lens[b])
+            elif t < 7 or b < 2:
+                rows[b] = (rows[b] + toks[b])[:int(kept[b])]
+                assert len(rows[b]) == int(kept[b]) == before[b] + 1 + int(r.accepted[b])
+                went_on += t > 7 and refusals > 0
+            pos = torch.arange(len(rows[b]), dtype=torch.int32, device="cuda")
+            if len(pos):
+                x = packed[torch.tensor(rows[b], device="cuda")]
+                _, kr = ops.rope_qk(x[:, :HQ], x[:, HQ:HQ + HKV], pos, freqs)
+                ck, cv = ops.paged_read(kc, vc, (table[b, (pos // P).long()] * P + pos % P).int())
+                assert torch.equal(ck, kr) and torch.equal(cv, x[:, HQ + HKV:]), (t, b)
+    assert refusals > 3 and went_on > 3
