@@ -208,6 +208,35 @@ def test_in_place_where_a_dimension_is_one(T, Hq):
     assert got[0] is out and torch.equal(out, want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("T,Hq,Hkv,D", [(360000, 32, 8, 128), (2200000, 4, 2, 128)])
+def test_rows_past_32_bits_of_values(T, Hq, Hkv, D):
+    """Each token is its own: the last ones have the bits of a call on them alone, one or several tokens a workgroup."""
+    from gmlx_amd import ops
+    _say("long", T)
+    n, P, step = 777, 256, Hq + 2 * Hkv
+    assert T * step * D > 2 ** 31
+    packed = torch.empty(T, step, D, dtype=F16, device="cuda")
+    for c in packed.split(100000):
+        c.normal_()
+    q, k, v = packed[:, :Hq], packed[:, Hq:Hq + Hkv], packed[:, Hq + Hkv:]
+    pos = torch.arange(T, dtype=torch.int32, device="cuda") * 3
+    freqs, w = _freqs(D), torch.randn(D, device="cuda")
+    pages = -(-T // P)
+    slots = pos // 3
+    kw = dict(q_weight=w, k_weight=w)
+    last = packed[-n:].clone()
+    lq, lk, lv = last[:, :Hq], last[:, Hq:Hq + Hkv], last[:, Hq + Hkv:]
+    want = ops.rope_qk(lq, lk, pos[-n:].clone(), freqs, **kw)
+    got = ops.rope_qk(q, k, pos, freqs, **kw)
+    assert torch.equal(got[0][-n:], want[0]) and torch.equal(got[1][-n:], want[1])
+    del got
+    kc, vc = (torch.zeros(pages, Hkv, P, D, dtype=F16, device="cuda") for _ in range(2))
+    out = ops.paged_write_rope(q, k, v, kc, vc, slots, pos, freqs, q_out=q, **kw)
+    assert torch.equal(out[-n:], want[0])
+    ck, cv = ops.paged_read(kc, vc, slots[-n:].clone())
+    assert torch.equal(ck, want[1]) and torch.equal(cv, lv)
+
+
 def test_captured_and_on_another_stream():
     from gmlx_amd import ops
     torch.manual_seed(3)

@@ -135,6 +135,29 @@ def test_many_rows_of_drafts_past_the_64th_slice(B):
     _check(_late_case(ns, 66000, F32, F32, B, 0.7))
 
 
+@pytest.mark.parametrize("pt", [None, BF16])
+def test_a_vocabulary_of_thousands_of_slices(pt):
+    V = (1 << 24) + 5  # 8193 slices, five tokens in the last
+    rng = np.random.default_rng(3)
+    x = torch.randn(3, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    x[:, V - 3] = 16.0
+    x[0, [5, 1 << 23]] = 15.0
+    x = x.to(BF16)
+    p = None
+    if pt is not None:
+        p = torch.softmax(x.float(), 1).to(pt)
+        p[:, V - 3] *= 1.5
+    for temp in (1.0, 0.0):
+        for draft, draw in ((V - 3, 0.0), (V - 3, 0.999), (7, 0.3), (V, 0.97), (1 << 23, 0.5)):
+            c = dict(logits=x, tokens=torch.tensor([0, V - 3, draft], dtype=torch.int32, device="cuda"),
+                     cu=torch.tensor([0, 3], dtype=torch.int32, device="cuda"),
+                     uniforms=torch.tensor([0.0, rng.random(), 0.0], device="cuda").float(),
+                     draws=torch.tensor([draw], device="cuda"), draft_probs=p, temperature=temp,
+                     kv_lens=torch.tensor([9], dtype=torch.int32, device="cuda"))
+            _say("vocabulary", pt, temp, draft, draw)
+            _check(c)
+
+
 def test_equal_logits_in_slices_of_one_lane():
     """The largest logit in slices 3, 67 and 131 (one lane's), 130 (an earlier lane's) and within a slice twice."""
     from gmlx_amd import ops
