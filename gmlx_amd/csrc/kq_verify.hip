@@ -13,6 +13,8 @@
 // hundred on the other side of some border at V = 10^5.  So is a temperature given
 // as a number: 0.7 rounded to fp32 alone, off by 1.7 10^-8, moved 16 of 60000 draws
 // at V = 152064.
+#include <algorithm>
+
 #include "kq_attn.h"
 
 namespace {
@@ -31,7 +33,7 @@ struct VerifyArgs {
     int64_t stride, probs_stride;
     const int32_t *tokens, *cu, *kv;
     const float *u, *draws, *temps;
-    double temp;
+    double rate;  // log2(e) / c without temps, 0 at a temperature of 0
     int32_t T, B, V, S;  // S: slices a row
     int32_t probs_type;
     Part *part;    // [T][S]
@@ -107,13 +109,12 @@ __device__ __forceinline__ void values(const void *row, int i, int V, float past
 // weight of either is right as it is.)
 __device__ __forceinline__ float counted(float x) { return x != x ? -INFINITY : fminf(x, 3.4028235e38f); }
 
-__device__ __forceinline__ double temp_of(const VerifyArgs &a, int b) { return a.temps ? (double)a.temps[b] : a.temp; }
-__device__ __forceinline__ bool greedy(const VerifyArgs &a, int b) { return !(temp_of(a, b) > 0.0); }
+__device__ __forceinline__ bool greedy(const VerifyArgs &a, int b) { return a.temps ? !(a.temps[b] > 0.f) : a.rate == 0.0; }
 
-// log2(e) / c of row b.  Past either limit of c any two fp32 logits are as far apart, or
-// as near, as at it, and at them the rate is finite and no 0.
+// log2(e) / c of row b.
+__host__ __device__ __forceinline__ double rate_at(double c) { return 1.4426950408889634074 / c; }
 __device__ __forceinline__ double rate_of(const VerifyArgs &a, int b) {
-    return 1.4426950408889634074 / fmin(fmax(temp_of(a, b), 1e-300), 1e300);
+    return a.temps ? rate_at(fminf(a.temps[b], 3.4028235e38f)) : a.rate;
 }
 
 // The weight of x <= m (both fp64 steps are exact for x = m), and the same, 0 below 2^-1000.
@@ -619,7 +620,8 @@ int kq_verify_drafts(const void *logits, int dtype, int64_t row_stride, const in
     a.u = uniforms;
     a.draws = draws;
     a.temps = temperatures;
-    a.temp = temperature;
+    // (at either limit fp32 logits are as far apart, or as near, as past it, and the rate is finite and not 0)
+    a.rate = temperature > 0.0 ? rate_at(std::min(std::max(temperature, 1e-300), 1e300)) : 0.0;
     a.T = T;
     a.B = B;
     a.V = V;
