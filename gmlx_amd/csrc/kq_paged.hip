@@ -25,9 +25,9 @@
 // keys through registers; 16 rows of 1 k to 131 k keys, head dim 128, 2.01 GB
 // in 371 us, 5.4 TB/s.  Chunks: bound by the MFMA, exp and LDS pipes together,
 // tiles in LDS shared by the workgroup's columns; 2048 tokens behind 6000, head
-// dim 128, 236 GFLOP in 247 to 255 us over runs, 925 to 950 TFLOP/s (1.19 PFLOP/s
-// for a plain 8192^3 product on the same card): MFMA pipes busy 45 % of the cycles,
-// LDS 35 %, a third of that in bank conflicts.
+// dim 128, 236 GFLOP in 247 to 277 us over cards and runs, 850 to 950 TFLOP/s (1.19
+// PFLOP/s for a plain 8192^3 product on the card of the 247): MFMA pipes busy 45 % of
+// the cycles, LDS 35 %, a third of that in bank conflicts.
 #include "kq_once.h"
 #include "kq_paged.h"
 
@@ -1937,8 +1937,10 @@ int attend(const void *q, int64_t q_stride, const kq_paged_pool *pool, const int
     int64_t many = blocks * (has_waves(D) ? plan.many : most);
     if (has_waves(D)) {
         // A chunk's splits times its blocks are no more than group_slots, or it has one:
-        // without this bound workgroups that find no unit queue up behind the others
-        // (2048 tokens behind 6000 keys 276 us in place of 291, through 2000 of them 96 / 101).
+        // without this bound workgroups that find no unit queue up behind the others (us,
+        // without / with it: 4096 tokens alone 175 / 167, in 8 bits 327 / 307, four rows
+        // of 1000 over 5000 386 / 371, 2048 through a window of 2000 99 / 93; 2048 behind
+        // 6000 276 / 276).
         const int64_t filled = rows * a.group_slots + (blocks > a.group_slots ? blocks - a.group_slots : 0);
         many = many < filled ? many : filled;
     }

@@ -455,7 +455,7 @@ __global__ __launch_bounds__(kThreads) void kq_verify_pick_kernel(VerifyArgs a) 
         }
     };
     // A lone draft's slice is summed again without it: taken off the slice's sum, what is
-    // left would keep that sum's error, up to all of its digits (10.5 us in place of 11.5,
+    // left would keep that sum's error, up to all of its digits (10.8 us in place of 11.4,
     // 16 rows of 64 slices; only where the draft holds half of the slice or more 12.3).
     const int own = lone ? r.draft / (kThreads * N) : -1;
     double without = 0.0;
