@@ -584,8 +584,9 @@ int kq_sdpa_paged(const void *q, int64_t q_stride, const kq_paged_pool *pool, co
  * read: table entries between the sinks and the first new token's window may be
  * anything.  Their pages may be put on the free stack between two plans; such a row is
  * then ended as kq_paged_plan says.  Splits of rows of few columns follow the
- * window's length up to 16384 keys, past it the row's; with a window that no row
- * passes, what kq_sdpa_paged gives to its rounding.
+ * length of a window of up to 16384 keys (sinks and pieces of 16 at its ends counted),
+ * past that the row's; with a window that no row passes, what kq_sdpa_paged gives to
+ * its rounding.
  * Everything else as kq_sdpa_paged has it, the workspace's size apart. */
 size_t kq_sdpa_paged_window_workspace_bytes(int32_t T, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_q,
                                             int32_t max_kv, int q8, int32_t window, int32_t sinks);
